@@ -233,6 +233,20 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dpa_conv3x3_thin_wgrad": (
         c_int, [c_void_p, c_int, c_void_p, c_void_p] + [c_int] * 5 + [c_void_p, c_int64, c_void_p],
     ),
+    "dpa_cross_attention_fwd_workspace_bytes": (c_int64, [c_void_p]),
+    "dpa_cross_attention_fwd": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
+    "dpa_cross_attention_bwd_workspace_bytes": (c_int64, [c_void_p]),
+    "dpa_cross_attention_bwd": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
+    "dpa_dropout": (c_int, [c_void_p] * 3 + [c_int, c_int64, c_void_p, c_float, c_void_p]),
+    "dpa_embedding_fwd": (
+        c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_int, c_float,
+                c_void_p, c_float, c_void_p],
+    ),
+    "dpa_embedding_bwd_workspace_bytes": (c_int64, [c_int64, c_int]),
+    "dpa_embedding_bwd": (
+        c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_int, c_float,
+                c_int64, c_void_p, c_float, c_void_p, c_int64, c_void_p],
+    ),
 }
 
 _lock = threading.Lock()

@@ -268,6 +268,36 @@ __device__ __forceinline__ uint32_t perm_b32(uint32_t hi, uint32_t lo, uint32_t 
   return __builtin_amdgcn_perm(hi, lo, sel);
 }
 
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// Elements by DPA_DTYPE_*: the 16-bit ones in pairs of a word.
+template <int DT>
+struct Elem;
+template <>
+struct Elem<DPA_DTYPE_F32> {
+  static constexpr int size = 4;
+};
+template <>
+struct Elem<DPA_DTYPE_BF16> {
+  static constexpr int size = 2;
+  static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+};
+template <>
+struct Elem<DPA_DTYPE_F16> {
+  static constexpr int size = 2;
+  static __device__ __forceinline__ float lo(uint32_t w) {
+    return (float)__builtin_bit_cast(f16x2, w).x;
+  }
+  static __device__ __forceinline__ float hi(uint32_t w) {
+    return (float)__builtin_bit_cast(f16x2, w).y;
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, f16x2));
+  }
+};
+
 // ---------------------------------------------------------------------------------------
 // Global -> LDS DMA and the explicit waits that pipeline it.
 // ---------------------------------------------------------------------------------------
@@ -346,6 +376,41 @@ inline FastDiv make_fastdiv(uint32_t d) {
 }
 
 // ---------------------------------------------------------------------------------------
+// Dropout: element idx is kept when bits [16 (idx % 4), 16 (idx % 4) + 16) of
+// splitmix64(seed + (idx / 4) * golden ratio), as a 16-bit number, are >= floor(p * 2^16).
+// ---------------------------------------------------------------------------------------
+constexpr uint64_t kDropGolden = 0x9E3779B97F4A7C15ull;
+
+// hash input of element idx (a multiple of 4)
+__device__ __forceinline__ uint64_t drop_z(uint64_t seed, int64_t idx) {
+  return seed + (uint64_t)(idx >> 2) * kDropGolden;
+}
+
+__device__ __forceinline__ uint32_t drop_mask2(uint32_t r, uint32_t keep2) {
+  uint32_t m;
+  // (as instructions of its own: the compiler turns the form into compares and selects)
+  asm("v_pk_sub_u16 %0, %1, %2 clamp\n\tv_pk_min_u16 %0, %0, %3\n\tv_pk_sub_i16 %0, %0, %3"
+      : "=&v"(m)
+      : "v"(keep2), "v"(r), "v"(0x00010001u));
+  return m;
+}
+
+// Masks of the 8 elements whose hash input starts at z0; keep2: the threshold in both halves.
+__device__ __forceinline__ uint4 drop_mask8(uint64_t z0, uint32_t keep2) {
+  uint32_t m[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint64_t z = z0 + (uint64_t)i * kDropGolden;
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    z ^= z >> 31;
+    m[2 * i] = drop_mask2((uint32_t)z, keep2);
+    m[2 * i + 1] = drop_mask2((uint32_t)(z >> 32), keep2);
+  }
+  return uint4{m[0], m[1], m[2], m[3]};
+}
+
+// ---------------------------------------------------------------------------------------
 // Host helpers
 // ---------------------------------------------------------------------------------------
 inline int launch_status() {
@@ -355,6 +420,15 @@ inline int launch_status() {
 
 // CUs of the device (256 where there is none to ask)
 int num_cus();
+
+// The threshold and the kept values' scale 1 / (1 - p), rounded as torch's dropout forms it (1 - p
+// in double, rounded to fp32, its reciprocal rounded to fp32); 0 <= p < 1.
+inline bool drop_p_ok(float p) { return p >= 0.0f && p < 1.0f; }
+inline uint32_t drop_threshold(float p) { return (uint32_t)((double)p * 65536.0); }
+inline float drop_scale_of(float p) {
+  const float pa = (float)(1.0 - (double)p);
+  return (float)(1.0 / (double)pa);
+}
 
 inline bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p % a) == 0; }
 

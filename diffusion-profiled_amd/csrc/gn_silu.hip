@@ -87,40 +87,9 @@ struct GnArgs {
 // a 16-bit number, are >= floor(p * 2^16). Four elements per 64-bit hash halve the hash's vector
 // instructions against one per pair (its multiplies are done in 32-bit halves); 16 bits
 // still give a drop rate within 2^-16 of p.
-// The decisions come as masks of bf16 pairs (0xffff: kept), to be and'ed into packed values:
+// The decisions (drop_mask8) come as masks of bf16 pairs (0xffff: kept), to be and'ed into packed values:
 // four packed 16-bit instructions per pair instead of an extract, a compare and a select per
 // element. r >= k is sat(k - r) == 0 in 16 bits, and min(., 1) - 1 turns that into the mask.
-constexpr uint64_t kDropGolden = 0x9E3779B97F4A7C15ull;
-
-// hash input of element idx (a multiple of 4)
-__device__ __forceinline__ uint64_t drop_z(uint64_t seed, int64_t idx) {
-  return seed + (uint64_t)(idx >> 2) * kDropGolden;
-}
-
-__device__ __forceinline__ uint32_t drop_mask2(uint32_t r, uint32_t keep2) {
-  uint32_t m;
-  // (as instructions of its own: the compiler turns the form into compares and selects)
-  asm("v_pk_sub_u16 %0, %1, %2 clamp\n\tv_pk_min_u16 %0, %0, %3\n\tv_pk_sub_i16 %0, %0, %3"
-      : "=&v"(m)
-      : "v"(keep2), "v"(r), "v"(0x00010001u));
-  return m;
-}
-
-// Masks of the 8 elements whose hash input starts at z0; keep2: the threshold in both halves.
-__device__ __forceinline__ uint4 drop_mask8(uint64_t z0, uint32_t keep2) {
-  uint32_t m[4];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    uint64_t z = z0 + (uint64_t)i * kDropGolden;
-    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-    z ^= z >> 31;
-    m[2 * i] = drop_mask2((uint32_t)z, keep2);
-    m[2 * i + 1] = drop_mask2((uint32_t)(z >> 32), keep2);
-  }
-  return uint4{m[0], m[1], m[2], m[3]};
-}
-
 __device__ __forceinline__ uint32_t drop_keep2(const GnArgs& p) {
   return p.drop_keep | (p.drop_keep << 16);
 }

@@ -1,0 +1,265 @@
+// Cross attention of B images' query tokens to an encoder's states of another length: what the
+// forward and the backward kernels share. Per (batch, key/value head g), with the G = H / KVH
+// query heads that read g taken together as rows = G Lq query rows (row r: head g G + r / Lq,
+// token r % Lq):
+//   S = c Q K^T over the visible keys, P = softmax(S), O = P V, lse = log sum exp S.
+// A key is visible below its batch's length and where its mask byte is not 0. Rows of keys and
+// values that are not visible are never read (they may hold NaN): zeros take their place in LDS,
+// and their scores are -inf. A row without a visible key gives O = 0 and lse = -inf.
+//
+// Products run on v_mfma_f32_32x32x16 (bf16 or fp16 operands, fp32 sums): against the 16x16x32
+// form it needs half the LDS reads per product, and one query per lane column, so a row's
+// softmax needs one exchange (with lane ^ 32). Head dims are multiples of 8 up to 128, padded
+// with zeros to DP = 32, 64 or 128 in LDS and registers only.
+#pragma once
+#include "dpa_common.hpp"
+
+namespace dpa {
+namespace xattn {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct Stride {
+  int64_t b, l, h;  // elements between batches, tokens, heads
+};
+
+struct Args {
+  const uint16_t *q, *k, *v, *dout;
+  uint16_t *out, *dq, *dk, *dv;  // out and dq dense [B][Lq][H][D]
+  float* lse;                    // [B][H][Lq], natural logarithm
+  const int32_t* klen;           // [B] or null
+  const uint8_t* kmask;          // [B][Lk] or null
+  Stride qs, ks, vs, gs, dks, dvs;
+  int64_t mask_b;
+  float* part;   // fp32 partial sums of a split axis
+  float2* stat;  // forward: their (max, sum); backward: per query row (lse in base 2 - kShift, rowsum(dO O))
+  int B, Lq, Lk, H, KVH, G, D, rows, tiles;
+  int splits, per_split;  // workgroups that share one tile's loop, and its steps each
+  uint32_t total;         // workgroups with work
+  float c2, scale;        // scale log2(e), scale
+  FastDiv by_lq;
+};
+
+// kShift: the backward forms 2^kShift P and takes the factor out of its fp32 sums at the end. In
+// bf16, whose exponents have the room, that keeps probabilities down to 2^-150, where v_exp_f32
+// alone gives 0 below 2^-126; it costs nothing. fp16 has no room for it.
+struct Bf16 {
+  static constexpr int kShift = 24;
+  static __device__ __forceinline__ v16f mfma(uint4 a, uint4 b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+  static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+};
+
+struct F16 {
+  static constexpr int kShift = 0;
+  static __device__ __forceinline__ v16f mfma(uint4 a, uint4 b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, f16x2));
+  }
+  static __device__ __forceinline__ float lo(uint32_t w) {
+    return (float)__builtin_bit_cast(f16x2, w).x;
+  }
+  static __device__ __forceinline__ float hi(uint32_t w) {
+    return (float)__builtin_bit_cast(f16x2, w).y;
+  }
+};
+
+// Fragments of v_mfma_f32_32x32x16: lane l supplies row (column of B) l & 31 and 8 k-elements of
+// slice h = l >> 5; it receives D[8 (r / 4) + 4 h + r % 4][l & 31] in register r of 16. Two
+// products chain without moving data: registers 8 s .. 8 s + 7 of a result, packed, are the B
+// operand of a product over its rows 16 s + {4 h + j, 8 + 4 h + j}, whose A operand comes from
+// transpose reads of those rows.
+__device__ __forceinline__ v16f zero16() {
+  return v16f{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+}
+
+__device__ __forceinline__ uint4 ld16(const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); }
+
+// A rows array in LDS: rows of DP elements, the 16-B granule g of row r at g ^ swz(r). 16 rows
+// read at one granule, and the 4 rows x 2 granules of a transpose read, then lie in 64 different
+// banks each.
+template <int DP>
+__device__ __forceinline__ int swz(int r) {
+  if (DP == 32) return (r >> 2) & 3;
+  if (DP == 64) return (r & 6) | ((r >> 3) & 1);
+  return ((r & 7) << 1) | ((r >> 3) & 1);
+}
+
+// 8 elements of row r at granule g
+template <int DP>
+__device__ __forceinline__ uint4 frag_row(const uint16_t* x, int r, int g) {
+  return ld16(x + r * DP + ((g ^ swz<DP>(r)) << 3));
+}
+
+// Operand of the transpose of the array: dims 32 db + (lane & 31), k over its rows r0 + 4 h +
+// {0..3, 8..11} (r0 a multiple of 16). The transpose read gives lane j of a group of 16 column j
+// of 4 rows, the group's lanes addressing 4 elements of a row each.
+template <int DP>
+__device__ __forceinline__ uint4 frag_tr(const uint16_t* x, int r0, int db, int lane) {
+  const int k = lane & 15, rr = k >> 2;
+  const int g = 4 * db + 2 * ((lane >> 4) & 1) + ((k & 3) >> 1), half = 4 * (k & 1);
+  const int r1 = r0 + 4 * (lane >> 5) + rr, r2 = r1 + 8;
+  typedef v4s __attribute__((address_space(3))) * LP;
+  const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(x + r1 * DP + ((g ^ swz<DP>(r1)) << 3) + half));
+  const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(x + r2 * DP + ((g ^ swz<DP>(r2)) << 3) + half));
+  const uint2 lo = __builtin_bit_cast(uint2, a), hi = __builtin_bit_cast(uint2, b);
+  return uint4{lo.x, lo.y, hi.x, hi.y};
+}
+
+static __device__ __attribute__((aligned(64))) uint32_t g_zero16[4];
+
+// 64 transfers of 16 B of a wave: chunks c0 .. c0 + 63 (c0 wave-uniform) of the rows array at lds,
+// from the row pointers that src(row) gives (null: zeros).
+template <int DP, class Src>
+__device__ __forceinline__ void dma_rows(uint32_t lds, int c0, int lane, int D, Src src) {
+  constexpr int NG = DP / 8;
+  const int c = c0 + lane, row = c / NG;
+  const int g = (c % NG) ^ swz<DP>(row);
+  const uint16_t* s = src(row);
+  const void* a = (s && 8 * g < D) ? static_cast<const void*>(s + 8 * g) : g_zero16;
+  dma16_lds(a, lds + (uint32_t)c0 * 16);
+}
+
+// 4 B per lane to lds + 4 * lane (lds wave-uniform).
+__device__ __forceinline__ void dma4_lds(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "m0");
+}
+
+// Which keys of a workgroup's range [k0, k1) are visible, in words of 32 or 64 keys. Mask bytes are
+// packed into LDS first: loaded in the loop over the keys, their waits would take in the tiles in
+// flight. The host splits the keys so that a range has at most kMaxRange.
+constexpr int kMaxRange = 16384;
+
+struct KeyBits {
+  const uint32_t* seen;  // LDS, null without a mask
+  int klen, k0;
+  __device__ __forceinline__ KeyBits(const Args& p, int b, int klen_, int k0_, int k1,
+                                     uint32_t* lds, int tid)
+      : seen(p.kmask ? lds : nullptr), klen(klen_), k0(k0_) {
+    if (!seen) return;
+    const uint8_t* mb = p.kmask + b * p.mask_b;
+    const int lane = tid & 63;
+    k1 = min((k1 + 63) & ~63, k0 + kMaxRange);
+    for (int k = k0 + (tid & ~63); k < k1; k += blockDim.x) {
+      const int key = k + lane;
+      const uint64_t w = __ballot(key < klen && mb[key < klen ? key : 0] != 0);
+      if (lane < 2) lds[(k - k0) / 32 + lane] = (uint32_t)(w >> (32 * lane));
+    }
+    __syncthreads();
+  }
+  // keys KT t .. KT t + KT - 1 (inside the range)
+  template <int KT>
+  __device__ __forceinline__ uint64_t word(int t) const {
+    if (seen) {
+      const uint32_t* s = seen + (t * KT - k0) / 32;
+      const uint32_t lo = __builtin_amdgcn_readfirstlane(s[0]);
+      return KT == 64 ? lo | (uint64_t)__builtin_amdgcn_readfirstlane(s[1]) << 32 : lo;
+    }
+    const int n = klen - t * KT;
+    const uint64_t all = KT == 64 ? ~0ull : 0xffffffffull;
+    return n >= KT ? all : n <= 0 ? 0 : (1ull << n) - 1;
+  }
+};
+
+// Workgroup i of the launch goes to XCD i % 8: neighbours in the order of work (the row tiles and
+// splits of one key/value head) go to one XCD, whose L2 then holds their keys.
+__device__ __forceinline__ uint32_t xcd_order(uint32_t i, uint32_t n8) { return (i & 7) * n8 + (i >> 3); }
+
+// ---- host ------------------------------------------------------------------------------
+// Shapes and sizes of a call (its pointers apart). Everything that the kernels index in 32 bits
+// (rows, keys, workgroups) is bounded here; element offsets are 64-bit.
+inline int check_shape(const DpaCrossAttention& a) {
+  if (a.dtype != DPA_DTYPE_BF16 && a.dtype != DPA_DTYPE_F16) return DPA_ERR_SHAPE;
+  if (a.batch < 0 || a.q_len < 0 || a.kv_len < 0 || a.heads <= 0 || a.kv_heads <= 0) return DPA_ERR_SIZE;
+  if (a.heads % a.kv_heads || a.head_dim <= 0 || a.head_dim > 128 || a.head_dim % 8) return DPA_ERR_SHAPE;
+  if (!(a.scale > 0.f) || !(a.scale <= 3.4e38f)) return DPA_ERR_SIZE;
+  const int64_t most = 1ll << 30;
+  const int64_t rows = (int64_t)a.heads / a.kv_heads * a.q_len;
+  if (rows >= most || a.kv_len >= most || (int64_t)a.batch * a.kv_heads >= most) return DPA_ERR_SIZE;
+  const int64_t bkv = (int64_t)a.batch * a.kv_heads;
+  if (bkv * (rows / 32 + 1) >= most || bkv * (a.kv_len / 128 + 1) >= most ||
+      bkv * rows >= most * 8 || bkv * a.kv_len >= most * 8)
+    return DPA_ERR_SIZE;
+  return DPA_OK;
+}
+
+inline bool strides_ok(const int64_t* s) { return s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0; }
+inline Stride stride_of(const int64_t* s) { return Stride{s[0], s[1], s[2]}; }
+
+inline Args make_args(const DpaCrossAttention& a) {
+  Args p{};
+  p.q = (const uint16_t*)a.q, p.k = (const uint16_t*)a.k, p.v = (const uint16_t*)a.v;
+  p.dout = (const uint16_t*)a.dout;
+  p.out = (uint16_t*)a.out, p.dq = (uint16_t*)a.dq, p.dk = (uint16_t*)a.dk, p.dv = (uint16_t*)a.dv;
+  p.lse = a.lse;
+  p.klen = a.key_lengths;
+  p.kmask = a.key_mask;
+  p.mask_b = a.mask_stride;
+  p.qs = stride_of(a.q_stride), p.ks = stride_of(a.k_stride), p.vs = stride_of(a.v_stride);
+  p.gs = stride_of(a.dout_stride), p.dks = stride_of(a.dk_stride), p.dvs = stride_of(a.dv_stride);
+  p.B = a.batch, p.Lq = a.q_len, p.Lk = a.kv_len, p.H = a.heads, p.KVH = a.kv_heads;
+  p.G = a.heads / a.kv_heads, p.D = a.head_dim, p.rows = p.G * p.Lq;
+  p.c2 = a.scale * kLog2e;
+  p.scale = a.scale;
+  p.by_lq = make_fastdiv(p.Lq > 0 ? p.Lq : 1);
+  return p;
+}
+
+// Splits the `steps` of a loop over `groups` workgroups' worth of launches so that about `want`
+// workgroups run, each of at least `least` and at most `most` steps (a multiple of `unit`).
+inline void choose_splits(Args& p, int64_t groups, int64_t steps, int64_t want, int64_t least,
+                          int64_t most, int64_t unit) {
+  int64_t n = groups > 0 ? want / groups : 1;
+  if (n > steps / least) n = steps / least;
+  if (n < 1) n = 1;
+  int64_t per = ceil_div(ceil_div(steps > 0 ? steps : 1, n), unit) * unit;
+  if (per > most) per = most;
+  p.per_split = (int)per;
+  p.splits = (int)ceil_div(steps > 0 ? steps : 1, per);
+}
+
+inline unsigned xcd_grid(uint32_t total) { return (total + 7) / 8 * 8; }
+
+// The forward's and dQ's tiles: rows of up to 32 go to the form whose waves share them
+inline bool few_rows(const Args& p) { return p.rows <= 32; }
+
+inline void plan_rows(Args& p) {
+  const bool few = few_rows(p);
+  p.tiles = few ? 1 : (int)ceil_div(p.rows, 128);
+  const int64_t groups = (int64_t)p.B * p.KVH * p.tiles, kt = few ? 32 : 64;
+  choose_splits(p, groups, ceil_div(p.Lk, kt), 2 * num_cus(), few ? 16 : 8, kMaxRange / kt, few ? 4 : 1);
+  p.total = (uint32_t)(groups * p.splits);
+}
+
+inline void plan_keys(Args& p) {
+  p.tiles = (int)ceil_div(p.Lk, 128);
+  const int64_t groups = (int64_t)p.B * p.KVH * p.tiles;
+  choose_splits(p, groups, ceil_div(p.rows, 64), 2 * num_cus(), 4, 1ll << 30, 1);
+  p.total = (uint32_t)(groups * p.splits);
+}
+
+inline int64_t part_rows_bytes(const Args& p) {
+  return p.splits > 1 ? (int64_t)p.splits * p.B * p.KVH * p.rows * p.D * 4 : 0;
+}
+inline int64_t part_keys_bytes(const Args& p) {
+  return p.splits > 1 ? (int64_t)p.splits * 2 * p.B * p.KVH * p.Lk * p.D * 4 : 0;
+}
+inline int64_t align256(int64_t n) { return (n + 255) & ~255ll; }
+
+inline int dim_pad(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
+}  // namespace xattn
+}  // namespace dpa

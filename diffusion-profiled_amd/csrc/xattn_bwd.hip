@@ -1,0 +1,493 @@
+// Cross attention, backward. With P recomputed from the saved lse and D = rowsum(dO O):
+//   dP = dO V^T, dS = P (dP - D), dQ = c dS K, dK = c dS^T Q, dV = P^T dO.
+// Two kernels, each recomputing S and dP, so that every gradient has one writer and a fixed order
+// of sums: one of query rows (dQ, and D for the other), one of keys (dK, dV, summed over the query
+// heads that share them).
+#include <type_traits>
+
+#include "xattn.hpp"
+
+namespace dpa {
+namespace xattn {
+
+// ---------------------------------------------------------------------------------------
+// dQ: the forward's tiles and layouts (S^T = K Q^T, dP^T = V dO^T: a query per lane column), then
+// dQ^T += K^T dS^T from transpose reads of the key rows.
+// ---------------------------------------------------------------------------------------
+template <class T, int DP, int WK>
+__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_dq_kernel(const Args p) {
+  constexpr int KT = WK == 1 ? 64 : 32, NKB = KT / 32;
+  constexpr int NG = DP / 8, KS = DP / 16, NDB = DP / 32;
+  constexpr float kUnshift = 1.f / (1 << T::kShift);
+  constexpr int kTile = KT * DP;
+  constexpr int kXfer = KT * NG / (WK == 1 ? 256 : 64);
+  constexpr int kBufs = 2 * (WK == 1 ? 1 : 4);
+  __shared__ __attribute__((aligned(1024))) uint16_t kv[kBufs][2][kTile];
+  __shared__ uint32_t seen[kMaxRange / 32];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, h = lane >> 5;
+  const uint32_t id = xcd_order(blockIdx.x, gridDim.x >> 3);
+  if (id >= p.total) return;
+  const int split = id % (uint32_t)p.splits;
+  const uint32_t bt = id / (uint32_t)p.splits;
+  const int tile = bt % (uint32_t)p.tiles;
+  const int bkv = bt / (uint32_t)p.tiles;
+  const int b = bkv / p.KVH, g = bkv - b * p.KVH;
+
+  int klen = p.Lk;
+  if (p.klen) {
+    const int n = p.klen[b];
+    klen = n < 0 ? 0 : n < klen ? n : klen;
+  }
+  const int nt = (klen + KT - 1) / KT;
+  const int t_lo = split * p.per_split + (WK == 1 ? 0 : wave);
+  const int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
+  const uint16_t* kb = p.k + b * p.ks.b + g * p.ks.h;
+  const uint16_t* vb = p.v + b * p.vs.b + g * p.vs.h;
+  const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
+
+  const int buf0 = WK == 1 ? 0 : wave * 2;
+  auto fetch = [&](int t, int buf, uint64_t word) __attribute__((always_inline)) {
+    const int64_t k0 = (int64_t)t * KT;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const uint16_t* base = x == 0 ? kb + k0 * p.ks.l : vb + k0 * p.vs.l;
+      const int64_t pitch = x == 0 ? p.ks.l : p.vs.l;
+      const uint32_t lds = LDS_ADDR(kv[buf0 + buf][x]);
+#pragma unroll
+      for (int r = 0; r < kXfer; ++r) {
+        const int c0 = WK == 1 ? wave * 64 + 256 * r : 64 * r;
+        dma_rows<DP>(lds, c0, lane, p.D, [&](int row) __attribute__((always_inline)) {
+          return (word >> row) & 1 ? base + row * pitch : static_cast<const uint16_t*>(nullptr);
+        });
+      }
+    }
+  };
+  uint64_t word = 0;
+  if (t_lo < t_hi) {
+    word = bits.template word<KT>(t_lo);
+    fetch(t_lo, 0, word);
+  }
+
+  const int row = (WK == 1 ? tile * 128 + wave * 32 : 0) + col;
+  const bool has_row = row < p.rows;
+  const uint32_t hg = fdiv(has_row ? row : 0, p.by_lq), tok = (has_row ? row : 0) - hg * p.Lq;
+  const int head = g * p.G + hg;
+  const int64_t orow = ((int64_t)b * p.Lq + tok) * p.H + head;
+  uint4 qf[KS], gf[KS];
+  float lse2 = __builtin_inff(), dd = 0.f;
+  {
+    const uint16_t* qr = p.q + b * p.qs.b + (int64_t)tok * p.qs.l + head * p.qs.h;
+    const uint16_t* gr = p.dout + b * p.gs.b + (int64_t)tok * p.gs.l + head * p.gs.h;
+    const uint16_t* orp = p.out + orow * p.D;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int dim = 16 * ks + 8 * h;
+      qf[ks] = gf[ks] = uint4{0u, 0u, 0u, 0u};
+      if (has_row && dim < p.D) {
+        qf[ks] = ld16(qr + dim);
+        gf[ks] = ld16(gr + dim);
+        const uint4 ov = ld16(orp + dim);
+        const uint32_t gw[4] = {gf[ks].x, gf[ks].y, gf[ks].z, gf[ks].w};
+        const uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          dd = __builtin_fmaf(T::lo(gw[i]), T::lo(ow[i]), dd);
+          dd = __builtin_fmaf(T::hi(gw[i]), T::hi(ow[i]), dd);
+        }
+      }
+    }
+    if (has_row) {
+      const float e = p.lse[((int64_t)b * p.H + head) * p.Lq + tok];
+      lse2 = e == -__builtin_inff() ? __builtin_inff() : e * kLog2e - (float)T::kShift;
+    }
+    dd += __shfl_xor(dd, 32, 64);
+    if (has_row && split == 0 && h == 0 && (WK == 1 || wave == 0))
+      p.stat[(int64_t)bkv * p.rows + row] = float2{lse2, dd};
+  }
+  wait_vmcnt<0>();
+
+  const float unscale = p.scale * kUnshift;
+  v16f dq[NDB];
+#pragma unroll
+  for (int i = 0; i < NDB; ++i) dq[i] = zero16();
+
+  for (int t = t_lo, buf = 0; t < t_hi; t += WK, buf ^= 1) {
+    uint64_t word_next = 0;
+    if (WK == 1) {
+      wait_vmcnt<0>();
+      lds_barrier();
+      if (t + WK < t_hi) {
+        word_next = bits.template word<KT>(t + WK);
+        fetch(t + WK, buf ^ 1, word_next);
+      }
+    } else if (t + WK < t_hi) {
+      word_next = bits.template word<KT>(t + WK);
+      wait_lgkmcnt0();
+      asm volatile("" ::: "memory");
+      fetch(t + WK, buf ^ 1, word_next);
+      wait_vmcnt<2 * kXfer>();
+      asm volatile("" ::: "memory");
+    } else {
+      wait_vmcnt<0>();
+      asm volatile("" ::: "memory");
+    }
+    const uint16_t *kr = kv[buf0 + buf][0], *vr = kv[buf0 + buf][1];
+#pragma unroll
+    for (int i = 0; i < NKB; ++i) {
+      const uint32_t wi = (uint32_t)(word >> (32 * i));
+      if (!wi) continue;
+      v16f s = zero16(), dp = zero16();
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        s = T::mfma(frag_row<DP>(kr, 32 * i + col, 2 * k + h), qf[k], s);
+        dp = T::mfma(frag_row<DP>(vr, 32 * i + col, 2 * k + h), gf[k], dp);
+      }
+      if (wi != 0xffffffffu) {
+        const uint32_t w = wi >> (4 * h);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!((w >> (8 * (r / 4) + r % 4)) & 1)) s[r] = -__builtin_inff();
+      }
+      uint32_t sw[8];
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, -lse2));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, -lse2));
+        sw[r / 2] = T::pack(p0 * (dp[r] - dd), p1 * (dp[r + 1] - dd));
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        const uint4 sf = {sw[4 * s2], sw[4 * s2 + 1], sw[4 * s2 + 2], sw[4 * s2 + 3]};
+#pragma unroll
+        for (int d = 0; d < NDB; ++d)
+          dq[d] = T::mfma(frag_tr<DP>(kr, 32 * i + 16 * s2, d, lane), sf, dq[d]);
+      }
+    }
+    word = word_next;
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  if constexpr (WK == 4) {
+    __syncthreads();
+    float* ox = reinterpret_cast<float*>(&kv[0][0][0]);  // [4][DP][32]
+    static_assert(sizeof(kv) >= 4 * DP * 32 * 4, "the waves' dQ fit the buffers");
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        ox[(wave * DP + 32 * d + 8 * (r / 4) + 4 * h + r % 4) * 32 + col] = dq[d][r];
+    __syncthreads();
+    constexpr int ND = DP / 8;
+    const int q8 = tid >> 5;
+    if (!has_row) return;
+#pragma unroll
+    for (int i = 0; i < ND; i += 4) {
+      float a[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        a[j] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) a[j] += ox[(w * DP + q8 * ND + i + j) * 32 + col];
+      }
+      const int dim = q8 * ND + i;
+      if (dim >= p.D) continue;
+      if (p.splits > 1)
+        *reinterpret_cast<float4*>(
+            p.part + (((int64_t)split * p.B * p.KVH + bkv) * p.rows + row) * p.D + dim) =
+            float4{a[0], a[1], a[2], a[3]};
+      else
+        *reinterpret_cast<uint2*>(p.dq + orow * p.D + dim) =
+            uint2{T::pack(a[0] * unscale, a[1] * unscale), T::pack(a[2] * unscale, a[3] * unscale)};
+    }
+    return;
+  }
+  if (!has_row) return;
+#pragma unroll
+  for (int d = 0; d < NDB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int dim = 32 * d + 8 * (r / 4) + 4 * h;
+      if (dim >= p.D) continue;
+      if (p.splits > 1)
+        *reinterpret_cast<float4*>(
+            p.part + (((int64_t)split * p.B * p.KVH + bkv) * p.rows + row) * p.D + dim) =
+            float4{dq[d][r], dq[d][r + 1], dq[d][r + 2], dq[d][r + 3]};
+      else
+        *reinterpret_cast<uint2*>(p.dq + orow * p.D + dim) =
+            uint2{T::pack(dq[d][r] * unscale, dq[d][r + 1] * unscale),
+                  T::pack(dq[d][r + 2] * unscale, dq[d][r + 3] * unscale)};
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// dK, dV: a workgroup's four waves take 32 keys each (their K and V rows as B operands and the two
+// accumulators in registers); tiles of 64 query rows, with their dO, lse and D, pass through LDS.
+// S = Q K^T and dP = dO V^T put a key in each lane column, so P and dS are the B operands of
+// dV^T += dO^T P and dK^T += Q^T dS, whose A operands are transpose reads of the same rows.
+// ---------------------------------------------------------------------------------------
+constexpr int kQT = 64;
+static __device__ __attribute__((aligned(8))) float g_pad_stat[2] = {__builtin_inff(), 0.f};
+
+template <class T, int DP>
+__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_dkdv_kernel(const Args p) {
+  constexpr int NG = DP / 8, KS = DP / 16, NDB = DP / 32;
+  constexpr float kUnshift = 1.f / (1 << T::kShift);
+  constexpr int kXfer = kQT * NG / 256;
+  __shared__ __attribute__((aligned(1024))) uint16_t qg[2][2][kQT * DP];
+  __shared__ __attribute__((aligned(256))) float2 st[2][kQT];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, h = lane >> 5;
+  const uint32_t id = xcd_order(blockIdx.x, gridDim.x >> 3);
+  if (id >= p.total) return;
+  const int split = id % (uint32_t)p.splits;
+  const uint32_t bt = id / (uint32_t)p.splits;
+  const int tile = bt % (uint32_t)p.tiles;
+  const int bkv = bt / (uint32_t)p.tiles;
+  const int b = bkv / p.KVH, g = bkv - b * p.KVH;
+
+  int klen = p.Lk;
+  if (p.klen) {
+    const int n = p.klen[b];
+    klen = n < 0 ? 0 : n < klen ? n : klen;
+  }
+  const int key = tile * 128 + wave * 32 + col;
+  const bool vis = key < klen && (!p.kmask || p.kmask[b * p.mask_b + key] != 0);
+  const bool any_vis = __any(vis);  // (wave-uniform)
+  uint4 kf[KS], vf[KS];
+  {
+    const uint16_t* kr = p.k + b * p.ks.b + key * p.ks.l + g * p.ks.h;
+    const uint16_t* vr = p.v + b * p.vs.b + key * p.vs.l + g * p.vs.h;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      kf[ks] = vf[ks] = uint4{0u, 0u, 0u, 0u};
+      if (vis && 16 * ks + 8 * h < p.D) {
+        kf[ks] = ld16(kr + 16 * ks + 8 * h);
+        vf[ks] = ld16(vr + 16 * ks + 8 * h);
+      }
+    }
+  }
+  const bool wg_vis = __syncthreads_or(vis);
+  const int nt = wg_vis ? (p.rows + kQT - 1) / kQT : 0;
+  const int t_lo = split * p.per_split;
+  const int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
+
+  const uint16_t* qb = p.q + b * p.qs.b + (int64_t)g * p.G * p.qs.h;
+  const uint16_t* gb = p.dout + b * p.gs.b + (int64_t)g * p.G * p.gs.h;
+  const float* sb = reinterpret_cast<const float*>(p.stat + (int64_t)bkv * p.rows);
+  auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
+    const int r0 = t * kQT;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const uint16_t* base = x == 0 ? qb : gb;
+      const Stride s = x == 0 ? p.qs : p.gs;
+#pragma unroll
+      for (int r = 0; r < kXfer; ++r)
+        dma_rows<DP>(LDS_ADDR(qg[buf][x]), wave * 64 + 256 * r, lane, p.D,
+                     [&](int row) __attribute__((always_inline)) {
+                       row += r0;
+                       if (row >= p.rows) return static_cast<const uint16_t*>(nullptr);
+                       const uint32_t hg = fdiv(row, p.by_lq), tok = row - hg * p.Lq;
+                       return base + (int64_t)tok * s.l + hg * s.h;
+                     });
+    }
+    if (wave < 2) {  // (lse, D) of 32 rows each
+      const int row = r0 + 32 * wave + (lane >> 1);
+      const float* a = row < p.rows ? sb + 2 * (int64_t)row + (lane & 1) : g_pad_stat + (lane & 1);
+      dma4_lds(a, (uint32_t)__builtin_amdgcn_readfirstlane(LDS_ADDR(st[buf]) + 256 * wave));
+    }
+  };
+  wait_vmcnt<0>();  // (no wait on keys and values inside the loop)
+  if (t_lo < t_hi) fetch(t_lo, 0);
+
+  v16f dk[NDB], dv[NDB];
+#pragma unroll
+  for (int i = 0; i < NDB; ++i) dk[i] = dv[i] = zero16();
+  for (int t = t_lo, buf = 0; t < t_hi; ++t, buf ^= 1) {
+    wait_vmcnt<0>();
+    lds_barrier();
+    if (t + 1 < t_hi) fetch(t + 1, buf ^ 1);
+    if (!any_vis) continue;
+    const uint16_t *qr = qg[buf][0], *gr = qg[buf][1];
+#pragma unroll
+    for (int i = 0; i < kQT / 32; ++i) {
+      v16f s = zero16(), dp = zero16();
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        s = T::mfma(frag_row<DP>(qr, 32 * i + col, 2 * k + h), kf[k], s);
+        dp = T::mfma(frag_row<DP>(gr, 32 * i + col, 2 * k + h), vf[k], dp);
+      }
+      uint32_t pw[8], sw[8];
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float4 e = *reinterpret_cast<const float4*>(&st[buf][32 * i + 8 * (r / 4) + 4 * h + r % 4]);
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, -e.x));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, -e.z));
+        pw[r / 2] = T::pack(p0, p1);
+        sw[r / 2] = T::pack(p0 * (dp[r] - e.y), p1 * (dp[r + 1] - e.w));
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        const uint4 pf = {pw[4 * s2], pw[4 * s2 + 1], pw[4 * s2 + 2], pw[4 * s2 + 3]};
+        const uint4 sf = {sw[4 * s2], sw[4 * s2 + 1], sw[4 * s2 + 2], sw[4 * s2 + 3]};
+#pragma unroll
+        for (int d = 0; d < NDB; ++d) {
+          dv[d] = T::mfma(frag_tr<DP>(gr, 32 * i + 16 * s2, d, lane), pf, dv[d]);
+          dk[d] = T::mfma(frag_tr<DP>(qr, 32 * i + 16 * s2, d, lane), sf, dk[d]);
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  if (key >= p.Lk) return;
+  const int64_t n = (int64_t)p.B * p.KVH * p.Lk, at = (int64_t)bkv * p.Lk + key;
+  const float fk = p.scale * kUnshift;
+#pragma unroll
+  for (int d = 0; d < NDB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int dim = 32 * d + 8 * (r / 4) + 4 * h;
+      if (dim >= p.D) continue;
+      float4 a = {dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
+      float4 c = {dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+      if (!vis) a = c = float4{0.f, 0.f, 0.f, 0.f};
+      if (p.splits > 1) {
+        *reinterpret_cast<float4*>(p.part + (split * 2 * n + at) * p.D + dim) = a;
+        *reinterpret_cast<float4*>(p.part + ((split * 2 + 1) * n + at) * p.D + dim) = c;
+      } else {
+        *reinterpret_cast<uint2*>(p.dk + b * p.dks.b + key * p.dks.l + g * p.dks.h + dim) =
+            uint2{T::pack(a.x * fk, a.y * fk), T::pack(a.z * fk, a.w * fk)};
+        *reinterpret_cast<uint2*>(p.dv + b * p.dvs.b + key * p.dvs.l + g * p.dvs.h + dim) =
+            uint2{T::pack(c.x * kUnshift, c.y * kUnshift), T::pack(c.z * kUnshift, c.w * kUnshift)};
+      }
+    }
+}
+
+// Sums of the splits, in order: of dQ (kDq), or of dK and dV. Thread: 8 dims of a row.
+template <class T, bool kDq>
+__global__ __launch_bounds__(256) void xattn_sum_kernel(const Args p) {
+  const int nd = p.D / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = kDq ? p.rows : p.Lk;
+  const int64_t n = (int64_t)p.B * p.KVH * per, all = kDq ? n : 2 * n;
+  if (i >= all * nd) return;
+  const int64_t at = i / nd;
+  const int d0 = (int)(i - at * nd) * 8;
+  float o[8] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    const float* src = p.part + (s * all + at) * p.D + d0;
+    const float4 a = *reinterpret_cast<const float4*>(src), c = *reinterpret_cast<const float4*>(src + 4);
+    o[0] += a.x, o[1] += a.y, o[2] += a.z, o[3] += a.w;
+    o[4] += c.x, o[5] += c.y, o[6] += c.z, o[7] += c.w;
+  }
+  const bool is_v = !kDq && at >= n;
+  const int64_t r = is_v ? at - n : at;
+  const int bkv = (int)(r / per), x = (int)(r - (int64_t)bkv * per);
+  const int b = bkv / p.KVH, g = bkv - b * p.KVH;
+  uint16_t* dst;
+  if (kDq) {
+    const uint32_t hg = fdiv(x, p.by_lq), tok = x - hg * p.Lq;
+    dst = p.dq + (((int64_t)b * p.Lq + tok) * p.H + g * p.G + hg) * p.D;
+  } else if (is_v) {
+    dst = p.dv + b * p.dvs.b + x * p.dvs.l + g * p.dvs.h;
+  } else {
+    dst = p.dk + b * p.dks.b + x * p.dks.l + g * p.dks.h;
+  }
+  const float f = (is_v ? 1.f : p.scale) / (1 << T::kShift);
+  *reinterpret_cast<uint4*>(dst + d0) = uint4{T::pack(o[0] * f, o[1] * f), T::pack(o[2] * f, o[3] * f),
+                                              T::pack(o[4] * f, o[5] * f), T::pack(o[6] * f, o[7] * f)};
+}
+
+}  // namespace xattn
+}  // namespace dpa
+
+using namespace dpa;
+using namespace dpa::xattn;
+
+// (lse, D) of every row, then room for one kernel's partial sums at a time
+static int64_t stat_bytes(const Args& p) { return align256((int64_t)p.B * p.KVH * p.rows * 8); }
+
+static int64_t bwd_workspace(const Args& rows, const Args& keys) {
+  const int64_t a = part_rows_bytes(rows), b = part_keys_bytes(keys);
+  return stat_bytes(rows) + (a > b ? a : b);
+}
+
+extern "C" int64_t dpa_cross_attention_bwd_workspace_bytes(const DpaCrossAttention* a) {
+  if (!a || check_shape(*a) != DPA_OK) return 0;
+  Args r = make_args(*a), k = r;
+  plan_rows(r);
+  plan_keys(k);
+  return bwd_workspace(r, k);
+}
+
+template <class T, int DP>
+static int launch_bwd(const Args& r, const Args& k, hipStream_t s) {
+  if (r.total > 0) {
+    if (few_rows(r))
+      xattn_dq_kernel<T, DP, 4><<<xcd_grid(r.total), 256, 0, s>>>(r);
+    else
+      xattn_dq_kernel<T, DP, 1><<<xcd_grid(r.total), 256, 0, s>>>(r);
+    int st = launch_status();
+    if (st != DPA_OK) return st;
+    if (r.splits > 1) {
+      const int64_t n = (int64_t)r.B * r.KVH * r.rows * (r.D / 8);
+      xattn_sum_kernel<T, true><<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(r);
+      st = launch_status();
+      if (st != DPA_OK) return st;
+    }
+  }
+  if (k.total > 0) {
+    xattn_dkdv_kernel<T, DP><<<xcd_grid(k.total), 256, 0, s>>>(k);
+    int st = launch_status();
+    if (st != DPA_OK || k.splits <= 1) return st;
+    const int64_t n = (int64_t)k.B * k.KVH * k.Lk * 2 * (k.D / 8);
+    xattn_sum_kernel<T, false><<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(k);
+    return launch_status();
+  }
+  return DPA_OK;
+}
+
+template <class T>
+static int run_bwd(const Args& r, const Args& k, hipStream_t s) {
+  switch (dim_pad(r.D)) {
+    case 32: return launch_bwd<T, 32>(r, k, s);
+    case 64: return launch_bwd<T, 64>(r, k, s);
+    default: return launch_bwd<T, 128>(r, k, s);
+  }
+}
+
+extern "C" int dpa_cross_attention_bwd(const DpaCrossAttention* a, void* workspace,
+                                       int64_t workspace_bytes, void* stream) {
+  if (!a) return DPA_ERR_NULL;
+  const int st = check_shape(*a);
+  if (st != DPA_OK) return st;
+  if (a->batch == 0) return DPA_OK;
+  if (a->q_len > 0 && (!a->q || !a->out || !a->lse || !a->dout || !a->dq)) return DPA_ERR_NULL;
+  if (a->kv_len > 0 && (!a->k || !a->v)) return DPA_ERR_NULL;
+  if (!a->dk != !a->dv) return DPA_ERR_NULL;
+  if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 16) ||
+      !aligned(a->dout, 16) || !aligned(a->dq, 16) || !aligned(a->dk, 16) || !aligned(a->dv, 16) ||
+      !aligned(a->lse, 4) || !aligned(a->key_lengths, 4) || !strides_ok(a->q_stride) ||
+      !strides_ok(a->k_stride) || !strides_ok(a->v_stride) || !strides_ok(a->dout_stride) ||
+      !strides_ok(a->dk_stride) || !strides_ok(a->dv_stride))
+    return DPA_ERR_ALIGN;
+  Args r = make_args(*a), k = r;
+  plan_rows(r);
+  plan_keys(k);
+  const int64_t need = bwd_workspace(r, k);
+  if (need) {
+    if (!workspace || workspace_bytes < need) return DPA_ERR_WORKSPACE;
+    if (!aligned(workspace, 16)) return DPA_ERR_ALIGN;
+    r.stat = k.stat = (float2*)workspace;
+    r.part = k.part = (float*)((uint8_t*)workspace + stat_bytes(r));
+  }
+  if (a->q_len == 0) r.total = 0;
+  if (!a->dk) k.total = 0;
+  hipStream_t s = (hipStream_t)stream;
+  return a->dtype == DPA_DTYPE_BF16 ? run_bwd<Bf16>(r, k, s) : run_bwd<F16>(r, k, s);
+}

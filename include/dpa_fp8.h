@@ -322,6 +322,7 @@ int dpa_gn_silu_film_bwd_bf16(const void* x, const void* dout, const float* gamm
 /* Element type of x (and dx) for the *_ex GroupNorm entries. */
 #define DPA_DTYPE_BF16 0
 #define DPA_DTYPE_F32 1
+#define DPA_DTYPE_F16 2         /* cross attention, embedding and dropout only */
 
 /* GroupNorm + FiLM + SiLU forward / backward with x (and dx) in bf16 or fp32, the other
  * arguments as in dpa_gn_silu_fwd_ws_bf16 / dpa_gn_silu_bwd_bf16 (one FiLM form at a time:
@@ -779,6 +780,70 @@ int64_t dpa_conv3x3_thin_wgrad_workspace_bytes(int N, int H, int W, int Cin, int
 int dpa_conv3x3_thin_wgrad(const void* x, int x_dtype, const void* dy, float* dw, int N, int H,
                            int W, int Cin, int Cout, void* workspace, int64_t workspace_bytes,
                            void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Conditioning of the U-Net on text: token embedding, cross attention to the encoder's states,
+ * dropout. No counterpart in the reference, whose U-Net is unconditional.
+ *
+ * Cross attention (csrc/xattn_fwd.hip, csrc/xattn_bwd.hip). Query head h of a batch reads
+ * key/value head h / (heads / kv_heads); head_dim a multiple of 8 up to 128; operands bf16 or
+ * fp16 (dtype DPA_DTYPE_BF16 / DPA_DTYPE_F16), sums and softmax in fp32. A key takes part when
+ * its index is below key_lengths[b] (NULL: all of kv_len; values are clamped to [0, kv_len]) and
+ * key_mask[b * mask_stride + key] is not 0 (NULL: all). Keys and values that take no part are
+ * not read. Without any: out = 0, lse = -inf, no gradient from that query.
+ *   fwd: out = softmax(scale q k^T) v, lse = log sum exp(scale q k^T)  (natural logarithm)
+ *   bwd: dq, dk, dv (dk and dv summed over the query heads that share them; zeros for keys that
+ *        take no part) from dout, out and lse; deterministic. dk and dv both NULL: not formed.
+ * q, out, dout, dq: [batch][q_len][heads][head_dim]; k, v, dk, dv: [batch][kv_len][kv_heads]
+ * [head_dim]; lse: [batch][heads][q_len]. out and dq are dense; the others have element strides
+ * {batch, token, head} (multiples of 8; 0 repeats k and v over the batch) and dense head_dim;
+ * pointers 16-B aligned. scale > 0. Lengths may be 0. The descriptor is host memory, read at
+ * the call.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct DpaCrossAttention {
+  const void *q, *k, *v;
+  void* out;               /* bwd: the forward's, read */
+  float* lse;              /* bwd: the forward's, read */
+  const int32_t* key_lengths;
+  const uint8_t* key_mask;
+  const void* dout;        /* bwd only, as dq, dk, dv */
+  void *dq, *dk, *dv;
+  int64_t mask_stride;
+  int64_t q_stride[3], k_stride[3], v_stride[3], dout_stride[3], dk_stride[3], dv_stride[3];
+  int32_t dtype, batch, q_len, kv_len, heads, kv_heads, head_dim;
+  float scale;
+} DpaCrossAttention;
+
+int64_t dpa_cross_attention_fwd_workspace_bytes(const DpaCrossAttention* a);
+int dpa_cross_attention_fwd(const DpaCrossAttention* a, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+int64_t dpa_cross_attention_bwd_workspace_bytes(const DpaCrossAttention* a);
+int dpa_cross_attention_bwd(const DpaCrossAttention* a, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+
+/* Dropout (csrc/dropout.hip): y = residual + keep x / (1 - p) over n elements of one dtype (bf16,
+ * fp16 or fp32; residual NULL for none), rounded once; element idx (its place in memory) is kept
+ * by the counter hash of dpa_gn_silu_fwd_ex on seed (a uint64 in device memory). 0 <= p < 1. A
+ * dropped element counts as 0 whatever it holds. The backward is the call on dy without a
+ * residual (whose gradient is dy). y may alias x or residual. */
+int dpa_dropout(const void* x, const void* residual, void* y, int dtype, int64_t n,
+                const void* seed, float p, void* stream);
+
+/* Token embedding (csrc/embed.hip): out[i] = scale weight[tokens[i]] for n tokens (token_bytes 4
+ * or 8: int32 or int64), weight [V][C] and out [n][C] dense, each bf16, fp16 or fp32; with
+ * drop_seed (a uint64 in device memory, NULL for none) followed by dropout of the element index
+ * i C + c. A token outside [0, V) gives a row of NaN.
+ * bwd: dweight [V][C], all of it written: scale times the sum, in order of i and in fp32, of
+ * (dropped) dout[i] over the tokens of a row; zeros for rows without tokens and for padding_idx
+ * (-1: none). Tokens outside [0, V) add nothing. Deterministic. dweight 16-B aligned. */
+int dpa_embedding_fwd(const void* tokens, int token_bytes, const void* weight, int weight_dtype,
+                      void* out, int out_dtype, int64_t n, int64_t V, int C, float scale,
+                      const void* drop_seed, float drop_p, void* stream);
+int64_t dpa_embedding_bwd_workspace_bytes(int64_t n, int C);
+int dpa_embedding_bwd(const void* dout, int dout_dtype, const void* tokens, int token_bytes,
+                      void* dweight, int weight_dtype, int64_t n, int64_t V, int C, float scale,
+                      int64_t padding_idx, const void* drop_seed, float drop_p, void* workspace,
+                      int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
