@@ -16,8 +16,7 @@ from __future__ import annotations
 
 import math
 import struct
-from functools import lru_cache
-from typing import Any
+from typing import Any, NamedTuple
 
 import torch
 from torch.amp.autocast_mode import custom_bwd, custom_fwd
@@ -32,6 +31,7 @@ _MAX_HEAD_DIM = 128
 # DpaCrossAttention of include/dpa_fp8.h: 11 pointers, the mask's stride, 6 x 3 strides, 7 sizes,
 # the scale
 _DESC = struct.Struct("=11Qq18q7if")
+_DESC_HEAD, _DESC_TAIL = struct.Struct("=11Q"), struct.Struct("=q18q7if")
 
 
 def _ptr(t: torch.Tensor | None) -> int:
@@ -39,26 +39,28 @@ def _ptr(t: torch.Tensor | None) -> int:
 
 
 def _on_one_gpu(*tensors: torch.Tensor | None) -> None:
-    first = tensors[0]
+    first = tensors[0].get_device()
     for t in tensors:
-        if t is not None and not (t.is_cuda and t.device == first.device):
-            raise ValueError(f"expected GPU tensors on one device, got {t.device} and {first.device}")
+        if t is not None and (first < 0 or t.get_device() != first):
+            raise ValueError(f"expected GPU tensors on one device, got {t.device} and {tensors[0].device}")
 
 
 # ---- cross attention ---------------------------------------------------------------------
 def _strides(t: torch.Tensor) -> tuple[int, int, int]:
-    """Batch, token and head strides; 0 where there is one element only."""
-    s, n = t.stride(), t.shape
-    return (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+    """Element strides of batch, token and head; those of dimensions of one element are 0."""
+    return tuple(0 if n <= 1 else s for n, s in zip(t.shape[:3], t.stride()[:3]))
+
+
+def _in_place(t: torch.Tensor) -> bool:
+    """Whether the kernels read t where it is (its 16-B alignment apart): dense head_dim, strides of
+    whole 16 B."""
+    return t.stride(3) == 1 and all(s % 8 == 0 for s in _strides(t))
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t as the kernels read it: dense head_dim, strides of whole 16 B, 16-B aligned; else a
-    dense copy."""
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0:
-        a, b, c = _strides(t)
-        if a % 8 == 0 and b % 8 == 0 and c % 8 == 0:
-            return t
+    """t as the kernels read it, else a dense copy."""
+    if _in_place(t) and t.data_ptr() % 16 == 0:
+        return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
 
 
@@ -104,7 +106,6 @@ def _check_masks(q, k, key_lengths, key_mask):
 def _scale_of(scale: float | None, head_dim: int) -> float:
     if scale is None:
         return 1.0 / math.sqrt(head_dim)
-    scale = float(scale)
     if not 0.0 < scale < 3.4e38:
         raise ValueError(f"cross attention: scale {scale} is not positive and finite")
     return scale
@@ -113,21 +114,68 @@ def _scale_of(scale: float | None, head_dim: int) -> float:
 _NONE3 = (0, 0, 0)
 
 
-def _describe(q, k, v, out, lse, lengths, mask, scale, dout=None, dq=None, dk=None, dv=None) -> bytes:
+class _Plan(NamedTuple):
+    """What a call's shapes, strides, dtypes and scale settle, once they have been checked."""
+    tail: bytes         # DpaCrossAttention behind its pointers
+    out_shape: tuple
+    lse_shape: tuple
+    fwd_bytes: int      # workspaces
+    bwd_bytes: int
+
+
+# An eager call on small operands costs more in checks than in its launch, so what they come to is
+# kept per layout of the operands: 4 x 1 queries over 77 keys 15.7 -> 9.6 us, their backward 28.5 ->
+# 18.0 us on the host. Addresses and values are looked at in every call.
+_PLANS: dict[tuple, _Plan] = {}
+_MOST_PLANS = 4096
+
+
+def _layout(t: torch.Tensor | None):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _attention_key(q, k, v, lengths, mask, scale, dout=None, dk=None, dv=None) -> tuple:
+    return (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype,
+            q.get_device(), k.get_device(), v.get_device(), scale, _layout(lengths), _layout(mask),
+            _layout(dout), _layout(dk), _layout(dv))
+
+
+def _attention_operands(q, k, v, lengths, mask, scale, dout=None, dk=None, dv=None):
+    """(plan, q, k, v, lengths, mask, dout) as the kernels read them, checked."""
+    if scale is not None:
+        scale = float(scale)
+    key = _attention_key(q, k, v, lengths, mask, scale, dout, dk, dv)
+    plan = _PLANS.get(key)
+    if plan is not None and not ((q.data_ptr() | k.data_ptr() | v.data_ptr()
+                                  | (0 if dout is None else dout.data_ptr())) & 15):
+        return plan, q, k, v, lengths, mask, dout
+    given = (q, k, v, lengths, mask, dout)
+    _check_qkv(q, k, v)
     b, lq, h, d = q.shape
-    return _DESC.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _ptr(lengths),
-        _ptr(mask), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv),
-        0 if mask is None else mask.stride(0), *_strides(q), *_strides(k), *_strides(v),
-        *(_NONE3 if dout is None else _strides(dout)), *(_NONE3 if dk is None else _strides(dk)),
-        *(_NONE3 if dv is None else _strides(dv)),
-        _DT[q.dtype], b, lq, k.shape[1], h, k.shape[2], d, scale)
-
-
-@lru_cache(maxsize=4096)
-def _attention_workspace(entry: str, b: int, lq: int, lk: int, h: int, g: int, d: int) -> int:
-    desc = _DESC.pack(*[0] * 30, 0, b, lq, lk, h, g, d, 1.0)
-    return _lib.query(entry, desc)
+    lk, g = k.shape[1], k.shape[2]
+    if dout is not None:
+        if dout.shape != q.shape or dout.dtype != q.dtype:
+            raise ValueError(f"cross attention: dout {dout.dtype} {tuple(dout.shape)} is not q's "
+                             f"{q.dtype} {tuple(q.shape)}")
+        _on_one_gpu(q, dout)
+        dout = _rows(dout)
+    lengths, mask = _check_masks(q, k, lengths, mask)
+    number = _scale_of(scale, d)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    sizes = (_DT[q.dtype], b, lq, lk, h, g, d)
+    strides = [_NONE3 if t is None else _strides(t) for t in (q, k, v, dout, dk, dv)]
+    tail = _DESC_TAIL.pack(0 if mask is None else mask.stride(0), *(s for t in strides for s in t),
+                           *sizes, number)
+    desc = _DESC_HEAD.pack(*[0] * 11) + tail
+    plan = _Plan(tail, (b, lq, h, d), (b, h, lq),
+                 _lib.query("dpa_cross_attention_fwd_workspace_bytes", desc),
+                 _lib.query("dpa_cross_attention_bwd_workspace_bytes", desc))
+    now = (q, k, v, lengths, mask, dout)
+    if all(a is b for a, b in zip(now, given)):     # nothing was copied: it holds for the next call
+        if len(_PLANS) >= _MOST_PLANS:
+            _PLANS.clear()
+        _PLANS[key] = plan
+    return plan, *now
 
 
 def _workspace(nbytes: int, device) -> torch.Tensor | None:
@@ -147,44 +195,39 @@ def cross_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     [B], clamped to [0, Lk]) and where key_mask ([B, Lk], bool or uint8) is true; keys that do not
     are never read. A query without any gets 0, and -inf as its log sum exp. scale: 1 / sqrt(D) by
     default, positive. Returns (out [B, Lq, H, D], lse [B, H, Lq] fp32)."""
-    _check_qkv(q, k, v)
-    key_lengths, key_mask = _check_masks(q, k, key_lengths, key_mask)
-    scale = _scale_of(scale, q.shape[3])
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    b, lq, h, d = q.shape
-    out = torch.empty((b, lq, h, d), device=q.device, dtype=q.dtype)
-    lse = torch.empty((b, h, lq), device=q.device, dtype=torch.float32)
+    plan, q, k, v, lengths, mask, _ = _attention_operands(q, k, v, key_lengths, key_mask, scale)
+    out = q.new_empty(plan.out_shape)
+    lse = q.new_empty(plan.lse_shape, dtype=torch.float32)
     if out.numel() == 0:
         return out, lse
-    desc = _describe(q, k, v, out, lse, key_lengths, key_mask, scale)
-    n = _attention_workspace("dpa_cross_attention_fwd_workspace_bytes", b, lq, k.shape[1], h, k.shape[2], d)
-    ws = _workspace(n, q.device)
-    _lib.call("dpa_cross_attention_fwd", desc, _ptr(ws), n, _lib.current_stream(q))
+    ws = _workspace(plan.fwd_bytes, q.device) if plan.fwd_bytes else None
+    desc = _DESC_HEAD.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                           _ptr(lengths), _ptr(mask), 0, 0, 0, 0) + plan.tail
+    _lib.call("dpa_cross_attention_fwd", desc, _ptr(ws), plan.fwd_bytes, _lib.current_stream(q))
     return out, lse
 
 
 def _attention_bwd(dout, q, k, v, out, lse, key_lengths, key_mask, scale, dk, dv):
-    _check_qkv(q, k, v)
-    b, lq, h, d = q.shape
-    if dout.shape != q.shape or out.shape != q.shape or dout.dtype != q.dtype or out.dtype != q.dtype:
-        raise ValueError(f"cross attention: dout {dout.dtype} {tuple(dout.shape)} and out {out.dtype} "
-                         f"{tuple(out.shape)} are not q's {q.dtype} {tuple(q.shape)}")
-    if lse.shape != (b, h, lq) or lse.dtype != torch.float32:
-        raise ValueError(f"cross attention: lse is fp32 [{b}, {h}, {lq}], got {lse.dtype} {tuple(lse.shape)}")
-    _on_one_gpu(q, dout, out, lse)
-    key_lengths, key_mask = _check_masks(q, k, key_lengths, key_mask)
-    scale = _scale_of(scale, d)
-    q, k, v, dout = _rows(q), _rows(k), _rows(v), _rows(dout)
+    plan, q, k, v, lengths, mask, dout = _attention_operands(q, k, v, key_lengths, key_mask, scale,
+                                                             dout, dk, dv)
+    device = q.get_device()
+    if out.shape != plan.out_shape or out.dtype != q.dtype or out.get_device() != device:
+        raise ValueError(f"cross attention: out {out.dtype} {tuple(out.shape)} on {out.device} is not "
+                         f"q's {q.dtype} {tuple(q.shape)} on {q.device}")
+    if lse.shape != plan.lse_shape or lse.dtype != torch.float32 or lse.get_device() != device:
+        raise ValueError(f"cross attention: lse is fp32 {list(plan.lse_shape)} on {q.device}, got "
+                         f"{lse.dtype} {tuple(lse.shape)} on {lse.device}")
     out, lse = out.contiguous(), lse.contiguous()
     if out.data_ptr() % 16:
         out = out.clone()
-    dq = torch.empty((b, lq, h, d), device=q.device, dtype=q.dtype)
-    if b == 0 or (dq.numel() == 0 and (dk is None or dk.numel() == 0)):
+    dq = q.new_empty(plan.out_shape)
+    if plan.out_shape[0] == 0 or (dq.numel() == 0 and (dk is None or dk.numel() == 0)):
         return dq
-    desc = _describe(q, k, v, out, lse, key_lengths, key_mask, scale, dout, dq, dk, dv)
-    n = _attention_workspace("dpa_cross_attention_bwd_workspace_bytes", b, lq, k.shape[1], h, k.shape[2], d)
-    ws = _workspace(n, q.device)
-    _lib.call("dpa_cross_attention_bwd", desc, _ptr(ws), n, _lib.current_stream(q))
+    ws = _workspace(plan.bwd_bytes, q.device)
+    desc = _DESC_HEAD.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                           _ptr(lengths), _ptr(mask), dout.data_ptr(), dq.data_ptr(), _ptr(dk),
+                           _ptr(dv)) + plan.tail
+    _lib.call("dpa_cross_attention_bwd", desc, _ptr(ws), plan.bwd_bytes, _lib.current_stream(q))
     return dq
 
 
@@ -196,8 +239,7 @@ def cross_attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v:
     """(dq, dk, dv) of ``cross_attention_fwd`` from its outputs and the gradient of out; dk and dv
     [B, Lk, G, D] summed over the query heads of a key head, zero for keys that take no part.
     Deterministic."""
-    _check_qkv(q, k, v)
-    dk, dv = (torch.empty(k.shape, device=k.device, dtype=k.dtype) for _ in range(2))
+    dk, dv = k.new_empty(k.shape), k.new_empty(k.shape)
     return _attention_bwd(dout, q, k, v, out, lse, key_lengths, key_mask, scale, dk, dv), dk, dv
 
 
@@ -390,7 +432,7 @@ def embedding_fwd(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 
     p_drop = _check_embedding(tokens, weight.dtype, out_dtype, p_drop, seed, weight)
     v, c = weight.shape
     weight, tokens = weight.contiguous(), tokens.contiguous()
-    out = torch.empty((*tokens.shape, c), device=weight.device, dtype=out_dtype)
+    out = weight.new_empty((*tokens.shape, c), dtype=out_dtype)
     _lib.call("dpa_embedding_fwd", tokens.data_ptr(), tokens.element_size(), weight.data_ptr(),
               _DT[weight.dtype], out.data_ptr(), _DT[out_dtype], tokens.numel(), v, c, float(scale),
               seed.data_ptr() if p_drop > 0.0 else None, p_drop, _lib.current_stream(weight))
@@ -414,7 +456,7 @@ def embedding_bwd(dout: torch.Tensor, tokens: torch.Tensor, num_embeddings: int,
         raise ValueError(f"embedding: padding_idx {padding_idx} is outside the {num_embeddings} rows")
     c, n = dout.shape[-1], tokens.numel()
     dout, tokens = dout.contiguous(), tokens.contiguous()
-    dw = torch.empty((num_embeddings, c), device=dout.device, dtype=dtype)
+    dw = dout.new_empty((num_embeddings, c), dtype=dtype)
     nbytes = _lib.query("dpa_embedding_bwd_workspace_bytes", n, c)
     ws = _workspace(nbytes, dout.device)
     _lib.call("dpa_embedding_bwd", dout.data_ptr(), _DT[dout.dtype], tokens.data_ptr(),
