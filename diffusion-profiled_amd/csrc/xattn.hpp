@@ -38,12 +38,15 @@ struct Args {
   Stride qs, ks, vs, gs, dks, dvs;
   int64_t mask_b;
   float* part;   // fp32 partial sums of a split axis
-  float2* stat;  // forward: their (max, sum); backward: per query row (lse in base 2 - kShift, rowsum(dO O))
+  float2* stat;  // forward: their (max, sum)
+  float* row_stat;  // backward: kShift - lse in base 2 of every query row, then their -rowsum(dO O)
   int B, Lq, Lk, H, KVH, G, D, rows, tiles;
   int splits, per_split;  // workgroups that share one tile's loop, and its steps each
   uint32_t total;         // workgroups with work
+  uint32_t grid;          // workgroups launched
+  uint32_t unit;          // neighbours among them that one XCD takes
   float c2, scale;        // scale log2(e), scale
-  FastDiv by_lq;
+  FastDiv by_lq, by_unit;
 };
 
 // kShift: the backward forms 2^kShift P and takes the factor out of its fp32 sums at the end. In
@@ -174,9 +177,100 @@ struct KeyBits {
   }
 };
 
-// Workgroup i of the launch goes to XCD i % 8: neighbours in the order of work (the row tiles and
-// splits of one key/value head) go to one XCD, whose L2 then holds their keys.
-__device__ __forceinline__ uint32_t xcd_order(uint32_t i, uint32_t n8) { return (i & 7) * n8 + (i >> 3); }
+// Keys of batch b below its length
+__device__ __forceinline__ int keys_of(const Args& p, int b) {
+  if (!p.klen) return p.Lk;
+  const int n = p.klen[b];
+  return n < 0 ? 0 : n < p.Lk ? n : p.Lk;
+}
+
+// A wave's kXfer transfers each of the tiles of keys and values from key k0 on into kl and vl,
+// chunks c0, c0 + kStep, ...; keys whose bit in word is 0 come as zeros.
+template <int DP, int kXfer, int kStep>
+__device__ __forceinline__ void fetch_keys(const Args& p, const uint16_t* kb, const uint16_t* vb, int64_t k0,
+                                           uint64_t word, const uint16_t* kl, const uint16_t* vl, int c0,
+                                           int lane) {
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const uint16_t* base = x == 0 ? kb + k0 * p.ks.l : vb + k0 * p.vs.l;
+    const int64_t pitch = x == 0 ? p.ks.l : p.vs.l;
+    const uint32_t lds = LDS_ADDR(x == 0 ? kl : vl);
+#pragma unroll
+    for (int r = 0; r < kXfer; ++r)
+      dma_rows<DP>(lds, c0 + kStep * r, lane, p.D, [&](int row) __attribute__((always_inline)) {
+        return (word >> row) & 1 ? base + row * pitch : static_cast<const uint16_t*>(nullptr);
+      });
+  }
+}
+
+// The B operands of a row of queries (or of their gradient)
+template <int KS>
+__device__ __forceinline__ void load_row(uint4 (&f)[KS], const uint16_t* src, bool on, int h, int D) {
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    f[ks] = uint4{0u, 0u, 0u, 0u};
+    if (on && 16 * ks + 8 * h < D) f[ks] = ld16(src + 16 * ks + 8 * h);
+  }
+}
+
+// Workgroup i of the launch goes to XCD i % 8. Units of neighbours in the order of work (the row
+// tiles and splits of one key/value head) go to one XCD, whose L2 then holds their keys; the units
+// are dealt out to the XCDs in turn, so that ragged lengths even out.
+__device__ __forceinline__ uint32_t work_item(const Args& p) {
+  const uint32_t j = blockIdx.x >> 3, u = fdiv(j, p.by_unit);
+  return (u * 8 + (blockIdx.x & 7)) * p.unit + (j - u * p.unit);
+}
+
+// A value's maximum or sum over lanes l and l ^ 32
+__device__ __forceinline__ float max_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// f x as row l & 31 of a dense array's rows at dst (dims in the registers of the accumulators, on:
+// whether the lane's row exists). Lanes l and l ^ 32 hold 4 dims of every 8; they trade halves of
+// neighbouring eights, so that each stores 16 B.
+template <class T, int NDB>
+__device__ __forceinline__ void store_row(uint16_t* dst, bool on, const v16f (&x)[NDB], float f, int h, int D) {
+#pragma unroll
+  for (int d = 0; d < NDB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 8) {
+      const auto a = __builtin_amdgcn_permlane32_swap(T::pack(x[d][r] * f, x[d][r + 1] * f),
+                                                      T::pack(x[d][r + 4] * f, x[d][r + 5] * f), false, false);
+      const auto b = __builtin_amdgcn_permlane32_swap(T::pack(x[d][r + 2] * f, x[d][r + 3] * f),
+                                                      T::pack(x[d][r + 6] * f, x[d][r + 7] * f), false, false);
+      const int dim = 32 * d + 2 * r + 8 * h;
+      if (on && dim < D) *reinterpret_cast<uint4*>(dst + dim) = uint4{a[0], b[0], a[1], b[1]};
+    }
+}
+// the same rows in fp32
+template <int NDB>
+__device__ __forceinline__ void store_part(float* dst, const v16f (&x)[NDB], int h, int D) {
+#pragma unroll
+  for (int d = 0; d < NDB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int dim = 32 * d + 2 * r + 4 * h;
+      if (dim < D)
+        *reinterpret_cast<float4*>(dst + dim) = float4{x[d][r], x[d][r + 1], x[d][r + 2], x[d][r + 3]};
+    }
+}
+
+// The accumulator of a product whose 32 rows start from b[0 .. 31] (LDS, 16-B aligned)
+__device__ __forceinline__ v16f start_from(const float* b, int h) {
+  v16f s;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const float4 v = *reinterpret_cast<const float4*>(b + 8 * x + 4 * h);
+    s[4 * x] = v.x, s[4 * x + 1] = v.y, s[4 * x + 2] = v.z, s[4 * x + 3] = v.w;
+  }
+  return s;
+}
 
 // ---- host ------------------------------------------------------------------------------
 // Shapes and sizes of a call (its pointers apart). Everything that the kernels index in 32 bits
@@ -231,7 +325,19 @@ inline void choose_splits(Args& p, int64_t groups, int64_t steps, int64_t want, 
   p.splits = (int)ceil_div(steps > 0 ? steps : 1, per);
 }
 
-inline unsigned xcd_grid(uint32_t total) { return (total + 7) / 8 * 8; }
+// Sets p.unit for `total` workgroups, `per_head` of them to a key/value head, and p.grid. A
+// unit is a head's work, or a batch's where a head's rows are no whole cache lines (two XCDs would
+// fetch each line); with few units, an eighth of all.
+inline void set_grid(Args& p, int64_t total, int64_t per_head) {
+  int64_t unit = per_head * (p.D % 64 ? p.KVH : 1);
+  const int64_t n = unit ? total / unit : 0;
+  if (n % 8 && n < 32) unit = ceil_div(total, 8);
+  if (unit < 1) unit = 1;
+  p.total = (uint32_t)total;
+  p.unit = (uint32_t)unit;
+  p.by_unit = make_fastdiv(p.unit);
+  p.grid = (uint32_t)(ceil_div(total, 8 * unit) * 8 * unit);
+}
 
 // The forward's and dQ's tiles: rows of up to 32 go to the form whose waves share them
 inline bool few_rows(const Args& p) { return p.rows <= 32; }
@@ -241,14 +347,14 @@ inline void plan_rows(Args& p) {
   p.tiles = few ? 1 : (int)ceil_div(p.rows, 128);
   const int64_t groups = (int64_t)p.B * p.KVH * p.tiles, kt = few ? 32 : 64;
   choose_splits(p, groups, ceil_div(p.Lk, kt), 2 * num_cus(), few ? 16 : 8, kMaxRange / kt, few ? 4 : 1);
-  p.total = (uint32_t)(groups * p.splits);
+  set_grid(p, groups * p.splits, (int64_t)p.tiles * p.splits);
 }
 
 inline void plan_keys(Args& p) {
   p.tiles = (int)ceil_div(p.Lk, 128);
   const int64_t groups = (int64_t)p.B * p.KVH * p.tiles;
   choose_splits(p, groups, ceil_div(p.rows, 64), 2 * num_cus(), 4, 1ll << 30, 1);
-  p.total = (uint32_t)(groups * p.splits);
+  set_grid(p, groups * p.splits, (int64_t)p.tiles * p.splits);
 }
 
 inline int64_t part_rows_bytes(const Args& p) {

@@ -3,8 +3,6 @@
 // Two kernels, each recomputing S and dP, so that every gradient has one writer and a fixed order
 // of sums: one of query rows (dQ, and D for the other), one of keys (dK, dV, summed over the query
 // heads that share them).
-#include <type_traits>
-
 #include "xattn.hpp"
 
 namespace dpa {
@@ -12,23 +10,26 @@ namespace xattn {
 
 // ---------------------------------------------------------------------------------------
 // dQ: the forward's tiles and layouts (S^T = K Q^T, dP^T = V dO^T: a query per lane column), then
-// dQ^T += K^T dS^T from transpose reads of the key rows.
+// dQ^T += K^T dS^T from transpose reads of the key rows. The product for dP^T starts from -D, as the
+// one for S^T from the keys' bias, so that dS = P (dP - D) is one multiplication.
+// WK = 1: four waves of 32 query rows each share tiles of 64 keys. WK = 4, for up to 32 rows: the
+// four waves share them and take every fourth tile of 32 keys each.
 // ---------------------------------------------------------------------------------------
 template <class T, int DP, int WK>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_dq_kernel(const Args p) {
+__global__ __launch_bounds__(256, WK == 4 ? 1 : DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_dq_kernel(const Args p) {
   constexpr int KT = WK == 1 ? 64 : 32, NKB = KT / 32;
   constexpr int NG = DP / 8, KS = DP / 16, NDB = DP / 32;
   constexpr float kUnshift = 1.f / (1 << T::kShift);
-  constexpr int kTile = KT * DP;
-  constexpr int kXfer = KT * NG / (WK == 1 ? 256 : 64);
-  constexpr int kBufs = 2 * (WK == 1 ? 1 : 4);
-  __shared__ __attribute__((aligned(1024))) uint16_t kv[kBufs][2][kTile];
+  constexpr int kStep = WK == 1 ? 256 : 64;
+  constexpr int kXfer = KT * NG / kStep;
+  __shared__ __attribute__((aligned(1024))) uint16_t kv[WK][2][2][KT * DP];
+  __shared__ __attribute__((aligned(16))) float bias[WK][2][KT];
   __shared__ uint32_t seen[kMaxRange / 32];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, h = lane >> 5;
-  const uint32_t id = xcd_order(blockIdx.x, gridDim.x >> 3);
+  const uint32_t id = work_item(p);
   if (id >= p.total) return;
   const int split = id % (uint32_t)p.splits;
   const uint32_t bt = id / (uint32_t)p.splits;
@@ -36,11 +37,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_dq_kernel(const 
   const int bkv = bt / (uint32_t)p.tiles;
   const int b = bkv / p.KVH, g = bkv - b * p.KVH;
 
-  int klen = p.Lk;
-  if (p.klen) {
-    const int n = p.klen[b];
-    klen = n < 0 ? 0 : n < klen ? n : klen;
-  }
+  const int klen = keys_of(p, b);
   const int nt = (klen + KT - 1) / KT;
   const int t_lo = split * p.per_split + (WK == 1 ? 0 : wave);
   const int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
@@ -48,22 +45,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_dq_kernel(const 
   const uint16_t* vb = p.v + b * p.vs.b + g * p.vs.h;
   const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
 
-  const int buf0 = WK == 1 ? 0 : wave * 2;
+  const int own = WK == 1 ? 0 : wave;  // the buffers
   auto fetch = [&](int t, int buf, uint64_t word) __attribute__((always_inline)) {
-    const int64_t k0 = (int64_t)t * KT;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const uint16_t* base = x == 0 ? kb + k0 * p.ks.l : vb + k0 * p.vs.l;
-      const int64_t pitch = x == 0 ? p.ks.l : p.vs.l;
-      const uint32_t lds = LDS_ADDR(kv[buf0 + buf][x]);
-#pragma unroll
-      for (int r = 0; r < kXfer; ++r) {
-        const int c0 = WK == 1 ? wave * 64 + 256 * r : 64 * r;
-        dma_rows<DP>(lds, c0, lane, p.D, [&](int row) __attribute__((always_inline)) {
-          return (word >> row) & 1 ? base + row * pitch : static_cast<const uint16_t*>(nullptr);
-        });
-      }
-    }
+    fetch_keys<DP, kXfer, kStep>(p, kb, vb, (int64_t)t * KT, word, kv[own][buf][0], kv[own][buf][1],
+                                 WK == 1 ? wave * 64 : 0, lane);
+    if (WK == 1 ? wave == 0 : h == 0)
+      bias[own][buf][WK == 1 ? lane : col] = (word >> (WK == 1 ? lane : col)) & 1 ? 0.f : -__builtin_inff();
   };
   uint64_t word = 0;
   if (t_lo < t_hi) {
@@ -77,90 +64,83 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_dq_kernel(const 
   const int head = g * p.G + hg;
   const int64_t orow = ((int64_t)b * p.Lq + tok) * p.H + head;
   uint4 qf[KS], gf[KS];
-  float lse2 = __builtin_inff(), dd = 0.f;
+  float nlse2 = -__builtin_inff(), nd = 0.f;
   {
-    const uint16_t* qr = p.q + b * p.qs.b + (int64_t)tok * p.qs.l + head * p.qs.h;
-    const uint16_t* gr = p.dout + b * p.gs.b + (int64_t)tok * p.gs.l + head * p.gs.h;
-    const uint16_t* orp = p.out + orow * p.D;
+    uint4 of[KS];
+    load_row<KS>(qf, p.q + b * p.qs.b + (int64_t)tok * p.qs.l + head * p.qs.h, has_row, h, p.D);
+    load_row<KS>(gf, p.dout + b * p.gs.b + (int64_t)tok * p.gs.l + head * p.gs.h, has_row, h, p.D);
+    load_row<KS>(of, p.out + orow * p.D, has_row, h, p.D);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const int dim = 16 * ks + 8 * h;
-      qf[ks] = gf[ks] = uint4{0u, 0u, 0u, 0u};
-      if (has_row && dim < p.D) {
-        qf[ks] = ld16(qr + dim);
-        gf[ks] = ld16(gr + dim);
-        const uint4 ov = ld16(orp + dim);
-        const uint32_t gw[4] = {gf[ks].x, gf[ks].y, gf[ks].z, gf[ks].w};
-        const uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w};
+      const uint32_t gw[4] = {gf[ks].x, gf[ks].y, gf[ks].z, gf[ks].w};
+      const uint32_t ow[4] = {of[ks].x, of[ks].y, of[ks].z, of[ks].w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          dd = __builtin_fmaf(T::lo(gw[i]), T::lo(ow[i]), dd);
-          dd = __builtin_fmaf(T::hi(gw[i]), T::hi(ow[i]), dd);
-        }
+      for (int i = 0; i < 4; ++i) {
+        nd = __builtin_fmaf(-T::lo(gw[i]), T::lo(ow[i]), nd);
+        nd = __builtin_fmaf(-T::hi(gw[i]), T::hi(ow[i]), nd);
       }
     }
     if (has_row) {
       const float e = p.lse[((int64_t)b * p.H + head) * p.Lq + tok];
-      lse2 = e == -__builtin_inff() ? __builtin_inff() : e * kLog2e - (float)T::kShift;
+      nlse2 = e == -__builtin_inff() ? -__builtin_inff() : (float)T::kShift - e * kLog2e;
     }
-    dd += __shfl_xor(dd, 32, 64);
-    if (has_row && split == 0 && h == 0 && (WK == 1 || wave == 0))
-      p.stat[(int64_t)bkv * p.rows + row] = float2{lse2, dd};
+    nd = sum_halves(nd);
+    if (has_row && split == 0 && h == 0 && (WK == 1 || wave == 0)) {
+      const int64_t all = (int64_t)p.B * p.KVH * p.rows, at = (int64_t)bkv * p.rows + row;
+      p.row_stat[at] = nlse2;
+      p.row_stat[all + at] = nd;
+    }
   }
   wait_vmcnt<0>();
 
-  const float unscale = p.scale * kUnshift;
-  v16f dq[NDB];
+  v16f dq[NDB], nd16;
 #pragma unroll
   for (int i = 0; i < NDB; ++i) dq[i] = zero16();
+#pragma unroll
+  for (int r = 0; r < 16; ++r) nd16[r] = nd;
 
   for (int t = t_lo, buf = 0; t < t_hi; t += WK, buf ^= 1) {
     uint64_t word_next = 0;
     if (WK == 1) {
       wait_vmcnt<0>();
+      wait_lgkmcnt0();
       lds_barrier();
       if (t + WK < t_hi) {
         word_next = bits.template word<KT>(t + WK);
         fetch(t + WK, buf ^ 1, word_next);
       }
-    } else if (t + WK < t_hi) {
-      word_next = bits.template word<KT>(t + WK);
+    } else {
       wait_lgkmcnt0();
       asm volatile("" ::: "memory");
-      fetch(t + WK, buf ^ 1, word_next);
-      wait_vmcnt<2 * kXfer>();
-      asm volatile("" ::: "memory");
-    } else {
-      wait_vmcnt<0>();
+      if (t + WK < t_hi) {
+        word_next = bits.template word<KT>(t + WK);
+        fetch(t + WK, buf ^ 1, word_next);
+        wait_vmcnt<2 * kXfer>();
+      } else {
+        wait_vmcnt<0>();
+      }
       asm volatile("" ::: "memory");
     }
-    const uint16_t *kr = kv[buf0 + buf][0], *vr = kv[buf0 + buf][1];
+    const uint16_t *kr = kv[own][buf][0], *vr = kv[own][buf][1];
 #pragma unroll
     for (int i = 0; i < NKB; ++i) {
-      const uint32_t wi = (uint32_t)(word >> (32 * i));
-      if (!wi) continue;
-      v16f s = zero16(), dp = zero16();
+      if (!(uint32_t)(word >> (32 * i))) continue;
+      v16f s = start_from(bias[own][buf] + 32 * i, h), dp = nd16;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         s = T::mfma(frag_row<DP>(kr, 32 * i + col, 2 * k + h), qf[k], s);
         dp = T::mfma(frag_row<DP>(vr, 32 * i + col, 2 * k + h), gf[k], dp);
       }
-      if (wi != 0xffffffffu) {
-        const uint32_t w = wi >> (4 * h);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!((w >> (8 * (r / 4) + r % 4)) & 1)) s[r] = -__builtin_inff();
-      }
-      uint32_t sw[8];
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, -lse2));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, -lse2));
-        sw[r / 2] = T::pack(p0 * (dp[r] - dd), p1 * (dp[r + 1] - dd));
-      }
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
-        const uint4 sf = {sw[4 * s2], sw[4 * s2 + 1], sw[4 * s2 + 2], sw[4 * s2 + 3]};
+        uint32_t sw[4];
+#pragma unroll
+        for (int r = 8 * s2; r < 8 * s2 + 8; r += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, nlse2));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, nlse2));
+          sw[(r & 7) / 2] = T::pack(p0 * dp[r], p1 * dp[r + 1]);
+        }
+        const uint4 sf = {sw[0], sw[1], sw[2], sw[3]};
 #pragma unroll
         for (int d = 0; d < NDB; ++d)
           dq[d] = T::mfma(frag_tr<DP>(kr, 32 * i + 16 * s2, d, lane), sf, dq[d]);
@@ -170,10 +150,11 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_dq_kernel(const 
     __builtin_amdgcn_sched_barrier(0);
   }
 
+  const float unscale = p.scale * kUnshift;
   if constexpr (WK == 4) {
     __syncthreads();
-    float* ox = reinterpret_cast<float*>(&kv[0][0][0]);  // [4][DP][32]
-    static_assert(sizeof(kv) >= 4 * DP * 32 * 4, "the waves' dQ fit the buffers");
+    float* ox = reinterpret_cast<float*>(&kv[0][0][0][0]);  // [4][DP][32]
+    static_assert(sizeof(kv) >= WK * DP * 32 * 4, "the waves' dQ fit the buffers");
 #pragma unroll
     for (int d = 0; d < NDB; ++d)
 #pragma unroll
@@ -204,22 +185,11 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_dq_kernel(const 
     }
     return;
   }
-  if (!has_row) return;
-#pragma unroll
-  for (int d = 0; d < NDB; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int dim = 32 * d + 8 * (r / 4) + 4 * h;
-      if (dim >= p.D) continue;
-      if (p.splits > 1)
-        *reinterpret_cast<float4*>(
-            p.part + (((int64_t)split * p.B * p.KVH + bkv) * p.rows + row) * p.D + dim) =
-            float4{dq[d][r], dq[d][r + 1], dq[d][r + 2], dq[d][r + 3]};
-      else
-        *reinterpret_cast<uint2*>(p.dq + orow * p.D + dim) =
-            uint2{T::pack(dq[d][r] * unscale, dq[d][r + 1] * unscale),
-                  T::pack(dq[d][r + 2] * unscale, dq[d][r + 3] * unscale)};
-    }
+  if (p.splits > 1) {
+    if (has_row) store_part(p.part + (((int64_t)split * p.B * p.KVH + bkv) * p.rows + row) * p.D, dq, h, p.D);
+    return;
+  }
+  store_row<T>(p.dq + orow * p.D, has_row, dq, unscale, h, p.D);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -229,20 +199,20 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_dq_kernel(const 
 // dV^T += dO^T P and dK^T += Q^T dS, whose A operands are transpose reads of the same rows.
 // ---------------------------------------------------------------------------------------
 constexpr int kQT = 64;
-static __device__ __attribute__((aligned(8))) float g_pad_stat[2] = {__builtin_inff(), 0.f};
+static __device__ float g_pad_stat[2] = {-__builtin_inff(), 0.f};
 
 template <class T, int DP>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_dkdv_kernel(const Args p) {
+__global__ __launch_bounds__(256, DP == 128 ? 1 : DP == 64 ? 2 : 4) void xattn_dkdv_kernel(const Args p) {
   constexpr int NG = DP / 8, KS = DP / 16, NDB = DP / 32;
   constexpr float kUnshift = 1.f / (1 << T::kShift);
   constexpr int kXfer = kQT * NG / 256;
   __shared__ __attribute__((aligned(1024))) uint16_t qg[2][2][kQT * DP];
-  __shared__ __attribute__((aligned(256))) float2 st[2][kQT];
+  __shared__ __attribute__((aligned(256))) float st[2][2][kQT];  // -lse, -D
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, h = lane >> 5;
-  const uint32_t id = xcd_order(blockIdx.x, gridDim.x >> 3);
+  const uint32_t id = work_item(p);
   if (id >= p.total) return;
   const int split = id % (uint32_t)p.splits;
   const uint32_t bt = id / (uint32_t)p.splits;
@@ -250,27 +220,13 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_dkdv_kernel(cons
   const int bkv = bt / (uint32_t)p.tiles;
   const int b = bkv / p.KVH, g = bkv - b * p.KVH;
 
-  int klen = p.Lk;
-  if (p.klen) {
-    const int n = p.klen[b];
-    klen = n < 0 ? 0 : n < klen ? n : klen;
-  }
+  const int klen = keys_of(p, b);
   const int key = tile * 128 + wave * 32 + col;
   const bool vis = key < klen && (!p.kmask || p.kmask[b * p.mask_b + key] != 0);
   const bool any_vis = __any(vis);  // (wave-uniform)
   uint4 kf[KS], vf[KS];
-  {
-    const uint16_t* kr = p.k + b * p.ks.b + key * p.ks.l + g * p.ks.h;
-    const uint16_t* vr = p.v + b * p.vs.b + key * p.vs.l + g * p.vs.h;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      kf[ks] = vf[ks] = uint4{0u, 0u, 0u, 0u};
-      if (vis && 16 * ks + 8 * h < p.D) {
-        kf[ks] = ld16(kr + 16 * ks + 8 * h);
-        vf[ks] = ld16(vr + 16 * ks + 8 * h);
-      }
-    }
-  }
+  load_row<KS>(kf, p.k + b * p.ks.b + key * p.ks.l + g * p.ks.h, vis, h, p.D);
+  load_row<KS>(vf, p.v + b * p.vs.b + key * p.vs.l + g * p.vs.h, vis, h, p.D);
   const bool wg_vis = __syncthreads_or(vis);
   const int nt = wg_vis ? (p.rows + kQT - 1) / kQT : 0;
   const int t_lo = split * p.per_split;
@@ -278,27 +234,27 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_dkdv_kernel(cons
 
   const uint16_t* qb = p.q + b * p.qs.b + (int64_t)g * p.G * p.qs.h;
   const uint16_t* gb = p.dout + b * p.gs.b + (int64_t)g * p.G * p.gs.h;
-  const float* sb = reinterpret_cast<const float*>(p.stat + (int64_t)bkv * p.rows);
+  const float* sb = p.row_stat + (int64_t)bkv * p.rows;
+  const int64_t all_rows = (int64_t)p.B * p.KVH * p.rows;
   auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
     const int r0 = t * kQT;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const uint16_t* base = x == 0 ? qb : gb;
-      const Stride s = x == 0 ? p.qs : p.gs;
-#pragma unroll
-      for (int r = 0; r < kXfer; ++r)
-        dma_rows<DP>(LDS_ADDR(qg[buf][x]), wave * 64 + 256 * r, lane, p.D,
-                     [&](int row) __attribute__((always_inline)) {
-                       row += r0;
-                       if (row >= p.rows) return static_cast<const uint16_t*>(nullptr);
-                       const uint32_t hg = fdiv(row, p.by_lq), tok = row - hg * p.Lq;
-                       return base + (int64_t)tok * s.l + hg * s.h;
-                     });
+    for (int r = 0; r < kXfer; ++r) {
+      const int c0 = wave * 64 + 256 * r;
+      const int row = r0 + (c0 + lane) / NG;
+      const bool on = row < p.rows;
+      const uint32_t hg = fdiv(on ? row : 0, p.by_lq), tok = (on ? row : 0) - hg * p.Lq;
+      const uint16_t* qr = qb + (int64_t)tok * p.qs.l + hg * p.qs.h;
+      const uint16_t* gr = gb + (int64_t)tok * p.gs.l + hg * p.gs.h;
+      dma_rows<DP>(LDS_ADDR(qg[buf][0]), c0, lane, p.D,
+                   [&](int) __attribute__((always_inline)) { return on ? qr : static_cast<const uint16_t*>(nullptr); });
+      dma_rows<DP>(LDS_ADDR(qg[buf][1]), c0, lane, p.D,
+                   [&](int) __attribute__((always_inline)) { return on ? gr : static_cast<const uint16_t*>(nullptr); });
     }
-    if (wave < 2) {  // (lse, D) of 32 rows each
-      const int row = r0 + 32 * wave + (lane >> 1);
-      const float* a = row < p.rows ? sb + 2 * (int64_t)row + (lane & 1) : g_pad_stat + (lane & 1);
-      dma4_lds(a, (uint32_t)__builtin_amdgcn_readfirstlane(LDS_ADDR(st[buf]) + 256 * wave));
+    if (wave < 2) {  // -lse (wave 0) and -D (wave 1)
+      const int row = r0 + lane;
+      const float* a = row < p.rows ? sb + wave * all_rows + row : g_pad_stat + wave;
+      dma4_lds(a, (uint32_t)__builtin_amdgcn_readfirstlane(LDS_ADDR(st[buf][wave])));
     }
   };
   wait_vmcnt<0>();  // (no wait on keys and values inside the loop)
@@ -311,61 +267,58 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_dkdv_kernel(cons
     wait_vmcnt<0>();
     lds_barrier();
     if (t + 1 < t_hi) fetch(t + 1, buf ^ 1);
-    if (!any_vis) continue;
-    const uint16_t *qr = qg[buf][0], *gr = qg[buf][1];
+    if (any_vis) {
+      const uint16_t *qr = qg[buf][0], *gr = qg[buf][1];
 #pragma unroll
-    for (int i = 0; i < kQT / 32; ++i) {
-      v16f s = zero16(), dp = zero16();
+      for (int i = 0; i < kQT / 32; ++i) {
+        v16f s = zero16(), dp = start_from(st[buf][1] + 32 * i, h);
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        s = T::mfma(frag_row<DP>(qr, 32 * i + col, 2 * k + h), kf[k], s);
-        dp = T::mfma(frag_row<DP>(gr, 32 * i + col, 2 * k + h), vf[k], dp);
-      }
-      uint32_t pw[8], sw[8];
+        for (int k = 0; k < KS; ++k) {
+          s = T::mfma(frag_row<DP>(qr, 32 * i + col, 2 * k + h), kf[k], s);
+          dp = T::mfma(frag_row<DP>(gr, 32 * i + col, 2 * k + h), vf[k], dp);
+        }
 #pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        const float4 e = *reinterpret_cast<const float4*>(&st[buf][32 * i + 8 * (r / 4) + 4 * h + r % 4]);
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, -e.x));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, -e.z));
-        pw[r / 2] = T::pack(p0, p1);
-        sw[r / 2] = T::pack(p0 * (dp[r] - e.y), p1 * (dp[r + 1] - e.w));
-      }
+        for (int s2 = 0; s2 < 2; ++s2) {
+          uint32_t pw[4], sw[4];
 #pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        const uint4 pf = {pw[4 * s2], pw[4 * s2 + 1], pw[4 * s2 + 2], pw[4 * s2 + 3]};
-        const uint4 sf = {sw[4 * s2], sw[4 * s2 + 1], sw[4 * s2 + 2], sw[4 * s2 + 3]};
+          for (int x = 0; x < 2; ++x) {
+            const float4 e = *reinterpret_cast<const float4*>(&st[buf][0][32 * i + 16 * s2 + 8 * x + 4 * h]);
+            const int r = 8 * s2 + 4 * x;
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, e.x));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, e.y));
+            const float p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 2], p.c2, e.z));
+            const float p3 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 3], p.c2, e.w));
+            pw[2 * x] = T::pack(p0, p1), pw[2 * x + 1] = T::pack(p2, p3);
+            sw[2 * x] = T::pack(p0 * dp[r], p1 * dp[r + 1]);
+            sw[2 * x + 1] = T::pack(p2 * dp[r + 2], p3 * dp[r + 3]);
+          }
+          const uint4 pf = {pw[0], pw[1], pw[2], pw[3]}, sf = {sw[0], sw[1], sw[2], sw[3]};
 #pragma unroll
-        for (int d = 0; d < NDB; ++d) {
-          dv[d] = T::mfma(frag_tr<DP>(gr, 32 * i + 16 * s2, d, lane), pf, dv[d]);
-          dk[d] = T::mfma(frag_tr<DP>(qr, 32 * i + 16 * s2, d, lane), sf, dk[d]);
+          for (int d = 0; d < NDB; ++d) {
+            dv[d] = T::mfma(frag_tr<DP>(gr, 32 * i + 16 * s2, d, lane), pf, dv[d]);
+            dk[d] = T::mfma(frag_tr<DP>(qr, 32 * i + 16 * s2, d, lane), sf, dk[d]);
+          }
         }
       }
     }
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  if (key >= p.Lk) return;
-  const int64_t n = (int64_t)p.B * p.KVH * p.Lk, at = (int64_t)bkv * p.Lk + key;
-  const float fk = p.scale * kUnshift;
+  const bool on = key < p.Lk;
+  if (!vis) {  // (in the products an invisible key's column holds what a key of zeros would get)
 #pragma unroll
-  for (int d = 0; d < NDB; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int dim = 32 * d + 8 * (r / 4) + 4 * h;
-      if (dim >= p.D) continue;
-      float4 a = {dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
-      float4 c = {dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
-      if (!vis) a = c = float4{0.f, 0.f, 0.f, 0.f};
-      if (p.splits > 1) {
-        *reinterpret_cast<float4*>(p.part + (split * 2 * n + at) * p.D + dim) = a;
-        *reinterpret_cast<float4*>(p.part + ((split * 2 + 1) * n + at) * p.D + dim) = c;
-      } else {
-        *reinterpret_cast<uint2*>(p.dk + b * p.dks.b + key * p.dks.l + g * p.dks.h + dim) =
-            uint2{T::pack(a.x * fk, a.y * fk), T::pack(a.z * fk, a.w * fk)};
-        *reinterpret_cast<uint2*>(p.dv + b * p.dvs.b + key * p.dvs.l + g * p.dvs.h + dim) =
-            uint2{T::pack(c.x * kUnshift, c.y * kUnshift), T::pack(c.z * kUnshift, c.w * kUnshift)};
-      }
+    for (int i = 0; i < NDB; ++i) dk[i] = dv[i] = zero16();
+  }
+  if (p.splits > 1) {
+    const int64_t n = (int64_t)p.B * p.KVH * p.Lk, at = (int64_t)bkv * p.Lk + key;
+    if (on) {
+      store_part(p.part + (split * 2 * n + at) * p.D, dk, h, p.D);
+      store_part(p.part + ((split * 2 + 1) * n + at) * p.D, dv, h, p.D);
     }
+    return;
+  }
+  store_row<T>(p.dk + b * p.dks.b + key * p.dks.l + g * p.dks.h, on, dk, p.scale * kUnshift, h, p.D);
+  store_row<T>(p.dv + b * p.dvs.b + key * p.dvs.l + g * p.dvs.h, on, dv, kUnshift, h, p.D);
 }
 
 // Sums of the splits, in order: of dQ (kDq), or of dK and dV. Thread: 8 dims of a row.
@@ -409,7 +362,7 @@ __global__ __launch_bounds__(256) void xattn_sum_kernel(const Args p) {
 using namespace dpa;
 using namespace dpa::xattn;
 
-// (lse, D) of every row, then room for one kernel's partial sums at a time
+// lse and D of every row, then room for one kernel's partial sums at a time
 static int64_t stat_bytes(const Args& p) { return align256((int64_t)p.B * p.KVH * p.rows * 8); }
 
 static int64_t bwd_workspace(const Args& rows, const Args& keys) {
@@ -429,9 +382,9 @@ template <class T, int DP>
 static int launch_bwd(const Args& r, const Args& k, hipStream_t s) {
   if (r.total > 0) {
     if (few_rows(r))
-      xattn_dq_kernel<T, DP, 4><<<xcd_grid(r.total), 256, 0, s>>>(r);
+      xattn_dq_kernel<T, DP, 4><<<r.grid, 256, 0, s>>>(r);
     else
-      xattn_dq_kernel<T, DP, 1><<<xcd_grid(r.total), 256, 0, s>>>(r);
+      xattn_dq_kernel<T, DP, 1><<<r.grid, 256, 0, s>>>(r);
     int st = launch_status();
     if (st != DPA_OK) return st;
     if (r.splits > 1) {
@@ -442,7 +395,7 @@ static int launch_bwd(const Args& r, const Args& k, hipStream_t s) {
     }
   }
   if (k.total > 0) {
-    xattn_dkdv_kernel<T, DP><<<xcd_grid(k.total), 256, 0, s>>>(k);
+    xattn_dkdv_kernel<T, DP><<<k.grid, 256, 0, s>>>(k);
     int st = launch_status();
     if (st != DPA_OK || k.splits <= 1) return st;
     const int64_t n = (int64_t)k.B * k.KVH * k.Lk * 2 * (k.D / 8);
@@ -483,7 +436,7 @@ extern "C" int dpa_cross_attention_bwd(const DpaCrossAttention* a, void* workspa
   if (need) {
     if (!workspace || workspace_bytes < need) return DPA_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return DPA_ERR_ALIGN;
-    r.stat = k.stat = (float2*)workspace;
+    r.row_stat = k.row_stat = (float*)workspace;
     r.part = k.part = (float*)((uint8_t*)workspace + stat_bytes(r));
   }
   if (a->q_len == 0) r.total = 0;

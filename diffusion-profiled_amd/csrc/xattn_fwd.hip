@@ -1,36 +1,39 @@
 // Cross attention, forward: one pass over the keys with the running maximum and sum of each
 // row's softmax.
-#include <type_traits>
-
 #include "xattn.hpp"
 
 namespace dpa {
 namespace xattn {
 
 // ---------------------------------------------------------------------------------------
-// WK = 1: four waves of 32 query rows each share tiles of 64 keys, double-buffered by DMA.
-// WK = 4, for up to 32 rows: the four waves share the rows and take every fourth tile of 32 keys
-// each, through buffers of their own, and join their softmaxes in LDS at the end.
+// More than 32 rows: four waves of 32 query rows each share tiles of 64 keys, double-buffered by
+// DMA.
 //
 // Per tile a wave forms S^T = K Q^T (A: key rows from LDS, B: its queries, in registers), so lane
 // l holds scores of query l & 31 at keys 8 i + 4 (l >> 5) + j; then the row's running maximum and
 // sum, P = 2^(c2 S - m) rounded to the operands' type for the product (its sum is of the fp32
-// values), and O^T += V^T P^T with P^T straight from those registers.
+// values), and O^T += V^T P^T with P^T straight from those registers. A product over a tile starts
+// from 0 for the visible keys and -inf for the others, which costs no instruction per score.
+//
+// The maximum that O and its sum stand at moves up only when a score passes it by 2^8: P then
+// stays below 2^8, which fp32 and both operand types have room for, and nearly every tile goes
+// without the products that move it.
 // ---------------------------------------------------------------------------------------
-template <class T, int DP, int WK>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_fwd_kernel(const Args p) {
-  constexpr int KT = WK == 1 ? 64 : 32, NKB = KT / 32;
+constexpr float kSlack = 8.f;
+
+template <class T, int DP>
+__global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_fwd_kernel(const Args p) {
+  constexpr int KT = 64;
   constexpr int NG = DP / 8, KS = DP / 16, NDB = DP / 32;
-  constexpr int kTile = KT * DP;                         // elements of a K (or V) tile
-  constexpr int kXfer = KT * NG / (WK == 1 ? 256 : 64);  // a wave's transfers per K (or V) tile
-  constexpr int kBufs = 2 * (WK == 1 ? 1 : 4);
-  __shared__ __attribute__((aligned(1024))) uint16_t kv[kBufs][2][kTile];
+  constexpr int kXfer = KT * NG / 256;  // a wave's transfers per K (or V) tile
+  __shared__ __attribute__((aligned(1024))) uint16_t kv[2][2][KT * DP];
+  __shared__ __attribute__((aligned(16))) float bias[2][KT];
   __shared__ uint32_t seen[kMaxRange / 32];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, h = lane >> 5;
-  const uint32_t id = xcd_order(blockIdx.x, gridDim.x >> 3);
+  const uint32_t id = work_item(p);
   if (id >= p.total) return;
   const int split = id % (uint32_t)p.splits;
   const uint32_t bt = id / (uint32_t)p.splits;
@@ -38,41 +41,20 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_fwd_kernel(const
   const int bkv = bt / (uint32_t)p.tiles;
   const int b = bkv / p.KVH, g = bkv - b * p.KVH;
 
-  // the keys of this workgroup
-  int klen = p.Lk;
-  if (p.klen) {
-    const int n = p.klen[b];
-    klen = n < 0 ? 0 : n < klen ? n : klen;
-  }
+  const int klen = keys_of(p, b);
   const int nt = (klen + KT - 1) / KT;
-  const int t_lo = split * p.per_split + (WK == 1 ? 0 : wave);
+  const int t_lo = split * p.per_split;
   const int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
-
   const uint16_t* kb = p.k + b * p.ks.b + g * p.ks.h;
   const uint16_t* vb = p.v + b * p.vs.b + g * p.vs.h;
-
   const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
 
-  // this lane's query row
-  const int row = (WK == 1 ? tile * 128 + wave * 32 : 0) + col;
+  const int row = tile * 128 + wave * 32 + col;
   const bool has_row = row < p.rows;
   const uint32_t head = fdiv(has_row ? row : 0, p.by_lq), tok = (has_row ? row : 0) - head * p.Lq;
-  const int buf0 = WK == 1 ? 0 : wave * 2;
   auto fetch = [&](int t, int buf, uint64_t word) __attribute__((always_inline)) {
-    const int64_t k0 = (int64_t)t * KT;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const uint16_t* base = x == 0 ? kb + k0 * p.ks.l : vb + k0 * p.vs.l;
-      const int64_t pitch = x == 0 ? p.ks.l : p.vs.l;
-      const uint32_t lds = LDS_ADDR(kv[buf0 + buf][x]);
-#pragma unroll
-      for (int r = 0; r < kXfer; ++r) {
-        const int c0 = WK == 1 ? wave * 64 + 256 * r : 64 * r;
-        dma_rows<DP>(lds, c0, lane, p.D, [&](int row) __attribute__((always_inline)) {
-          return (word >> row) & 1 ? base + row * pitch : static_cast<const uint16_t*>(nullptr);
-        });
-      }
-    }
+    fetch_keys<DP, kXfer, 256>(p, kb, vb, (int64_t)t * KT, word, kv[buf][0], kv[buf][1], wave * 64, lane);
+    if (wave == 0) bias[buf][lane] = (word >> lane) & 1 ? 0.f : -__builtin_inff();
   };
 
   uint64_t word = 0;
@@ -81,196 +63,244 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_fwd_kernel(const
     fetch(t_lo, 0, word);
   }
   uint4 qf[KS];
-  {
-    const uint16_t* qr = p.q + b * p.qs.b + (int64_t)tok * p.qs.l + (g * p.G + head) * p.qs.h;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      qf[ks] = uint4{0u, 0u, 0u, 0u};
-      if (has_row && 16 * ks + 8 * h < p.D) qf[ks] = ld16(qr + 16 * ks + 8 * h);
-    }
-  }
+  load_row<KS>(qf, p.q + b * p.qs.b + (int64_t)tok * p.qs.l + (g * p.G + head) * p.qs.h, has_row, h, p.D);
   wait_vmcnt<0>();  // (no wait on the queries inside the loop: it would take in the tile in flight)
 
   v16f o[NDB];
 #pragma unroll
   for (int i = 0; i < NDB; ++i) o[i] = zero16();
-  float m = -__builtin_inff();  // running maximum of c2 S
+  float m = -__builtin_inff();  // what O and l stand at, in units of c2 S
   float l = 0.f;                // this lane's half of the running sum
 
-  // one tile: NB blocks of 32 keys
-  auto step = [&](const uint16_t* ks_, const uint16_t* vs_, uint64_t word, auto nb)
-                  __attribute__((always_inline)) {
-    constexpr int NB = decltype(nb)::value;
-    v16f s[NB];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      s[i] = zero16();
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-        s[i] = T::mfma(frag_row<DP>(ks_, 32 * i + col, 2 * k + h), qf[k], s[i]);
+  for (int t = t_lo, buf = 0; t < t_hi; ++t, buf ^= 1) {
+    uint64_t word_next = 0;
+    wait_vmcnt<0>();
+    wait_lgkmcnt0();
+    lds_barrier();  // tile t is there, and every wave is past its reads of the other buffer
+    if (t + 1 < t_hi) {
+      word_next = bits.template word<KT>(t + 1);
+      fetch(t + 1, buf ^ 1, word_next);
     }
-    if (word != (NB * 32 == 64 ? ~0ull : 0xffffffffull)) {
-      const uint64_t w = word >> (4 * h);
+    if (word) {
+      const uint16_t *ks_ = kv[buf][0], *vs_ = kv[buf][1];
+      v16f s[2];
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
+      for (int i = 0; i < 2; ++i) {
+        s[i] = start_from(bias[buf] + 32 * i, h);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!((w >> (32 * i + 8 * (r / 4) + r % 4)) & 1)) s[i][r] = -__builtin_inff();
-    }
-    float top = -__builtin_inff();
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
-    top = fmaxf(top, __shfl_xor(top, 32, 64)) * p.c2;
-    if (__any(top > m)) {
-      const float mn = fmaxf(top, m);
-      const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= f;
-#pragma unroll
-      for (int d = 0; d < NDB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] *= f;
-    }
-    const float ms = m == -__builtin_inff() ? 0.f : m;  // nothing visible yet: P = 0
-    uint32_t pk[NB][8];
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], p.c2, -ms));
-        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r + 1], p.c2, -ms));
-        l += e0 + e1;
-        pk[i][r / 2] = T::pack(e0, e1);
+        for (int k = 0; k < KS; ++k)
+          s[i] = T::mfma(frag_row<DP>(ks_, 32 * i + col, 2 * k + h), qf[k], s[i]);
       }
+      float top = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        const uint4 pf = {pk[i][4 * s2], pk[i][4 * s2 + 1], pk[i][4 * s2 + 2], pk[i][4 * s2 + 3]};
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
+      top = max_halves(top) * p.c2;
+      if (__any(top > m + kSlack)) {
+        const float mn = fmaxf(top, m);
+        const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
 #pragma unroll
         for (int d = 0; d < NDB; ++d)
-          o[d] = T::mfma(frag_tr<DP>(vs_, 32 * i + 16 * s2, d, lane), pf, o[d]);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= f;
       }
-  };
-
-  for (int t = t_lo, buf = 0; t < t_hi; t += WK, buf ^= 1) {
-    uint64_t word_next = 0;
-    if (WK == 1) {
-      wait_vmcnt<0>();
-      lds_barrier();  // tile t is there, and every wave is past its reads of the other buffer
-      if (t + WK < t_hi) {
-        word_next = bits.template word<KT>(t + WK);
-        fetch(t + WK, buf ^ 1, word_next);
-      }
-    } else if (t + WK < t_hi) {
-      word_next = bits.template word<KT>(t + WK);
-      wait_lgkmcnt0();
-      asm volatile("" ::: "memory");
-      fetch(t + WK, buf ^ 1, word_next);
-      wait_vmcnt<2 * kXfer>();  // all but the transfers just issued
-      asm volatile("" ::: "memory");
-    } else {
-      wait_vmcnt<0>();
-      asm volatile("" ::: "memory");
-    }
-    const uint16_t *ks_ = kv[buf0 + buf][0], *vs_ = kv[buf0 + buf][1];
-    if (word) {
-      if (NKB == 2 && (word >> 32))
-        step(ks_, vs_, word, std::integral_constant<int, NKB>());
-      else
-        step(ks_, vs_, word, std::integral_constant<int, 1>());
+      const float ms = m == -__builtin_inff() ? 0.f : m;  // nothing visible yet: P = 0
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+          uint32_t pk[4];
+#pragma unroll
+          for (int r = 0; r < 8; r += 2) {
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][8 * s2 + r], p.c2, -ms));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][8 * s2 + r + 1], p.c2, -ms));
+            l += e0 + e1;
+            pk[r / 2] = T::pack(e0, e1);
+          }
+          const uint4 pf = {pk[0], pk[1], pk[2], pk[3]};
+#pragma unroll
+          for (int d = 0; d < NDB; ++d)
+            o[d] = T::mfma(frag_tr<DP>(vs_, 32 * i + 16 * s2, d, lane), pf, o[d]);
+        }
     }
     word = word_next;
     __builtin_amdgcn_sched_barrier(0);
   }
-  l += __shfl_xor(l, 32, 64);
+  l = sum_halves(l);
 
-  if constexpr (WK == 4) {
-    // join the waves: wave w leaves its (m, l) and O, then adds up a quarter of the dims
-    __syncthreads();  // (every wave is past its buffers)
-    float* ox = reinterpret_cast<float*>(&kv[0][0][0]);  // [4][DP][32]
-    static_assert(sizeof(kv) >= 4 * DP * 32 * 4, "the waves' O fit the buffers");
-#pragma unroll
-    for (int d = 0; d < NDB; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        ox[(wave * DP + 32 * d + 8 * (r / 4) + 4 * h + r % 4) * 32 + col] = o[d][r];
-    __shared__ float ml[2][4][32];
-    if (h == 0) {
-      ml[0][wave][col] = m;
-      ml[1][wave][col] = l;
-    }
-    __syncthreads();
-    m = fmaxf(fmaxf(ml[0][0][col], ml[0][1][col]), fmaxf(ml[0][2][col], ml[0][3][col]));
-    const float ms = m == -__builtin_inff() ? 0.f : m;
-    float f[4];
-    l = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      f[w] = __builtin_amdgcn_exp2f(ml[0][w][col] - ms);
-      l += f[w] * ml[1][w][col];
-    }
-    // 8 threads per row: dims [q8 DP / 8, (q8 + 1) DP / 8) of row tid & 31
-    const int q8 = tid >> 5;
-    constexpr int ND = DP / 8;
-    float acc[ND];
-#pragma unroll
-    for (int i = 0; i < ND; ++i) {
-      acc[i] = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) acc[i] += f[w] * ox[(w * DP + q8 * ND + i) * 32 + col];
-    }
-    if (!has_row) return;
-    if (p.splits > 1) {
-      const int64_t at = ((int64_t)split * p.B * p.KVH + bkv) * p.rows + row;
-      if (q8 == 0) p.stat[at] = float2{m, l};
-#pragma unroll
-      for (int i = 0; i < ND; ++i)
-        if (q8 * ND + i < p.D) p.part[at * p.D + q8 * ND + i] = acc[i];
-      return;
-    }
-    const int64_t orow = ((int64_t)b * p.Lq + tok) * p.H + g * p.G + head;
-    if (q8 == 0)
-      p.lse[((int64_t)b * p.H + g * p.G + head) * p.Lq + tok] = (m + __builtin_amdgcn_logf(l)) * kLn2;
-    const float il = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int i = 0; i < ND; i += 4)
-      if (q8 * ND + i < p.D)
-        *reinterpret_cast<uint2*>(p.out + orow * p.D + q8 * ND + i) =
-            uint2{T::pack(acc[i] * il, acc[i + 1] * il), T::pack(acc[i + 2] * il, acc[i + 3] * il)};
-    return;
-  }
-
-  if (!has_row) return;
   if (p.splits > 1) {
+    if (!has_row) return;
     const int64_t at = ((int64_t)split * p.B * p.KVH + bkv) * p.rows + row;
     if (h == 0) p.stat[at] = float2{m, l};
-#pragma unroll
-    for (int d = 0; d < NDB; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int dim = 32 * d + 8 * (r / 4) + 4 * h;
-        if (dim < p.D)
-          *reinterpret_cast<float4*>(p.part + at * p.D + dim) =
-              float4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
-      }
+    store_part(p.part + at * p.D, o, h, p.D);
     return;
   }
-  const int64_t orow = ((int64_t)b * p.Lq + tok) * p.H + g * p.G + head;
-  if (h == 0)
+  if (has_row && h == 0)
     p.lse[((int64_t)b * p.H + g * p.G + head) * p.Lq + tok] = (m + __builtin_amdgcn_logf(l)) * kLn2;
-  const float il = l == 0.f ? 0.f : 1.f / l;
+  store_row<T>(p.out + (((int64_t)b * p.Lq + tok) * p.H + g * p.G + head) * p.D, has_row, o,
+               l == 0.f ? 0.f : 1.f / l, h, p.D);
+}
+
+// ---------------------------------------------------------------------------------------
+// Up to 32 rows: the four waves share them and take every fourth tile of 32 keys each, through
+// buffers of their own, and join their softmaxes in LDS at the end. Products as above.
+// ---------------------------------------------------------------------------------------
+template <class T, int DP>
+__global__ __launch_bounds__(256, 1) void xattn_few_kernel(const Args p) {
+  constexpr int KT = 32;
+  constexpr int NG = DP / 8, KS = DP / 16, NDB = DP / 32;
+  constexpr int kXfer = KT * NG / 64;
+  __shared__ __attribute__((aligned(1024))) uint16_t kv[4][2][2][KT * DP];
+  __shared__ __attribute__((aligned(16))) float bias[4][2][KT];
+  __shared__ uint32_t seen[kMaxRange / 32];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, h = lane >> 5;
+  const uint32_t id = work_item(p);
+  if (id >= p.total) return;
+  const int split = id % (uint32_t)p.splits;
+  const int bkv = id / (uint32_t)p.splits;
+  const int b = bkv / p.KVH, g = bkv - b * p.KVH;
+
+  const int klen = keys_of(p, b);
+  const int nt = (klen + KT - 1) / KT;
+  const int t_lo = split * p.per_split + wave;
+  const int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
+  const uint16_t* kb = p.k + b * p.ks.b + g * p.ks.h;
+  const uint16_t* vb = p.v + b * p.vs.b + g * p.vs.h;
+  const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
+
+  const int row = col;
+  const bool has_row = row < p.rows;
+  const uint32_t head = fdiv(has_row ? row : 0, p.by_lq), tok = (has_row ? row : 0) - head * p.Lq;
+  auto fetch = [&](int t, int buf, uint32_t word) __attribute__((always_inline)) {
+    fetch_keys<DP, kXfer, 64>(p, kb, vb, (int64_t)t * KT, word, kv[wave][buf][0], kv[wave][buf][1], 0, lane);
+    if (h == 0) bias[wave][buf][col] = (word >> col) & 1 ? 0.f : -__builtin_inff();
+  };
+  uint32_t word = 0;
+  if (t_lo < t_hi) {
+    word = (uint32_t)bits.template word<KT>(t_lo);
+    fetch(t_lo, 0, word);
+  }
+  uint4 qf[KS];
+  load_row<KS>(qf, p.q + b * p.qs.b + (int64_t)tok * p.qs.l + (g * p.G + head) * p.qs.h, has_row, h, p.D);
+  wait_vmcnt<0>();
+
+  v16f o[NDB];
+#pragma unroll
+  for (int i = 0; i < NDB; ++i) o[i] = zero16();
+  float m = -__builtin_inff(), l = 0.f;
+
+  for (int t = t_lo, buf = 0; t < t_hi; t += 4, buf ^= 1) {
+    uint32_t word_next = 0;
+    wait_lgkmcnt0();  // the reads of the other buffer are done
+    asm volatile("" ::: "memory");
+    if (t + 4 < t_hi) {
+      word_next = (uint32_t)bits.template word<KT>(t + 4);
+      fetch(t + 4, buf ^ 1, word_next);
+      wait_vmcnt<2 * kXfer>();  // all but the transfers just issued
+    } else {
+      wait_vmcnt<0>();
+    }
+    asm volatile("" ::: "memory");
+    if (word) {
+      const uint16_t *ks_ = kv[wave][buf][0], *vs_ = kv[wave][buf][1];
+      v16f s = start_from(bias[wave][buf], h);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) s = T::mfma(frag_row<DP>(ks_, col, 2 * k + h), qf[k], s);
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+      top = max_halves(top) * p.c2;
+      if (__any(top > m + kSlack)) {
+        const float mn = fmaxf(top, m);
+        const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < NDB; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= f;
+      }
+      const float ms = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        uint32_t pk[4];
+#pragma unroll
+        for (int r = 0; r < 8; r += 2) {
+          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * s2 + r], p.c2, -ms));
+          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * s2 + r + 1], p.c2, -ms));
+          l += e0 + e1;
+          pk[r / 2] = T::pack(e0, e1);
+        }
+        const uint4 pf = {pk[0], pk[1], pk[2], pk[3]};
+#pragma unroll
+        for (int d = 0; d < NDB; ++d) o[d] = T::mfma(frag_tr<DP>(vs_, 16 * s2, d, lane), pf, o[d]);
+      }
+    }
+    word = word_next;
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  l = sum_halves(l);
+
+  // wave w leaves its (m, l) and O, then adds up a quarter of the dims
+  __syncthreads();  // (every wave is past its buffers)
+  float* ox = reinterpret_cast<float*>(&kv[0][0][0][0]);  // [4][DP][32]
+  static_assert(sizeof(kv) >= 4 * DP * 32 * 4, "the waves' O fit the buffers");
 #pragma unroll
   for (int d = 0; d < NDB; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int dim = 32 * d + 8 * (r / 4) + 4 * h;
-      if (dim < p.D)
-        *reinterpret_cast<uint2*>(p.out + orow * p.D + dim) =
-            uint2{T::pack(o[d][r] * il, o[d][r + 1] * il), T::pack(o[d][r + 2] * il, o[d][r + 3] * il)};
-    }
+    for (int r = 0; r < 16; ++r)
+      ox[(wave * DP + 32 * d + 8 * (r / 4) + 4 * h + r % 4) * 32 + col] = o[d][r];
+  __shared__ float ml[2][4][32];
+  if (h == 0) {
+    ml[0][wave][col] = m;
+    ml[1][wave][col] = l;
+  }
+  __syncthreads();
+  m = fmaxf(fmaxf(ml[0][0][col], ml[0][1][col]), fmaxf(ml[0][2][col], ml[0][3][col]));
+  const float ms = m == -__builtin_inff() ? 0.f : m;
+  float f[4];
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = __builtin_amdgcn_exp2f(ml[0][w][col] - ms);
+    l += f[w] * ml[1][w][col];
+  }
+  // 8 threads per row: dims [q8 DP / 8, (q8 + 1) DP / 8) of row tid & 31
+  const int q8 = tid >> 5;
+  constexpr int ND = DP / 8;
+  float acc[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    acc[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) acc[i] += f[w] * ox[(w * DP + q8 * ND + i) * 32 + col];
+  }
+  if (!has_row) return;
+  if (p.splits > 1) {
+    const int64_t at = ((int64_t)split * p.B * p.KVH + bkv) * p.rows + row;
+    if (q8 == 0) p.stat[at] = float2{m, l};
+#pragma unroll
+    for (int i = 0; i < ND; i += 4)
+      if (q8 * ND + i < p.D)
+        *reinterpret_cast<float4*>(p.part + at * p.D + q8 * ND + i) =
+            float4{acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
+    return;
+  }
+  const int64_t orow = ((int64_t)b * p.Lq + tok) * p.H + g * p.G + head;
+  if (q8 == 0)
+    p.lse[((int64_t)b * p.H + g * p.G + head) * p.Lq + tok] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+  const float il = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < ND; i += 4)
+    if (q8 * ND + i < p.D)
+      *reinterpret_cast<uint2*>(p.out + orow * p.D + q8 * ND + i) =
+          uint2{T::pack(acc[i] * il, acc[i + 1] * il), T::pack(acc[i + 2] * il, acc[i + 3] * il)};
 }
 
 // Joins the splits of a row: O = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s. Thread: 8 dims.
@@ -327,9 +357,9 @@ extern "C" int64_t dpa_cross_attention_fwd_workspace_bytes(const DpaCrossAttenti
 template <class T, int DP>
 static void launch_fwd(const Args& p, hipStream_t s) {
   if (few_rows(p))
-    xattn_fwd_kernel<T, DP, 4><<<xcd_grid(p.total), 256, 0, s>>>(p);
+    xattn_few_kernel<T, DP><<<p.grid, 256, 0, s>>>(p);
   else
-    xattn_fwd_kernel<T, DP, 1><<<xcd_grid(p.total), 256, 0, s>>>(p);
+    xattn_fwd_kernel<T, DP><<<p.grid, 256, 0, s>>>(p);
 }
 
 template <class T>
