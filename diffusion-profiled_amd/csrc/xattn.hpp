@@ -342,6 +342,23 @@ inline void set_grid(Args& p, int64_t total, int64_t per_head) {
 // The forward's and dQ's tiles: rows of up to 32 go to the form whose waves share them
 inline bool few_rows(const Args& p) { return p.rows <= 32; }
 
+inline int dim_pad(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
+// Forms that keep a head's keys in LDS (xattn_short.hip). The backward's takes up to 96 keys of more
+// than 64 dims: its buffers for more pass a CU's LDS.
+inline bool short_keys_fwd(const Args& p) { return !few_rows(p) && p.Lk <= 128; }
+inline bool short_keys_bwd(const Args& p) { return !few_rows(p) && p.Lk <= (dim_pad(p.D) == 128 ? 96 : 128); }
+
+inline void plan_short(Args& p, int per_cu, int least) {
+  p.tiles = (int)ceil_div(p.rows, 128);
+  const int64_t groups = (int64_t)p.B * p.KVH;
+  choose_splits(p, groups, p.tiles, per_cu * num_cus(), least, 1ll << 30, 1);
+  set_grid(p, groups * p.splits, p.splits);
+}
+
+int short_fwd(const Args& p, int dtype, hipStream_t s);
+int short_bwd(const Args& p, int dtype, hipStream_t s);
+
 inline void plan_rows(Args& p) {
   const bool few = few_rows(p);
   p.tiles = few ? 1 : (int)ceil_div(p.rows, 128);
@@ -364,8 +381,6 @@ inline int64_t part_keys_bytes(const Args& p) {
   return p.splits > 1 ? (int64_t)p.splits * 2 * p.B * p.KVH * p.Lk * p.D * 4 : 0;
 }
 inline int64_t align256(int64_t n) { return (n + 255) & ~255ll; }
-
-inline int dim_pad(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 }  // namespace xattn
 }  // namespace dpa

@@ -370,12 +370,24 @@ static int64_t bwd_workspace(const Args& rows, const Args& keys) {
   return stat_bytes(rows) + (a > b ? a : b);
 }
 
+// (the most that a call with or without dk and dv needs)
 extern "C" int64_t dpa_cross_attention_bwd_workspace_bytes(const DpaCrossAttention* a) {
   if (!a || check_shape(*a) != DPA_OK) return 0;
-  Args r = make_args(*a), k = r;
+  Args r = make_args(*a), k = r, one = r;
   plan_rows(r);
   plan_keys(k);
-  return bwd_workspace(r, k);
+  const int64_t two = bwd_workspace(r, k);
+  if (!short_keys_bwd(one)) return two;
+  plan_short(one, 2, 2);
+  return two > part_keys_bytes(one) ? two : part_keys_bytes(one);
+}
+
+template <class T>
+static int sum_keys(const Args& k, hipStream_t s) {
+  if (k.splits <= 1) return DPA_OK;
+  const int64_t n = (int64_t)k.B * k.KVH * k.Lk * 2 * (k.D / 8);
+  xattn_sum_kernel<T, false><<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(k);
+  return launch_status();
 }
 
 template <class T, int DP>
@@ -396,11 +408,8 @@ static int launch_bwd(const Args& r, const Args& k, hipStream_t s) {
   }
   if (k.total > 0) {
     xattn_dkdv_kernel<T, DP><<<k.grid, 256, 0, s>>>(k);
-    int st = launch_status();
-    if (st != DPA_OK || k.splits <= 1) return st;
-    const int64_t n = (int64_t)k.B * k.KVH * k.Lk * 2 * (k.D / 8);
-    xattn_sum_kernel<T, false><<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(k);
-    return launch_status();
+    const int st = launch_status();
+    return st != DPA_OK ? st : sum_keys<T>(k, s);
   }
   return DPA_OK;
 }
@@ -430,6 +439,17 @@ extern "C" int dpa_cross_attention_bwd(const DpaCrossAttention* a, void* workspa
       !strides_ok(a->dk_stride) || !strides_ok(a->dv_stride))
     return DPA_ERR_ALIGN;
   Args r = make_args(*a), k = r;
+  hipStream_t s = (hipStream_t)stream;
+  if (short_keys_bwd(k)) {
+    plan_short(k, 2, 2);
+    const int64_t need = a->dk ? part_keys_bytes(k) : 0;
+    if (need && (!workspace || workspace_bytes < need)) return DPA_ERR_WORKSPACE;
+    if (!aligned(workspace, 16)) return DPA_ERR_ALIGN;
+    k.part = (float*)workspace;
+    const int status = short_bwd(k, a->dtype, s);
+    if (status != DPA_OK || !a->dk) return status;
+    return a->dtype == DPA_DTYPE_BF16 ? sum_keys<Bf16>(k, s) : sum_keys<F16>(k, s);
+  }
   plan_rows(r);
   plan_keys(k);
   const int64_t need = bwd_workspace(r, k);
@@ -441,6 +461,5 @@ extern "C" int dpa_cross_attention_bwd(const DpaCrossAttention* a, void* workspa
   }
   if (a->q_len == 0) r.total = 0;
   if (!a->dk) k.total = 0;
-  hipStream_t s = (hipStream_t)stream;
   return a->dtype == DPA_DTYPE_BF16 ? run_bwd<Bf16>(r, k, s) : run_bwd<F16>(r, k, s);
 }

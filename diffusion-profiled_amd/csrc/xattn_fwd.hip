@@ -350,6 +350,7 @@ static int64_t fwd_workspace(const Args& p) {
 extern "C" int64_t dpa_cross_attention_fwd_workspace_bytes(const DpaCrossAttention* a) {
   if (!a || check_shape(*a) != DPA_OK) return 0;
   Args p = make_args(*a);
+  if (short_keys_fwd(p)) return 0;
   plan_rows(p);
   return fwd_workspace(p);
 }
@@ -388,6 +389,11 @@ extern "C" int dpa_cross_attention_fwd(const DpaCrossAttention* a, void* workspa
       !strides_ok(a->k_stride) || !strides_ok(a->v_stride))
     return DPA_ERR_ALIGN;
   Args p = make_args(*a);
+  hipStream_t s = (hipStream_t)stream;
+  if (short_keys_fwd(p)) {
+    plan_short(p, 4, 1);
+    return short_fwd(p, a->dtype, s);
+  }
   plan_rows(p);
   const int64_t need = fwd_workspace(p);
   if (need) {
@@ -396,6 +402,5 @@ extern "C" int dpa_cross_attention_fwd(const DpaCrossAttention* a, void* workspa
     p.part = (float*)workspace;
     p.stat = (float2*)((uint8_t*)workspace + align256(part_rows_bytes(p)));
   }
-  hipStream_t s = (hipStream_t)stream;
   return a->dtype == DPA_DTYPE_BF16 ? run_fwd<Bf16>(p, s) : run_fwd<F16>(p, s);
 }
