@@ -54,7 +54,8 @@ struct Args {
 // alone gives 0 below 2^-126; it costs nothing. fp16 has no room for it.
 struct Bf16 {
   static constexpr int kShift = 24;
-  static __device__ __forceinline__ v16f mfma(uint4 a, uint4 b, v16f c) {
+  template <class A>
+  static __device__ __forceinline__ v16f mfma(A a, uint4 b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -65,7 +66,8 @@ struct Bf16 {
 
 struct F16 {
   static constexpr int kShift = 0;
-  static __device__ __forceinline__ v16f mfma(uint4 a, uint4 b, v16f c) {
+  template <class A>
+  static __device__ __forceinline__ v16f mfma(A a, uint4 b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -120,6 +122,76 @@ __device__ __forceinline__ uint4 frag_tr(const uint16_t* x, int r0, int db, int 
   const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(x + r2 * DP + ((g ^ swz<DP>(r2)) << 3) + half));
   const uint2 lo = __builtin_bit_cast(uint2, a), hi = __builtin_bit_cast(uint2, b);
   return uint4{lo.x, lo.y, hi.x, hi.y};
+}
+
+// The same reads with what depends on the lane in registers, made once: byte addresses in an array
+// that starts at `base` (a multiple of 1024), to which a read adds constants (another array, its
+// rows in steps of 16 or 32), which become the instruction's immediate offset. (opaque: else the
+// compiler keeps a register for every sum.)
+__device__ __forceinline__ uint32_t opaque(uint32_t x) {
+  asm("" : "+v"(x));
+  return x;
+}
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// (a vector: as a struct the load falls apart)
+__device__ __forceinline__ u32x4 lds_ld16(uint32_t a) {
+  return *(const __attribute__((address_space(3))) u32x4*)(a);
+}
+__device__ __forceinline__ void lds_st16(uint32_t a, uint4 v) {
+  *(__attribute__((address_space(3))) u32x4*)(a) = __builtin_bit_cast(u32x4, v);
+}
+__device__ __forceinline__ void lds_st8(uint32_t a, uint32_t x, uint32_t y) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  *(__attribute__((address_space(3))) u32x2*)(a) = u32x2{x, y};
+}
+
+// frag_row of row l & 31, granules 2 k + (l >> 5)
+template <int DP>
+struct RowAt {
+  uint32_t a[DP / 16];
+  __device__ __forceinline__ RowAt(int lane, uint32_t base) {
+    const int r = lane & 31;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k)
+      a[k] = opaque(base + r * DP * 2 + (((2 * k + (lane >> 5)) ^ swz<DP>(r)) << 4));
+  }
+  __device__ __forceinline__ u32x4 get(int k, uint32_t at) const { return lds_ld16(a[k] + at); }
+};
+
+// frag_tr of rows 0 .. 15, dims 32 (db0 + d) ..
+template <int DP, int ND>
+struct TrAt {
+  uint32_t a[ND][2];
+  __device__ __forceinline__ TrAt(int lane, uint32_t base, int db0 = 0, int step = 1) {
+    const int k = lane & 15, r = 4 * (lane >> 5) + (k >> 2);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int g = 4 * (db0 + step * d) + 2 * ((lane >> 4) & 1) + ((k & 3) >> 1), rr = r + 8 * x;
+        a[d][x] = opaque(base + rr * DP * 2 + ((g ^ swz<DP>(rr)) << 4) + 8 * (k & 1));
+      }
+  }
+  __device__ __forceinline__ uint4 get(int d, uint32_t at) const {
+    typedef v4s __attribute__((address_space(3))) * LP;
+    const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(a[d][0] + at));
+    const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(a[d][1] + at));
+    const uint2 lo = __builtin_bit_cast(uint2, x), hi = __builtin_bit_cast(uint2, y);
+    return uint4{lo.x, lo.y, hi.x, hi.y};
+  }
+};
+
+// start_from of 32 floats at byte address at (with the lane's 16 h in it)
+__device__ __forceinline__ v16f start_at(uint32_t at) {
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  v16f s;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const f32x4 v = *(const __attribute__((address_space(3))) f32x4*)(at + 32 * x);
+    s[4 * x] = v.x, s[4 * x + 1] = v.y, s[4 * x + 2] = v.z, s[4 * x + 3] = v.w;
+  }
+  return s;
 }
 
 static __device__ __attribute__((aligned(64))) uint32_t g_zero16[4];
@@ -203,13 +275,14 @@ __device__ __forceinline__ void fetch_keys(const Args& p, const uint16_t* kb, co
   }
 }
 
-// The B operands of a row of queries (or of their gradient)
+// The B operands of a row of queries (or of their gradient). Lanes without one load zeros: a branch
+// around each load would keep the loads from going out together.
 template <int KS>
 __device__ __forceinline__ void load_row(uint4 (&f)[KS], const uint16_t* src, bool on, int h, int D) {
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
-    f[ks] = uint4{0u, 0u, 0u, 0u};
-    if (on && 16 * ks + 8 * h < D) f[ks] = ld16(src + 16 * ks + 8 * h);
+    const int dim = 16 * ks + 8 * h;
+    f[ks] = *static_cast<const uint4*>(on && dim < D ? static_cast<const void*>(src + dim) : g_zero16);
   }
 }
 

@@ -2,6 +2,8 @@
 // keys in LDS and walks over its query rows, so that a row's scores are all in registers at once.
 // The forward needs no running maximum; the backward forms D = rowsum(P dP) from its own fp32 P and
 // dP (it reads no output of the forward but lse) and all three gradients in one pass over q and dO.
+#include <type_traits>
+
 #include "xattn.hpp"
 
 namespace dpa {
@@ -10,7 +12,7 @@ namespace xattn {
 // Brings the head's keys and values to kl and vl (rows of NB x 32 keys) and its bias (0: visible,
 // -inf: not) and gives which blocks of 32 keys have a visible one. Ends with a barrier.
 template <int DP, int NB>
-__device__ __forceinline__ uint32_t resident_keys(const Args& p, int b, int g, uint16_t* kl, uint16_t* vl,
+__device__ __forceinline__ uint32_t resident_keys(const Args& p, int b, int g, uint32_t kl, uint32_t vl,
                                                   float* bias, int tid, int wave, int lane) {
   constexpr int NG = DP / 8;
   const int klen = keys_of(p, b);
@@ -20,10 +22,10 @@ __device__ __forceinline__ uint32_t resident_keys(const Args& p, int b, int g, u
   const uint16_t* vb = p.v + b * p.vs.b + g * p.vs.h;
   for (int c0 = wave * 64; c0 < NB * 32 * NG; c0 += 256) {
     const bool vis = visible((c0 + lane) / NG);
-    dma_rows<DP>(LDS_ADDR(kl), c0, lane, p.D, [&](int row) __attribute__((always_inline)) {
+    dma_rows<DP>(kl, c0, lane, p.D, [&](int row) __attribute__((always_inline)) {
       return vis ? kb + row * p.ks.l : static_cast<const uint16_t*>(nullptr);
     });
-    dma_rows<DP>(LDS_ADDR(vl), c0, lane, p.D, [&](int row) __attribute__((always_inline)) {
+    dma_rows<DP>(vl, c0, lane, p.D, [&](int row) __attribute__((always_inline)) {
       return vis ? vb + row * p.vs.l : static_cast<const uint16_t*>(nullptr);
     });
   }
@@ -44,8 +46,10 @@ __device__ __forceinline__ uint32_t resident_keys(const Args& p, int b, int g, u
 template <class T, int DP, int NB>
 __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_short_fwd_kernel(const Args p) {
   constexpr int KS = DP / 16, NDB = DP / 32;
-  __shared__ __attribute__((aligned(1024))) uint16_t kv[2][NB * 32 * DP];
-  __shared__ __attribute__((aligned(16))) float bias[NB * 32];
+  constexpr uint32_t kBlock = 32 * DP * 2, kV = NB * kBlock, kBias = 2 * kV;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kBias + NB * 128];
+  const uint32_t l0 = LDS_ADDR(lds);
+  float* bias = reinterpret_cast<float*>(lds + kBias);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -66,7 +70,10 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_s
   };
   uint4 qf[KS];
   load(t_lo, qf);
-  const uint32_t act = resident_keys<DP, NB>(p, b, g, kv[0], kv[1], bias, tid, wave, lane);
+  const uint32_t act = resident_keys<DP, NB>(p, b, g, l0, l0 + kV, bias, tid, wave, lane);
+  const RowAt<DP> row_at(lane, l0);
+  const TrAt<DP, NDB> tr_at(lane, l0);
+  const uint32_t bias_at = opaque(l0 + kBias + 16 * h);
 
   for (int t = t_lo; t < t_hi; ++t) {
     v16f s[NB];
@@ -74,9 +81,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_s
 #pragma unroll
     for (int i = 0; i < NB; ++i)
       if ((act >> i) & 1) {
-        s[i] = start_from(bias + 32 * i, h);
+        s[i] = start_at(bias_at + 128 * i);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) s[i] = T::mfma(frag_row<DP>(kv[0], 32 * i + col, 2 * k + h), qf[k], s[i]);
+        for (int k = 0; k < KS; ++k) s[i] = T::mfma(row_at.get(k, kBlock * i), qf[k], s[i]);
 #pragma unroll
         for (int r = 0; r < 16; ++r) m = fmaxf(m, s[i][r]);
       }
@@ -103,7 +110,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_s
           const uint4 pf = {pk[0], pk[1], pk[2], pk[3]};
 #pragma unroll
           for (int d = 0; d < NDB; ++d)
-            o[d] = T::mfma(frag_tr<DP>(kv[1], 32 * i + 16 * s2, d, lane), pf, o[d]);
+            o[d] = T::mfma(tr_at.get(d, kV + kBlock * i + kBlock / 2 * s2), pf, o[d]);
         }
       }
     l = sum_halves(l);
@@ -129,10 +136,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_short_bwd_kernel
   constexpr int KS = DP / 16, NDB = DP / 32;
   constexpr int NT = DP == 128 ? 2 : 1;  // tiles of a wave per block
   constexpr float kUnshift = 1.f / (1 << T::kShift);
-  __shared__ __attribute__((aligned(1024))) uint16_t kv[2][NB * 32 * DP];
-  __shared__ __attribute__((aligned(1024))) uint16_t qg[2][128 * DP];  // Q, dO
-  __shared__ __attribute__((aligned(1024))) uint16_t ps[2][128 * 32];  // dS, P of a block
-  __shared__ __attribute__((aligned(16))) float bias[NB * 32];
+  // LDS: keys, values, their bias; dS and P of a block (rows of 32 keys); Q and dO of the tile
+  constexpr uint32_t kBlock = 32 * DP * 2, kV = NB * kBlock, kBias = 2 * kV, kPS = kBias + 1024;
+  constexpr uint32_t kQG = kPS + 2 * 128 * 64, kTile = 128 * DP * 2;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kKeys ? kQG + 2 * kTile : kPS];
+  const uint32_t l0 = LDS_ADDR(lds);
+  float* bias = reinterpret_cast<float*>(lds + kBias);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -159,7 +168,10 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_short_bwd_kernel
     if (on) lse = lb[row];
   };
   load(t_lo);
-  const uint32_t act = resident_keys<DP, NB>(p, b, g, kv[0], kv[1], bias, tid, wave, lane);
+  const uint32_t act = resident_keys<DP, NB>(p, b, g, l0, l0 + kV, bias, tid, wave, lane);
+  const RowAt<DP> row_at(lane, l0);
+  const TrAt<DP, NDB> tr_at(lane, l0);
+  const uint32_t bias_at = opaque(l0 + kBias + 16 * h);
 
   // this wave's tiles: of dK (mat 0) or dV, dims 32 (db0 + 2 j); with one block of dims, rows
   // 64 part .. 64 part + 63 of each tile
@@ -172,93 +184,105 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_short_bwd_kernel
     for (int j = 0; j < NT; ++j) acc[i][j] = zero16();
 
   const int mine = wave * 32 + col;  // row of the tile
-  for (int t = t_lo; t < t_hi; ++t) {
+  const uint32_t my_rows = kQG + wave * kBlock;
+  uint32_t ps_at[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) ps_at[x] = opaque(l0 + kPS + wave * 2048 + col * 64 + ((x ^ swz<32>(col)) << 4) + 8 * h);
+  const TrAt<32, 1> ps_tr(lane, l0 + kPS + mat * 8192 + part * 4096);
+  const TrAt<DP, NT> qg_tr(lane, l0 + kQG + mat * kTile + part * 2 * kBlock, db0, 2);
+  // one tile over the first N blocks of keys
+  auto tile = [&](int t, auto blocks) __attribute__((always_inline)) {
+    constexpr int N = decltype(blocks)::value;
     v16f dq[NDB];
 #pragma unroll
     for (int d = 0; d < NDB; ++d) dq[d] = zero16();
-    if (act) {
+    if constexpr (N == 0) {
+      load(t + 1);
+    } else {
 #pragma unroll
       for (int k = 0; kKeys && k < KS; ++k) {  // (every wave is past its reads of the last tile)
-        const int at = mine * DP + (((2 * k + h) ^ swz<DP>(mine)) << 3);
-        *reinterpret_cast<uint4*>(&qg[0][at]) = qf[k];
-        *reinterpret_cast<uint4*>(&qg[1][at]) = gf[k];
+        lds_st16(row_at.a[k] + my_rows, qf[k]);
+        lds_st16(row_at.a[k] + my_rows + kTile, gf[k]);
       }
       const float nlse2 = lse == -__builtin_inff() ? -__builtin_inff() : (float)T::kShift - lse * kLog2e;
-      v16f s[NB], dp[NB];  // (s: then P)
+      v16f s[N], dp[N];  // (s: then P)
       float nd = 0.f;
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
-        {
-          s[i] = start_from(bias + 32 * i, h);
-          dp[i] = zero16();
+      for (int i = 0; i < N; ++i) {
+        s[i] = start_at(bias_at + 128 * i);
+        dp[i] = zero16();
 #pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            s[i] = T::mfma(frag_row<DP>(kv[0], 32 * i + col, 2 * k + h), qf[k], s[i]);
-            dp[i] = T::mfma(frag_row<DP>(kv[1], 32 * i + col, 2 * k + h), gf[k], dp[i]);
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            s[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], p.c2, nlse2));
-            nd = __builtin_fmaf(-s[i][r], dp[i][r], nd);
-          }
-          __builtin_amdgcn_sched_barrier(0);
+        for (int k = 0; k < KS; ++k) {
+          s[i] = T::mfma(row_at.get(k, kBlock * i), qf[k], s[i]);
+          dp[i] = T::mfma(row_at.get(k, kV + kBlock * i), gf[k], dp[i]);
         }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], p.c2, nlse2));
+          nd = __builtin_fmaf(-s[i][r], dp[i][r], nd);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (DP == 32) load(t + 1);
       nd = sum_halves(nd) * kUnshift;
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
-        {
+      for (int i = 0; i < N; ++i) {
 #pragma unroll
-          for (int s2 = 0; s2 < 2; ++s2) {
-            uint32_t pw[4], sw[4];
+        for (int s2 = 0; s2 < 2; ++s2) {
+          uint32_t pw[4], sw[4];
 #pragma unroll
-            for (int r = 0; r < 8; r += 2) {
-              const float p0 = s[i][8 * s2 + r], p1 = s[i][8 * s2 + r + 1];
-              pw[r / 2] = T::pack(p0, p1);
-              sw[r / 2] = T::pack(p0 * (dp[i][8 * s2 + r] + nd), p1 * (dp[i][8 * s2 + r + 1] + nd));
-            }
-#pragma unroll
-            for (int x = 0; kKeys && x < 2; ++x) {
-              const int at = mine * 32 + (((2 * s2 + x) ^ swz<32>(mine)) << 3) + 4 * h;
-              *reinterpret_cast<uint2*>(&ps[0][at]) = uint2{sw[2 * x], sw[2 * x + 1]};
-              *reinterpret_cast<uint2*>(&ps[1][at]) = uint2{pw[2 * x], pw[2 * x + 1]};
-            }
-            const uint4 sf = {sw[0], sw[1], sw[2], sw[3]};
-#pragma unroll
-            for (int d = 0; d < NDB; ++d)
-              dq[d] = T::mfma(frag_tr<DP>(kv[0], 32 * i + 16 * s2, d, lane), sf, dq[d]);
+          for (int r = 0; r < 8; r += 2) {
+            const float p0 = s[i][8 * s2 + r], p1 = s[i][8 * s2 + r + 1];
+            pw[r / 2] = T::pack(p0, p1);
+            sw[r / 2] = T::pack(p0 * (dp[i][8 * s2 + r] + nd), p1 * (dp[i][8 * s2 + r + 1] + nd));
           }
-          if constexpr (kKeys) {
-            wait_lgkmcnt0();
-            lds_barrier();  // the block's P and dS (and the tile's Q and dO) are there
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-              const int r0 = 64 * part + 16 * k;
-              const uint4 x = frag_tr<32>(ps[mat], r0, 0, lane);
-#pragma unroll
-              for (int j = 0; j < NT; ++j)
-                acc[i][j] = T::mfma(frag_tr<DP>(qg[mat], r0, db0 + 2 * j, lane), x, acc[i][j]);
-            }
-            wait_lgkmcnt0();
-            lds_barrier();  // and read
+          for (int x = 0; kKeys && x < 2; ++x) {
+            const uint32_t at = ps_at[2 * s2 + x];
+            lds_st8(at, sw[2 * x], sw[2 * x + 1]);
+            lds_st8(at + 8192, pw[2 * x], pw[2 * x + 1]);
           }
-          if (i == 0) load(t + 1);  // (no sooner: the registers that they need are the scores')
+          const uint4 sf = {sw[0], sw[1], sw[2], sw[3]};
+#pragma unroll
+          for (int d = 0; d < NDB; ++d) dq[d] = T::mfma(tr_at.get(d, kBlock * i + kBlock / 2 * s2), sf, dq[d]);
         }
-    } else {
-      load(t + 1);
+        if constexpr (kKeys) {
+          wait_lgkmcnt0();
+          lds_barrier();  // the block's P and dS (and the tile's Q and dO) are there
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) {
+            const uint4 x = ps_tr.get(0, 1024 * k);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = T::mfma(qg_tr.get(j, kBlock / 2 * k), x, acc[i][j]);
+          }
+          wait_lgkmcnt0();
+          lds_barrier();  // and read
+        }
+        if (DP != 32 && i == 0) load(t + 1);  // (no sooner: the registers that they need are the scores')
+      }
     }
     const int row = t * 128 + mine;
     const bool on = row < p.rows;
     const uint32_t hg = fdiv(on ? row : 0, p.by_lq), tok = (on ? row : 0) - hg * p.Lq;
     store_row<T>(p.dq + (((int64_t)b * p.Lq + tok) * p.H + g * p.G + hg) * p.D, on, dq, p.scale * kUnshift, h, p.D);
-  }
+  };
+  // (a loop for each number of blocks up to the last with a visible key)
+  auto walk = [&](auto blocks) __attribute__((always_inline)) {
+    for (int t = t_lo; t < t_hi; ++t) tile(t, blocks);
+  };
+  if (act >= 1u << (NB - 1)) walk(std::integral_constant<int, NB>());
+  else if (NB == 4 && act >= 4) walk(std::integral_constant<int, 3>());
+  else if (act >= 2) walk(std::integral_constant<int, 2>());
+  else if (act) walk(std::integral_constant<int, 1>());
+  else walk(std::integral_constant<int, 0>());
 
   if constexpr (!kKeys) return;
   const int64_t n = (int64_t)p.B * p.KVH * p.Lk;
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
     if constexpr (DP == 32) {  // the two halves of the rows
-      float* x = reinterpret_cast<float*>(&qg[0][0]) + mat * 1024 + lane;
-      static_assert(DP != 32 || sizeof(qg) >= 2 * 1024 * 4, "the tiles fit");
+      float* x = reinterpret_cast<float*>(lds + kQG) + mat * 1024 + lane;
+      static_assert(2 * kTile >= 2 * 1024 * 4, "the tiles fit");
       __syncthreads();
       if (part)
 #pragma unroll
