@@ -208,6 +208,11 @@ __device__ __forceinline__ void dma_rows(uint32_t lds, int c0, int lane, int D, 
   dma16_lds(a, lds + (uint32_t)c0 * 16);
 }
 
+// 16 B per lane from base (wave-uniform) + off bytes
+__device__ __forceinline__ void dma16_lds_from(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "m0");
+}
+
 // 4 B per lane to lds + 4 * lane (lds wave-uniform).
 __device__ __forceinline__ void dma4_lds(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "m0");
@@ -255,6 +260,71 @@ __device__ __forceinline__ int keys_of(const Args& p, int b) {
   const int n = p.klen[b];
   return n < 0 ? 0 : n < p.Lk ? n : p.Lk;
 }
+
+// Tiles of 64 keys and values that a workgroup of four waves brings to LDS (rows arrays of 64 x DP:
+// keys at l0 + buf * 2 kBytes, values kBytes behind). Tiles whose 64 keys are all below the length
+// go by one instruction per transfer, its lane part a constant offset; then their rows that the mask
+// hides are cleared in LDS (ready(), once the tile has landed). The others, heads that are not DP
+// wide and rows that are far apart choose an address per row.
+template <int DP>
+struct KeyTiles {
+  static constexpr int NG = DP / 8, kXfer = 64 * NG / 256;
+  static constexpr uint32_t kBytes = 64 * DP * 2;
+  const uint16_t *kb, *vb;  // key 0 of the head
+  int64_t kl, vl;
+  uint32_t ko[kXfer], vo[kXfer], l0;
+  int lane, wave, klen, D;
+  bool fast;
+
+  __device__ __forceinline__ KeyTiles(const Args& p, int b, int g, int klen_, uint32_t lds, int wave_, int lane_)
+      : kb(p.k + b * p.ks.b + g * p.ks.h), vb(p.v + b * p.vs.b + g * p.vs.h), kl(p.ks.l), vl(p.vs.l),
+        l0(lds), lane(lane_), wave(wave_), klen(klen_), D(p.D) {
+    fast = D == DP && kl >= 0 && vl >= 0 && kl < (1 << 24) && vl < (1 << 24);
+#pragma unroll
+    for (int r = 0; r < kXfer; ++r) {
+      const int c = wave * 64 + 256 * r + lane, row = c / NG, g8 = ((c % NG) ^ swz<DP>(row)) << 3;
+      ko[r] = (uint32_t)(row * (int)kl + g8) * 2;
+      vo[r] = (uint32_t)(row * (int)vl + g8) * 2;
+    }
+  }
+  __device__ __forceinline__ bool whole(int t) const { return fast && t * 64 + 64 <= klen; }
+
+  __device__ __forceinline__ void fetch(int t, int buf, uint64_t word) const {
+    const uint16_t *kt = kb + (int64_t)t * 64 * kl, *vt = vb + (int64_t)t * 64 * vl;
+    const uint32_t at = l0 + buf * 2 * kBytes + wave * 1024;
+    if (whole(t)) {
+#pragma unroll
+      for (int r = 0; r < kXfer; ++r) {
+        dma16_lds_from(kt, ko[r], at + 4096 * r);
+        dma16_lds_from(vt, vo[r], at + kBytes + 4096 * r);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < kXfer; ++r) {
+        const int c0 = wave * 64 + 256 * r;
+        dma_rows<DP>(l0 + buf * 2 * kBytes, c0, lane, D, [&](int row) __attribute__((always_inline)) {
+          return (word >> row) & 1 ? kt + row * kl : static_cast<const uint16_t*>(nullptr);
+        });
+        dma_rows<DP>(l0 + buf * 2 * kBytes + kBytes, c0, lane, D, [&](int row) __attribute__((always_inline)) {
+          return (word >> row) & 1 ? vt + row * vl : static_cast<const uint16_t*>(nullptr);
+        });
+      }
+    }
+  }
+  // (before the barrier behind which tile t is read)
+  __device__ __forceinline__ void ready(int t, int buf, uint64_t word) const {
+    if (word == ~0ull || !whole(t)) return;
+    const uint32_t at = l0 + buf * 2 * kBytes + wave * 1024 + lane * 16;
+#pragma unroll
+    for (int r = 0; r < kXfer; ++r) {
+      const int row = (wave * 64 + 256 * r + lane) / NG;
+      if (!((word >> row) & 1)) {
+        lds_st16(at + 4096 * r, uint4{0u, 0u, 0u, 0u});
+        lds_st16(at + kBytes + 4096 * r, uint4{0u, 0u, 0u, 0u});
+      }
+    }
+  }
+};
 
 // A wave's kXfer transfers each of the tiles of keys and values from key k0 on into kl and vl,
 // chunks c0, c0 + kStep, ...; keys whose bit in word is 0 come as zeros.
@@ -440,10 +510,15 @@ inline void plan_rows(Args& p) {
   set_grid(p, groups * p.splits, (int64_t)p.tiles * p.splits);
 }
 
+constexpr int kQT = 64;  // rows of a tile of the kernel of dK and dV
+
+// Its workgroups take 128 keys, or 64 where that leaves less than four to a CU
+inline bool few_keys(const Args& p) { return (int64_t)p.B * p.KVH * ceil_div(p.Lk, 128) < 4 * num_cus(); }
+
 inline void plan_keys(Args& p) {
-  p.tiles = (int)ceil_div(p.Lk, 128);
+  p.tiles = (int)ceil_div(p.Lk, few_keys(p) ? 64 : 128);
   const int64_t groups = (int64_t)p.B * p.KVH * p.tiles;
-  choose_splits(p, groups, ceil_div(p.rows, 64), 2 * num_cus(), 4, 1ll << 30, 1);
+  choose_splits(p, groups, ceil_div(p.rows, kQT), 2 * num_cus(), 4, 1ll << 30, 1);
   set_grid(p, groups * p.splits, (int64_t)p.tiles * p.splits);
 }
 

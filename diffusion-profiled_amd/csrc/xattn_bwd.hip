@@ -3,6 +3,8 @@
 // Two kernels, each recomputing S and dP, so that every gradient has one writer and a fixed order
 // of sums: one of query rows (dQ, and D for the other), one of keys (dK, dV, summed over the query
 // heads that share them).
+#include <type_traits>
+
 #include "xattn.hpp"
 
 namespace dpa {
@@ -12,64 +14,25 @@ namespace xattn {
 // dQ: the forward's tiles and layouts (S^T = K Q^T, dP^T = V dO^T: a query per lane column), then
 // dQ^T += K^T dS^T from transpose reads of the key rows. The product for dP^T starts from -D, as the
 // one for S^T from the keys' bias, so that dS = P (dP - D) is one multiplication.
-// WK = 1: four waves of 32 query rows each share tiles of 64 keys. WK = 4, for up to 32 rows: the
-// four waves share them and take every fourth tile of 32 keys each.
 // ---------------------------------------------------------------------------------------
-template <class T, int DP, int WK>
-__global__ __launch_bounds__(256, WK == 4 ? 1 : DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_dq_kernel(const Args p) {
-  constexpr int KT = WK == 1 ? 64 : 32, NKB = KT / 32;
-  constexpr int NG = DP / 8, KS = DP / 16, NDB = DP / 32;
-  constexpr float kUnshift = 1.f / (1 << T::kShift);
-  constexpr int kStep = WK == 1 ? 256 : 64;
-  constexpr int kXfer = KT * NG / kStep;
-  __shared__ __attribute__((aligned(1024))) uint16_t kv[WK][2][2][KT * DP];
-  __shared__ __attribute__((aligned(16))) float bias[WK][2][KT];
-  __shared__ uint32_t seen[kMaxRange / 32];
 
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 31, h = lane >> 5;
-  const uint32_t id = work_item(p);
-  if (id >= p.total) return;
-  const int split = id % (uint32_t)p.splits;
-  const uint32_t bt = id / (uint32_t)p.splits;
-  const int tile = bt % (uint32_t)p.tiles;
-  const int bkv = bt / (uint32_t)p.tiles;
-  const int b = bkv / p.KVH, g = bkv - b * p.KVH;
-
-  const int klen = keys_of(p, b);
-  const int nt = (klen + KT - 1) / KT;
-  const int t_lo = split * p.per_split + (WK == 1 ? 0 : wave);
-  const int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
-  const uint16_t* kb = p.k + b * p.ks.b + g * p.ks.h;
-  const uint16_t* vb = p.v + b * p.vs.b + g * p.vs.h;
-  const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
-
-  const int own = WK == 1 ? 0 : wave;  // the buffers
-  auto fetch = [&](int t, int buf, uint64_t word) __attribute__((always_inline)) {
-    fetch_keys<DP, kXfer, kStep>(p, kb, vb, (int64_t)t * KT, word, kv[own][buf][0], kv[own][buf][1],
-                                 WK == 1 ? wave * 64 : 0, lane);
-    if (WK == 1 ? wave == 0 : h == 0)
-      bias[own][buf][WK == 1 ? lane : col] = (word >> (WK == 1 ? lane : col)) & 1 ? 0.f : -__builtin_inff();
-  };
-  uint64_t word = 0;
-  if (t_lo < t_hi) {
-    word = bits.template word<KT>(t_lo);
-    fetch(t_lo, 0, word);
-  }
-
-  const int row = (WK == 1 ? tile * 128 + wave * 32 : 0) + col;
-  const bool has_row = row < p.rows;
-  const uint32_t hg = fdiv(has_row ? row : 0, p.by_lq), tok = (has_row ? row : 0) - hg * p.Lq;
-  const int head = g * p.G + hg;
-  const int64_t orow = ((int64_t)b * p.Lq + tok) * p.H + head;
+// What the kernels of dQ keep of a lane's query row: q and dO as B operands, kShift - lse in base 2
+// and -D, which they leave for the kernel of dK and dV (leave: this wave does).
+template <class T, int KS>
+struct QueryRow {
   uint4 qf[KS], gf[KS];
-  float nlse2 = -__builtin_inff(), nd = 0.f;
-  {
+  float nlse2, nd;
+  int64_t orow;
+  __device__ __forceinline__ QueryRow(const Args& p, int b, int g, int bkv, int row, bool leave, int h) {
+    const bool on = row < p.rows;
+    const uint32_t hg = fdiv(on ? row : 0, p.by_lq), tok = (on ? row : 0) - hg * p.Lq;
+    const int head = g * p.G + hg;
+    orow = ((int64_t)b * p.Lq + tok) * p.H + head;
     uint4 of[KS];
-    load_row<KS>(qf, p.q + b * p.qs.b + (int64_t)tok * p.qs.l + head * p.qs.h, has_row, h, p.D);
-    load_row<KS>(gf, p.dout + b * p.gs.b + (int64_t)tok * p.gs.l + head * p.gs.h, has_row, h, p.D);
-    load_row<KS>(of, p.out + orow * p.D, has_row, h, p.D);
+    load_row<KS>(qf, p.q + b * p.qs.b + (int64_t)tok * p.qs.l + head * p.qs.h, on, h, p.D);
+    load_row<KS>(gf, p.dout + b * p.gs.b + (int64_t)tok * p.gs.l + head * p.gs.h, on, h, p.D);
+    load_row<KS>(of, p.out + orow * p.D, on, h, p.D);
+    nlse2 = -__builtin_inff(), nd = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const uint32_t gw[4] = {gf[ks].x, gf[ks].y, gf[ks].z, gf[ks].w};
@@ -80,70 +43,200 @@ __global__ __launch_bounds__(256, WK == 4 ? 1 : DP == 128 ? 2 : DP == 64 ? 3 : 4
         nd = __builtin_fmaf(-T::hi(gw[i]), T::hi(ow[i]), nd);
       }
     }
-    if (has_row) {
+    if (on) {
       const float e = p.lse[((int64_t)b * p.H + head) * p.Lq + tok];
       nlse2 = e == -__builtin_inff() ? -__builtin_inff() : (float)T::kShift - e * kLog2e;
     }
     nd = sum_halves(nd);
-    if (has_row && split == 0 && h == 0 && (WK == 1 || wave == 0)) {
+    if (on && leave && h == 0) {
       const int64_t all = (int64_t)p.B * p.KVH * p.rows, at = (int64_t)bkv * p.rows + row;
       p.row_stat[at] = nlse2;
       p.row_stat[all + at] = nd;
     }
   }
+};
+
+// More than 32 rows: four waves of 32 query rows each share tiles of 64 keys.
+template <class T, int DP>
+__global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_dq_kernel(const Args p) {
+  constexpr int KT = 64;
+  constexpr int KS = DP / 16, NDB = DP / 32;
+  constexpr float kUnshift = 1.f / (1 << T::kShift);
+  constexpr uint32_t kBytes = KT * DP * 2, kBias = 4 * kBytes;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kBias + 2 * KT * 4];
+  __shared__ uint32_t seen[kMaxRange / 32];
+  const uint32_t l0 = LDS_ADDR(lds);
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, h = lane >> 5;
+  const uint32_t id = work_item(p);
+  if (id >= p.total) return;
+  const int split = id % (uint32_t)p.splits;
+  const uint32_t bt = id / (uint32_t)p.splits;
+  const int tile = bt % (uint32_t)p.tiles;
+  const int bkv = bt / (uint32_t)p.tiles;
+  const int b = bkv / p.KVH, g = bkv - b * p.KVH;
+
+  const int klen = __builtin_amdgcn_readfirstlane(keys_of(p, b));
+  const int nt = (klen + KT - 1) / KT;
+  const int t_lo = split * p.per_split;
+  const int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
+  const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
+  const KeyTiles<DP> keys(p, b, g, klen, l0, wave, lane);
+  auto fetch = [&](int t, int buf, uint64_t word) __attribute__((always_inline)) {
+    keys.fetch(t, buf, word);
+    if (wave == 0)
+      *reinterpret_cast<float*>(lds + kBias + buf * KT * 4 + lane * 4) = (word >> lane) & 1 ? 0.f : -__builtin_inff();
+  };
+  uint64_t word = 0;
+  if (t_lo < t_hi) {
+    word = bits.template word<KT>(t_lo);
+    fetch(t_lo, 0, word);
+  }
+
+  const int row = tile * 128 + wave * 32 + col;
+  const QueryRow<T, KS> q(p, b, g, bkv, row, split == 0, h);
+  const RowAt<DP> row_at(lane, l0);
+  const TrAt<DP, NDB> tr_at(lane, l0);
+  const uint32_t bias_at = opaque(l0 + kBias + 16 * h);
   wait_vmcnt<0>();
 
   v16f dq[NDB], nd16;
 #pragma unroll
   for (int i = 0; i < NDB; ++i) dq[i] = zero16();
 #pragma unroll
-  for (int r = 0; r < 16; ++r) nd16[r] = nd;
+  for (int r = 0; r < 16; ++r) nd16[r] = q.nd;
 
-  for (int t = t_lo, buf = 0; t < t_hi; t += WK, buf ^= 1) {
+  auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buffer)::value;
     uint64_t word_next = 0;
-    if (WK == 1) {
-      wait_vmcnt<0>();
-      wait_lgkmcnt0();
-      lds_barrier();
-      if (t + WK < t_hi) {
-        word_next = bits.template word<KT>(t + WK);
-        fetch(t + WK, buf ^ 1, word_next);
-      }
-    } else {
-      wait_lgkmcnt0();
-      asm volatile("" ::: "memory");
-      if (t + WK < t_hi) {
-        word_next = bits.template word<KT>(t + WK);
-        fetch(t + WK, buf ^ 1, word_next);
-        wait_vmcnt<2 * kXfer>();
-      } else {
-        wait_vmcnt<0>();
-      }
-      asm volatile("" ::: "memory");
+    wait_vmcnt<0>();
+    keys.ready(t, buf, word);
+    wait_lgkmcnt0();
+    lds_barrier();
+    if (t + 1 < t_hi) {
+      word_next = bits.template word<KT>(t + 1);
+      fetch(t + 1, buf ^ 1, word_next);
     }
-    const uint16_t *kr = kv[own][buf][0], *vr = kv[own][buf][1];
 #pragma unroll
-    for (int i = 0; i < NKB; ++i) {
+    for (int i = 0; i < 2; ++i) {
       if (!(uint32_t)(word >> (32 * i))) continue;
-      v16f s = start_from(bias[own][buf] + 32 * i, h), dp = nd16;
+      constexpr uint32_t at = buf * 2 * kBytes;
+      v16f s = start_at(bias_at + buf * KT * 4 + 128 * i), dp = nd16;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        s = T::mfma(frag_row<DP>(kr, 32 * i + col, 2 * k + h), qf[k], s);
-        dp = T::mfma(frag_row<DP>(vr, 32 * i + col, 2 * k + h), gf[k], dp);
+        s = T::mfma(row_at.get(k, at + kBytes / 2 * i), q.qf[k], s);
+        dp = T::mfma(row_at.get(k, at + kBytes + kBytes / 2 * i), q.gf[k], dp);
       }
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         uint32_t sw[4];
 #pragma unroll
         for (int r = 8 * s2; r < 8 * s2 + 8; r += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, nlse2));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, nlse2));
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, q.nlse2));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, q.nlse2));
           sw[(r & 7) / 2] = T::pack(p0 * dp[r], p1 * dp[r + 1]);
         }
         const uint4 sf = {sw[0], sw[1], sw[2], sw[3]};
 #pragma unroll
-        for (int d = 0; d < NDB; ++d)
-          dq[d] = T::mfma(frag_tr<DP>(kr, 32 * i + 16 * s2, d, lane), sf, dq[d]);
+        for (int d = 0; d < NDB; ++d) dq[d] = T::mfma(tr_at.get(d, at + kBytes / 2 * i + kBytes / 4 * s2), sf, dq[d]);
+      }
+    }
+    word = word_next;
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  for (int t = t_lo; t < t_hi; t += 2) {
+    step(t, std::integral_constant<int, 0>());
+    if (t + 1 < t_hi) step(t + 1, std::integral_constant<int, 1>());
+  }
+
+  const bool has_row = row < p.rows;
+  if (p.splits > 1) {
+    if (has_row) store_part(p.part + (((int64_t)split * p.B * p.KVH + bkv) * p.rows + row) * p.D, dq, h, p.D);
+    return;
+  }
+  store_row<T>(p.dq + q.orow * p.D, has_row, dq, p.scale * kUnshift, h, p.D);
+}
+
+// Up to 32 rows: the four waves share them and take every fourth tile of 32 keys each.
+template <class T, int DP>
+__global__ __launch_bounds__(256, 1) void xattn_dq_few_kernel(const Args p) {
+  constexpr int KT = 32;
+  constexpr int NG = DP / 8, KS = DP / 16, NDB = DP / 32;
+  constexpr float kUnshift = 1.f / (1 << T::kShift);
+  constexpr int kXfer = KT * NG / 64;
+  __shared__ __attribute__((aligned(1024))) uint16_t kv[4][2][2][KT * DP];
+  __shared__ __attribute__((aligned(16))) float bias[4][2][KT];
+  __shared__ uint32_t seen[kMaxRange / 32];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, h = lane >> 5;
+  const uint32_t id = work_item(p);
+  if (id >= p.total) return;
+  const int split = id % (uint32_t)p.splits;
+  const int bkv = id / (uint32_t)p.splits;
+  const int b = bkv / p.KVH, g = bkv - b * p.KVH;
+
+  const int klen = keys_of(p, b);
+  const int nt = (klen + KT - 1) / KT;
+  const int t_lo = split * p.per_split + wave;
+  const int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
+  const uint16_t* kb = p.k + b * p.ks.b + g * p.ks.h;
+  const uint16_t* vb = p.v + b * p.vs.b + g * p.vs.h;
+  const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
+  auto fetch = [&](int t, int buf, uint32_t word) __attribute__((always_inline)) {
+    fetch_keys<DP, kXfer, 64>(p, kb, vb, (int64_t)t * KT, word, kv[wave][buf][0], kv[wave][buf][1], 0, lane);
+    if (h == 0) bias[wave][buf][col] = (word >> col) & 1 ? 0.f : -__builtin_inff();
+  };
+  uint32_t word = 0;
+  if (t_lo < t_hi) {
+    word = (uint32_t)bits.template word<KT>(t_lo);
+    fetch(t_lo, 0, word);
+  }
+  const int row = col;
+  const QueryRow<T, KS> q(p, b, g, bkv, row, split == 0 && wave == 0, h);
+  wait_vmcnt<0>();
+
+  v16f dq[NDB], nd16;
+#pragma unroll
+  for (int i = 0; i < NDB; ++i) dq[i] = zero16();
+#pragma unroll
+  for (int r = 0; r < 16; ++r) nd16[r] = q.nd;
+
+  for (int t = t_lo, buf = 0; t < t_hi; t += 4, buf ^= 1) {
+    uint32_t word_next = 0;
+    wait_lgkmcnt0();
+    asm volatile("" ::: "memory");
+    if (t + 4 < t_hi) {
+      word_next = (uint32_t)bits.template word<KT>(t + 4);
+      fetch(t + 4, buf ^ 1, word_next);
+      wait_vmcnt<2 * kXfer>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    asm volatile("" ::: "memory");
+    if (word) {
+      const uint16_t *kr = kv[wave][buf][0], *vr = kv[wave][buf][1];
+      v16f s = start_from(bias[wave][buf], h), dp = nd16;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        s = T::mfma(frag_row<DP>(kr, col, 2 * k + h), q.qf[k], s);
+        dp = T::mfma(frag_row<DP>(vr, col, 2 * k + h), q.gf[k], dp);
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        uint32_t sw[4];
+#pragma unroll
+        for (int r = 8 * s2; r < 8 * s2 + 8; r += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, q.nlse2));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, q.nlse2));
+          sw[(r & 7) / 2] = T::pack(p0 * dp[r], p1 * dp[r + 1]);
+        }
+        const uint4 sf = {sw[0], sw[1], sw[2], sw[3]};
+#pragma unroll
+        for (int d = 0; d < NDB; ++d) dq[d] = T::mfma(frag_tr<DP>(kr, 16 * s2, d, lane), sf, dq[d]);
       }
     }
     word = word_next;
@@ -151,63 +244,56 @@ __global__ __launch_bounds__(256, WK == 4 ? 1 : DP == 128 ? 2 : DP == 64 ? 3 : 4
   }
 
   const float unscale = p.scale * kUnshift;
-  if constexpr (WK == 4) {
-    __syncthreads();
-    float* ox = reinterpret_cast<float*>(&kv[0][0][0][0]);  // [4][DP][32]
-    static_assert(sizeof(kv) >= WK * DP * 32 * 4, "the waves' dQ fit the buffers");
+  __syncthreads();
+  float* ox = reinterpret_cast<float*>(&kv[0][0][0][0]);  // [4][DP][32]
+  static_assert(sizeof(kv) >= 4 * DP * 32 * 4, "the waves' dQ fit the buffers");
 #pragma unroll
-    for (int d = 0; d < NDB; ++d)
+  for (int d = 0; d < NDB; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        ox[(wave * DP + 32 * d + 8 * (r / 4) + 4 * h + r % 4) * 32 + col] = dq[d][r];
-    __syncthreads();
-    constexpr int ND = DP / 8;
-    const int q8 = tid >> 5;
-    if (!has_row) return;
+    for (int r = 0; r < 16; ++r)
+      ox[(wave * DP + 32 * d + 8 * (r / 4) + 4 * h + r % 4) * 32 + col] = dq[d][r];
+  __syncthreads();
+  constexpr int ND = DP / 8;
+  const int q8 = tid >> 5;
+  if (row >= p.rows) return;
 #pragma unroll
-    for (int i = 0; i < ND; i += 4) {
-      float a[4];
+  for (int i = 0; i < ND; i += 4) {
+    float a[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        a[j] = 0.f;
+    for (int j = 0; j < 4; ++j) {
+      a[j] = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) a[j] += ox[(w * DP + q8 * ND + i + j) * 32 + col];
-      }
-      const int dim = q8 * ND + i;
-      if (dim >= p.D) continue;
-      if (p.splits > 1)
-        *reinterpret_cast<float4*>(
-            p.part + (((int64_t)split * p.B * p.KVH + bkv) * p.rows + row) * p.D + dim) =
-            float4{a[0], a[1], a[2], a[3]};
-      else
-        *reinterpret_cast<uint2*>(p.dq + orow * p.D + dim) =
-            uint2{T::pack(a[0] * unscale, a[1] * unscale), T::pack(a[2] * unscale, a[3] * unscale)};
+      for (int w = 0; w < 4; ++w) a[j] += ox[(w * DP + q8 * ND + i + j) * 32 + col];
     }
-    return;
+    const int dim = q8 * ND + i;
+    if (dim >= p.D) continue;
+    if (p.splits > 1)
+      *reinterpret_cast<float4*>(p.part + (((int64_t)split * p.B * p.KVH + bkv) * p.rows + row) * p.D + dim) =
+          float4{a[0], a[1], a[2], a[3]};
+    else
+      *reinterpret_cast<uint2*>(p.dq + q.orow * p.D + dim) =
+          uint2{T::pack(a[0] * unscale, a[1] * unscale), T::pack(a[2] * unscale, a[3] * unscale)};
   }
-  if (p.splits > 1) {
-    if (has_row) store_part(p.part + (((int64_t)split * p.B * p.KVH + bkv) * p.rows + row) * p.D, dq, h, p.D);
-    return;
-  }
-  store_row<T>(p.dq + orow * p.D, has_row, dq, unscale, h, p.D);
 }
 
 // ---------------------------------------------------------------------------------------
-// dK, dV: a workgroup's four waves take 32 keys each (their K and V rows as B operands and the two
+// dK, dV: a workgroup's waves take 32 keys each (their K and V rows as B operands and the two
 // accumulators in registers); tiles of 64 query rows, with their dO, lse and D, pass through LDS.
 // S = Q K^T and dP = dO V^T put a key in each lane column, so P and dS are the B operands of
 // dV^T += dO^T P and dK^T += Q^T dS, whose A operands are transpose reads of the same rows.
+// KB = 4: four blocks of keys. KB = 2: two, each of two waves with 32 rows of every tile, which join
+// in LDS at the end: twice the workgroups, for when there are few.
 // ---------------------------------------------------------------------------------------
-constexpr int kQT = 64;
 static __device__ float g_pad_stat[2] = {-__builtin_inff(), 0.f};
 
-template <class T, int DP>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : DP == 64 ? 2 : 4) void xattn_dkdv_kernel(const Args p) {
+template <class T, int DP, int KB>
+__global__ __launch_bounds__(256, DP == 128 ? 1 : DP == 64 ? 3 : 4) void xattn_dkdv_kernel(const Args p) {
   constexpr int NG = DP / 8, KS = DP / 16, NDB = DP / 32;
   constexpr float kUnshift = 1.f / (1 << T::kShift);
   constexpr int kXfer = kQT * NG / 256;
-  __shared__ __attribute__((aligned(1024))) uint16_t qg[2][2][kQT * DP];
-  __shared__ __attribute__((aligned(256))) float st[2][2][kQT];  // -lse, -D
+  constexpr uint32_t kBytes = kQT * DP * 2, kStat = 4 * kBytes;  // [2][Q, dO], [2][-lse, -D]
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kStat + 4 * kQT * 4];
+  const uint32_t l0 = LDS_ADDR(lds);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -221,7 +307,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : DP == 64 ? 2 : 4) void xattn_d
   const int b = bkv / p.KVH, g = bkv - b * p.KVH;
 
   const int klen = keys_of(p, b);
-  const int key = tile * 128 + wave * 32 + col;
+  const int key = tile * 32 * KB + wave % KB * 32 + col;
   const bool vis = key < klen && (!p.kmask || p.kmask[b * p.mask_b + key] != 0);
   const bool any_vis = __any(vis);  // (wave-uniform)
   uint4 kf[KS], vf[KS];
@@ -236,74 +322,124 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : DP == 64 ? 2 : 4) void xattn_d
   const uint16_t* gb = p.dout + b * p.gs.b + (int64_t)g * p.G * p.gs.h;
   const float* sb = p.row_stat + (int64_t)bkv * p.rows;
   const int64_t all_rows = (int64_t)p.B * p.KVH * p.rows;
+  // tiles of 64 rows of one head go by constant lane offsets, the others by an address per row
+  const bool fast = p.D == DP && p.qs.l >= 0 && p.gs.l >= 0 && p.qs.l < (1 << 24) && p.gs.l < (1 << 24);
+  uint32_t qo[kXfer], go[kXfer];
+#pragma unroll
+  for (int r = 0; r < kXfer; ++r) {
+    const int c = wave * 64 + 256 * r + lane, row = c / NG, g8 = ((c % NG) ^ swz<DP>(row)) << 3;
+    qo[r] = (uint32_t)(row * (int)p.qs.l + g8) * 2;
+    go[r] = (uint32_t)(row * (int)p.gs.l + g8) * 2;
+  }
   auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
     const int r0 = t * kQT;
+    const uint32_t hg = fdiv(r0, p.by_lq), at = l0 + buf * 2 * kBytes;
+    const int tok = r0 - hg * p.Lq;
+    if (fast && tok + kQT <= p.Lq) {
+      const uint16_t* qt = qb + (int64_t)tok * p.qs.l + hg * p.qs.h;
+      const uint16_t* gt = gb + (int64_t)tok * p.gs.l + hg * p.gs.h;
 #pragma unroll
-    for (int r = 0; r < kXfer; ++r) {
-      const int c0 = wave * 64 + 256 * r;
-      const int row = r0 + (c0 + lane) / NG;
-      const bool on = row < p.rows;
-      const uint32_t hg = fdiv(on ? row : 0, p.by_lq), tok = (on ? row : 0) - hg * p.Lq;
-      const uint16_t* qr = qb + (int64_t)tok * p.qs.l + hg * p.qs.h;
-      const uint16_t* gr = gb + (int64_t)tok * p.gs.l + hg * p.gs.h;
-      dma_rows<DP>(LDS_ADDR(qg[buf][0]), c0, lane, p.D,
-                   [&](int) __attribute__((always_inline)) { return on ? qr : static_cast<const uint16_t*>(nullptr); });
-      dma_rows<DP>(LDS_ADDR(qg[buf][1]), c0, lane, p.D,
-                   [&](int) __attribute__((always_inline)) { return on ? gr : static_cast<const uint16_t*>(nullptr); });
+      for (int r = 0; r < kXfer; ++r) {
+        dma16_lds_from(qt, qo[r], at + wave * 1024 + 4096 * r);
+        dma16_lds_from(gt, go[r], at + kBytes + wave * 1024 + 4096 * r);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < kXfer; ++r) {
+        const int c0 = wave * 64 + 256 * r;
+        const int row = r0 + (c0 + lane) / NG;
+        const bool on = row < p.rows;
+        const uint32_t hr = fdiv(on ? row : 0, p.by_lq), tr = (on ? row : 0) - hr * p.Lq;
+        const uint16_t* qr = qb + (int64_t)tr * p.qs.l + hr * p.qs.h;
+        const uint16_t* gr = gb + (int64_t)tr * p.gs.l + hr * p.gs.h;
+        dma_rows<DP>(at, c0, lane, p.D,
+                     [&](int) __attribute__((always_inline)) { return on ? qr : static_cast<const uint16_t*>(nullptr); });
+        dma_rows<DP>(at + kBytes, c0, lane, p.D,
+                     [&](int) __attribute__((always_inline)) { return on ? gr : static_cast<const uint16_t*>(nullptr); });
+      }
     }
     if (wave < 2) {  // -lse (wave 0) and -D (wave 1)
       const int row = r0 + lane;
       const float* a = row < p.rows ? sb + wave * all_rows + row : g_pad_stat + wave;
-      dma4_lds(a, (uint32_t)__builtin_amdgcn_readfirstlane(LDS_ADDR(st[buf][wave])));
+      dma4_lds(a, l0 + kStat + (buf * 2 + wave) * kQT * 4);
     }
   };
   wait_vmcnt<0>();  // (no wait on keys and values inside the loop)
   if (t_lo < t_hi) fetch(t_lo, 0);
 
+  const int r_lo = KB == 4 ? 0 : wave / KB;  // this wave's block of 32 rows, the first of its blocks
+  const RowAt<DP> row_at(lane, l0 + r_lo * kBytes / 2);
+  const TrAt<DP, NDB> tr_at(lane, l0 + r_lo * kBytes / 2);
+  const uint32_t stat_at = opaque(l0 + kStat + r_lo * 128 + 16 * h);
   v16f dk[NDB], dv[NDB];
 #pragma unroll
   for (int i = 0; i < NDB; ++i) dk[i] = dv[i] = zero16();
-  for (int t = t_lo, buf = 0; t < t_hi; ++t, buf ^= 1) {
+  auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buffer)::value;
     wait_vmcnt<0>();
     lds_barrier();
     if (t + 1 < t_hi) fetch(t + 1, buf ^ 1);
     if (any_vis) {
-      const uint16_t *qr = qg[buf][0], *gr = qg[buf][1];
 #pragma unroll
-      for (int i = 0; i < kQT / 32; ++i) {
-        v16f s = zero16(), dp = start_from(st[buf][1] + 32 * i, h);
+      for (int i = 0; i < KB / 2; ++i) {
+        constexpr uint32_t at0 = buf * 2 * kBytes, st0 = buf * 2 * kQT * 4;
+        const uint32_t at = at0 + kBytes / 2 * i, st = st0 + 128 * i;
+        v16f s = zero16(), dp = start_at(stat_at + st + kQT * 4);
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          s = T::mfma(frag_row<DP>(qr, 32 * i + col, 2 * k + h), kf[k], s);
-          dp = T::mfma(frag_row<DP>(gr, 32 * i + col, 2 * k + h), vf[k], dp);
+          s = T::mfma(row_at.get(k, at), kf[k], s);
+          dp = T::mfma(row_at.get(k, at + kBytes), vf[k], dp);
         }
+        const v16f e = start_at(stat_at + st);
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
           uint32_t pw[4], sw[4];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float4 e = *reinterpret_cast<const float4*>(&st[buf][0][32 * i + 16 * s2 + 8 * x + 4 * h]);
-            const int r = 8 * s2 + 4 * x;
-            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, e.x));
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, e.y));
-            const float p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 2], p.c2, e.z));
-            const float p3 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 3], p.c2, e.w));
-            pw[2 * x] = T::pack(p0, p1), pw[2 * x + 1] = T::pack(p2, p3);
-            sw[2 * x] = T::pack(p0 * dp[r], p1 * dp[r + 1]);
-            sw[2 * x + 1] = T::pack(p2 * dp[r + 2], p3 * dp[r + 3]);
+          for (int r = 8 * s2; r < 8 * s2 + 8; r += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, e[r]));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, e[r + 1]));
+            pw[(r & 7) / 2] = T::pack(p0, p1);
+            sw[(r & 7) / 2] = T::pack(p0 * dp[r], p1 * dp[r + 1]);
           }
           const uint4 pf = {pw[0], pw[1], pw[2], pw[3]}, sf = {sw[0], sw[1], sw[2], sw[3]};
 #pragma unroll
           for (int d = 0; d < NDB; ++d) {
-            dv[d] = T::mfma(frag_tr<DP>(gr, 32 * i + 16 * s2, d, lane), pf, dv[d]);
-            dk[d] = T::mfma(frag_tr<DP>(qr, 32 * i + 16 * s2, d, lane), sf, dk[d]);
+            dv[d] = T::mfma(tr_at.get(d, at + kBytes + kBytes / 4 * s2), pf, dv[d]);
+            dk[d] = T::mfma(tr_at.get(d, at + kBytes / 4 * s2), sf, dk[d]);
           }
         }
       }
     }
     __builtin_amdgcn_sched_barrier(0);
+  };
+  for (int t = t_lo; t < t_hi; t += 2) {
+    step(t, std::integral_constant<int, 0>());
+    if (t + 1 < t_hi) step(t + 1, std::integral_constant<int, 1>());
   }
 
+  if constexpr (KB == 2) {
+    __syncthreads();
+    float* x = reinterpret_cast<float*>(lds) + wave % KB * (2 * NDB * 1024) + lane;
+    static_assert(KB * 2 * NDB * 1024 * 4 <= 4 * kBytes, "two waves' sums fit the buffers");
+    if (wave >= KB) {
+#pragma unroll
+      for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          x[(d * 32 + r) * 64] = dk[d][r];
+          x[(d * 32 + 16 + r) * 64] = dv[d][r];
+        }
+    }
+    __syncthreads();
+    if (wave >= KB) return;
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        dk[d][r] += x[(d * 32 + r) * 64];
+        dv[d][r] += x[(d * 32 + 16 + r) * 64];
+      }
+  }
   const bool on = key < p.Lk;
   if (!vis) {  // (in the products an invisible key's column holds what a key of zeros would get)
 #pragma unroll
@@ -394,9 +530,9 @@ template <class T, int DP>
 static int launch_bwd(const Args& r, const Args& k, hipStream_t s) {
   if (r.total > 0) {
     if (few_rows(r))
-      xattn_dq_kernel<T, DP, 4><<<r.grid, 256, 0, s>>>(r);
+      xattn_dq_few_kernel<T, DP><<<r.grid, 256, 0, s>>>(r);
     else
-      xattn_dq_kernel<T, DP, 1><<<r.grid, 256, 0, s>>>(r);
+      xattn_dq_kernel<T, DP><<<r.grid, 256, 0, s>>>(r);
     int st = launch_status();
     if (st != DPA_OK) return st;
     if (r.splits > 1) {
@@ -407,7 +543,10 @@ static int launch_bwd(const Args& r, const Args& k, hipStream_t s) {
     }
   }
   if (k.total > 0) {
-    xattn_dkdv_kernel<T, DP><<<k.grid, 256, 0, s>>>(k);
+    if (few_keys(k))
+      xattn_dkdv_kernel<T, DP, 2><<<k.grid, 256, 0, s>>>(k);
+    else
+      xattn_dkdv_kernel<T, DP, 4><<<k.grid, 256, 0, s>>>(k);
     const int st = launch_status();
     return st != DPA_OK ? st : sum_keys<T>(k, s);
   }

@@ -1,5 +1,7 @@
 // Cross attention, forward: one pass over the keys with the running maximum and sum of each
 // row's softmax.
+#include <type_traits>
+
 #include "xattn.hpp"
 
 namespace dpa {
@@ -24,11 +26,11 @@ constexpr float kSlack = 8.f;
 template <class T, int DP>
 __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_fwd_kernel(const Args p) {
   constexpr int KT = 64;
-  constexpr int NG = DP / 8, KS = DP / 16, NDB = DP / 32;
-  constexpr int kXfer = KT * NG / 256;  // a wave's transfers per K (or V) tile
-  __shared__ __attribute__((aligned(1024))) uint16_t kv[2][2][KT * DP];
-  __shared__ __attribute__((aligned(16))) float bias[2][KT];
+  constexpr int KS = DP / 16, NDB = DP / 32;
+  constexpr uint32_t kBytes = KT * DP * 2, kBias = 4 * kBytes;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kBias + 2 * KT * 4];
   __shared__ uint32_t seen[kMaxRange / 32];
+  const uint32_t l0 = LDS_ADDR(lds);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -41,20 +43,20 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_fwd_kernel(const
   const int bkv = bt / (uint32_t)p.tiles;
   const int b = bkv / p.KVH, g = bkv - b * p.KVH;
 
-  const int klen = keys_of(p, b);
+  const int klen = __builtin_amdgcn_readfirstlane(keys_of(p, b));
   const int nt = (klen + KT - 1) / KT;
   const int t_lo = split * p.per_split;
   const int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
-  const uint16_t* kb = p.k + b * p.ks.b + g * p.ks.h;
-  const uint16_t* vb = p.v + b * p.vs.b + g * p.vs.h;
   const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
+  const KeyTiles<DP> keys(p, b, g, klen, l0, wave, lane);
 
   const int row = tile * 128 + wave * 32 + col;
   const bool has_row = row < p.rows;
   const uint32_t head = fdiv(has_row ? row : 0, p.by_lq), tok = (has_row ? row : 0) - head * p.Lq;
   auto fetch = [&](int t, int buf, uint64_t word) __attribute__((always_inline)) {
-    fetch_keys<DP, kXfer, 256>(p, kb, vb, (int64_t)t * KT, word, kv[buf][0], kv[buf][1], wave * 64, lane);
-    if (wave == 0) bias[buf][lane] = (word >> lane) & 1 ? 0.f : -__builtin_inff();
+    keys.fetch(t, buf, word);
+    if (wave == 0)
+      *reinterpret_cast<float*>(lds + kBias + buf * KT * 4 + lane * 4) = (word >> lane) & 1 ? 0.f : -__builtin_inff();
   };
 
   uint64_t word = 0;
@@ -64,6 +66,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_fwd_kernel(const
   }
   uint4 qf[KS];
   load_row<KS>(qf, p.q + b * p.qs.b + (int64_t)tok * p.qs.l + (g * p.G + head) * p.qs.h, has_row, h, p.D);
+  const RowAt<DP> row_at(lane, l0);
+  const TrAt<DP, NDB> tr_at(lane, l0 + kBytes);
+  const uint32_t bias_at = opaque(l0 + kBias + 16 * h);
   wait_vmcnt<0>();  // (no wait on the queries inside the loop: it would take in the tile in flight)
 
   v16f o[NDB];
@@ -72,9 +77,11 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_fwd_kernel(const
   float m = -__builtin_inff();  // what O and l stand at, in units of c2 S
   float l = 0.f;                // this lane's half of the running sum
 
-  for (int t = t_lo, buf = 0; t < t_hi; ++t, buf ^= 1) {
+  auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buffer)::value;
     uint64_t word_next = 0;
     wait_vmcnt<0>();
+    keys.ready(t, buf, word);
     wait_lgkmcnt0();
     lds_barrier();  // tile t is there, and every wave is past its reads of the other buffer
     if (t + 1 < t_hi) {
@@ -82,14 +89,13 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_fwd_kernel(const
       fetch(t + 1, buf ^ 1, word_next);
     }
     if (word) {
-      const uint16_t *ks_ = kv[buf][0], *vs_ = kv[buf][1];
       v16f s[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        s[i] = start_from(bias[buf] + 32 * i, h);
+        s[i] = start_at(bias_at + buf * KT * 4 + 128 * i);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
-          s[i] = T::mfma(frag_row<DP>(ks_, 32 * i + col, 2 * k + h), qf[k], s[i]);
+          s[i] = T::mfma(row_at.get(k, buf * 2 * kBytes + kBytes / 2 * i), qf[k], s[i]);
       }
       float top = -__builtin_inff();
 #pragma unroll
@@ -123,11 +129,15 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_fwd_kernel(const
           const uint4 pf = {pk[0], pk[1], pk[2], pk[3]};
 #pragma unroll
           for (int d = 0; d < NDB; ++d)
-            o[d] = T::mfma(frag_tr<DP>(vs_, 32 * i + 16 * s2, d, lane), pf, o[d]);
+            o[d] = T::mfma(tr_at.get(d, buf * 2 * kBytes + kBytes / 2 * i + kBytes / 4 * s2), pf, o[d]);
         }
     }
     word = word_next;
     __builtin_amdgcn_sched_barrier(0);
+  };
+  for (int t = t_lo; t < t_hi; t += 2) {
+    step(t, std::integral_constant<int, 0>());
+    if (t + 1 < t_hi) step(t + 1, std::integral_constant<int, 1>());
   }
   l = sum_halves(l);
 
