@@ -226,9 +226,10 @@ constexpr int kMaxRange = 16384;
 struct KeyBits {
   const uint32_t* seen;  // LDS, null without a mask
   int klen, k0;
+  int last;  // keys from here on are invisible (a multiple of 64, or the range's end)
   __device__ __forceinline__ KeyBits(const Args& p, int b, int klen_, int k0_, int k1,
                                      uint32_t* lds, int tid)
-      : seen(p.kmask ? lds : nullptr), klen(klen_), k0(k0_) {
+      : seen(p.kmask ? lds : nullptr), klen(klen_), k0(k0_), last(k1) {
     if (!seen) return;
     const uint8_t* mb = p.kmask + b * p.mask_b;
     const int lane = tid & 63;
@@ -239,6 +240,18 @@ struct KeyBits {
       if (lane < 2) lds[(k - k0) / 32 + lane] = (uint32_t)(w >> (32 * lane));
     }
     __syncthreads();
+    last = k0;
+    for (int k = k0; k < k1; k += 64 * 64) {  // (a lane per 64 keys)
+      const int at = k + 64 * lane;
+      const uint64_t any = __ballot(at < k1 && (lds[(at - k0) / 32] | lds[(at - k0) / 32 + 1]) != 0);
+      if (any) last = k + 64 * (64 - __builtin_clzll(any));
+    }
+    last = __builtin_amdgcn_readfirstlane(last);
+  }
+  // tiles [.., t_hi) without the invisible ones at their end
+  template <int KT>
+  __device__ __forceinline__ int tiles_to(int t_hi) const {
+    return seen ? min(t_hi, (last + KT - 1) / KT) : t_hi;
   }
   // keys KT t .. KT t + KT - 1 (inside the range)
   template <int KT>
@@ -506,7 +519,7 @@ inline void plan_rows(Args& p) {
   const bool few = few_rows(p);
   p.tiles = few ? 1 : (int)ceil_div(p.rows, 128);
   const int64_t groups = (int64_t)p.B * p.KVH * p.tiles, kt = few ? 32 : 64;
-  choose_splits(p, groups, ceil_div(p.Lk, kt), 2 * num_cus(), few ? 16 : 8, kMaxRange / kt, few ? 4 : 1);
+  choose_splits(p, groups, ceil_div(p.Lk, kt), (few ? 4 : 2) * num_cus(), 8, kMaxRange / kt, few ? 4 : 1);
   set_grid(p, groups * p.splits, (int64_t)p.tiles * p.splits);
 }
 

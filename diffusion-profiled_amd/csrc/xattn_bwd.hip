@@ -81,8 +81,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_d
   const int klen = __builtin_amdgcn_readfirstlane(keys_of(p, b));
   const int nt = (klen + KT - 1) / KT;
   const int t_lo = split * p.per_split;
-  const int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
+  int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
   const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
+  t_hi = bits.tiles_to<KT>(t_hi);
   const KeyTiles<DP> keys(p, b, g, klen, l0, wave, lane);
   auto fetch = [&](int t, int buf, uint64_t word) __attribute__((always_inline)) {
     keys.fetch(t, buf, word);
@@ -182,10 +183,11 @@ __global__ __launch_bounds__(256, 1) void xattn_dq_few_kernel(const Args p) {
   const int klen = keys_of(p, b);
   const int nt = (klen + KT - 1) / KT;
   const int t_lo = split * p.per_split + wave;
-  const int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
+  int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
   const uint16_t* kb = p.k + b * p.ks.b + g * p.ks.h;
   const uint16_t* vb = p.v + b * p.vs.b + g * p.vs.h;
   const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
+  t_hi = bits.tiles_to<KT>(t_hi);
   auto fetch = [&](int t, int buf, uint32_t word) __attribute__((always_inline)) {
     fetch_keys<DP, kXfer, 64>(p, kb, vb, (int64_t)t * KT, word, kv[wave][buf][0], kv[wave][buf][1], 0, lane);
     if (h == 0) bias[wave][buf][col] = (word >> col) & 1 ? 0.f : -__builtin_inff();

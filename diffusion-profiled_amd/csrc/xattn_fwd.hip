@@ -46,8 +46,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_fwd_kernel(const
   const int klen = __builtin_amdgcn_readfirstlane(keys_of(p, b));
   const int nt = (klen + KT - 1) / KT;
   const int t_lo = split * p.per_split;
-  const int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
+  int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
   const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
+  t_hi = bits.tiles_to<KT>(t_hi);
   const KeyTiles<DP> keys(p, b, g, klen, l0, wave, lane);
 
   const int row = tile * 128 + wave * 32 + col;
@@ -155,17 +156,20 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_fwd_kernel(const
 }
 
 // ---------------------------------------------------------------------------------------
-// Up to 32 rows: the four waves share them and take every fourth tile of 32 keys each, through
-// buffers of their own, and join their softmaxes in LDS at the end. Products as above.
+// Up to 32 rows: the four waves share them and take every fourth tile of 32 keys each, and join
+// their softmaxes in LDS at the end. Products as above. This form reads the keys and values once
+// and does little with them, so it is made for bytes in flight: keys go straight to registers as A
+// operands, values to LDS, each one tile ahead, and two workgroups of 128 dims fit a CU.
 // ---------------------------------------------------------------------------------------
 template <class T, int DP>
-__global__ __launch_bounds__(256, 1) void xattn_few_kernel(const Args p) {
+__global__ __launch_bounds__(256, 2) void xattn_few_kernel(const Args p) {
   constexpr int KT = 32;
   constexpr int NG = DP / 8, KS = DP / 16, NDB = DP / 32;
   constexpr int kXfer = KT * NG / 64;
-  __shared__ __attribute__((aligned(1024))) uint16_t kv[4][2][2][KT * DP];
-  __shared__ __attribute__((aligned(16))) float bias[4][2][KT];
+  constexpr uint32_t kBytes = KT * DP * 2, kBias = 8 * kBytes;  // [4 waves][2]
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kBias + 4 * 2 * KT * 4];
   __shared__ uint32_t seen[kMaxRange / 32];
+  const uint32_t l0 = LDS_ADDR(lds);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -176,52 +180,62 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(const Args p) {
   const int bkv = id / (uint32_t)p.splits;
   const int b = bkv / p.KVH, g = bkv - b * p.KVH;
 
-  const int klen = keys_of(p, b);
+  const int klen = __builtin_amdgcn_readfirstlane(keys_of(p, b));
   const int nt = (klen + KT - 1) / KT;
   const int t_lo = split * p.per_split + wave;
-  const int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
+  int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
   const uint16_t* kb = p.k + b * p.ks.b + g * p.ks.h;
   const uint16_t* vb = p.v + b * p.vs.b + g * p.vs.h;
   const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
+  t_hi = bits.tiles_to<KT>(t_hi);
 
   const int row = col;
   const bool has_row = row < p.rows;
   const uint32_t head = fdiv(has_row ? row : 0, p.by_lq), tok = (has_row ? row : 0) - head * p.Lq;
-  auto fetch = [&](int t, int buf, uint32_t word) __attribute__((always_inline)) {
-    fetch_keys<DP, kXfer, 64>(p, kb, vb, (int64_t)t * KT, word, kv[wave][buf][0], kv[wave][buf][1], 0, lane);
-    if (h == 0) bias[wave][buf][col] = (word >> col) & 1 ? 0.f : -__builtin_inff();
+  uint4 kf[2][KS];
+  auto fetch = [&](int t, uint4(&k)[KS], int buf, uint32_t word) __attribute__((always_inline)) {
+    const uint16_t* vt = vb + (int64_t)t * KT * p.vs.l;
+    const uint32_t at = __builtin_amdgcn_readfirstlane(l0 + (wave * 2 + buf) * kBytes);
+#pragma unroll
+    for (int r = 0; r < kXfer; ++r)
+      dma_rows<DP>(at, 64 * r, lane, p.D, [&](int row) __attribute__((always_inline)) {
+        return (word >> row) & 1 ? vt + row * p.vs.l : static_cast<const uint16_t*>(nullptr);
+      });
+    load_row<KS>(k, kb + ((int64_t)t * KT + col) * p.ks.l, (word >> col) & 1, h, p.D);
+    if (h == 0)
+      *reinterpret_cast<float*>(lds + kBias + (wave * 2 + buf) * 128 + col * 4) = (word >> col) & 1 ? 0.f : -__builtin_inff();
   };
   uint32_t word = 0;
   if (t_lo < t_hi) {
     word = (uint32_t)bits.template word<KT>(t_lo);
-    fetch(t_lo, 0, word);
+    fetch(t_lo, kf[0], 0, word);
   }
   uint4 qf[KS];
   load_row<KS>(qf, p.q + b * p.qs.b + (int64_t)tok * p.qs.l + (g * p.G + head) * p.qs.h, has_row, h, p.D);
-  wait_vmcnt<0>();
+  const TrAt<DP, NDB> tr_at(lane, l0 + wave * 2 * kBytes);
+  const uint32_t bias_at = opaque(l0 + kBias + wave * 256 + 16 * h);
 
   v16f o[NDB];
 #pragma unroll
   for (int i = 0; i < NDB; ++i) o[i] = zero16();
   float m = -__builtin_inff(), l = 0.f;
 
-  for (int t = t_lo, buf = 0; t < t_hi; t += 4, buf ^= 1) {
+  auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buffer)::value;
     uint32_t word_next = 0;
-    wait_lgkmcnt0();  // the reads of the other buffer are done
+    wait_vmcnt<0>();
+    wait_lgkmcnt0();  // the tile is there, and the reads of the other buffer are done
     asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
     if (t + 4 < t_hi) {
       word_next = (uint32_t)bits.template word<KT>(t + 4);
-      fetch(t + 4, buf ^ 1, word_next);
-      wait_vmcnt<2 * kXfer>();  // all but the transfers just issued
-    } else {
-      wait_vmcnt<0>();
+      fetch(t + 4, kf[buf ^ 1], buf ^ 1, word_next);
     }
     asm volatile("" ::: "memory");
     if (word) {
-      const uint16_t *ks_ = kv[wave][buf][0], *vs_ = kv[wave][buf][1];
-      v16f s = start_from(bias[wave][buf], h);
+      v16f s = start_at(bias_at + buf * 128);
 #pragma unroll
-      for (int k = 0; k < KS; ++k) s = T::mfma(frag_row<DP>(ks_, col, 2 * k + h), qf[k], s);
+      for (int k = 0; k < KS; ++k) s = T::mfma(kf[buf][k], qf[k], s);
       float top = -__builtin_inff();
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
@@ -249,18 +263,22 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(const Args p) {
         }
         const uint4 pf = {pk[0], pk[1], pk[2], pk[3]};
 #pragma unroll
-        for (int d = 0; d < NDB; ++d) o[d] = T::mfma(frag_tr<DP>(vs_, 16 * s2, d, lane), pf, o[d]);
+        for (int d = 0; d < NDB; ++d) o[d] = T::mfma(tr_at.get(d, buf * kBytes + kBytes / 2 * s2), pf, o[d]);
       }
     }
     word = word_next;
     __builtin_amdgcn_sched_barrier(0);
+  };
+  for (int t = t_lo; t < t_hi; t += 8) {
+    step(t, std::integral_constant<int, 0>());
+    if (t + 4 < t_hi) step(t + 4, std::integral_constant<int, 1>());
   }
   l = sum_halves(l);
 
   // wave w leaves its (m, l) and O, then adds up a quarter of the dims
   __syncthreads();  // (every wave is past its buffers)
-  float* ox = reinterpret_cast<float*>(&kv[0][0][0][0]);  // [4][DP][32]
-  static_assert(sizeof(kv) >= 4 * DP * 32 * 4, "the waves' O fit the buffers");
+  float* ox = reinterpret_cast<float*>(lds);  // [4][DP][32]
+  static_assert(8 * kBytes >= 4 * DP * 32 * 4, "the waves' O fit the buffers");
 #pragma unroll
   for (int d = 0; d < NDB; ++d)
 #pragma unroll
@@ -313,37 +331,53 @@ __global__ __launch_bounds__(256, 1) void xattn_few_kernel(const Args p) {
           uint2{T::pack(acc[i] * il, acc[i + 1] * il), T::pack(acc[i + 2] * il, acc[i + 3] * il)};
 }
 
-// Joins the splits of a row: O = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s. Thread: 8 dims.
+// Joins the splits of a row: O = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s. A wave per row, two
+// dims per lane; its splits' (max, sum) come in one load, so that the sums over the splits, whose
+// loads wait for nothing else, are the only loop.
 template <class T>
 __global__ __launch_bounds__(256) void xattn_join_kernel(const Args p) {
-  const int nd = p.D / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int lane = threadIdx.x & 63;
   const int64_t rows = (int64_t)p.B * p.KVH * p.rows;
-  if (i >= rows * nd) return;
-  const int64_t at = i / nd;
-  const int d0 = (int)(i - at * nd) * 8;
-  float m = -__builtin_inff();
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.stat[s * rows + at].x);
-  const float ms = m == -__builtin_inff() ? 0.f : m;
-  float l = 0.f, o[8] = {};
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = p.stat[s * rows + at];
-    const float f = __builtin_amdgcn_exp2f(ml.x - ms);
-    l += f * ml.y;
-    const float* src = p.part + (s * rows + at) * p.D + d0;
-    const float4 a = *reinterpret_cast<const float4*>(src), c = *reinterpret_cast<const float4*>(src + 4);
-    o[0] += f * a.x, o[1] += f * a.y, o[2] += f * a.z, o[3] += f * a.w;
-    o[4] += f * c.x, o[5] += f * c.y, o[6] += f * c.z, o[7] += f * c.w;
+  const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (at >= rows) return;
+  const int d0 = 2 * lane;
+  const bool on = d0 < p.D;
+  float m = -__builtin_inff(), l = 0.f, a = 0.f, c = 0.f;
+  for (int s0 = 0; s0 < p.splits; s0 += 64) {
+    const int n = min(64, p.splits - s0);
+    float2 ml = {-__builtin_inff(), 0.f};
+    if (lane < n) ml = p.stat[(s0 + lane) * rows + at];
+    float top = ml.x;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+    const float mn = fmaxf(m, top), ms = mn == -__builtin_inff() ? 0.f : mn;
+    const float keep = __builtin_amdgcn_exp2f(m - ms), f = __builtin_amdgcn_exp2f(ml.x - ms);
+    float sum = f * ml.y;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x, 64);
+    l = l * keep + sum, a *= keep, c *= keep, m = mn;
+    const float* src = p.part + ((int64_t)s0 * rows + at) * p.D + (on ? d0 : 0);
+    const int64_t pitch = rows * p.D;
+    for (int s = 0; s < n; s += 8) {  // (past the last one: that one again, with no weight)
+      float2 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const float2*>(src + min(s + i, n - 1) * pitch);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float fs = s + i < n ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s + i)) : 0.f;
+        a = __builtin_fmaf(fs, v[i].x, a), c = __builtin_fmaf(fs, v[i].y, c);
+      }
+    }
   }
   const int bkv = (int)(at / p.rows), row = (int)(at - (int64_t)bkv * p.rows);
   const int b = bkv / p.KVH, g = bkv - b * p.KVH;
   const uint32_t head = fdiv(row, p.by_lq), tok = row - head * p.Lq;
-  if (d0 == 0)
+  if (lane == 0)
     p.lse[((int64_t)b * p.H + g * p.G + head) * p.Lq + tok] = (m + __builtin_amdgcn_logf(l)) * kLn2;
   const float il = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint4*>(p.out + (((int64_t)b * p.Lq + tok) * p.H + g * p.G + head) * p.D + d0) =
-      uint4{T::pack(o[0] * il, o[1] * il), T::pack(o[2] * il, o[3] * il), T::pack(o[4] * il, o[5] * il),
-            T::pack(o[6] * il, o[7] * il)};
+  if (on)
+    *reinterpret_cast<uint32_t*>(p.out + (((int64_t)b * p.Lq + tok) * p.H + g * p.G + head) * p.D + d0) =
+        T::pack(a * il, c * il);
 }
 
 }  // namespace xattn
@@ -382,8 +416,7 @@ static int run_fwd(const Args& p, hipStream_t s) {
   }
   int st = launch_status();
   if (st != DPA_OK || p.splits <= 1) return st;
-  const int64_t n = (int64_t)p.B * p.KVH * p.rows * (p.D / 8);
-  xattn_join_kernel<T><<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(p);
+  xattn_join_kernel<T><<<(unsigned)ceil_div((int64_t)p.B * p.KVH * p.rows, 4), 256, 0, s>>>(p);
   return launch_status();
 }
 
