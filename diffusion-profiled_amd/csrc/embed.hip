@@ -112,26 +112,36 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const Args p) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Sorting the tokens (stable, so that a run keeps the order of positions). One workgroup sorts a
-// chunk of up to 16384 in LDS, by radix 256; the runs of several chunks are then merged, 16 at a
-// time, by rank. The other workgroups of the first launch clear dW meanwhile: with a large table
-// that is most of the backward's bytes, and it hides the sort.
+// Sorting the tokens (stable, so that a run keeps the order of positions). A workgroup sorts a chunk
+// of 1024 in LDS, by radix 256, which takes about 5 us however many chunks there are; the sorted runs
+// are then merged 16 at a time by rank, with every 32nd key of a run in LDS to search first. The
+// other workgroups of these launches clear dW meanwhile, each launch a part of it: with a large
+// table that is most of the backward's bytes, and it hides most of the sort.
 // ---------------------------------------------------------------------------------------
-constexpr int kChunk = 16384, kSortThreads = 1024, kSortWaves = 16, kMerge = 16;
+constexpr int kChunk = 1024, kSortWaves = kChunk / 64, kMerge = 16, kSample = 32;
+
+struct Fill {  // clears 16-B units and the bytes past them
+  uint4* at;
+  int64_t n;
+  int tail;
+  __device__ __forceinline__ void run(int block, int blocks, int threads, int tid) const {
+    const int64_t step = (int64_t)blocks * threads, i0 = (int64_t)block * threads + tid;
+    for (int64_t i = i0; i < n; i += step) at[i] = uint4{0u, 0u, 0u, 0u};
+    if (i0 < tail) reinterpret_cast<uint8_t*>(at + n)[i0] = 0;
+  }
+};
 
 struct SortArgs {
   const void* tokens;
-  uint32_t *key, *pos;
+  uint32_t *key, *pos, *sample;
   int64_t n;
   uint32_t V, pad;
-  int chunk, chunks, passes;
-  uint4* zero;     // dW, 16-B units
-  int64_t nzero;
-  int tail;        // bytes past them
+  int chunks, passes;
+  Fill fill;
 };
 
 template <int TB>
-__global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(const SortArgs p) {
+__global__ __launch_bounds__(kChunk) void embed_sort_kernel(const SortArgs p) {
   __shared__ uint32_t key[kChunk];
   __shared__ uint16_t idx[2][kChunk];
   __shared__ uint32_t hist[kSortWaves][256];
@@ -139,44 +149,51 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(const SortArgs
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 
   if ((int)blockIdx.x >= p.chunks) {
-    const int64_t step = (int64_t)(gridDim.x - p.chunks) * kSortThreads;
-    const int64_t i0 = (int64_t)(blockIdx.x - p.chunks) * kSortThreads + tid;
-    for (int64_t i = i0; i < p.nzero; i += step) p.zero[i] = uint4{0u, 0u, 0u, 0u};
-    if (i0 < p.tail) reinterpret_cast<uint8_t*>(p.zero + p.nzero)[i0] = 0;
+    p.fill.run(blockIdx.x - p.chunks, gridDim.x - p.chunks, kChunk, tid);
     return;
   }
 
-  const int64_t c0 = (int64_t)blockIdx.x * p.chunk;
-  const int m = (int)(p.n - c0 < p.chunk ? p.n - c0 : p.chunk);
-  for (int i = tid; i < m; i += kSortThreads) {
-    const int64_t t = token_at<TB>(p.tokens, c0 + i);
-    key[i] = t < 0 || t >= (int64_t)p.V || t == (int64_t)p.pad ? p.V : (uint32_t)t;
-    idx[0][i] = (uint16_t)i;
+  const int64_t c0 = (int64_t)blockIdx.x * kChunk;
+  const int m = (int)(p.n - c0 < kChunk ? p.n - c0 : kChunk);
+  const bool on = tid < m;
+  if (on) {
+    const int64_t t = token_at<TB>(p.tokens, c0 + tid);
+    key[tid] = t < 0 || t >= (int64_t)p.V || t == (int64_t)p.pad ? p.V : (uint32_t)t;
+    idx[0][tid] = (uint16_t)tid;
   }
-  const int per = (m + kSortWaves * 64 - 1) / (kSortWaves * 64) * 64;  // a wave's part
-  const int lo = wave * per, hi = min(m, lo + per);
   for (int pass = 0; pass < p.passes; ++pass) {
     const uint16_t* a = idx[pass & 1];
     uint16_t* o = idx[(pass & 1) ^ 1];
-    const int shift = 8 * pass;
-    for (int i = tid; i < kSortWaves * 256; i += kSortThreads) (&hist[0][0])[i] = 0;
+    for (int i = tid; i < kSortWaves * 256; i += kChunk) (&hist[0][0])[i] = 0;
     __syncthreads();
-    for (int i = lo + lane; i < hi; i += 64) atomicAdd(&hist[wave][(key[a[i]] >> shift) & 255], 1u);
+    // a wave's places in order: how many lower lanes share this one's digit, and how many lanes do
+    const uint32_t x = on ? a[tid] : 0;
+    const uint32_t d = on ? (key[x] >> (8 * pass)) & 255 : 0;
+    uint64_t same = __ballot(on);
+#pragma unroll
+    for (int bit = 0; bit < 8; ++bit) {
+      const uint64_t ones = __ballot((d >> bit) & 1);
+      same &= (d >> bit) & 1 ? ones : ~ones;
+    }
+    const int before = __popcll(same & ((1ull << lane) - 1));
+    if (on && before == 0) hist[wave][d] = (uint32_t)__popcll(same);
     __syncthreads();
     // each (digit, wave)'s first place: digits in order, waves in order within a digit
-    uint32_t sum = 0;
+    uint32_t sum = 0, first[kSortWaves];
     if (tid < 256) {
 #pragma unroll
+      for (int w = 0; w < kSortWaves; ++w) first[w] = hist[w][tid];
+#pragma unroll
       for (int w = 0; w < kSortWaves; ++w) {
-        const uint32_t c = hist[w][tid];
-        hist[w][tid] = sum;
+        const uint32_t c = first[w];
+        first[w] = sum;
         sum += c;
       }
       uint32_t incl = sum;
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t x = __shfl_up(incl, off, 64);
-        if (lane >= off) incl += x;
+        const uint32_t y = __shfl_up(incl, off, 64);
+        if (lane >= off) incl += y;
       }
       if (lane == 63) wsum[wave] = incl;
       sum = incl - sum;
@@ -185,69 +202,75 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(const SortArgs
     if (tid < 256) {
       for (int w = 0; w < wave; ++w) sum += wsum[w];
 #pragma unroll
-      for (int w = 0; w < kSortWaves; ++w) hist[w][tid] += sum;
+      for (int w = 0; w < kSortWaves; ++w) hist[w][tid] = first[w] + sum;
     }
     __syncthreads();
-    // 64 at a time, in order: a lane's place is its digit's next one plus the equal digits in
-    // lower lanes
-    for (int i0 = lo; i0 < hi; i0 += 64) {
-      const int i = i0 + lane;
-      const bool on = i < hi;
-      const uint32_t x = on ? a[i] : 0;
-      const uint32_t d = on ? (key[x] >> shift) & 255 : 0;
-      uint64_t same = __ballot(on);
-#pragma unroll
-      for (int bit = 0; bit < 8; ++bit) {
-        const uint64_t ones = __ballot((d >> bit) & 1);
-        same &= (d >> bit) & 1 ? ones : ~ones;
-      }
-      const int before = __popcll(same & ((1ull << lane) - 1));
-      uint32_t base = 0;
-      if (on) base = hist[wave][d];
-      __builtin_amdgcn_wave_barrier();
-      asm volatile("" ::: "memory");
-      if (on && before == 0) hist[wave][d] = base + (uint32_t)__popcll(same);
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_wave_barrier();
-      if (on) o[base + before] = (uint16_t)x;
-    }
+    if (on) o[hist[wave][d] + before] = (uint16_t)x;
     __syncthreads();
   }
-  const uint16_t* a = idx[p.passes & 1];
-  for (int i = tid; i < m; i += kSortThreads) {
-    p.key[c0 + i] = key[a[i]];
-    p.pos[c0 + i] = (uint32_t)(c0 + a[i]);
+  if (on) {
+    const uint32_t x = idx[p.passes & 1][tid], k = key[x];
+    p.key[c0 + tid] = k;
+    p.pos[c0 + tid] = (uint32_t)(c0 + x);
+    if (tid % kSample == 0) p.sample[(c0 + tid) / kSample] = k;
   }
 }
 
-// One round of merges: groups of kMerge sorted runs of len. An element goes to the place that the
-// elements before it take: those of its own run, the not larger ones of the runs before, the
-// smaller ones of the runs after.
-__global__ __launch_bounds__(256) void embed_merge_kernel(const uint32_t* __restrict__ key,
-                                                          const uint32_t* __restrict__ pos,
-                                                          uint32_t* __restrict__ okey,
-                                                          uint32_t* __restrict__ opos, int64_t n,
-                                                          int64_t len) {
+// One round of merges: groups of kMerge sorted runs of len (a multiple of kChunk). An element goes to
+// the place that the elements before it take: those of its own run, the not larger ones of the runs
+// before, the smaller ones of the runs after.
+constexpr int kTable = 512;  // keys of a run in LDS
+
+struct MergeArgs {
+  const uint32_t *key, *pos, *sample;
+  uint32_t *okey, *opos, *osample;
+  int64_t n, len;
+  int blocks;  // of len's groups of 256 places; the others clear
+  Fill fill;
+};
+
+__global__ __launch_bounds__(256) void embed_merge_kernel(const MergeArgs p) {
+  __shared__ uint32_t table[kMerge * kTable];
+  if ((int)blockIdx.x >= p.blocks) {
+    p.fill.run(blockIdx.x - p.blocks, gridDim.x - p.blocks, 256, threadIdx.x);
+    return;
+  }
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const uint32_t k = key[i];
-  const int64_t run = i / len, first = run / kMerge * kMerge;
-  int64_t at = first * len + (i - run * len);
+  const int64_t run = (int64_t)blockIdx.x * 256 / p.len, first = run / kMerge * kMerge;  // (of the workgroup)
+  const int64_t per = p.len / kTable > kSample ? p.len / kTable : kSample;  // keys from one of a table to the next
+  const int rows = (int)(p.len / per);
+  for (int x = threadIdx.x; x < kMerge * rows; x += 256) {
+    const int64_t at = first * p.len + (int64_t)x * per;
+    table[x] = at < p.n ? p.sample[at / kSample] : 0xffffffffu;
+  }
+  __syncthreads();
+  if (i >= p.n) return;
+  const uint32_t k = p.key[i];
+  int64_t place = first * p.len + (i - run * p.len);
 #pragma unroll 4
   for (int r = 0; r < kMerge; ++r) {
-    const int64_t s = (first + r) * len;
-    if (first + r == run || s >= n) continue;
+    const int64_t s = (first + r) * p.len;
+    if (first + r == run || s >= p.n) continue;
     const uint32_t want = first + r < run ? k + 1 : k;  // count keys < want (k <= V < 2^31)
-    int64_t lo = s, hi = s + len < n ? s + len : n;
+    const uint32_t* t = table + r * rows;
+    int a = 0, b = rows;  // (entries past the end are never smaller)
+    while (a < b) {
+      const int mid = (a + b) >> 1;
+      if (t[mid] < want) a = mid + 1;
+      else b = mid;
+    }
+    if (a == 0) continue;
+    int64_t lo = s + (a - 1) * per + 1, hi = s + a * per < p.n ? s + a * per : p.n;
     while (lo < hi) {
       const int64_t mid = (lo + hi) >> 1;
-      if (key[mid] < want) lo = mid + 1;
+      if (p.key[mid] < want) lo = mid + 1;
       else hi = mid;
     }
-    at += lo - s;
+    place += lo - s;
   }
-  okey[at] = k;
-  opos[at] = pos[i];
+  p.okey[place] = k;
+  p.opos[place] = p.pos[i];
+  if (place % kSample == 0) p.osample[place / kSample] = k;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -256,8 +279,10 @@ __global__ __launch_bounds__(256) void embed_merge_kernel(const uint32_t* __rest
 // each owned by the wave of the piece's first place: its fp32 sums go to `part`, and a second
 // launch adds them up in order. Slot of a piece that starts at place i: 2 (i / 64) + (1 if it is
 // the run's first): a run with several pieces is longer than 64, so no two meet.
+// The runs that a wave sums lie side by side, so their places load together, kBatch rows at a time
+// whatever runs they belong to, and a run is stored where the next one begins.
 // ---------------------------------------------------------------------------------------
-constexpr int kOwn = 16, kPiece = 64;
+constexpr int kOwn = 16, kPiece = 64, kBatch = 16;
 
 __device__ __forceinline__ int64_t lower_bound(const uint32_t* key, int64_t n, uint32_t want) {
   int64_t lo = 0, hi = n;
@@ -276,70 +301,77 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const Args p) {
   const int64_t i0 = ((int64_t)blockIdx.x * 4 + wave) * kOwn;
   const int c = (blockIdx.y * 64 + lane) * VEC, cl = c < p.C ? c : 0;
   if (i0 >= p.n) return;
-  // lanes 0 .. 15: the places' keys, those before them and those 64 before
+  // the keys of places i0 + lane and i0 + 64 + lane, those before the first and 64 before, and the
+  // places' positions (V: no gradient, and past the end)
   const int64_t i = i0 + lane;
-  const bool mine = lane < kOwn && i < p.n;
-  const uint32_t k = mine ? p.key[i] : p.V;
-  const bool valid = k != p.V;
-  const uint32_t k1 = mine && i >= 1 ? p.key[i - 1] : p.V, k64 = mine && i >= kPiece ? p.key[i - kPiece] : p.V;
-  uint64_t starts = __ballot(valid && (i == 0 || k1 != k));
-  const uint64_t firsts = starts;
-  const uint64_t deep = __ballot(valid && i >= kPiece && k64 == k);
+  const uint32_t k = i < p.n ? p.key[i] : p.V, kn = i + 64 < p.n && lane <= kOwn ? p.key[i + 64] : p.V;
+  const uint32_t k1 = i >= 1 && i < p.n ? p.key[i - 1] : p.V;
+  const uint32_t k64 = i >= kPiece && i < p.n ? p.key[i - kPiece] : p.V;
+  const uint32_t ps = i < p.n ? p.pos[i] : 0, psn = i + 64 < p.n && lane <= kOwn ? p.pos[i + 64] : 0;
+  const uint64_t own = (1ull << kOwn) - 1;
+  const uint64_t firsts = __ballot(k != p.V && (i == 0 || k1 != k));  // (all 64 places)
+  uint64_t starts = firsts & own;
+  const uint64_t deep = __ballot(k != p.V && i >= kPiece && k64 == k) & own;
   if (deep) {  // places of one long run: where its next piece starts
     const uint32_t kd = __builtin_amdgcn_readlane(k, __builtin_ctzll(deep));
     const int64_t s = lower_bound(p.key, p.n, kd);
     const int64_t next = s + (i0 - s + kPiece - 1) / kPiece * kPiece;
     if (next >= i0 && next < i0 + kOwn) starts |= deep & (1ull << (next - i0));
   }
+  if (!starts) return;
+  // the last of them ends at place `end`: 64 further on, or at the next run
+  const int j_last = 63 - __builtin_clzll(starts);
+  const uint32_t k_last = (uint32_t)__builtin_amdgcn_readlane(k, j_last);
+  const uint64_t away = __ballot(k != k_last) & ~((2ull << j_last) - 1);
+  const uint64_t away_n = __ballot(kn != k_last);
+  int end = away ? __builtin_ctzll(away) : 64 + __builtin_ctzll(away_n | 1ull << (kOwn + 1));
+  const bool more = end > j_last + kPiece;  // it goes on behind its piece
+  if (end > j_last + kPiece) end = j_last + kPiece;
+
   const uint64_t seed = p.seed ? *p.seed : 0;
-  while (starts) {
-    const int j0 = __builtin_ctzll(starts);
-    starts &= starts - 1;
-    const int64_t s = i0 + j0;
-    const uint32_t kr = (uint32_t)__builtin_amdgcn_readlane(k, j0);
-    const bool here = s + lane < p.n && p.key[s + lane] == kr;
-    const uint64_t run = __ballot(here);
-    const int len = run == ~0ull ? 64 : __builtin_ctzll(~run);
-    const uint32_t ps = here ? p.pos[s + lane] : 0;
-    const bool first = (firsts >> j0) & 1;
-    const bool more = len == 64 && s + 64 < p.n && p.key[s + 64] == kr;
-    float acc[VEC];
+  float acc[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
-    // (every lane goes through the loads, lanes past the row at its start: the positions come
-    // from other lanes' registers)
-    int j = 0;
-    for (; j + 8 <= len; j += 8) {
-      float v[8][VEC];
+  for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+  int from = __builtin_ctzll(starts);  // the run at work
+  auto finish = [&]() __attribute__((always_inline)) {
+    const bool first = (firsts >> from) & 1;
+    if (c < p.C && ((starts >> from) & 1)) {
+      if (!first || (from == j_last && more)) {
+        store<DPA_DTYPE_F32, VEC>(p.part, (2 * ((i0 + from) / kPiece) + (first ? 1 : 0)) * p.C + c, acc);
+      } else {
+        const uint32_t kr = (uint32_t)__builtin_amdgcn_readlane(k, from);
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        load<GT, VEC>(p.src, (int64_t)(uint32_t)__builtin_amdgcn_readlane(ps, j + u) * p.C + cl, v[u]);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        if (p.seed)
-          drop<VEC>(seed, (int64_t)(uint32_t)__builtin_amdgcn_readlane(ps, j + u) * p.C + cl,
-                    p.keep2 & 0xffffu, v[u]);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += v[u][e];
+        for (int e = 0; e < VEC; ++e) acc[e] *= p.scale * p.keep_scale;
+        store<WT, VEC>(p.dst, (int64_t)kr * p.C + c, acc);
       }
     }
-    for (; j < len; ++j) {
-      const int64_t at = (int64_t)(uint32_t)__builtin_amdgcn_readlane(ps, j) * p.C + cl;
-      float v[VEC];
-      load<GT, VEC>(p.src, at, v);
-      if (p.seed) drop<VEC>(seed, at, p.keep2 & 0xffffu, v);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[e] += v[e];
+    for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+  };
+  // (every lane goes through the loads, lanes past the row at its start: the positions come from
+  // other lanes' registers)
+  for (int j = from; j < end; j += kBatch) {
+    float v[kBatch][VEC];
+    uint32_t pj[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int x = j + u < end ? j + u : end - 1;
+      pj[u] = (uint32_t)(x < 64 ? __builtin_amdgcn_readlane(ps, x) : __builtin_amdgcn_readlane(psn, x - 64));
+      load<GT, VEC>(p.src, (int64_t)pj[u] * p.C + cl, v[u]);
     }
-    if (c >= p.C) continue;
-    if (!first || more) {
-      store<DPA_DTYPE_F32, VEC>(p.part, (2 * (s / kPiece) + (first ? 1 : 0)) * p.C + c, acc);
-    } else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[e] *= p.scale * p.keep_scale;
-      store<WT, VEC>(p.dst, (int64_t)kr * p.C + c, acc);
+    for (int u = 0; u < kBatch; ++u) {
+      if (j + u >= end) break;
+      if (j + u > from && j + u < kOwn && ((starts >> (j + u)) & 1)) {
+        finish();
+        from = j + u;
+      }
+      if (p.seed) drop<VEC>(seed, (int64_t)pj[u] * p.C + cl, p.keep2 & 0xffffu, v[u]);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] += v[u][e];
     }
   }
+  finish();
 }
 
 // The pieces of the long run that starts among a workgroup's 64 places, if one does: each wave adds
@@ -448,10 +480,6 @@ static int launch_sum(const Args& a, hipStream_t s) {
     default: CALL(DPA_DTYPE_F16, DPA_DTYPE_F16); break;                    \
   }
 
-// Up to kChunk tokens in one workgroup; more in runs of half that, which sort in half the time on
-// more CUs and are merged
-static int chunk_of(int64_t n) { return n <= kChunk ? kChunk : kChunk / 2; }
-
 static int64_t align256(int64_t n) { return (n + 255) & ~255ll; }
 
 }  // namespace embed
@@ -482,10 +510,10 @@ extern "C" int dpa_embedding_fwd(const void* tokens, int token_bytes, const void
   return launch_status();
 }
 
-// two key and two position arrays, and the pieces' sums
+// two arrays of keys, two of positions and two of samples, and the pieces' sums
 extern "C" int64_t dpa_embedding_bwd_workspace_bytes(int64_t n, int C) {
   if (n <= 0 || C <= 0) return 0;
-  return 4 * align256(4 * n) + ceil_div(n, kPiece) * 2 * C * 4;
+  return 4 * align256(4 * n) + 2 * align256(4 * ceil_div(n, kSample)) + ceil_div(n, kPiece) * 2 * C * 4;
 }
 
 extern "C" int dpa_embedding_bwd(const void* dout, int dout_dtype, const void* tokens,
@@ -502,37 +530,51 @@ extern "C" int dpa_embedding_bwd(const void* dout, int dout_dtype, const void* t
     return DPA_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return DPA_ERR_ALIGN;
   uint8_t* w = (uint8_t*)workspace;
-  const int64_t arr = align256(4 * n);
+  const int64_t arr = align256(4 * n), smp = align256(4 * ceil_div(n, kSample));
   uint32_t* key[2] = {(uint32_t*)w, (uint32_t*)(w + arr)};
   uint32_t* pos[2] = {(uint32_t*)(w + 2 * arr), (uint32_t*)(w + 3 * arr)};
+  uint32_t* sample[2] = {(uint32_t*)(w + 4 * arr), (uint32_t*)(w + 4 * arr + smp)};
   hipStream_t s = (hipStream_t)stream;
 
+  // dW, in equal parts to the launches of the sort
+  int launches = 1;
+  for (int64_t len = kChunk; len < n; len *= kMerge) ++launches;
+  const int64_t bytes = V * C * dtype_size(weight_dtype), units = bytes / 16, part = ceil_div(units, launches);
+  auto fill = [&](int i, int threads, int* blocks) {
+    const int64_t lo = i * part < units ? i * part : units, hi = lo + part < units ? lo + part : units;
+    const int64_t most = 2 * num_cus() * (1024 / threads), want = ceil_div(hi - lo + 1, threads * 4);
+    *blocks = (int)(want < most ? want : most);
+    return Fill{(uint4*)dweight + lo, hi - lo, i + 1 == launches ? (int)(bytes % 16) : 0};
+  };
+
   SortArgs q{};
-  q.tokens = tokens, q.key = key[0], q.pos = pos[0], q.n = n;
+  q.tokens = tokens, q.key = key[0], q.pos = pos[0], q.sample = sample[0], q.n = n;
   q.V = (uint32_t)V;
   q.pad = padding_idx >= 0 && padding_idx < V ? (uint32_t)padding_idx : 0xffffffffu;
-  q.chunk = chunk_of(n);
-  q.chunks = (int)ceil_div(n, q.chunk);
+  q.chunks = (int)ceil_div(n, kChunk);
   while ((V >> (8 * q.passes)) > 0) ++q.passes;
-  const int64_t bytes = V * C * dtype_size(weight_dtype);
-  q.zero = (uint4*)dweight, q.nzero = bytes / 16, q.tail = (int)(bytes % 16);
-  int64_t fill = ceil_div(q.nzero + 1, kSortThreads * 4);
-  if (fill > 2 * num_cus()) fill = 2 * num_cus();
-  const unsigned grid = (unsigned)(q.chunks + fill);
-  if (token_bytes == 8) embed_sort_kernel<8><<<grid, kSortThreads, 0, s>>>(q);
-  else embed_sort_kernel<4><<<grid, kSortThreads, 0, s>>>(q);
+  int blocks;
+  q.fill = fill(0, kChunk, &blocks);
+  const unsigned grid = (unsigned)(q.chunks + blocks);
+  if (token_bytes == 8) embed_sort_kernel<8><<<grid, kChunk, 0, s>>>(q);
+  else embed_sort_kernel<4><<<grid, kChunk, 0, s>>>(q);
   st = launch_status();
   if (st != DPA_OK || n == 0) return st;
-  int at = 0;
-  for (int64_t len = q.chunk; len < n; len *= kMerge, at ^= 1) {
-    embed_merge_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(key[at], pos[at], key[at ^ 1],
-                                                                   pos[at ^ 1], n, len);
+  int at = 0, round = 0;
+  for (int64_t len = kChunk; len < n; len *= kMerge, at ^= 1) {
+    MergeArgs m{};
+    m.key = key[at], m.pos = pos[at], m.sample = sample[at];
+    m.okey = key[at ^ 1], m.opos = pos[at ^ 1], m.osample = sample[at ^ 1];
+    m.n = n, m.len = len;
+    m.blocks = (int)ceil_div(n, 256);
+    m.fill = fill(++round, 256, &blocks);
+    embed_merge_kernel<<<(unsigned)(m.blocks + blocks), 256, 0, s>>>(m);
     st = launch_status();
     if (st != DPA_OK) return st;
   }
   Args a{};
   a.src = dout, a.dst = dweight, a.n = n, a.V = (uint32_t)V, a.C = C, a.scale = scale;
-  a.key = key[at], a.pos = pos[at], a.part = (float*)(w + 4 * arr);
+  a.key = key[at], a.pos = pos[at], a.part = (float*)(w + 4 * arr + 2 * smp);
   set_drop(a, drop_seed, drop_p);
 #define SUM(A, B) st = launch_sum<A, B>(a, s)
   EMBED_BY_TYPES(dout_dtype, weight_dtype, SUM)
