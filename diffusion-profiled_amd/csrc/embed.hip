@@ -20,22 +20,33 @@ struct Args {
   // backward
   uint32_t *key, *pos;  // sorted tokens (V: no gradient) and their positions
   float* part;          // sums of the pieces of long runs
+  // forward: 16-B units of out's rows, as the table has them
+  uint32_t units;
+  FastDiv by_row;
 };
 
-// VEC (1 or 4) elements of type DT at p, in fp32 and back
+// VEC (1, 4 or 8) elements of type DT at p, in fp32 and back
 template <int DT, int VEC>
 __device__ __forceinline__ void load(const void* p, int64_t i, float (&v)[VEC]) {
   if constexpr (DT == DPA_DTYPE_F32) {
-    if constexpr (VEC == 4) {
-      const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    const float* q = static_cast<const float*>(p) + i;
+    if constexpr (VEC == 1) {
+      v[0] = *q;
     } else {
-      v[0] = static_cast<const float*>(p)[i];
+#pragma unroll
+      for (int x = 0; x < VEC; x += 4) {
+        const float4 a = *reinterpret_cast<const float4*>(q + x);
+        v[x] = a.x, v[x + 1] = a.y, v[x + 2] = a.z, v[x + 3] = a.w;
+      }
     }
   } else {
     typedef Elem<DT> E;
     const uint16_t* q = static_cast<const uint16_t*>(p) + i;
-    if constexpr (VEC == 4) {
+    if constexpr (VEC == 8) {
+      const uint4 a = *reinterpret_cast<const uint4*>(q);
+      v[0] = E::lo(a.x), v[1] = E::hi(a.x), v[2] = E::lo(a.y), v[3] = E::hi(a.y);
+      v[4] = E::lo(a.z), v[5] = E::hi(a.z), v[6] = E::lo(a.w), v[7] = E::hi(a.w);
+    } else if constexpr (VEC == 4) {
       const uint2 a = *reinterpret_cast<const uint2*>(q);
       v[0] = E::lo(a.x), v[1] = E::hi(a.x), v[2] = E::lo(a.y), v[3] = E::hi(a.y);
     } else {
@@ -47,14 +58,21 @@ __device__ __forceinline__ void load(const void* p, int64_t i, float (&v)[VEC]) 
 template <int DT, int VEC>
 __device__ __forceinline__ void store(void* p, int64_t i, const float (&v)[VEC]) {
   if constexpr (DT == DPA_DTYPE_F32) {
-    if constexpr (VEC == 4)
-      *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = float4{v[0], v[1], v[2], v[3]};
-    else
-      static_cast<float*>(p)[i] = v[0];
+    float* q = static_cast<float*>(p) + i;
+    if constexpr (VEC == 1) {
+      *q = v[0];
+    } else {
+#pragma unroll
+      for (int x = 0; x < VEC; x += 4)
+        *reinterpret_cast<float4*>(q + x) = float4{v[x], v[x + 1], v[x + 2], v[x + 3]};
+    }
   } else {
     typedef Elem<DT> E;
     uint16_t* q = static_cast<uint16_t*>(p) + i;
-    if constexpr (VEC == 4)
+    if constexpr (VEC == 8)
+      *reinterpret_cast<uint4*>(q) = uint4{E::pack(v[0], v[1]), E::pack(v[2], v[3]), E::pack(v[4], v[5]),
+                                           E::pack(v[6], v[7])};
+    else if constexpr (VEC == 4)
       *reinterpret_cast<uint2*>(q) = uint2{E::pack(v[0], v[1]), E::pack(v[2], v[3])};
     else
       *q = (uint16_t)E::pack(v[0], 0.f);
@@ -81,33 +99,69 @@ __device__ __forceinline__ int64_t token_at(const void* t, int64_t i) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Forward. A wave per row: 4 channels per lane and step. A token outside the table gives a row of
-// NaN (nothing is read for it).
+// Forward. A token outside the table gives a row of NaN (nothing is read for it). Bound by HBM: rows
+// of the table read, out written.
+// Where rows are whole units of 16 B of the table's type: a thread per unit, four of them apart, so
+// that their tokens load together and then their rows. Else a wave per row, an element per lane.
 // ---------------------------------------------------------------------------------------
-template <int WT, int OT, int TB, int VEC>
-__global__ __launch_bounds__(256) void embed_fwd_kernel(const Args p) {
+template <int WT, int OT, int VEC>
+__device__ __forceinline__ void embed_store(const Args& p, uint64_t seed, bool in, int64_t at, float (&v)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = in ? v[i] * p.scale : __builtin_nanf("");
+  if (p.seed && in) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] *= p.keep_scale;
+    if constexpr (VEC == 8) {
+      float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
+      drop<4>(seed, at, p.keep2 & 0xffffu, a);
+      drop<4>(seed, at + 4, p.keep2 & 0xffffu, b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+    } else {
+      drop<VEC>(seed, at, p.keep2 & 0xffffu, v);
+    }
+  }
+  store<OT, VEC>(p.dst, at, v);
+}
+
+template <int WT, int OT, int TB>
+__global__ __launch_bounds__(256) void embed_units_kernel(const Args p) {
+  constexpr int VEC = 16 / (WT == DPA_DTYPE_F32 ? 4 : 2), U = 4;
+  const uint64_t seed = p.seed ? *p.seed : 0;
+  const uint32_t i0 = blockIdx.x * (256 * U) + threadIdx.x;
+  int64_t t[U];
+  uint32_t c[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t i = i0 + 256 * u, row = fdiv(i < p.units ? i : 0, p.by_row);
+    c[u] = ((i < p.units ? i : 0) - row * p.by_row.d) * VEC;
+    t[u] = token_at<TB>(p.tokens, row);
+  }
+  float v[U][VEC];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const bool in = t[u] >= 0 && t[u] < (int64_t)p.V;
+    load<WT, VEC>(p.src, (in ? t[u] * p.C : 0) + c[u], v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t i = i0 + 256 * u;
+    if (i < p.units) embed_store<WT, OT, VEC>(p, seed, t[u] >= 0 && t[u] < (int64_t)p.V, (int64_t)i * VEC, v[u]);
+  }
+}
+
+template <int WT, int OT, int TB>
+__global__ __launch_bounds__(256) void embed_rows_kernel(const Args p) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= p.n) return;
   const int64_t t = token_at<TB>(p.tokens, row);
   const bool in = t >= 0 && t < (int64_t)p.V;
   const uint64_t seed = p.seed ? *p.seed : 0;
-  for (int c = lane * VEC; c < p.C; c += 64 * VEC) {
-    float v[VEC];
-    if (in) {
-      load<WT, VEC>(p.src, t * p.C + c, v);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] *= p.scale;
-      if (p.seed) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] *= p.keep_scale;
-        drop<VEC>(seed, row * p.C + c, p.keep2 & 0xffffu, v);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = __builtin_nanf("");
-    }
-    store<OT, VEC>(p.dst, row * p.C + c, v);
+  for (int c = lane; c < p.C; c += 64) {
+    float v[1] = {0.f};
+    if (in) load<WT, 1>(p.src, t * p.C + c, v);
+    embed_store<WT, OT, 1>(p, seed, in, row * p.C + c, v);
   }
 }
 
@@ -246,28 +300,33 @@ __global__ __launch_bounds__(256) void embed_merge_kernel(const MergeArgs p) {
   __syncthreads();
   if (i >= p.n) return;
   const uint32_t k = p.key[i];
-  int64_t place = first * p.len + (i - run * p.len);
-#pragma unroll 4
-  for (int r = 0; r < kMerge; ++r) {
-    const int64_t s = (first + r) * p.len;
-    if (first + r == run || s >= p.n) continue;
-    const uint32_t want = first + r < run ? k + 1 : k;  // count keys < want (k <= V < 2^31)
-    const uint32_t* t = table + r * rows;
-    int a = 0, b = rows;  // (entries past the end are never smaller)
-    while (a < b) {
-      const int mid = (a + b) >> 1;
-      if (t[mid] < want) a = mid + 1;
-      else b = mid;
-    }
-    if (a == 0) continue;
-    int64_t lo = s + (a - 1) * per + 1, hi = s + a * per < p.n ? s + a * per : p.n;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (p.key[mid] < want) lo = mid + 1;
-      else hi = mid;
-    }
-    place += lo - s;
+  // how many table entries, then keys up to the next entry, are smaller: halving steps, the same for
+  // every run, so that the runs' reads go out together
+  int a[kMerge];
+#pragma unroll
+  for (int r = 0; r < kMerge; ++r) a[r] = 0;
+  const auto want = [&](int r) __attribute__((always_inline)) { return first + r < run ? k + 1 : k; };  // (k <= V < 2^31)
+  for (int st = rows / 2; st > 0; st >>= 1) {
+#pragma unroll
+    for (int r = 0; r < kMerge; ++r) a[r] += table[r * rows + a[r] + st - 1] < want(r) ? st : 0;
   }
+#pragma unroll
+  for (int r = 0; r < kMerge; ++r) a[r] += table[r * rows + a[r]] < want(r) ? 1 : 0;
+  // (the run's key at (a - 1) per is smaller: c counts from there)
+  int c[kMerge];
+#pragma unroll
+  for (int r = 0; r < kMerge; ++r) c[r] = 0;
+  for (int st = (int)(per / 2); st > 0; st >>= 1) {
+#pragma unroll
+    for (int r = 0; r < kMerge; ++r) {
+      const int64_t at = (first + r) * p.len + (a[r] - 1) * per + c[r] + st;
+      if (a[r] > 0 && at < p.n && p.key[at] < want(r)) c[r] += st;
+    }
+  }
+  int64_t place = first * p.len + (i - run * p.len);
+#pragma unroll
+  for (int r = 0; r < kMerge; ++r)
+    if (first + r != run && a[r] > 0) place += (a[r] - 1) * per + c[r] + 1;
   p.okey[place] = k;
   p.opos[place] = p.pos[i];
   if (place % kSample == 0) p.osample[place / kSample] = k;
@@ -284,12 +343,16 @@ __global__ __launch_bounds__(256) void embed_merge_kernel(const MergeArgs p) {
 // ---------------------------------------------------------------------------------------
 constexpr int kOwn = 16, kPiece = 64, kBatch = 16;
 
-__device__ __forceinline__ int64_t lower_bound(const uint32_t* key, int64_t n, uint32_t want) {
+// The first of the n sorted keys that is not smaller than want, by a wave: 64 probes a step
+__device__ __forceinline__ int64_t lower_bound(const uint32_t* key, int64_t n, uint32_t want, int lane) {
   int64_t lo = 0, hi = n;
   while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (key[mid] < want) lo = mid + 1;
-    else hi = mid;
+    const int64_t step = (hi - lo + 63) >> 6, at = lo + lane * step;
+    const int below = __popcll(__ballot(at < hi && key[at < hi ? at : lo] < want));
+    if (below == 0) break;
+    const int64_t next = lo + below * step;
+    lo += (below - 1) * step + 1;
+    hi = next < hi ? next : hi;
   }
   return lo;
 }
@@ -314,7 +377,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const Args p) {
   const uint64_t deep = __ballot(k != p.V && i >= kPiece && k64 == k) & own;
   if (deep) {  // places of one long run: where its next piece starts
     const uint32_t kd = __builtin_amdgcn_readlane(k, __builtin_ctzll(deep));
-    const int64_t s = lower_bound(p.key, p.n, kd);
+    const int64_t s = lower_bound(p.key, i0, kd, lane);
     const int64_t next = s + (i0 - s + kPiece - 1) / kPiece * kPiece;
     if (next >= i0 && next < i0 + kOwn) starts |= deep & (1ull << (next - i0));
   }
@@ -389,7 +452,7 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const Args p) {
   const int j0 = __builtin_ctzll(m);
   const int64_t s = (int64_t)blockIdx.x * kPiece + j0;
   const uint32_t kr = (uint32_t)__builtin_amdgcn_readlane(k, j0);
-  const int64_t pieces = (lower_bound(p.key, p.n, kr + 1) - s + kPiece - 1) / kPiece;
+  const int64_t pieces = (lower_bound(p.key, p.n, kr + 1, lane) - s + kPiece - 1) / kPiece;
   const int64_t per = (pieces + 3) / 4, lo = wave * per, hi = lo + per < pieces ? lo + per : pieces;
   const int c = (blockIdx.y * 64 + lane) * VEC;
   float acc[VEC];
@@ -440,16 +503,21 @@ static bool vec_ok(const Args& a, int t_src, int t_dst) {
 }
 
 template <int WT, int OT>
-static void launch_fwd(const Args& a, int token_bytes, hipStream_t s) {
-  const unsigned grid = (unsigned)ceil_div(a.n, 4);
-  const bool v = vec_ok(a, WT, OT);
-  if (token_bytes == 8) {
-    if (v) embed_fwd_kernel<WT, OT, 8, 4><<<grid, 256, 0, s>>>(a);
-    else embed_fwd_kernel<WT, OT, 8, 1><<<grid, 256, 0, s>>>(a);
-  } else {
-    if (v) embed_fwd_kernel<WT, OT, 4, 4><<<grid, 256, 0, s>>>(a);
-    else embed_fwd_kernel<WT, OT, 4, 1><<<grid, 256, 0, s>>>(a);
+static void launch_fwd(Args& a, int token_bytes, hipStream_t s) {
+  constexpr int VEC = 16 / (WT == DPA_DTYPE_F32 ? 4 : 2);
+  const int64_t units = a.n * (a.C / VEC);
+  if (a.C % VEC == 0 && units < 1ll << 31 && aligned(a.src, 16) &&
+      aligned(a.dst, VEC * dtype_size(OT) < 16 ? VEC * dtype_size(OT) : 16)) {
+    a.units = (uint32_t)units;
+    a.by_row = make_fastdiv(a.C / VEC);
+    const unsigned grid = (unsigned)ceil_div(units, 1024);
+    if (token_bytes == 8) embed_units_kernel<WT, OT, 8><<<grid, 256, 0, s>>>(a);
+    else embed_units_kernel<WT, OT, 4><<<grid, 256, 0, s>>>(a);
+    return;
   }
+  const unsigned grid = (unsigned)ceil_div(a.n, 4);
+  if (token_bytes == 8) embed_rows_kernel<WT, OT, 8><<<grid, 256, 0, s>>>(a);
+  else embed_rows_kernel<WT, OT, 4><<<grid, 256, 0, s>>>(a);
 }
 
 template <int GT, int WT>
