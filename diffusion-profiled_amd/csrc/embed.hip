@@ -318,9 +318,11 @@ __global__ __launch_bounds__(256) void embed_merge_kernel(const MergeArgs p) {
   for (int r = 0; r < kMerge; ++r) c[r] = 0;
   for (int st = (int)(per / 2); st > 0; st >>= 1) {
 #pragma unroll
-    for (int r = 0; r < kMerge; ++r) {
+    for (int r = 0; r < kMerge; ++r) {  // (loads without a branch around them, for that reason too)
       const int64_t at = (first + r) * p.len + (a[r] - 1) * per + c[r] + st;
-      if (a[r] > 0 && at < p.n && p.key[at] < want(r)) c[r] += st;
+      const bool on = (a[r] > 0) & (at < p.n);
+      const uint32_t x = p.key[on ? at : 0];
+      c[r] += on & (x < want(r)) ? st : 0;
     }
   }
   int64_t place = first * p.len + (i - run * p.len);
@@ -334,14 +336,14 @@ __global__ __launch_bounds__(256) void embed_merge_kernel(const MergeArgs p) {
 
 // ---------------------------------------------------------------------------------------
 // Sums of the runs. A wave owns 16 sorted places and 256 channels (4 per lane) and sums each run
-// that starts there, up to 64 places of it. A longer run is cut into pieces of 64 from its start,
+// that starts there, up to 32 places of it. A longer run is cut into pieces of 32 from its start,
 // each owned by the wave of the piece's first place: its fp32 sums go to `part`, and a second
-// launch adds them up in order. Slot of a piece that starts at place i: 2 (i / 64) + (1 if it is
-// the run's first): a run with several pieces is longer than 64, so no two meet.
+// launch adds them up in order. Slot of a piece that starts at place i: 2 (i / 32) + (1 if it is
+// the run's first): a run with several pieces is longer than 32, so no two meet.
 // The runs that a wave sums lie side by side, so their places load together, kBatch rows at a time
 // whatever runs they belong to, and a run is stored where the next one begins.
 // ---------------------------------------------------------------------------------------
-constexpr int kOwn = 16, kPiece = 64, kBatch = 16;
+constexpr int kOwn = 16, kPiece = 32, kBatch = 16;
 
 // The first of the n sorted keys that is not smaller than want, by a wave: 64 probes a step
 __device__ __forceinline__ int64_t lower_bound(const uint32_t* key, int64_t n, uint32_t want, int lane) {
@@ -364,13 +366,13 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const Args p) {
   const int64_t i0 = ((int64_t)blockIdx.x * 4 + wave) * kOwn;
   const int c = (blockIdx.y * 64 + lane) * VEC, cl = c < p.C ? c : 0;
   if (i0 >= p.n) return;
-  // the keys of places i0 + lane and i0 + 64 + lane, those before the first and 64 before, and the
-  // places' positions (V: no gradient, and past the end)
+  // the keys of places i0 + lane, those one and 32 before, and the places' positions (V: no gradient,
+  // and past the end)
   const int64_t i = i0 + lane;
-  const uint32_t k = i < p.n ? p.key[i] : p.V, kn = i + 64 < p.n && lane <= kOwn ? p.key[i + 64] : p.V;
+  const uint32_t k = i < p.n ? p.key[i] : p.V;
   const uint32_t k1 = i >= 1 && i < p.n ? p.key[i - 1] : p.V;
   const uint32_t k64 = i >= kPiece && i < p.n ? p.key[i - kPiece] : p.V;
-  const uint32_t ps = i < p.n ? p.pos[i] : 0, psn = i + 64 < p.n && lane <= kOwn ? p.pos[i + 64] : 0;
+  const uint32_t ps = i < p.n ? p.pos[i] : 0;
   const uint64_t own = (1ull << kOwn) - 1;
   const uint64_t firsts = __ballot(k != p.V && (i == 0 || k1 != k));  // (all 64 places)
   uint64_t starts = firsts & own;
@@ -382,12 +384,12 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const Args p) {
     if (next >= i0 && next < i0 + kOwn) starts |= deep & (1ull << (next - i0));
   }
   if (!starts) return;
-  // the last of them ends at place `end`: 64 further on, or at the next run
+  // the last of them ends at place `end`: 32 further on, or at the next run
   const int j_last = 63 - __builtin_clzll(starts);
   const uint32_t k_last = (uint32_t)__builtin_amdgcn_readlane(k, j_last);
   const uint64_t away = __ballot(k != k_last) & ~((2ull << j_last) - 1);
-  const uint64_t away_n = __ballot(kn != k_last);
-  int end = away ? __builtin_ctzll(away) : 64 + __builtin_ctzll(away_n | 1ull << (kOwn + 1));
+  static_assert(kOwn + kPiece < 64, "a wave's runs and what follows are in its lanes");
+  int end = away ? __builtin_ctzll(away) : 64;
   const bool more = end > j_last + kPiece;  // it goes on behind its piece
   if (end > j_last + kPiece) end = j_last + kPiece;
 
@@ -419,7 +421,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const Args p) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const int x = j + u < end ? j + u : end - 1;
-      pj[u] = (uint32_t)(x < 64 ? __builtin_amdgcn_readlane(ps, x) : __builtin_amdgcn_readlane(psn, x - 64));
+      pj[u] = (uint32_t)__builtin_amdgcn_readlane(ps, x);
       load<GT, VEC>(p.src, (int64_t)pj[u] * p.C + cl, v[u]);
     }
 #pragma unroll
@@ -437,7 +439,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const Args p) {
   finish();
 }
 
-// The pieces of the long run that starts among a workgroup's 64 places, if one does: each wave adds
+// The pieces of the long run that starts among a workgroup's 32 places, if one does: each wave adds
 // up a quarter of them in order, then the quarters.
 template <int WT, int VEC>
 __global__ __launch_bounds__(256) void embed_join_kernel(const Args p) {
@@ -445,7 +447,7 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const Args p) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t i = (int64_t)blockIdx.x * kPiece + lane;
-  const uint32_t k = i < p.n ? p.key[i] : p.V;
+  const uint32_t k = lane < kPiece && i < p.n ? p.key[i] : p.V;
   const bool start = k != p.V && (i == 0 || p.key[i - 1] != k) && i + kPiece < p.n && p.key[i + kPiece] == k;
   const uint64_t m = __ballot(start);
   if (!m) return;  // (the same in every wave)
