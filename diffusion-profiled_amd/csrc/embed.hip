@@ -279,7 +279,8 @@ struct MergeArgs {
   const uint32_t *key, *pos, *sample;
   uint32_t *okey, *opos, *osample;
   int64_t n, len;
-  int blocks;  // of len's groups of 256 places; the others clear
+  int log_per, log_rows;  // keys from one table entry to the next, entries of a run
+  int blocks;             // of 256 places; the others clear
   Fill fill;
 };
 
@@ -291,44 +292,42 @@ __global__ __launch_bounds__(256) void embed_merge_kernel(const MergeArgs p) {
   }
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t run = (int64_t)blockIdx.x * 256 / p.len, first = run / kMerge * kMerge;  // (of the workgroup)
-  const int64_t per = p.len / kTable > kSample ? p.len / kTable : kSample;  // keys from one of a table to the next
-  const int rows = (int)(p.len / per);
-  for (int x = threadIdx.x; x < kMerge * rows; x += 256) {
-    const int64_t at = first * p.len + (int64_t)x * per;
+  for (int x = threadIdx.x; x < kMerge << p.log_rows; x += 256) {
+    const int64_t at = first * p.len + ((int64_t)x << p.log_per);
     table[x] = at < p.n ? p.sample[at / kSample] : 0xffffffffu;
   }
   __syncthreads();
   if (i >= p.n) return;
-  const uint32_t k = p.key[i];
+  const uint32_t k = p.key[i], n = (uint32_t)p.n;
   // how many table entries, then keys up to the next entry, are smaller: halving steps, the same for
   // every run, so that the runs' reads go out together
-  int a[kMerge];
+  uint32_t a[kMerge], want[kMerge];  // (k <= V < 2^31)
 #pragma unroll
-  for (int r = 0; r < kMerge; ++r) a[r] = 0;
-  const auto want = [&](int r) __attribute__((always_inline)) { return first + r < run ? k + 1 : k; };  // (k <= V < 2^31)
-  for (int st = rows / 2; st > 0; st >>= 1) {
+  for (int r = 0; r < kMerge; ++r) a[r] = r << p.log_rows, want[r] = first + r < run ? k + 1 : k;
+  for (int st = 1 << p.log_rows >> 1; st > 0; st >>= 1) {
 #pragma unroll
-    for (int r = 0; r < kMerge; ++r) a[r] += table[r * rows + a[r] + st - 1] < want(r) ? st : 0;
+    for (int r = 0; r < kMerge; ++r) a[r] += table[a[r] + st - 1] < want[r] ? st : 0;
   }
 #pragma unroll
-  for (int r = 0; r < kMerge; ++r) a[r] += table[r * rows + a[r]] < want(r) ? 1 : 0;
-  // (the run's key at (a - 1) per is smaller: c counts from there)
-  int c[kMerge];
+  for (int r = 0; r < kMerge; ++r) a[r] = a[r] - (r << p.log_rows) + (table[a[r]] < want[r] ? 1 : 0);
+  // (with a entries smaller, so is the run's key at (a - 1) per: the count goes on behind it)
+  uint32_t at[kMerge];
 #pragma unroll
-  for (int r = 0; r < kMerge; ++r) c[r] = 0;
-  for (int st = (int)(per / 2); st > 0; st >>= 1) {
+  for (int r = 0; r < kMerge; ++r) {
+    const int64_t s = (first + r) * p.len;
+    at[r] = (uint32_t)(s < p.n ? s : p.n) + ((a[r] ? a[r] - 1 : 0) << p.log_per);
+  }
+  for (uint32_t st = 1u << p.log_per >> 1; st > 0; st >>= 1) {
+    uint32_t x[kMerge];
 #pragma unroll
-    for (int r = 0; r < kMerge; ++r) {  // (loads without a branch around them, for that reason too)
-      const int64_t at = (first + r) * p.len + (a[r] - 1) * per + c[r] + st;
-      const bool on = (a[r] > 0) & (at < p.n);
-      const uint32_t x = p.key[on ? at : 0];
-      c[r] += on & (x < want(r)) ? st : 0;
-    }
+    for (int r = 0; r < kMerge; ++r) x[r] = p.key[min(at[r] + st, n - 1)];
+#pragma unroll
+    for (int r = 0; r < kMerge; ++r) at[r] += (at[r] + st < n) & (x[r] < want[r]) ? st : 0;
   }
   int64_t place = first * p.len + (i - run * p.len);
 #pragma unroll
   for (int r = 0; r < kMerge; ++r)
-    if (first + r != run && a[r] > 0) place += (a[r] - 1) * per + c[r] + 1;
+    if (first + r != run && a[r] > 0) place += (int64_t)at[r] + 1 - (first + r) * p.len;
   p.okey[place] = k;
   p.opos[place] = p.pos[i];
   if (place % kSample == 0) p.osample[place / kSample] = k;
@@ -636,6 +635,8 @@ extern "C" int dpa_embedding_bwd(const void* dout, int dout_dtype, const void* t
     m.key = key[at], m.pos = pos[at], m.sample = sample[at];
     m.okey = key[at ^ 1], m.opos = pos[at ^ 1], m.osample = sample[at ^ 1];
     m.n = n, m.len = len;
+    while ((kSample << m.log_rows) < len && (1 << m.log_rows) < kTable) ++m.log_rows;
+    while (((int64_t)1 << (m.log_rows + m.log_per)) < len) ++m.log_per;
     m.blocks = (int)ceil_div(n, 256);
     m.fill = fill(++round, 256, &blocks);
     embed_merge_kernel<<<(unsigned)(m.blocks + blocks), 256, 0, s>>>(m);
