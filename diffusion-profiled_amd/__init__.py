@@ -6,6 +6,8 @@ from ``csrc/*.hip`` by ``build.build_library()``.
 """
 from . import _lib, attention, build, conditioning, fp8_kernels, gn_silu  # noqa: F401
 from . import ddpm, unet, trainer  # noqa: F401
+from . import text_unet  # noqa: F401
+from .conditioning import cross_attention, cross_attention_kv, dropout, embedding  # noqa: F401
 from .fp8_kernels import (  # noqa: F401
     FP8_DTYPE,
     FP8_MAX_E4M3,

@@ -21,6 +21,7 @@ import torch
 
 from .ddpm import DiffusionWrapper, EWMAWrapper
 from .optim import FusedAdamWEMA
+from .text_unet import TextConfig, TextUNet
 from .unet import UNet, UNetConfig
 
 
@@ -110,13 +111,16 @@ def prepare_cuda_graph(ddpm: DiffusionWrapper, model: torch.nn.Module, ema_ddpm:
 
 class TrainState:
     """Model + AdamW + DDPM + EMA with static input buffers (the reference's train.py setup:
-    channels-last model, fused capturable AdamW, EMA beta 0.9999)."""
+    channels-last model, fused capturable AdamW, EMA beta 0.9999). With ``text`` the model is a
+    ``text_unet.TextUNet`` and the prompts' tokens [batch, prompt_length] a static buffer too."""
 
     def __init__(self, config: UNetConfig, batch: int, lr: float = 2e-4, max_t: int = 1000,
                  schedule_type: str = "linear", ema_beta: float = 0.9999, device: str = "cuda",
-                 seed: int = 0, fixed_noise: bool = False, fused_tail: bool = True):
+                 seed: int = 0, fixed_noise: bool = False, fused_tail: bool = True,
+                 text: TextConfig | None = None, prompt_length: int = 77):
         torch.manual_seed(seed)
-        model = UNet(config).to(memory_format=torch.channels_last)
+        model = UNet(config) if text is None else TextUNet(config, text)
+        model = model.to(memory_format=torch.channels_last)
         self.model = model.to(device)
         self.optimizer = torch.optim.AdamW(self.model.parameters(), lr=lr, fused=True,
                                            capturable=True)
@@ -138,12 +142,19 @@ class TrainState:
         self.static_t = torch.zeros(batch, dtype=torch.long, device=device) if fixed_noise else None
         self.static_eps = (torch.zeros(shape, device=device).contiguous(
             memory_format=torch.channels_last) if fixed_noise else None)
+        self.static_tokens = None
+        if text is not None:
+            self.static_tokens = torch.full((batch, prompt_length), text.padding_idx, device=device)
+            self.model.prompt = self.static_tokens
         self.loss_acc = torch.zeros((), device=device)
         self.graph: torch.cuda.CUDAGraph | None = None
 
     def set_batch(self, images: torch.Tensor, t: torch.Tensor | None = None,
-                  eps: torch.Tensor | None = None) -> None:
+                  eps: torch.Tensor | None = None, tokens: torch.Tensor | None = None) -> None:
         self.static_batch.copy_(images)
+        if tokens is not None:
+            assert self.static_tokens is not None
+            self.static_tokens.copy_(tokens)
         if t is not None:
             assert self.static_t is not None
             self.static_t.copy_(t)

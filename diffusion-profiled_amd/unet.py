@@ -630,10 +630,19 @@ class UNet(nn.Module):
         self._wprep.active = True
         return self._wprep
 
+    def _dropouts(self) -> int:
+        """Dropout seeds that a forward takes."""
+        return sum(1 for m in self.modules()
+                   if isinstance(m, ResidualBlock) and m.training and m.dropout.p > 0.0)
+
+    def _after_stage(self, name: str, act: torch.Tensor) -> torch.Tensor:
+        """What a model that is conditioned on more than the timestep does behind a stage (down<i>,
+        mid, up<i>)."""
+        return act
+
     def forward(self, x: torch.Tensor, t: torch.Tensor) -> torch.Tensor:
         plan = self._weight_prep(x)
-        n_drop = sum(1 for m in self.modules()
-                     if isinstance(m, ResidualBlock) and m.training and m.dropout.p > 0.0)
+        n_drop = self._dropouts()
         if n_drop and _on_gpu(x):
             DROPOUT_SEEDS.fill(x.device, n_drop)
         try:
@@ -691,9 +700,9 @@ class UNet(nn.Module):
                     act, hs[-1] = downsample2_tee(act)
                 else:
                     act = downsample2(act)
-            act = stage(act, t_emb)
+            act = self._after_stage(f"down{i}", stage(act, t_emb))
             hs.append(act)
-        act = self.mid(act, t_emb)
+        act = self._after_stage("mid", self.mid(act, t_emb))
         for i, stage in enumerate(self.up_stages):
             h = hs.pop()
             # torch.concat([self.upsample(act) if i > 0 else act, h], dim=1): one pass on the
@@ -702,6 +711,7 @@ class UNet(nn.Module):
                 act = stage(CatInput(act, h, True), t_emb)
             else:
                 act = stage(upsample_concat(act, h, up=i > 0), t_emb)
+            act = self._after_stage(f"up{i}", act)
         return self.out(act)
 
 

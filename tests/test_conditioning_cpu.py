@@ -173,3 +173,25 @@ def test_dropout_and_embedding_refuse():
 def test_p_as_fp32_below_one():
     assert struct.unpack("f", struct.pack("f", 1.0 - 1e-12))[0] == 1.0     # what the check is for
     assert C._check_p(0.999999, "dropout") == 0.999999
+
+
+def test_text_unet_structure():
+    U, X = dpa_mod("unet"), dpa_mod("text_unet")
+    cfg = U.UNetConfig(in_channels=3, base_hidden=64, scales=[1, 2, 2], n_heads=2, p_drop=0.1,
+                       attn_resolutions=[16], in_resolution=32, n_resblocks=2)
+    m = X.TextUNet(cfg, X.TextConfig(vocab=11, width=24))
+    base = U.UNet(cfg)
+    assert set(base.state_dict()) <= set(m.state_dict())
+    assert sorted(m.cross) == ["down1", "mid", "up1"]
+    assert m.cross["down1"].q.in_features == 128 and m.cross["up1"].q.in_features == 128
+    assert not m.text.weight[0].any() and all(not b.out.weight.any() for b in m.cross.values())
+    m.train()
+    assert m._dropouts() == base.train()._dropouts() + 4
+    assert m.eval()._dropouts() == 0
+    # without a prompt it runs as the base model does, on the CPU too
+    x, t = torch.randn(1, 3, 32, 32), torch.tensor([3])
+    assert torch.equal(m(x, t), base.eval()(x, t))            # (both start at zero)
+    with pytest.raises(ValueError, match="cross attention block"):
+        X.CrossAttentionBlock(60, X.TextConfig(vocab=11, width=24), 8)
+    with pytest.raises(ValueError, match="GPU"):
+        m(x, t, torch.ones((1, 5), dtype=torch.int64))
