@@ -525,8 +525,12 @@ inline void plan_rows(Args& p) {
 
 constexpr int kQT = 64;  // rows of a tile of the kernel of dK and dV
 
-// Its workgroups take 128 keys, or 64 where that leaves less than four to a CU
-inline bool few_keys(const Args& p) { return (int64_t)p.B * p.KVH * ceil_div(p.Lk, 128) < 4 * num_cus(); }
+// Its workgroups take 128 keys, or 64 where that leaves few of them: less than four to a CU, of the
+// form for more than 64 dims, which runs one to a CU, less than two. (8 x 4096 queries of 64 dims over
+// 700 of 1031 keys 251 -> 197 us with 64; 16 x 1024 of 128 dims over 512 keys 173 us with 128, 196.)
+inline bool few_keys(const Args& p) {
+  return (int64_t)p.B * p.KVH * ceil_div(p.Lk, 128) < (dim_pad(p.D) == 128 ? 2 : 4) * num_cus();
+}
 
 inline void plan_keys(Args& p) {
   p.tiles = (int)ceil_div(p.Lk, few_keys(p) ? 64 : 128);
