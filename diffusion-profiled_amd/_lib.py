@@ -7,6 +7,7 @@ fallback: if the library is missing, every op raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import threading
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_void_p
 
@@ -298,3 +299,26 @@ def call(name: str, *args) -> None:
 def query(name: str, *args) -> int:
     """Call an entry point that returns a size."""
     return getattr(_lib or load(), name)(*args)
+
+
+_FAST_ENTRIES = ("dpa_cross_attention_fwd", "dpa_cross_attention_fwd_workspace_bytes",
+                 "dpa_cross_attention_bwd", "dpa_cross_attention_bwd_workspace_bytes", "dpa_dropout",
+                 "dpa_embedding_fwd", "dpa_embedding_bwd", "dpa_embedding_bwd_workspace_bytes",
+                 "dpa_status_string")
+
+
+def fast_calls():
+    """The module of ``csrc/fast_calls.cpp`` on this library's entries, or None where it is not built
+    or was built for another torch."""
+    path = _build.FAST_PATH
+    lib = load()
+    if not path.exists():
+        return None
+    spec = importlib.util.spec_from_file_location("dpa_fast_calls", path)
+    try:
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except ImportError:
+        return None
+    module.init(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in _FAST_ENTRIES))
+    return module

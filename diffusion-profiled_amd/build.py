@@ -1,13 +1,16 @@
 """Build the gfx950 HIP library ``lib/libdpa_fp8.so`` from ``csrc/*.hip``.
 
-The library has a plain C ABI (``include/dpa_fp8.h``); nothing here links against torch.
-Sources compile in parallel (one ``hipcc -c`` per file) and link with ``hipcc -shared``.
+The library has a plain C ABI (``include/dpa_fp8.h``) and does not link against torch.
+Sources compile in parallel (one ``hipcc -c`` per file) and link with ``hipcc -shared``. Beside it
+``lib/dpa_fast_calls.so`` (``csrc/fast_calls.cpp``, host code only) is a Python module for the torch
+of this interpreter.
 """
 from __future__ import annotations
 
 import os
 import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -15,6 +18,7 @@ CSRC_DIR = PKG_DIR / "csrc"
 BUILD_DIR = PKG_DIR / "_build"
 LIB_DIR = PKG_DIR / "lib"
 LIB_PATH = LIB_DIR / "libdpa_fp8.so"
+FAST_PATH = LIB_DIR / "dpa_fast_calls.so"
 
 OFFLOAD_ARCH = "gfx950"
 
@@ -45,6 +49,20 @@ def sources() -> list[Path]:
     return sorted(CSRC_DIR.glob("*.hip"))
 
 
+def _fast_calls_command() -> list[str]:
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include",
+            f"-I{sysconfig.get_paths()['include']}", f"-I{rocm}/include",
+            str(CSRC_DIR / "fast_calls.cpp"), "-o", str(FAST_PATH.with_suffix(".so.tmp")),
+            f"-L{root}/lib", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+
+
 def build_library(verbose: bool = False) -> Path:
     """Compile every csrc/*.hip for gfx950 and link lib/libdpa_fp8.so. Always rebuilds."""
     BUILD_DIR.mkdir(parents=True, exist_ok=True)
@@ -59,6 +77,8 @@ def build_library(verbose: bool = False) -> Path:
         if verbose:
             print(" ".join(cmd), flush=True)
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
+    fast = subprocess.Popen(_fast_calls_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+    procs.append((CSRC_DIR / "fast_calls.cpp", fast))
     errors = []
     for src, p in procs:
         out, _ = p.communicate()
@@ -79,6 +99,7 @@ def build_library(verbose: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError("hipcc link failed:\n" + r.stdout.decode(errors="replace"))
     os.replace(tmp, LIB_PATH)
+    os.replace(FAST_PATH.with_suffix(".so.tmp"), FAST_PATH)
     return LIB_PATH
 
 

@@ -34,6 +34,25 @@ _DESC = struct.Struct("=11Qq18q7if")
 _DESC_HEAD, _DESC_TAIL = struct.Struct("=11Q"), struct.Struct("=q18q7if")
 
 
+class _General:
+    """Stands for the native calls where they are not built: every call goes the general way."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+_FAST: Any = None
+
+
+def _fast():
+    """``csrc/fast_calls.cpp``: each of its functions does a whole call on operands that need no
+    conversion, and returns None for any other, which the code behind it copies or refuses."""
+    global _FAST
+    if _FAST is None:
+        _FAST = _lib.fast_calls() or _General()
+    return _FAST
+
+
 def _ptr(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -106,6 +125,7 @@ def _check_masks(q, k, key_lengths, key_mask):
 def _scale_of(scale: float | None, head_dim: int) -> float:
     if scale is None:
         return 1.0 / math.sqrt(head_dim)
+    scale = float(scale)
     if not 0.0 < scale < 3.4e38:
         raise ValueError(f"cross attention: scale {scale} is not positive and finite")
     return scale
@@ -114,45 +134,24 @@ def _scale_of(scale: float | None, head_dim: int) -> float:
 _NONE3 = (0, 0, 0)
 
 
-class _Plan(NamedTuple):
-    """What a call's shapes, strides, dtypes and scale settle, once they have been checked."""
+class _Call(NamedTuple):
+    """The operands of a call as the kernels read them, checked, and what follows from their layout."""
+    q: torch.Tensor
+    k: torch.Tensor
+    v: torch.Tensor
+    lengths: torch.Tensor | None
+    mask: torch.Tensor | None
+    dout: torch.Tensor | None
     tail: bytes         # DpaCrossAttention behind its pointers
-    out_shape: tuple
-    lse_shape: tuple
-    fwd_bytes: int      # workspaces
-    bwd_bytes: int
+
+    def describe(self, out, lse, dq=None, dk=None, dv=None) -> bytes:
+        return _DESC_HEAD.pack(self.q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), out.data_ptr(),
+                               lse.data_ptr(), _ptr(self.lengths), _ptr(self.mask), _ptr(self.dout),
+                               _ptr(dq), _ptr(dk), _ptr(dv)) + self.tail
 
 
-# An eager call on small operands costs more in checks than in its launch, so what they come to is
-# kept per layout of the operands: 4 x 1 queries over 77 keys 15.7 -> 9.6 us, their backward 28.5 ->
-# 18.0 us on the host. Addresses and values are looked at in every call.
-_PLANS: dict[tuple, _Plan] = {}
-_MOST_PLANS = 4096
-
-
-def _layout(t: torch.Tensor | None):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
-
-
-def _attention_key(q, k, v, lengths, mask, scale, dout=None, dk=None, dv=None) -> tuple:
-    return (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype,
-            q.get_device(), k.get_device(), v.get_device(), scale, _layout(lengths), _layout(mask),
-            _layout(dout), _layout(dk), _layout(dv))
-
-
-def _attention_operands(q, k, v, lengths, mask, scale, dout=None, dk=None, dv=None):
-    """(plan, q, k, v, lengths, mask, dout) as the kernels read them, checked."""
-    if scale is not None:
-        scale = float(scale)
-    key = _attention_key(q, k, v, lengths, mask, scale, dout, dk, dv)
-    plan = _PLANS.get(key)
-    if plan is not None and not ((q.data_ptr() | k.data_ptr() | v.data_ptr()
-                                  | (0 if dout is None else dout.data_ptr())) & 15):
-        return plan, q, k, v, lengths, mask, dout
-    given = (q, k, v, lengths, mask, dout)
+def _attention_call(q, k, v, lengths, mask, scale, dout=None, dk=None, dv=None) -> _Call:
     _check_qkv(q, k, v)
-    b, lq, h, d = q.shape
-    lk, g = k.shape[1], k.shape[2]
     if dout is not None:
         if dout.shape != q.shape or dout.dtype != q.dtype:
             raise ValueError(f"cross attention: dout {dout.dtype} {tuple(dout.shape)} is not q's "
@@ -160,22 +159,13 @@ def _attention_operands(q, k, v, lengths, mask, scale, dout=None, dk=None, dv=No
         _on_one_gpu(q, dout)
         dout = _rows(dout)
     lengths, mask = _check_masks(q, k, lengths, mask)
+    (b, lq, h, d), (lk, g) = q.shape, k.shape[1:3]
     number = _scale_of(scale, d)
     q, k, v = _rows(q), _rows(k), _rows(v)
-    sizes = (_DT[q.dtype], b, lq, lk, h, g, d)
     strides = [_NONE3 if t is None else _strides(t) for t in (q, k, v, dout, dk, dv)]
     tail = _DESC_TAIL.pack(0 if mask is None else mask.stride(0), *(s for t in strides for s in t),
-                           *sizes, number)
-    desc = _DESC_HEAD.pack(*[0] * 11) + tail
-    plan = _Plan(tail, (b, lq, h, d), (b, h, lq),
-                 _lib.query("dpa_cross_attention_fwd_workspace_bytes", desc),
-                 _lib.query("dpa_cross_attention_bwd_workspace_bytes", desc))
-    now = (q, k, v, lengths, mask, dout)
-    if all(a is b for a, b in zip(now, given)):     # nothing was copied: it holds for the next call
-        if len(_PLANS) >= _MOST_PLANS:
-            _PLANS.clear()
-        _PLANS[key] = plan
-    return plan, *now
+                           _DT[q.dtype], b, lq, lk, h, g, d, number)
+    return _Call(q, k, v, lengths, mask, dout, tail)
 
 
 def _workspace(nbytes: int, device) -> torch.Tensor | None:
@@ -195,40 +185,48 @@ def cross_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     [B], clamped to [0, Lk]) and where key_mask ([B, Lk], bool or uint8) is true; keys that do not
     are never read. A query without any gets 0, and -inf as its log sum exp. scale: 1 / sqrt(D) by
     default, positive. Returns (out [B, Lq, H, D], lse [B, H, Lq] fp32)."""
-    plan, q, k, v, lengths, mask, _ = _attention_operands(q, k, v, key_lengths, key_mask, scale)
-    out = q.new_empty(plan.out_shape)
-    lse = q.new_empty(plan.lse_shape, dtype=torch.float32)
+    done = _fast().attention_fwd(q, k, v, key_lengths, key_mask, scale)
+    if done is not None:
+        return done
+    call = _attention_call(q, k, v, key_lengths, key_mask, scale)
+    b, lq, h, d = q.shape
+    out = q.new_empty((b, lq, h, d))
+    lse = q.new_empty((b, h, lq), dtype=torch.float32)
     if out.numel() == 0:
         return out, lse
-    ws = _workspace(plan.fwd_bytes, q.device) if plan.fwd_bytes else None
-    desc = _DESC_HEAD.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-                           _ptr(lengths), _ptr(mask), 0, 0, 0, 0) + plan.tail
-    _lib.call("dpa_cross_attention_fwd", desc, _ptr(ws), plan.fwd_bytes, _lib.current_stream(q))
+    desc = call.describe(out, lse)
+    n = _lib.query("dpa_cross_attention_fwd_workspace_bytes", desc)
+    ws = _workspace(n, q.device)
+    _lib.call("dpa_cross_attention_fwd", desc, _ptr(ws), n, _lib.current_stream(q))
     return out, lse
 
 
 def _attention_bwd(dout, q, k, v, out, lse, key_lengths, key_mask, scale, dk, dv):
-    plan, q, k, v, lengths, mask, dout = _attention_operands(q, k, v, key_lengths, key_mask, scale,
-                                                             dout, dk, dv)
-    device = q.get_device()
-    if out.shape != plan.out_shape or out.dtype != q.dtype or out.get_device() != device:
+    """(dq, dk, dv); dk and dv: None (not formed), True (a new dense tensor) or where to write them."""
+    done = _fast().attention_bwd(dout, q, k, v, out, lse, key_lengths, key_mask, scale, dk, dv)
+    if done is not None:
+        return done
+    if dk is True:
+        dk, dv = k.new_empty(k.shape), k.new_empty(k.shape)
+    call = _attention_call(q, k, v, key_lengths, key_mask, scale, dout, dk, dv)
+    b, lq, h, d = q.shape
+    if out.shape != q.shape or out.dtype != q.dtype or out.get_device() != q.get_device():
         raise ValueError(f"cross attention: out {out.dtype} {tuple(out.shape)} on {out.device} is not "
                          f"q's {q.dtype} {tuple(q.shape)} on {q.device}")
-    if lse.shape != plan.lse_shape or lse.dtype != torch.float32 or lse.get_device() != device:
-        raise ValueError(f"cross attention: lse is fp32 {list(plan.lse_shape)} on {q.device}, got "
+    if lse.shape != (b, h, lq) or lse.dtype != torch.float32 or lse.get_device() != q.get_device():
+        raise ValueError(f"cross attention: lse is fp32 [{b}, {h}, {lq}] on {q.device}, got "
                          f"{lse.dtype} {tuple(lse.shape)} on {lse.device}")
     out, lse = out.contiguous(), lse.contiguous()
     if out.data_ptr() % 16:
         out = out.clone()
-    dq = q.new_empty(plan.out_shape)
-    if plan.out_shape[0] == 0 or (dq.numel() == 0 and (dk is None or dk.numel() == 0)):
-        return dq
-    ws = _workspace(plan.bwd_bytes, q.device)
-    desc = _DESC_HEAD.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-                           _ptr(lengths), _ptr(mask), dout.data_ptr(), dq.data_ptr(), _ptr(dk),
-                           _ptr(dv)) + plan.tail
-    _lib.call("dpa_cross_attention_bwd", desc, _ptr(ws), plan.bwd_bytes, _lib.current_stream(q))
-    return dq
+    dq = q.new_empty((b, lq, h, d))
+    if b == 0 or (dq.numel() == 0 and (dk is None or dk.numel() == 0)):
+        return dq, dk, dv
+    desc = call.describe(out, lse, dq, dk, dv)
+    n = _lib.query("dpa_cross_attention_bwd_workspace_bytes", desc)
+    ws = _workspace(n, q.device)
+    _lib.call("dpa_cross_attention_bwd", desc, _ptr(ws), n, _lib.current_stream(q))
+    return dq, dk, dv
 
 
 def cross_attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -239,8 +237,7 @@ def cross_attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v:
     """(dq, dk, dv) of ``cross_attention_fwd`` from its outputs and the gradient of out; dk and dv
     [B, Lk, G, D] summed over the query heads of a key head, zero for keys that take no part.
     Deterministic."""
-    dk, dv = k.new_empty(k.shape), k.new_empty(k.shape)
-    return _attention_bwd(dout, q, k, v, out, lse, key_lengths, key_mask, scale, dk, dv), dk, dv
+    return _attention_bwd(dout, q, k, v, out, lse, key_lengths, key_mask, scale, True, True)
 
 
 class CrossAttention(torch.autograd.Function):
@@ -258,11 +255,9 @@ class CrossAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, dout):
         q, k, v, out, lse, lengths, mask = ctx.saved_tensors
-        dk = dv = None
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dk, dv = (torch.empty(k.shape, device=k.device, dtype=k.dtype) for _ in range(2))
-        dq = _attention_bwd(dout, q, k, v, out, lse, lengths, mask, ctx.scale, dk, dv)
-        return dq, dk, dv, None, None, None
+        keys = True if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else None
+        return (*_attention_bwd(dout, q, k, v, out, lse, lengths, mask, ctx.scale, keys, keys),
+                None, None, None)
 
 
 class CrossAttentionKV(torch.autograd.Function):
@@ -284,7 +279,7 @@ class CrossAttentionKV(torch.autograd.Function):
         q, kv, out, lse, lengths, mask = ctx.saved_tensors
         dkv = torch.empty(kv.shape, device=kv.device, dtype=kv.dtype) if ctx.needs_input_grad[1] else None
         dk, dv = (None, None) if dkv is None else (dkv[:, :, 0], dkv[:, :, 1])
-        dq = _attention_bwd(dout, q, kv[:, :, 0], kv[:, :, 1], out, lse, lengths, mask, ctx.scale, dk, dv)
+        dq, _, _ = _attention_bwd(dout, q, kv[:, :, 0], kv[:, :, 1], out, lse, lengths, mask, ctx.scale, dk, dv)
         return dq, dkv, None, None, None
 
 
@@ -352,6 +347,9 @@ def dropout_fwd(x: torch.Tensor, p: float, seed: torch.Tensor, *,
     fp32 and rounded once. x is bf16, fp16 or fp32. An element's place in memory is its index for
     the mask (dense or channels-last tensors as they are, others as their dense copy); the result
     has x's layout. A dropped element counts as 0 whatever it holds."""
+    y = _fast().dropout(x, p, seed, residual)
+    if y is not None:
+        return y
     if x.dtype not in _DT:
         raise ValueError(f"dropout: bf16, fp16 or fp32, got {x.dtype}")
     p = _check_p(p, "dropout")
@@ -426,6 +424,9 @@ def embedding_fwd(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 
     """scale weight[tokens] in out_dtype (weight's by default), with p_drop > 0 followed by dropout
     (index: the element's place in the output; seed as in ``dropout_fwd``). tokens int32 or int64
     of any shape, weight [V, C] bf16, fp16 or fp32. A token outside [0, V) gives a row of NaN."""
+    out = _fast().embedding_fwd(tokens, weight, scale, p_drop, seed, out_dtype)
+    if out is not None:
+        return out
     if weight.ndim != 2 or weight.numel() == 0:
         raise ValueError(f"embedding: the weight is [V, C], got {tuple(weight.shape)}")
     out_dtype = weight.dtype if out_dtype is None else out_dtype
@@ -445,6 +446,10 @@ def embedding_bwd(dout: torch.Tensor, tokens: torch.Tensor, num_embeddings: int,
     """The gradient [num_embeddings, C] of ``embedding_fwd``'s weight in dtype (dout's by default):
     per row the fp32 sum over its tokens in order, rounded once; zeros for padding_idx. Tokens
     outside the table add nothing. Deterministic."""
+    dw = _fast().embedding_bwd(dout, tokens, num_embeddings, scale,
+                               -1 if padding_idx is None else padding_idx, p_drop, seed, dtype)
+    if dw is not None:
+        return dw
     if dout.ndim < 1 or dout.shape[:-1] != tokens.shape or dout.shape[-1] == 0 or num_embeddings <= 0:
         raise ValueError(f"embedding: dout {tuple(dout.shape)} does not go with tokens "
                          f"{tuple(tokens.shape)} and {num_embeddings} rows")

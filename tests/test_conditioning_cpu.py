@@ -195,3 +195,19 @@ def test_text_unet_structure():
         X.CrossAttentionBlock(60, X.TextConfig(vocab=11, width=24), 8)
     with pytest.raises(ValueError, match="GPU"):
         m(x, t, torch.ones((1, 5), dtype=torch.int64))
+
+
+def test_fast_calls_take_plain_gpu_tensors_only():
+    """The native calls leave everything else to the general way (None), without touching it."""
+    fast = L.fast_calls()
+    assert fast is not None
+    q, k, v = _qkv()
+    x, seed = torch.zeros(4, 8), torch.zeros(1, dtype=torch.int64)
+    t = torch.zeros(4, dtype=torch.int64)
+    assert fast.attention_fwd(q, k, v, None, None, None) is None
+    assert fast.attention_fwd(q, None, v, None, None, None) is None
+    assert fast.attention_fwd(q, k) is None and fast.attention_fwd(1, "a", [], {}, (), 0) is None
+    assert fast.attention_bwd(q, q, k, v, q, q, None, None, None, True, True) is None
+    assert fast.dropout(x, 0.1, seed, None) is None and fast.dropout(x) is None
+    assert fast.embedding_fwd(t, x, 1.0, 0.0, None, None) is None
+    assert fast.embedding_bwd(x, t, 5, 1.0, -1, 0.0, None, None) is None

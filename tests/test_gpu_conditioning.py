@@ -569,3 +569,68 @@ def test_captured_step_replays():
         torch.cuda.synchronize()
         for a, b in zip(held, want):
             assert torch.equal(a, b)
+
+
+# ---- the native calls and the general way -------------------------------------------------------
+def test_fast_calls_and_the_general_way_agree(monkeypatch):
+    """Both ways to a launch give the same bits, and the operands that need no conversion take the
+    native one."""
+    fast = C._fast()
+    assert not isinstance(fast, C._General)
+    q, kv, dout, lengths, mask, _ = _case("bf16", 3, 40, 77, 4, 2, 64, "both", seed=31)
+    kv = torch.nan_to_num(kv)
+    k, v = kv[:, :, 0], kv[:, :, 1]
+    g = _gen(32)
+    x = torch.randn((6, 33), generator=g).cuda()
+    img = torch.randn((2, 8, 4, 4), generator=g).cuda().contiguous(memory_format=torch.channels_last)
+    table = torch.randn((20, 24), generator=g).cuda()
+    tokens = torch.randint(0, 20, (4, 7), generator=g).cuda()
+    grad = torch.randn((4, 7, 24), generator=g).cuda()
+
+    def calls():
+        kw = dict(key_lengths=lengths, key_mask=mask)
+        out, lse = C.cross_attention_fwd(q, k, v, **kw)
+        dkv = torch.empty_like(kv)
+        return [out, lse, *C.cross_attention_bwd(dout, q, k, v, out, lse, **kw),
+                *C.cross_attention_fwd(q, k, v, scale=0.3),
+                C._attention_bwd(dout, q, k, v, out, lse, lengths, mask, None, None, None)[0],
+                *C._attention_bwd(dout, q, k, v, out, lse, lengths, mask, None, dkv[:, :, 0], dkv[:, :, 1]), dkv,
+                C.dropout_fwd(x, 0.3, _seed(5)), C.dropout_fwd(img, 0.3, _seed(5), residual=img),
+                C.embedding_fwd(tokens, table, scale=2.0, p_drop=0.2, seed=_seed(6), out_dtype=torch.bfloat16),
+                C.embedding_fwd(tokens.int(), table),
+                C.embedding_bwd(grad, tokens, 20, scale=2.0, padding_idx=3, p_drop=0.2, seed=_seed(6)),
+                C.embedding_bwd(grad, tokens, 20, dtype=torch.bfloat16)]
+    assert fast.attention_fwd(q, k, v, lengths, mask, None) is not None
+    assert fast.attention_fwd(q[:2], k, v, None, None, None) is None                   # another batch
+    assert fast.attention_fwd(q, k, v, lengths.long(), None, None) is None             # int64 is converted
+    assert fast.dropout(img, 0.3, _seed(5), img) is not None
+    assert fast.dropout(img, 1.0, _seed(5), None) is None and fast.dropout(img, 0.3, None, None) is None
+    assert fast.embedding_bwd(grad, tokens, 20, 1.0, 20, 0.0, None, None) is None      # padding outside the rows
+    here = calls()
+    monkeypatch.setattr(C, "_FAST", C._General())
+    there = calls()
+    assert len(here) == len(there)
+    for a, b in zip(here, there):
+        assert a.dtype == b.dtype and a.stride() == b.stride() and torch.equal(a, b)
+
+
+def test_fast_calls_keep_to_the_current_stream_and_free_what_they_make():
+    q = torch.randn((2, 64, 2, 64), device="cuda").bfloat16()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        big = torch.randn((1 << 24,), device="cuda")
+        x = (big * 0 + 2).view(-1)                 # work in flight that the call has to stand behind
+        y = C.dropout_fwd(x, 0.5, _seed(3))
+    torch.cuda.current_stream().wait_stream(side)
+    assert bool(((y == 0) | (y == 4)).all()) and bool(y.any())
+    del x, y, big
+    torch.cuda.synchronize()
+    for _ in range(3):
+        C.cross_attention_fwd(q, q, q)
+    before = torch.cuda.memory_allocated()
+    for _ in range(20):
+        o, lse = C.cross_attention_fwd(q, q, q)
+        C.cross_attention_bwd(q, q, q, q, o, lse)
+    del o, lse
+    assert torch.cuda.memory_allocated() == before
