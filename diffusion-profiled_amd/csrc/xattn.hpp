@@ -495,15 +495,23 @@ inline void set_grid(Args& p, int64_t total, int64_t per_head) {
   p.grid = (uint32_t)(ceil_div(total, 8 * unit) * 8 * unit);
 }
 
-// The forward's and dQ's tiles: rows of up to 32 go to the form whose waves share them
-inline bool few_rows(const Args& p) { return p.rows <= 32; }
-
 inline int dim_pad(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
+// The forward's and dQ's forms: four waves of 32 rows that share tiles of keys, or four waves that
+// share 32 rows and take every fourth tile each. The second reads the keys four times as often. It is
+// taken for up to 32 rows of a head, and by the forward where it comes to less than two workgroups a
+// CU: the first would leave CUs idle. (84 x 38 queries of 4 heads, 80 dims, over 412 keys of one: 13.4
+// against 17.4 us; 15 x 1869 of 2 heads over 522 keys, which has more: 30 against 21 us. dQ, whose
+// buffers leave a CU one workgroup of 128 dims, gains nothing: 26 against 19 us in the first case.)
+inline bool few_rows_dq(const Args& p) { return p.rows <= 32; }
+inline bool few_rows_fwd(const Args& p) {
+  return p.rows <= 32 || (int64_t)p.B * p.KVH * ceil_div(p.rows, 32) < 2 * num_cus();
+}
 
 // Forms that keep a head's keys in LDS (xattn_short.hip). The backward's takes up to 96 keys of more
 // than 64 dims: its buffers for more pass a CU's LDS.
-inline bool short_keys_fwd(const Args& p) { return !few_rows(p) && p.Lk <= 128; }
-inline bool short_keys_bwd(const Args& p) { return !few_rows(p) && p.Lk <= (dim_pad(p.D) == 128 ? 96 : 128); }
+inline bool short_keys_fwd(const Args& p) { return p.rows > 32 && p.Lk <= 128; }
+inline bool short_keys_bwd(const Args& p) { return p.rows > 32 && p.Lk <= (dim_pad(p.D) == 128 ? 96 : 128); }
 
 inline void plan_short(Args& p, int per_cu, int least) {
   p.tiles = (int)ceil_div(p.rows, 128);
@@ -515,9 +523,8 @@ inline void plan_short(Args& p, int per_cu, int least) {
 int short_fwd(const Args& p, int dtype, hipStream_t s);
 int short_bwd(const Args& p, int dtype, hipStream_t s);
 
-inline void plan_rows(Args& p) {
-  const bool few = few_rows(p);
-  p.tiles = few ? 1 : (int)ceil_div(p.rows, 128);
+inline void plan_rows(Args& p, bool few) {
+  p.tiles = (int)ceil_div(p.rows > 0 ? p.rows : 1, few ? 32 : 128);
   const int64_t groups = (int64_t)p.B * p.KVH * p.tiles, kt = few ? 32 : 64;
   choose_splits(p, groups, ceil_div(p.Lk, kt), (few ? 4 : 2) * num_cus(), 8, kMaxRange / kt, few ? 4 : 1);
   set_grid(p, groups * p.splits, (int64_t)p.tiles * p.splits);

@@ -56,7 +56,7 @@ struct QueryRow {
   }
 };
 
-// More than 32 rows: four waves of 32 query rows each share tiles of 64 keys.
+// Four waves of 32 query rows each share tiles of 64 keys.
 template <class T, int DP>
 __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_dq_kernel(const Args p) {
   constexpr int KT = 64;
@@ -512,7 +512,7 @@ static int64_t bwd_workspace(const Args& rows, const Args& keys) {
 extern "C" int64_t dpa_cross_attention_bwd_workspace_bytes(const DpaCrossAttention* a) {
   if (!a || check_shape(*a) != DPA_OK) return 0;
   Args r = make_args(*a), k = r, one = r;
-  plan_rows(r);
+  plan_rows(r, few_rows_dq(r));
   plan_keys(k);
   const int64_t two = bwd_workspace(r, k);
   if (!short_keys_bwd(one)) return two;
@@ -531,7 +531,7 @@ static int sum_keys(const Args& k, hipStream_t s) {
 template <class T, int DP>
 static int launch_bwd(const Args& r, const Args& k, hipStream_t s) {
   if (r.total > 0) {
-    if (few_rows(r))
+    if (few_rows_dq(r))
       xattn_dq_few_kernel<T, DP><<<r.grid, 256, 0, s>>>(r);
     else
       xattn_dq_kernel<T, DP><<<r.grid, 256, 0, s>>>(r);
@@ -591,7 +591,7 @@ extern "C" int dpa_cross_attention_bwd(const DpaCrossAttention* a, void* workspa
     if (status != DPA_OK || !a->dk) return status;
     return a->dtype == DPA_DTYPE_BF16 ? sum_keys<Bf16>(k, s) : sum_keys<F16>(k, s);
   }
-  plan_rows(r);
+  plan_rows(r, few_rows_dq(r));
   plan_keys(k);
   const int64_t need = bwd_workspace(r, k);
   if (need) {

@@ -8,7 +8,7 @@ namespace dpa {
 namespace xattn {
 
 // ---------------------------------------------------------------------------------------
-// More than 32 rows: four waves of 32 query rows each share tiles of 64 keys, double-buffered by
+// Four waves of 32 query rows each share tiles of 64 keys, double-buffered by
 // DMA.
 //
 // Per tile a wave forms S^T = K Q^T (A: key rows from LDS, B: its queries, in registers), so lane
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_fwd_kernel(const
 }
 
 // ---------------------------------------------------------------------------------------
-// Up to 32 rows: the four waves share them and take every fourth tile of 32 keys each, and join
+// Few workgroups: the four waves share 32 rows and take every fourth tile of 32 keys each, and join
 // their softmaxes in LDS at the end. Products as above. This form reads the keys and values once
 // and does little with them, so it is made for bytes in flight: keys go straight to registers as A
 // operands, values to LDS, each one tile ahead, and two workgroups of 128 dims fit a CU.
@@ -177,7 +177,9 @@ __global__ __launch_bounds__(256, 2) void xattn_few_kernel(const Args p) {
   const uint32_t id = work_item(p);
   if (id >= p.total) return;
   const int split = id % (uint32_t)p.splits;
-  const int bkv = id / (uint32_t)p.splits;
+  const uint32_t bt = id / (uint32_t)p.splits;
+  const int tile = bt % (uint32_t)p.tiles;
+  const int bkv = bt / (uint32_t)p.tiles;
   const int b = bkv / p.KVH, g = bkv - b * p.KVH;
 
   const int klen = __builtin_amdgcn_readfirstlane(keys_of(p, b));
@@ -189,7 +191,7 @@ __global__ __launch_bounds__(256, 2) void xattn_few_kernel(const Args p) {
   const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
   t_hi = bits.tiles_to<KT>(t_hi);
 
-  const int row = col;
+  const int row = tile * 32 + col;
   const bool has_row = row < p.rows;
   const uint32_t head = fdiv(has_row ? row : 0, p.by_lq), tok = (has_row ? row : 0) - head * p.Lq;
   uint4 kf[2][KS];
@@ -331,9 +333,51 @@ __global__ __launch_bounds__(256, 2) void xattn_few_kernel(const Args p) {
           uint2{T::pack(acc[i] * il, acc[i + 1] * il), T::pack(acc[i + 2] * il, acc[i + 3] * il)};
 }
 
-// Joins the splits of a row: O = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s. A wave per row, two
-// dims per lane; its splits' (max, sum) come in one load, so that the sums over the splits, whose
-// loads wait for nothing else, are the only loop.
+// Joins the splits of a row: O = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s. Up to kJoinSplits: a
+// thread per 4 dims of a row, all its loads at once. More: a wave per row, two dims per lane; its
+// splits' (max, sum) come in one load, so that the sums over the splits, whose loads wait for nothing
+// else, are the only loop. (32768 rows of 2 splits: 18 us by waves.)
+constexpr int kJoinSplits = 8;
+
+template <class T>
+__global__ __launch_bounds__(256) void xattn_join_few_kernel(const Args p) {
+  const int nd = p.D / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)p.B * p.KVH * p.rows;
+  if (i >= rows * nd) return;
+  const int64_t at = i / nd;
+  const int d0 = (int)(i - at * nd) * 4;
+  float2 ml[kJoinSplits];
+  float4 v[kJoinSplits];
+#pragma unroll
+  for (int s = 0; s < kJoinSplits; ++s)
+    if (s < p.splits) {
+      ml[s] = p.stat[s * rows + at];
+      v[s] = *reinterpret_cast<const float4*>(p.part + (s * rows + at) * p.D + d0);
+    }
+  float m = -__builtin_inff();
+#pragma unroll
+  for (int s = 0; s < kJoinSplits; ++s)
+    if (s < p.splits) m = fmaxf(m, ml[s].x);
+  const float ms = m == -__builtin_inff() ? 0.f : m;
+  float l = 0.f;
+  float4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < kJoinSplits; ++s)
+    if (s < p.splits) {
+      const float f = __builtin_amdgcn_exp2f(ml[s].x - ms);
+      l += f * ml[s].y;
+      o.x += f * v[s].x, o.y += f * v[s].y, o.z += f * v[s].z, o.w += f * v[s].w;
+    }
+  const int bkv = (int)(at / p.rows), row = (int)(at - (int64_t)bkv * p.rows);
+  const int b = bkv / p.KVH, g = bkv - b * p.KVH;
+  const uint32_t head = fdiv(row, p.by_lq), tok = row - head * p.Lq;
+  if (d0 == 0)
+    p.lse[((int64_t)b * p.H + g * p.G + head) * p.Lq + tok] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+  const float il = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(p.out + (((int64_t)b * p.Lq + tok) * p.H + g * p.G + head) * p.D + d0) =
+      uint2{T::pack(o.x * il, o.y * il), T::pack(o.z * il, o.w * il)};
+}
+
 template <class T>
 __global__ __launch_bounds__(256) void xattn_join_kernel(const Args p) {
   const int lane = threadIdx.x & 63;
@@ -395,13 +439,13 @@ extern "C" int64_t dpa_cross_attention_fwd_workspace_bytes(const DpaCrossAttenti
   if (!a || check_shape(*a) != DPA_OK) return 0;
   Args p = make_args(*a);
   if (short_keys_fwd(p)) return 0;
-  plan_rows(p);
+  plan_rows(p, few_rows_fwd(p));
   return fwd_workspace(p);
 }
 
 template <class T, int DP>
 static void launch_fwd(const Args& p, hipStream_t s) {
-  if (few_rows(p))
+  if (few_rows_fwd(p))
     xattn_few_kernel<T, DP><<<p.grid, 256, 0, s>>>(p);
   else
     xattn_fwd_kernel<T, DP><<<p.grid, 256, 0, s>>>(p);
@@ -416,7 +460,11 @@ static int run_fwd(const Args& p, hipStream_t s) {
   }
   int st = launch_status();
   if (st != DPA_OK || p.splits <= 1) return st;
-  xattn_join_kernel<T><<<(unsigned)ceil_div((int64_t)p.B * p.KVH * p.rows, 4), 256, 0, s>>>(p);
+  const int64_t rows = (int64_t)p.B * p.KVH * p.rows;
+  if (p.splits <= kJoinSplits)
+    xattn_join_few_kernel<T><<<(unsigned)ceil_div(rows * (p.D / 4), 256), 256, 0, s>>>(p);
+  else
+    xattn_join_kernel<T><<<(unsigned)ceil_div(rows, 4), 256, 0, s>>>(p);
   return launch_status();
 }
 
@@ -437,7 +485,7 @@ extern "C" int dpa_cross_attention_fwd(const DpaCrossAttention* a, void* workspa
     plan_short(p, 4, 1);
     return short_fwd(p, a->dtype, s);
   }
-  plan_rows(p);
+  plan_rows(p, few_rows_fwd(p));
   const int64_t need = fwd_workspace(p);
   if (need) {
     if (!workspace || workspace_bytes < need) return DPA_ERR_WORKSPACE;
