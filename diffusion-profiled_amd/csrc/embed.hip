@@ -173,6 +173,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const Args p) {
 // table that is most of the backward's bytes, and it hides most of the sort.
 // ---------------------------------------------------------------------------------------
 constexpr int kChunk = 1024, kSortWaves = kChunk / 64, kMerge = 16, kSample = 32;
+constexpr int kBatch = 16;  // rows that a wave loads together
 
 struct Fill {  // clears 16-B units and the bytes past them
   uint4* at;
@@ -194,35 +195,27 @@ struct SortArgs {
   Fill fill;
 };
 
-template <int TB>
-__global__ __launch_bounds__(kChunk) void embed_sort_kernel(const SortArgs p) {
-  __shared__ uint32_t key[kChunk];
-  __shared__ uint16_t idx[2][kChunk];
-  __shared__ uint32_t hist[kSortWaves][256];
-  __shared__ uint32_t wsum[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+struct ChunkLds {
+  uint32_t key[kChunk];
+  uint16_t idx[2][kChunk];
+  uint32_t hist[kSortWaves][256];
+  uint32_t wsum[4];
+};
 
-  if ((int)blockIdx.x >= p.chunks) {
-    p.fill.run(blockIdx.x - p.chunks, gridDim.x - p.chunks, kChunk, tid);
-    return;
-  }
-
-  const int64_t c0 = (int64_t)blockIdx.x * kChunk;
-  const int m = (int)(p.n - c0 < kChunk ? p.n - c0 : kChunk);
+// Sorts the chunk's m keys (key[0 .. m), by the workgroup, a thread each) by their lowest 8 `passes`
+// bits: gives the places' original places. Ends with a barrier.
+__device__ __forceinline__ const uint16_t* sort_chunk(ChunkLds& s, int m, int passes, int tid) {
+  const int lane = tid & 63, wave = tid >> 6;
   const bool on = tid < m;
-  if (on) {
-    const int64_t t = token_at<TB>(p.tokens, c0 + tid);
-    key[tid] = t < 0 || t >= (int64_t)p.V || t == (int64_t)p.pad ? p.V : (uint32_t)t;
-    idx[0][tid] = (uint16_t)tid;
-  }
-  for (int pass = 0; pass < p.passes; ++pass) {
-    const uint16_t* a = idx[pass & 1];
-    uint16_t* o = idx[(pass & 1) ^ 1];
-    for (int i = tid; i < kSortWaves * 256; i += kChunk) (&hist[0][0])[i] = 0;
+  if (on) s.idx[0][tid] = (uint16_t)tid;
+  for (int pass = 0; pass < passes; ++pass) {
+    const uint16_t* a = s.idx[pass & 1];
+    uint16_t* o = s.idx[(pass & 1) ^ 1];
+    for (int i = tid; i < kSortWaves * 256; i += kChunk) (&s.hist[0][0])[i] = 0;
     __syncthreads();
     // a wave's places in order: how many lower lanes share this one's digit, and how many lanes do
     const uint32_t x = on ? a[tid] : 0;
-    const uint32_t d = on ? (key[x] >> (8 * pass)) & 255 : 0;
+    const uint32_t d = on ? (s.key[x] >> (8 * pass)) & 255 : 0;
     uint64_t same = __ballot(on);
 #pragma unroll
     for (int bit = 0; bit < 8; ++bit) {
@@ -230,13 +223,13 @@ __global__ __launch_bounds__(kChunk) void embed_sort_kernel(const SortArgs p) {
       same &= (d >> bit) & 1 ? ones : ~ones;
     }
     const int before = __popcll(same & ((1ull << lane) - 1));
-    if (on && before == 0) hist[wave][d] = (uint32_t)__popcll(same);
+    if (on && before == 0) s.hist[wave][d] = (uint32_t)__popcll(same);
     __syncthreads();
     // each (digit, wave)'s first place: digits in order, waves in order within a digit
     uint32_t sum = 0, first[kSortWaves];
     if (tid < 256) {
 #pragma unroll
-      for (int w = 0; w < kSortWaves; ++w) first[w] = hist[w][tid];
+      for (int w = 0; w < kSortWaves; ++w) first[w] = s.hist[w][tid];
 #pragma unroll
       for (int w = 0; w < kSortWaves; ++w) {
         const uint32_t c = first[w];
@@ -249,24 +242,152 @@ __global__ __launch_bounds__(kChunk) void embed_sort_kernel(const SortArgs p) {
         const uint32_t y = __shfl_up(incl, off, 64);
         if (lane >= off) incl += y;
       }
-      if (lane == 63) wsum[wave] = incl;
+      if (lane == 63) s.wsum[wave] = incl;
       sum = incl - sum;
     }
     __syncthreads();
     if (tid < 256) {
-      for (int w = 0; w < wave; ++w) sum += wsum[w];
+      for (int w = 0; w < wave; ++w) sum += s.wsum[w];
 #pragma unroll
-      for (int w = 0; w < kSortWaves; ++w) hist[w][tid] = first[w] + sum;
+      for (int w = 0; w < kSortWaves; ++w) s.hist[w][tid] = first[w] + sum;
     }
     __syncthreads();
-    if (on) o[hist[wave][d] + before] = (uint16_t)x;
+    if (on) o[s.hist[wave][d] + before] = (uint16_t)x;
     __syncthreads();
   }
-  if (on) {
-    const uint32_t x = idx[p.passes & 1][tid], k = key[x];
+  return s.idx[passes & 1];
+}
+
+// a token's key: V for those without a gradient
+template <int TB>
+__device__ __forceinline__ uint32_t key_of(const void* tokens, int64_t i, uint32_t V, uint32_t pad) {
+  const int64_t t = token_at<TB>(tokens, i);
+  return t < 0 || t >= (int64_t)V || t == (int64_t)pad ? V : (uint32_t)t;
+}
+
+template <int TB>
+__global__ __launch_bounds__(kChunk) void embed_sort_kernel(const SortArgs p) {
+  __shared__ ChunkLds s;
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x >= p.chunks) {
+    p.fill.run(blockIdx.x - p.chunks, gridDim.x - p.chunks, kChunk, tid);
+    return;
+  }
+  const int64_t c0 = (int64_t)blockIdx.x * kChunk;
+  const int m = (int)(p.n - c0 < kChunk ? p.n - c0 : kChunk);
+  if (tid < m) s.key[tid] = key_of<TB>(p.tokens, c0 + tid, p.V, p.pad);
+  const uint16_t* order = sort_chunk(s, m, p.passes, tid);
+  if (tid < m) {
+    const uint32_t x = order[tid], k = s.key[x];
     p.key[c0 + tid] = k;
     p.pos[c0 + tid] = (uint32_t)(c0 + x);
     if (tid % kSample == 0) p.sample[(c0 + tid) / kSample] = k;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Up to kSmall tokens: the whole gradient in one launch, for whose others a small call would wait (512
+// tokens, 663 rows of 768: 12.2 us; with 1000 tokens it would be 17.9, and the three launches of the
+// form for more 14.7).
+// `slices` workgroups of 64 channels sort the tokens, each for itself, and sum: a wave takes 16, 32,
+// 48 or 64 sorted places; a run that goes on in the next wave is finished, in order, by the wave in which it
+// starts, from what the others leave in LDS. The other workgroups clear the rows that no token names
+// (a bit per row in LDS).
+// ---------------------------------------------------------------------------------------
+constexpr int kSmall = 512;
+constexpr int kSmallRows = 1 << 18;  // rows that the bits have room for
+
+template <int GT, int WT, int TB>
+__global__ __launch_bounds__(kChunk) void embed_small_kernel(const Args p, const void* tokens, int slices, int passes) {
+  __shared__ union {
+    struct {
+      ChunkLds sort;
+      float head[kSortWaves][64];
+    };
+    uint32_t named[kSmallRows / 32];
+  } s;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = (int)p.n;
+
+  if ((int)blockIdx.x >= slices) {
+    for (int i = tid; i < (int)(p.V + 31) / 32; i += kChunk) s.named[i] = 0;
+    __syncthreads();
+    if (tid < n) {
+      const uint32_t k = key_of<TB>(tokens, tid, p.V, p.pad);
+      if (k != p.V) atomicOr(&s.named[k / 32], 1u << (k % 32));
+    }
+    __syncthreads();
+    const int64_t step = (int64_t)(gridDim.x - slices) * kSortWaves;
+    const int bytes = p.C * Elem<WT>::size;
+    for (int64_t r = (int64_t)(blockIdx.x - slices) * kSortWaves + wave; r < p.V; r += step) {
+      if ((s.named[r / 32] >> (r % 32)) & 1) continue;
+      uint8_t* row = static_cast<uint8_t*>(p.dst) + r * bytes;
+      if (bytes % 16 == 0)
+        for (int i = lane * 16; i < bytes; i += 1024) *reinterpret_cast<uint4*>(row + i) = uint4{0u, 0u, 0u, 0u};
+      else
+        for (int i = lane * 2; i < bytes; i += 128) *reinterpret_cast<uint16_t*>(row + i) = 0;
+    }
+    return;
+  }
+
+  if (tid < n) s.sort.key[tid] = key_of<TB>(tokens, tid, p.V, p.pad);
+  const uint16_t* order = sort_chunk(s.sort, n, passes, tid);
+  const int per = (n + kSortWaves * kBatch - 1) / (kSortWaves * kBatch) * kBatch;  // a wave's places
+  const int place = wave * per + lane;
+  const bool on = lane < per && place < n;
+  const uint32_t at = on ? order[place] : 0;
+  const uint32_t k = on ? s.sort.key[at] : p.V;
+  const uint32_t before = on && place > 0 ? s.sort.key[order[place - 1]] : p.V;
+  const int count = __popcll(__ballot(k != p.V));  // (V's are behind the others)
+  const uint64_t starts = __ballot(k != p.V && (place == 0 || before != k));
+  const int c = blockIdx.x * 64 + lane, cl = c < p.C ? c : 0;
+  const uint64_t seed = p.seed ? *p.seed : 0;
+  const float factor = p.scale * p.keep_scale;
+
+  float acc = 0.f;
+  int from = starts & 1 ? 0 : -1;  // where the run at work starts (-1: in a wave before)
+  auto leave = [&](int end) __attribute__((always_inline)) {
+    if (from < 0) {
+      s.head[wave][lane] = acc;
+    } else if (end < per && c < p.C) {
+      const float v[1] = {acc * factor};
+      store<WT, 1>(p.dst, (int64_t)(uint32_t)__builtin_amdgcn_readlane(k, from) * p.C + c, v);
+    }
+  };
+  for (int j = 0; j < count; j += kBatch) {
+    float v[kBatch][1];
+    uint32_t pj[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      pj[u] = (uint32_t)__builtin_amdgcn_readlane(at, j + u < count ? j + u : count - 1);
+      load<GT, 1>(p.src, (int64_t)pj[u] * p.C + cl, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (j + u >= count) break;
+      if (j + u > 0 && ((starts >> (j + u)) & 1)) {
+        leave(j + u);
+        from = j + u;
+        acc = 0.f;
+      }
+      if (p.seed) drop<1>(seed, (int64_t)pj[u] * p.C + cl, p.keep2 & 0xffffu, v[u]);
+      acc += v[u][0];
+    }
+  }
+  if (count > 0) leave(count);
+  __syncthreads();
+  if (count < per || from < 0) return;
+  const uint32_t kr = (uint32_t)__builtin_amdgcn_readlane(k, from);
+  for (int w = wave + 1; w < kSortWaves; ++w) {
+    const int lo = w * per, hi = lo + per - 1;
+    if (lo >= n || s.sort.key[order[lo]] != kr) break;
+    acc += s.head[w][lane];
+    if (hi >= n || s.sort.key[order[hi]] != kr) break;
+  }
+  if (c < p.C) {
+    const float v[1] = {acc * factor};
+    store<WT, 1>(p.dst, (int64_t)kr * p.C + c, v);
   }
 }
 
@@ -342,7 +463,7 @@ __global__ __launch_bounds__(256) void embed_merge_kernel(const MergeArgs p) {
 // The runs that a wave sums lie side by side, so their places load together, kBatch rows at a time
 // whatever runs they belong to, and a run is stored where the next one begins.
 // ---------------------------------------------------------------------------------------
-constexpr int kOwn = 16, kPiece = 32, kBatch = 16;
+constexpr int kOwn = 16, kPiece = 32;
 
 // The first of the n sorted keys that is not smaller than want, by a wave: 64 probes a step
 __device__ __forceinline__ int64_t lower_bound(const uint32_t* key, int64_t n, uint32_t want, int lane) {
@@ -535,6 +656,17 @@ static int launch_sum(const Args& a, hipStream_t s) {
   return launch_status();
 }
 
+template <int GT, int WT>
+static int launch_small(const Args& a, const void* tokens, int token_bytes, int passes, hipStream_t s) {
+  const int slices = (int)ceil_div(a.C, 64);
+  int64_t fill = ceil_div(a.V, kSortWaves * 4);
+  if (fill > 2 * num_cus()) fill = 2 * num_cus();
+  const unsigned grid = (unsigned)(slices + fill);
+  if (token_bytes == 8) embed_small_kernel<GT, WT, 8><<<grid, kChunk, 0, s>>>(a, tokens, slices, passes);
+  else embed_small_kernel<GT, WT, 4><<<grid, kChunk, 0, s>>>(a, tokens, slices, passes);
+  return launch_status();
+}
+
 // f<T1, T2>(args ...) for the types d1, d2
 #define EMBED_BY_TYPES(d1, d2, CALL)                                        \
   switch ((d1) * 3 + (d2)) {                                               \
@@ -598,12 +730,25 @@ extern "C" int dpa_embedding_bwd(const void* dout, int dout_dtype, const void* t
   if (n > 0 && (!workspace || workspace_bytes < dpa_embedding_bwd_workspace_bytes(n, C)))
     return DPA_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return DPA_ERR_ALIGN;
+  hipStream_t s = (hipStream_t)stream;
+  const uint32_t pad = padding_idx >= 0 && padding_idx < V ? (uint32_t)padding_idx : 0xffffffffu;
+  int passes = 0;
+  while ((V >> (8 * passes)) > 0) ++passes;
+  Args a{};
+  a.src = dout, a.dst = dweight, a.n = n, a.V = (uint32_t)V, a.C = C, a.scale = scale, a.pad = pad;
+  set_drop(a, drop_seed, drop_p);
+  if (n > 0 && n <= kSmall && V <= kSmallRows) {
+#define SMALL(A, B) st = launch_small<A, B>(a, tokens, token_bytes, passes, s)
+    EMBED_BY_TYPES(dout_dtype, weight_dtype, SMALL)
+#undef SMALL
+    return st;
+  }
+
   uint8_t* w = (uint8_t*)workspace;
   const int64_t arr = align256(4 * n), smp = align256(4 * ceil_div(n, kSample));
   uint32_t* key[2] = {(uint32_t*)w, (uint32_t*)(w + arr)};
   uint32_t* pos[2] = {(uint32_t*)(w + 2 * arr), (uint32_t*)(w + 3 * arr)};
   uint32_t* sample[2] = {(uint32_t*)(w + 4 * arr), (uint32_t*)(w + 4 * arr + smp)};
-  hipStream_t s = (hipStream_t)stream;
 
   // dW, in equal parts to the launches of the sort
   int launches = 1;
@@ -618,10 +763,8 @@ extern "C" int dpa_embedding_bwd(const void* dout, int dout_dtype, const void* t
 
   SortArgs q{};
   q.tokens = tokens, q.key = key[0], q.pos = pos[0], q.sample = sample[0], q.n = n;
-  q.V = (uint32_t)V;
-  q.pad = padding_idx >= 0 && padding_idx < V ? (uint32_t)padding_idx : 0xffffffffu;
+  q.V = (uint32_t)V, q.pad = pad, q.passes = passes;
   q.chunks = (int)ceil_div(n, kChunk);
-  while ((V >> (8 * q.passes)) > 0) ++q.passes;
   int blocks;
   q.fill = fill(0, kChunk, &blocks);
   const unsigned grid = (unsigned)(q.chunks + blocks);
@@ -643,10 +786,7 @@ extern "C" int dpa_embedding_bwd(const void* dout, int dout_dtype, const void* t
     st = launch_status();
     if (st != DPA_OK) return st;
   }
-  Args a{};
-  a.src = dout, a.dst = dweight, a.n = n, a.V = (uint32_t)V, a.C = C, a.scale = scale;
   a.key = key[at], a.pos = pos[at], a.part = (float*)(w + 4 * arr + 2 * smp);
-  set_drop(a, drop_seed, drop_p);
 #define SUM(A, B) st = launch_sum<A, B>(a, s)
   EMBED_BY_TYPES(dout_dtype, weight_dtype, SUM)
 #undef SUM

@@ -193,6 +193,84 @@ def test_attention_against_64_bits(dtype, b, lq, lk, h, kvh, d, kind):
     assert all(torch.equal(x, y) for x, y in zip((dq, dk, dv), again))
 
 
+MORE = [
+    # up to 128 keys: blocks of 32 that are empty, one tile and several, splits of the rows, every
+    # padded head size
+    ("bf16", 2, 130, 1, 2, 2, 64, "none"),
+    ("fp16", 3, 128, 32, 2, 1, 32, "bool"),
+    ("bf16", 5, 400, 33, 2, 2, 64, "lengths"),
+    ("bf16", 1, 1500, 77, 2, 1, 40, "bool"),
+    ("fp16", 5, 50, 96, 3, 3, 128, "both"),
+    ("bf16", 4, 140, 97, 2, 2, 64, "lengths"),
+    ("fp16", 4, 200, 128, 4, 2, 32, "both"),
+    ("bf16", 5, 90, 97, 2, 2, 128, "bool"),
+    ("bf16", 5, 600, 128, 1, 1, 24, "lengths"),
+    # more: tiles at the length's border, whole tiles hidden, rows in both forms, heads that share keys
+    # in tiles that lie in one head or in two
+    ("bf16", 3, 64, 129, 2, 2, 64, "bool"),
+    ("fp16", 6, 1000, 192, 8, 2, 64, "both"),
+    ("bf16", 6, 1000, 320, 8, 2, 32, "lengths"),
+    ("bf16", 40, 300, 200, 4, 4, 64, "both"),
+    ("fp16", 20, 130, 640, 6, 3, 128, "lengths"),
+    ("bf16", 9, 512, 1024, 8, 8, 64, "none"),
+]
+
+
+@pytest.mark.parametrize("dtype,b,lq,lk,h,kvh,d,kind", MORE)
+def test_attention_forms_against_64_bits(dtype, b, lq, lk, h, kvh, d, kind):
+    test_attention_against_64_bits(dtype, b, lq, lk, h, kvh, d, kind)
+    # a frozen encoder: dq alone, the same bits
+    q, kv, dout, lengths, mask, _ = _case(dtype, b, lq, lk, h, kvh, d, kind, seed=lq + lk)
+    k, v = kv[:, :, 0], kv[:, :, 1]
+    kw = dict(key_lengths=lengths, key_mask=mask)
+    out, lse = C.cross_attention_fwd(q, k, v, **kw)
+    both = C.cross_attention_bwd(dout, q, k, v, out, lse, **kw)
+    alone = C._attention_bwd(dout, q, k, v, out, lse, lengths, mask, None, None, None)
+    assert alone[1] is None and alone[2] is None and torch.equal(alone[0], both[0])
+
+
+@pytest.mark.parametrize("lk", [50, 700])
+def test_attention_far_strides(lk):
+    """Rows of keys more than 2^24 elements apart and a whole cache past 2^31 of them."""
+    step = (1 << 32) // lk // 8 * 8 if lk == 50 else (1 << 23) + 8
+    room = torch.empty((lk - 1) * step + 2 * 64, device="cuda", dtype=torch.bfloat16)
+    far = room.as_strided((1, lk, 2, 64), (0, step, 64, 1))
+    g = _gen(41)
+    q = torch.randn((1, 100, 4, 64), generator=g).bfloat16().cuda()
+    near = torch.randn((1, lk, 2, 64), generator=g).bfloat16().cuda()
+    far.copy_(near)
+    a, c = C.cross_attention_fwd(q, far, far), C.cross_attention_fwd(q, near, near)
+    assert all(torch.equal(x, y) for x, y in zip(a, c))
+    dout = torch.randn(q.shape, generator=g).bfloat16().cuda()
+    a = C.cross_attention_bwd(dout, q, far, far, *a)
+    c = C.cross_attention_bwd(dout, q, near, near, *c)
+    assert all(torch.equal(x, y) for x, y in zip(a, c))
+    one = q[:, :1]
+    a, c = C.cross_attention_fwd(one, far, far), C.cross_attention_fwd(one, near, near)
+    assert all(torch.equal(x, y) for x, y in zip(a, c))
+
+
+def test_attention_extreme_masked_scores():
+    """Hidden keys whose scores would be the largest, rows whose scores are far below zero, and
+    batches whose mask hides everything, in every form."""
+    for lq, lk in ((1, 40), (70, 77), (70, 300), (300, 900)):
+        q, kv, dout, _, _, _ = _case("bf16", 3, lq, lk, 2, 2, 64, "none", seed=51)
+        mask = (torch.rand((3, lk), generator=_gen(52)) < 0.5).cuda()
+        mask[2] = False
+        kv = torch.where(mask[:, :, None, None, None], kv, torch.full_like(kv, 3e4))
+        q = q.clone()
+        q[0] *= 40.0                                   # scores of hundreds
+        k, v = kv[:, :, 0], kv[:, :, 1]
+        out, lse = C.cross_attention_fwd(q, k, v, key_mask=mask)
+        grads = C.cross_attention_bwd(dout, q, k, v, out, lse, key_mask=mask)
+        assert not out[2].any() and bool((lse[2] == -math.inf).all())
+        assert all(t.isfinite().all() for t in (out, *grads))
+        assert not grads[0][2].any() and not grads[1][2].any() and not grads[2][2].any()
+        clean = torch.where(mask[:, :, None, None, None], kv, torch.zeros_like(kv))
+        again = C.cross_attention_fwd(q, clean[:, :, 0], clean[:, :, 1], key_mask=mask)
+        assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
 @pytest.mark.parametrize("lq,lk", [(0, 5), (3, 0), (0, 0), (40, 0)])
 def test_attention_empty(lq, lk):
     q = torch.randn((2, lq, 4, 64), device="cuda").bfloat16()
@@ -498,6 +576,28 @@ def test_embedding_gradient(n, v, c, gt, wt, pad, p):
         assert torch.equal(dw, C.embedding_bwd(dout, tokens, v, **kw))
         if pad is not None:
             assert not dw[pad].any()
+
+
+@pytest.mark.parametrize("n,v,c", [(17, 2, 70), (255, 1, 64), (256, 3, 65), (257, 1000, 130), (512, 2, 3),
+                                   (512, 2**18, 8), (511, 2**18 + 1, 8), (513, 5, 64), (300, 40000, 1)])
+@pytest.mark.parametrize("gt,wt,pad", [("fp32", "fp32", None), ("bf16", "bf16", 0), ("fp16", "fp32", 1)])
+def test_embedding_gradient_few_tokens(n, v, c, gt, wt, pad):
+    """The form of one launch and its border: runs over several waves, rows that no token names, odd
+    widths, tokens outside the table."""
+    print(f"embedding_bwd n={n} v={v} c={c} {gt} {wt} pad={pad}", flush=True)
+    pad = pad if pad is None or pad < v else None
+    g = _gen(n * 31 + v)
+    t = torch.randint(0, v, (n,), generator=g)
+    t = torch.where(torch.rand(n, generator=g) < 0.05, torch.randint(-2, v + 2, (n,), generator=g), t).cuda()
+    dout = torch.randn((n, c), generator=g).to(DT[gt]).cuda()
+    for p in (0.0, 0.3):
+        dw = C.embedding_bwd(dout, t, v, scale=0.8, padding_idx=pad, dtype=DT[wt], p_drop=p,
+                             seed=_seed(77) if p else None)
+        torch.cuda.synchronize()
+        exact, bound = _dw_reference(dout, t, v, 0.8, pad, p, 77)
+        tiny = torch.finfo(DT[wt]).smallest_normal * torch.finfo(DT[wt]).eps
+        over = (dw.double() - exact).abs() - (bound + HALF[DT[wt]] * exact.abs() + tiny)
+        assert float(over.max()) <= 0, f"{int((over > 0).sum())} beyond the bound, worst {float(over.max()):.3e}"
 
 
 def test_embedding_gradient_without_tokens():
