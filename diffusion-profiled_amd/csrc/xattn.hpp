@@ -508,10 +508,11 @@ inline bool few_rows_fwd(const Args& p) {
   return p.rows <= 32 || (int64_t)p.B * p.KVH * ceil_div(p.rows, 32) < 2 * num_cus();
 }
 
-// Forms that keep a head's keys in LDS (xattn_short.hip). The backward's takes up to 96 keys of more
-// than 64 dims: its buffers for more pass a CU's LDS.
+// Forms that keep a head's keys in LDS (xattn_short.hip). The forward's is for more than 32 rows: one
+// wave would work on fewer. The backward's takes any number, since it is one launch for two, and up to
+// 96 keys of more than 64 dims: its buffers for more pass a CU's LDS.
 inline bool short_keys_fwd(const Args& p) { return p.rows > 32 && p.Lk <= 128; }
-inline bool short_keys_bwd(const Args& p) { return p.rows > 32 && p.Lk <= (dim_pad(p.D) == 128 ? 96 : 128); }
+inline bool short_keys_bwd(const Args& p) { return p.rows > 0 && p.Lk <= (dim_pad(p.D) == 128 ? 96 : 128); }
 
 inline void plan_short(Args& p, int per_cu, int least) {
   p.tiles = (int)ceil_div(p.rows, 128);

@@ -508,21 +508,24 @@ static int64_t bwd_workspace(const Args& rows, const Args& keys) {
   return stat_bytes(rows) + (a > b ? a : b);
 }
 
-// (the most that a call with or without dk and dv needs)
+// Never 0: a caller without one is told so at every size.
+static int64_t short_workspace(const Args& k) { return align256(part_keys_bytes(k) + 1); }
+
 extern "C" int64_t dpa_cross_attention_bwd_workspace_bytes(const DpaCrossAttention* a) {
   if (!a || check_shape(*a) != DPA_OK) return 0;
-  Args r = make_args(*a), k = r, one = r;
+  Args r = make_args(*a), k = r;
+  if (short_keys_bwd(k)) {
+    plan_short(k, 2, 2);
+    return short_workspace(k);
+  }
   plan_rows(r, few_rows_dq(r));
   plan_keys(k);
-  const int64_t two = bwd_workspace(r, k);
-  if (!short_keys_bwd(one)) return two;
-  plan_short(one, 2, 2);
-  return two > part_keys_bytes(one) ? two : part_keys_bytes(one);
+  return bwd_workspace(r, k);
 }
 
 template <class T>
 static int sum_keys(const Args& k, hipStream_t s) {
-  if (k.splits <= 1) return DPA_OK;
+  if (k.splits <= 1 || k.Lk == 0) return DPA_OK;
   const int64_t n = (int64_t)k.B * k.KVH * k.Lk * 2 * (k.D / 8);
   xattn_sum_kernel<T, false><<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(k);
   return launch_status();
@@ -583,8 +586,7 @@ extern "C" int dpa_cross_attention_bwd(const DpaCrossAttention* a, void* workspa
   hipStream_t s = (hipStream_t)stream;
   if (short_keys_bwd(k)) {
     plan_short(k, 2, 2);
-    const int64_t need = a->dk ? part_keys_bytes(k) : 0;
-    if (need && (!workspace || workspace_bytes < need)) return DPA_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < short_workspace(k)) return DPA_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return DPA_ERR_ALIGN;
     k.part = (float*)workspace;
     const int status = short_bwd(k, a->dtype, s);

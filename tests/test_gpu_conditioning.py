@@ -250,6 +250,16 @@ def test_attention_far_strides(lk):
     assert all(torch.equal(x, y) for x, y in zip(a, c))
 
 
+def test_attention_no_keys_many_queries():
+    """Rows that would be split over workgroups, and no key to sum for."""
+    q = torch.randn((1, 3000, 1, 64), device="cuda").bfloat16()
+    k = q[:, :0]
+    out, lse = C.cross_attention_fwd(q, k, k)
+    dq, dk, dv = C.cross_attention_bwd(q, q, k, k, out, lse)
+    assert not out.any() and bool((lse == -math.inf).all()) and not dq.any()
+    assert dk.shape == (1, 0, 1, 64) and dv.shape == dk.shape
+
+
 def test_attention_extreme_masked_scores():
     """Hidden keys whose scores would be the largest, rows whose scores are far below zero, and
     batches whose mask hides everything, in every form."""
