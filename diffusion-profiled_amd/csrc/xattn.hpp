@@ -514,10 +514,14 @@ inline bool few_rows_fwd(const Args& p) {
 inline bool short_keys_fwd(const Args& p) { return p.rows > 32 && p.Lk <= 128; }
 inline bool short_keys_bwd(const Args& p) { return p.rows > 0 && p.Lk <= (dim_pad(p.D) == 128 ? 96 : 128); }
 
-inline void plan_short(Args& p, int per_cu, int least) {
+// Rows are split so that the workgroups that fit the chip at once share them; the backward's splits
+// write fp32 sums of dK and dV each, so it leaves at least two tiles of rows to one.
+inline void plan_short(Args& p, bool backward) {
+  const int dp = dim_pad(p.D);
+  const int per_cu = backward ? (dp == 128 || (dp == 64 && p.Lk > 96) ? 1 : 2) : dp == 128 ? 2 : 4;
   p.tiles = (int)ceil_div(p.rows, 128);
   const int64_t groups = (int64_t)p.B * p.KVH;
-  choose_splits(p, groups, p.tiles, per_cu * num_cus(), least, 1ll << 30, 1);
+  choose_splits(p, groups, p.tiles, per_cu * num_cus(), backward ? 2 : 1, 1ll << 30, 1);
   set_grid(p, groups * p.splits, p.splits);
 }
 

@@ -515,7 +515,7 @@ extern "C" int64_t dpa_cross_attention_bwd_workspace_bytes(const DpaCrossAttenti
   if (!a || check_shape(*a) != DPA_OK) return 0;
   Args r = make_args(*a), k = r;
   if (short_keys_bwd(k)) {
-    plan_short(k, 2, 2);
+    plan_short(k, true);
     return short_workspace(k);
   }
   plan_rows(r, few_rows_dq(r));
@@ -585,7 +585,7 @@ extern "C" int dpa_cross_attention_bwd(const DpaCrossAttention* a, void* workspa
   Args r = make_args(*a), k = r;
   hipStream_t s = (hipStream_t)stream;
   if (short_keys_bwd(k)) {
-    plan_short(k, 2, 2);
+    plan_short(k, true);
     if (!workspace || workspace_bytes < short_workspace(k)) return DPA_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return DPA_ERR_ALIGN;
     k.part = (float*)workspace;

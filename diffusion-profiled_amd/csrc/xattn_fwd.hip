@@ -482,7 +482,7 @@ extern "C" int dpa_cross_attention_fwd(const DpaCrossAttention* a, void* workspa
   Args p = make_args(*a);
   hipStream_t s = (hipStream_t)stream;
   if (short_keys_fwd(p)) {
-    plan_short(p, 4, 1);
+    plan_short(p, false);
     return short_fwd(p, a->dtype, s);
   }
   plan_rows(p, few_rows_fwd(p));
