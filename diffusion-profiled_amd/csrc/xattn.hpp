@@ -512,7 +512,7 @@ inline bool few_rows_fwd(const Args& p) {
 // wave would work on fewer. The backward's takes any number, since it is one launch for two, and up to
 // 96 keys of more than 64 dims: its buffers for more pass a CU's LDS.
 inline bool short_keys_fwd(const Args& p) { return p.rows > 32 && p.Lk <= 128; }
-inline bool short_keys_bwd(const Args& p) { return p.rows > 0 && p.Lk <= (dim_pad(p.D) == 128 ? 96 : 128); }
+inline bool short_keys_bwd(const Args& p) { return p.rows > 0 && p.Lk <= 128; }
 
 // Rows are split so that the workgroups that fit the chip at once share them; the backward's splits
 // write fp32 sums of dK and dV each, so it leaves at least two tiles of rows to one.

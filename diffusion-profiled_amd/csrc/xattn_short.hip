@@ -343,7 +343,7 @@ static int run_short_bwd(const Args& p, hipStream_t s) {
   switch (dim_pad(p.D)) {
     case 32: return p.Lk <= 96 ? launch_short_bwd<T, 32, 3>(p, s) : launch_short_bwd<T, 32, 4>(p, s);
     case 64: return p.Lk <= 96 ? launch_short_bwd<T, 64, 3>(p, s) : launch_short_bwd<T, 64, 4>(p, s);
-    default: return launch_short_bwd<T, 128, 3>(p, s);
+    default: return p.Lk <= 96 ? launch_short_bwd<T, 128, 3>(p, s) : launch_short_bwd<T, 128, 4>(p, s);
   }
 }
 
