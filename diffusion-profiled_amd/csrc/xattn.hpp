@@ -508,9 +508,14 @@ inline bool few_rows_fwd(const Args& p) {
   return p.rows <= 32 || (int64_t)p.B * p.KVH * ceil_div(p.rows, 32) < 2 * num_cus();
 }
 
-// Forms that keep a head's keys in LDS (xattn_short.hip). The forward's is for more than 32 rows: one
-// wave would work on fewer. The backward's takes any number, since it is one launch for two, and up to
-// 96 keys of more than 64 dims: its buffers for more pass a CU's LDS.
+// Forms that keep a head's keys in LDS (xattn_short.hip), for up to 128 keys: what a CU's LDS holds of 128
+// dims beside the backward's rows of P and dS, and the registers of scores. The forward's is for more
+// than 32 rows, of which each of its waves takes 32; up to there the waves that split the keys are no
+// slower. The backward's takes any number: one launch for two.
+// (us, these forms against the others, replayed without the host. 128 x 256 queries of 4 heads of 64 dims
+// over 77 keys: forward 12.9, 14.4, backward 24, 40; 128 x 1024 of 32 dims 20, 26 and 39, 65; 64 x 512 of
+// 128 dims over 120 keys 20, 25 and 56, 84; 128 x 1024 of 64 dims over 128 keys 45, 50 and 107, 131; 128 x 64
+// over 77 keys 7.7, 9.4 and 15, 23; 128 x 16 6.3, 5.9 and 14, 21; 512 x 1 of 8 heads 24.7, 23.5 and 82, 83.)
 inline bool short_keys_fwd(const Args& p) { return p.rows > 32 && p.Lk <= 128; }
 inline bool short_keys_bwd(const Args& p) { return p.rows > 0 && p.Lk <= 128; }
 

@@ -14,6 +14,8 @@ namespace xattn {
 // dQ: the forward's tiles and layouts (S^T = K Q^T, dP^T = V dO^T: a query per lane column), then
 // dQ^T += K^T dS^T from transpose reads of the key rows. The product for dP^T starts from -D, as the
 // one for S^T from the keys' bias, so that dS = P (dP - D) is one multiplication.
+// Bound as the forward is, with three products to an exponential: bf16, 8 x 4096 queries of 8 heads of 64
+// dims over 1024 keys 132 us, 780 TFLOP/s, MFMA 50 % busy.
 // ---------------------------------------------------------------------------------------
 
 // What the kernels of dQ keep of a lane's query row: q and dO as B operands, kShift - lse in base 2
@@ -285,6 +287,9 @@ __global__ __launch_bounds__(256, 1) void xattn_dq_few_kernel(const Args p) {
 // dV^T += dO^T P and dK^T += Q^T dS, whose A operands are transpose reads of the same rows.
 // KB = 4: four blocks of keys. KB = 2: two, each of two waves with 32 rows of every tile, which join
 // in LDS at the end: twice the workgroups, for when there are few.
+// Keys are resident and rows pass because dK and dV are the two sums: four products to an exponential and
+// nothing but their operands through LDS. bf16, 8 x 4096 queries of 8 heads of 64 dims over 1024 keys 194
+// us (KB = 2), 707 TFLOP/s, MFMA 39 % busy. Heads of more than 64 dims need 304 registers: one wave a SIMD.
 // ---------------------------------------------------------------------------------------
 static __device__ float g_pad_stat[2] = {-__builtin_inff(), 0.f};
 

@@ -42,6 +42,8 @@ __device__ __forceinline__ uint32_t resident_keys(const Args& p, int b, int g, u
 // ---------------------------------------------------------------------------------------
 // Forward: four waves, each with its own 32 rows of every tile of 128; the next tile's queries load
 // while this one's are at work. Layouts and products as in xattn_fwd.hip.
+// Bound by HBM, less what a workgroup of few tiles leaves bare at its ends: 128 x 256 queries of 4 heads of
+// 64 dims over up to 77 keys 12.4 us (3.3 TB/s), 128 x 1024 of 32 dims 19.5 (3.7).
 // ---------------------------------------------------------------------------------------
 template <class T, int DP, int NB>
 __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_short_fwd_kernel(const Args p) {
@@ -130,6 +132,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_s
 // through LDS as rows of 32 keys, and each wave forms one 32 x 32 tile (or two) of dK^T = Q^T dS or
 // dV^T = dO^T P of the block over the tile's 128 rows, both operands by transpose reads. Without
 // kKeys only dQ is formed (the same bits).
+// The scores of all keys in registers leave two waves a SIMD (one of 128 dims), which bounds it, by LDS and
+// vector work in turn: the above shapes 22.4 us (2.3 TB/s) and 38.1 (2.8). Rows of P and dS laid 8 B askew
+// against their writes' conflicts: no more than 1 %.
 // ---------------------------------------------------------------------------------------
 template <class T, int DP, int NB, bool kKeys>
 __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_short_bwd_kernel(const Args p) {
