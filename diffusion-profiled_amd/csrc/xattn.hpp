@@ -281,11 +281,11 @@ __device__ __forceinline__ int keys_of(const Args& p, int b) {
 // wide and rows that are far apart choose an address per row.
 template <int DP>
 struct KeyTiles {
-  static constexpr int NG = DP / 8, kXfer = 64 * NG / 256;
+  static constexpr int NG = DP / 8, kXfer = 64 * NG / 256, kRows = 256 / NG;
   static constexpr uint32_t kBytes = 64 * DP * 2;
   const uint16_t *kb, *vb;  // key 0 of the head
   int64_t kl, vl;
-  uint32_t ko[kXfer], vo[kXfer], l0;
+  uint32_t ko, vo, l0;  // (transfers of a tile are kRows rows apart, a multiple of the period of swz)
   int lane, wave, klen, D;
   bool fast;
 
@@ -293,12 +293,9 @@ struct KeyTiles {
       : kb(p.k + b * p.ks.b + g * p.ks.h), vb(p.v + b * p.vs.b + g * p.vs.h), kl(p.ks.l), vl(p.vs.l),
         l0(lds), lane(lane_), wave(wave_), klen(klen_), D(p.D) {
     fast = D == DP && kl >= 0 && vl >= 0 && kl < (1 << 24) && vl < (1 << 24);
-#pragma unroll
-    for (int r = 0; r < kXfer; ++r) {
-      const int c = wave * 64 + 256 * r + lane, row = c / NG, g8 = ((c % NG) ^ swz<DP>(row)) << 3;
-      ko[r] = (uint32_t)(row * (int)kl + g8) * 2;
-      vo[r] = (uint32_t)(row * (int)vl + g8) * 2;
-    }
+    const int c = wave * 64 + lane, row = c / NG, g8 = ((c % NG) ^ swz<DP>(row)) << 3;
+    ko = (uint32_t)(row * (int)kl + g8) * 2;
+    vo = (uint32_t)(row * (int)vl + g8) * 2;
   }
   __device__ __forceinline__ bool whole(int t) const { return fast && t * 64 + 64 <= klen; }
 
@@ -308,8 +305,8 @@ struct KeyTiles {
     if (whole(t)) {
 #pragma unroll
       for (int r = 0; r < kXfer; ++r) {
-        dma16_lds_from(kt, ko[r], at + 4096 * r);
-        dma16_lds_from(vt, vo[r], at + kBytes + 4096 * r);
+        dma16_lds_from(kt + r * kRows * kl, ko, at + 4096 * r);
+        dma16_lds_from(vt + r * kRows * vl, vo, at + kBytes + 4096 * r);
       }
     } else {
 #pragma unroll
@@ -542,11 +539,12 @@ inline void plan_rows(Args& p, bool few) {
 
 constexpr int kQT = 64;  // rows of a tile of the kernel of dK and dV
 
-// Its workgroups take 128 keys, or 64 where that leaves few of them: less than four to a CU, of the
-// form for more than 64 dims, which runs one to a CU, less than two. (8 x 4096 queries of 64 dims over
-// 700 of 1031 keys 251 -> 197 us with 64; 16 x 1024 of 128 dims over 512 keys 173 us with 128, 196.)
+// Its workgroups take 128 keys, or 64 where that leaves few of them, less than four to a CU, and always of
+// more than 64 dims, whose sums leave a wave of the 128-key form a SIMD to itself. (8 x 4096 queries of 64
+// dims over 700 of 1031 keys 251 -> 197 us with 64. The backward of 128 dims with 128 and 64: 8 x 4096 of 8
+// heads over 1024 keys 549, 495; 16 x 1024 over 512 172, 159; 64 x 256 over 200 130, 121.)
 inline bool few_keys(const Args& p) {
-  return (int64_t)p.B * p.KVH * ceil_div(p.Lk, 128) < (dim_pad(p.D) == 128 ? 2 : 4) * num_cus();
+  return dim_pad(p.D) == 128 || (int64_t)p.B * p.KVH * ceil_div(p.Lk, 128) < 4 * num_cus();
 }
 
 inline void plan_keys(Args& p) {

@@ -286,15 +286,17 @@ __global__ __launch_bounds__(256, 1) void xattn_dq_few_kernel(const Args p) {
 // S = Q K^T and dP = dO V^T put a key in each lane column, so P and dS are the B operands of
 // dV^T += dO^T P and dK^T += Q^T dS, whose A operands are transpose reads of the same rows.
 // KB = 4: four blocks of keys. KB = 2: two, each of two waves with 32 rows of every tile, which join
-// in LDS at the end: twice the workgroups, for when there are few.
+// in LDS at the end: twice the workgroups, for when there are few, and registers for two of 128 dims
+// to a CU.
 // Keys are resident and rows pass because dK and dV are the two sums: four products to an exponential and
 // nothing but their operands through LDS. bf16, 8 x 4096 queries of 8 heads of 64 dims over 1024 keys 194
-// us (KB = 2), 707 TFLOP/s, MFMA 39 % busy. Heads of more than 64 dims need 304 registers: one wave a SIMD.
+// us (KB = 2), 707 TFLOP/s, MFMA 39 % busy. At 128 dims a block's operands pass through LDS (32 KB a wave) in
+// as many cycles as its products take.
 // ---------------------------------------------------------------------------------------
 static __device__ float g_pad_stat[2] = {-__builtin_inff(), 0.f};
 
 template <class T, int DP, int KB>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : DP == 64 ? 3 : 4) void xattn_dkdv_kernel(const Args p) {
+__global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_dkdv_kernel(const Args p) {
   constexpr int NG = DP / 8, KS = DP / 16, NDB = DP / 32;
   constexpr float kUnshift = 1.f / (1 << T::kShift);
   constexpr int kXfer = kQT * NG / 256;
@@ -331,13 +333,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : DP == 64 ? 3 : 4) void xattn_d
   const int64_t all_rows = (int64_t)p.B * p.KVH * p.rows;
   // tiles of 64 rows of one head go by constant lane offsets, the others by an address per row
   const bool fast = p.D == DP && p.qs.l >= 0 && p.gs.l >= 0 && p.qs.l < (1 << 24) && p.gs.l < (1 << 24);
-  uint32_t qo[kXfer], go[kXfer];
-#pragma unroll
-  for (int r = 0; r < kXfer; ++r) {
-    const int c = wave * 64 + 256 * r + lane, row = c / NG, g8 = ((c % NG) ^ swz<DP>(row)) << 3;
-    qo[r] = (uint32_t)(row * (int)p.qs.l + g8) * 2;
-    go[r] = (uint32_t)(row * (int)p.gs.l + g8) * 2;
-  }
+  constexpr int kRows = 256 / NG;  // from one transfer to the next (a multiple of the period of swz)
+  const int c = wave * 64 + lane, row0 = c / NG, g8 = ((c % NG) ^ swz<DP>(row0)) << 3;
+  const uint32_t qo = (uint32_t)(row0 * (int)p.qs.l + g8) * 2, go = (uint32_t)(row0 * (int)p.gs.l + g8) * 2;
   auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
     const int r0 = t * kQT;
     const uint32_t hg = fdiv(r0, p.by_lq), at = l0 + buf * 2 * kBytes;
@@ -347,8 +345,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : DP == 64 ? 3 : 4) void xattn_d
       const uint16_t* gt = gb + (int64_t)tok * p.gs.l + hg * p.gs.h;
 #pragma unroll
       for (int r = 0; r < kXfer; ++r) {
-        dma16_lds_from(qt, qo[r], at + wave * 1024 + 4096 * r);
-        dma16_lds_from(gt, go[r], at + kBytes + wave * 1024 + 4096 * r);
+        dma16_lds_from(qt + r * kRows * p.qs.l, qo, at + wave * 1024 + 4096 * r);
+        dma16_lds_from(gt + r * kRows * p.gs.l, go, at + kBytes + wave * 1024 + 4096 * r);
       }
     } else {
 #pragma unroll
@@ -555,7 +553,7 @@ static int launch_bwd(const Args& r, const Args& k, hipStream_t s) {
   if (k.total > 0) {
     if (few_keys(k))
       xattn_dkdv_kernel<T, DP, 2><<<k.grid, 256, 0, s>>>(k);
-    else
+    else if constexpr (DP != 128)  // (few_keys holds for 128)
       xattn_dkdv_kernel<T, DP, 4><<<k.grid, 256, 0, s>>>(k);
     const int st = launch_status();
     return st != DPA_OK ? st : sum_keys<T>(k, s);

@@ -316,6 +316,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_short_bwd_kernel
   }
 }
 
+// Up to 96 keys are three blocks of 32 in registers and LDS, more are four. (77 keys as four: 128 x 256
+// queries of 64 dims forward 14.5 us for 13.0, backward 30.6 for 23.9; 128 x 1024 of 32 dims 21.1 for 20.8
+// and 40.8 for 39.7.)
 template <class T, int DP>
 static int launch_short_fwd(const Args& p, hipStream_t s) {
   if (p.Lk <= 96) xattn_short_fwd_kernel<T, DP, 3><<<p.grid, 256, 0, s>>>(p);
