@@ -785,7 +785,7 @@ int dpa_conv3x3_thin_wgrad(const void* x, int x_dtype, const void* dy, float* dw
  * Conditioning of the U-Net on text: token embedding, cross attention to the encoder's states,
  * dropout. No counterpart in the reference, whose U-Net is unconditional.
  *
- * Cross attention (csrc/xattn_fwd.hip, csrc/xattn_bwd.hip). Query head h of a batch reads
+ * Cross attention (csrc/xattn_fwd.hip, xattn_bwd.hip, xattn_short.hip). Query head h of a batch reads
  * key/value head h / (heads / kv_heads); head_dim a multiple of 8 up to 128; operands bf16 or
  * fp16 (dtype DPA_DTYPE_BF16 / DPA_DTYPE_F16), sums and softmax in fp32. A key takes part when
  * its index is below key_lengths[b] (NULL: all of kv_len; values are clamped to [0, kv_len]) and
