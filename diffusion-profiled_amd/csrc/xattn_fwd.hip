@@ -21,7 +21,7 @@ namespace xattn {
 // without the products that move it.
 //
 // Bound by the products and the exponentials (a quarter-rate unit, one per score), which follow each
-// other within a wave and overlap between the waves of a SIMD: hence four of 64 dims (two of 128).
+// other within a wave and overlap between the waves of a SIMD: hence four waves of 64 dims to a SIMD (two of 128).
 // bf16, 8 x 4096 queries of 8 heads of 64 dims over 1024 keys: 108 us, 635 TFLOP/s, MFMA 34 % busy;
 // fp16, 16 x 1024 of 8 heads of 128 dims over 512 keys of 2: 61 us from cold operands, 49 from cached
 // ones (700 TFLOP/s). A third buffer of keys brought nothing (94 -> 98 us).
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_fwd_kernel(const
 // their softmaxes in LDS at the end. Products as above. This form reads the keys and values once
 // and does little with them, so it is made for bytes in flight: keys go straight to registers as A
 // operands, values to LDS, each one tile ahead, and two workgroups of 128 dims fit a CU.
-// fp16, 16 x 1 queries of 16 heads over 4 of up to 4097 keys of 128 dims (90 MB): 20 us, 4.5 TB/s.
+// fp16, 16 x 1 queries of 16 heads over 4 of up to 4097 keys of 128 dims: 20 us for 90 MB (72 of them from HBM).
 // Few keys as well: three dependent trips to memory (lengths, operands, store), 5.5 us for 4 x 1
 // queries over 77 keys.
 // ---------------------------------------------------------------------------------------

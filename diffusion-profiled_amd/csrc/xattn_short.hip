@@ -133,7 +133,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_s
 // dV^T = dO^T P of the block over the tile's 128 rows, both operands by transpose reads. Without
 // kKeys only dQ is formed (the same bits).
 // The scores of all keys in registers leave two waves a SIMD (one of 128 dims), which bounds it, by LDS and
-// vector work in turn: the above shapes 22.4 us (2.3 TB/s) and 38.1 (2.8). Rows of P and dS laid 8 B askew
+// vector work in turn: the above shapes 22.1 us (3.5 TB/s) and 37.8 (2.8). Rows of P and dS laid 8 B askew
 // against their writes' conflicts: no more than 1 %.
 // ---------------------------------------------------------------------------------------
 template <class T, int DP, int NB, bool kKeys>
