@@ -51,9 +51,13 @@ struct Args {
 
 // kShift: the backward forms 2^kShift P and takes the factor out of its fp32 sums at the end. In
 // bf16, whose exponents have the room, that keeps probabilities down to 2^-150, where v_exp_f32
-// alone gives 0 below 2^-126; it costs nothing. fp16 has no room for it.
+// alone gives 0 below 2^-126; it costs nothing. fp16 has room for 2^14 P, at most 1, which keeps all
+// bits of probabilities down to 2^-28.
+// kScaled: dS is scaled by a power of 2 that follows its size (in fp16: P (dP - D) over 4096 keys with
+// gradients of 1e-5 is mostly below its subnormals, and beyond 65504 with a large loss scale).
 struct Bf16 {
   static constexpr int kShift = 24;
+  static constexpr bool kScaled = false;
   template <class A>
   static __device__ __forceinline__ v16f mfma(A a, uint4 b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
@@ -65,7 +69,8 @@ struct Bf16 {
 };
 
 struct F16 {
-  static constexpr int kShift = 0;
+  static constexpr int kShift = 14;
+  static constexpr bool kScaled = true;
   template <class A>
   static __device__ __forceinline__ v16f mfma(A a, uint4 b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
@@ -383,6 +388,33 @@ __device__ __forceinline__ float sum_halves(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+// The power of 2, `up`, at which a lane's column of 2^kShift dS stands (fp16): moved down only when a
+// |dP - D| passes what the type holds, and then so far that values 2^4 larger fit too, so that nearly every
+// tile goes without moving the sums. Costs half a vector instruction per score and an exchange (dK's one
+// more): the fp16 backward of 16 x 1024 queries of 8 heads over 512 keys of 2, 128 dims, 168 -> 175 us, of 16 x 1
+// of 16 heads over 4097 keys of 4 133 -> 145, of 8 x 4096 of 64 dims over 1024 as before (293, 288).
+struct DsScale {
+  static constexpr int kFirst = 46;  // (nothing passes before it is 2^-45)
+  float up = __uint_as_float((127u + kFirst) << 23);
+  // the largest of these 16 of the column's values (and the 16 of lane ^ 32)
+  static __device__ __forceinline__ float largest(const v16f& dp) {
+    float t = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t = fmaxf(t, fabsf(dp[r]));
+    return max_halves(t);
+  }
+  // 2^kShift dS up stays below 2^15 (P is at most 1, but for its rounding)
+  __device__ __forceinline__ bool passes(float top) const { return top * up > 2.f; }
+  // the binary exponent by which it moves, 0 if top does not pass
+  __device__ __forceinline__ int move(float top) {
+    if (!passes(top)) return 0;
+    const int was = __builtin_amdgcn_frexp_expf(up) - 1;
+    const int k = min(was, -3 - __builtin_amdgcn_frexp_expf(top));  // (top < 2^its exponent)
+    up = ldexpf(1.f, k);
+    return k - was;
+  }
+};
 
 // f x as row l & 31 of a dense array's rows at dst (dims in the registers of the accumulators, on:
 // whether the lane's row exists). Lanes l and l ^ 32 hold 4 dims of every 8; they trade halves of

@@ -19,7 +19,9 @@ namespace xattn {
 // ---------------------------------------------------------------------------------------
 
 // What the kernels of dQ keep of a lane's query row: q and dO as B operands, kShift - lse in base 2
-// and -D, which they leave for the kernel of dK and dV (leave: this wave does).
+// and -D, which they leave for the kernel of dK and dV (leave: this wave does). D is formed from O as it was
+// rounded, half a step off per dim: the fp32 P and dP that it could be summed from pass only later, tile by
+// tile, and one more pass over the keys to get it would cost as much as dQ's.
 template <class T, int KS>
 struct QueryRow {
   uint4 qf[KS], gf[KS];
@@ -57,6 +59,24 @@ struct QueryRow {
     }
   }
 };
+
+template <int NDB>
+__device__ __forceinline__ void times(v16f (&x)[NDB], float f) {
+#pragma unroll
+  for (int d = 0; d < NDB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[d][r] *= f;
+}
+
+// Moves dS's scale, dq's with it, for these values of dP - D. The scale is part of P's exponent, in nlse2.
+template <int NDB>
+__device__ __forceinline__ void follow(DsScale& ds, const v16f& dp, v16f (&dq)[NDB], float& nlse2) {
+  const float top = DsScale::largest(dp);
+  if (!__any(ds.passes(top))) return;
+  const int by = ds.move(top);
+  times(dq, ldexpf(1.f, by));
+  nlse2 += (float)by;
+}
 
 // Four waves of 32 query rows each share tiles of 64 keys.
 template <class T, int DP>
@@ -110,6 +130,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_d
   for (int i = 0; i < NDB; ++i) dq[i] = zero16();
 #pragma unroll
   for (int r = 0; r < 16; ++r) nd16[r] = q.nd;
+  DsScale ds;
+  float nlse2 = T::kScaled ? q.nlse2 + DsScale::kFirst : q.nlse2;
 
   auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
     constexpr int buf = decltype(buffer)::value;
@@ -132,13 +154,14 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_d
         s = T::mfma(row_at.get(k, at + kBytes / 2 * i), q.qf[k], s);
         dp = T::mfma(row_at.get(k, at + kBytes + kBytes / 2 * i), q.gf[k], dp);
       }
+      if constexpr (T::kScaled) follow(ds, dp, dq, nlse2);
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         uint32_t sw[4];
 #pragma unroll
         for (int r = 8 * s2; r < 8 * s2 + 8; r += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, q.nlse2));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, q.nlse2));
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, nlse2));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, nlse2));
           sw[(r & 7) / 2] = T::pack(p0 * dp[r], p1 * dp[r + 1]);
         }
         const uint4 sf = {sw[0], sw[1], sw[2], sw[3]};
@@ -155,11 +178,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_d
   }
 
   const bool has_row = row < p.rows;
+  if constexpr (T::kScaled) times(dq, kUnshift / ds.up);
   if (p.splits > 1) {
     if (has_row) store_part(p.part + (((int64_t)split * p.B * p.KVH + bkv) * p.rows + row) * p.D, dq, h, p.D);
     return;
   }
-  store_row<T>(p.dq + q.orow * p.D, has_row, dq, p.scale * kUnshift, h, p.D);
+  store_row<T>(p.dq + q.orow * p.D, has_row, dq, T::kScaled ? p.scale : p.scale * kUnshift, h, p.D);
 }
 
 // Up to 32 rows: the four waves share them and take every fourth tile of 32 keys each.
@@ -208,6 +232,8 @@ __global__ __launch_bounds__(256, 1) void xattn_dq_few_kernel(const Args p) {
   for (int i = 0; i < NDB; ++i) dq[i] = zero16();
 #pragma unroll
   for (int r = 0; r < 16; ++r) nd16[r] = q.nd;
+  DsScale ds;
+  float nlse2 = T::kScaled ? q.nlse2 + DsScale::kFirst : q.nlse2;
 
   for (int t = t_lo, buf = 0; t < t_hi; t += 4, buf ^= 1) {
     uint32_t word_next = 0;
@@ -229,13 +255,14 @@ __global__ __launch_bounds__(256, 1) void xattn_dq_few_kernel(const Args p) {
         s = T::mfma(frag_row<DP>(kr, col, 2 * k + h), q.qf[k], s);
         dp = T::mfma(frag_row<DP>(vr, col, 2 * k + h), q.gf[k], dp);
       }
+      if constexpr (T::kScaled) follow(ds, dp, dq, nlse2);
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         uint32_t sw[4];
 #pragma unroll
         for (int r = 8 * s2; r < 8 * s2 + 8; r += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, q.nlse2));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, q.nlse2));
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, nlse2));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, nlse2));
           sw[(r & 7) / 2] = T::pack(p0 * dp[r], p1 * dp[r + 1]);
         }
         const uint4 sf = {sw[0], sw[1], sw[2], sw[3]};
@@ -247,7 +274,8 @@ __global__ __launch_bounds__(256, 1) void xattn_dq_few_kernel(const Args p) {
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  const float unscale = p.scale * kUnshift;
+  const float unscale = T::kScaled ? p.scale : p.scale * kUnshift;
+  if constexpr (T::kScaled) times(dq, kUnshift / ds.up);  // (each wave has its own)
   __syncthreads();
   float* ox = reinterpret_cast<float*>(&kv[0][0][0][0]);  // [4][DP][32]
   static_assert(sizeof(kv) >= 4 * DP * 32 * 4, "the waves' dQ fit the buffers");
@@ -379,6 +407,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_d
   v16f dk[NDB], dv[NDB];
 #pragma unroll
   for (int i = 0; i < NDB; ++i) dk[i] = dv[i] = zero16();
+  DsScale ds;  // (of the key in the lane)
   auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
     constexpr int buf = decltype(buffer)::value;
     wait_vmcnt<0>();
@@ -394,6 +423,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_d
         for (int k = 0; k < KS; ++k) {
           s = T::mfma(row_at.get(k, at), kf[k], s);
           dp = T::mfma(row_at.get(k, at + kBytes), vf[k], dp);
+        }
+        if constexpr (T::kScaled) {
+          const float top = DsScale::largest(dp);
+          if (__any(ds.passes(top))) times(dk, ldexpf(1.f, ds.move(top)));
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] *= ds.up;
         }
         const v16f e = start_at(stat_at + st);
 #pragma unroll
@@ -422,6 +457,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_d
     if (t + 1 < t_hi) step(t + 1, std::integral_constant<int, 1>());
   }
 
+  if constexpr (T::kScaled) times(dk, kUnshift / ds.up);
   if constexpr (KB == 2) {
     __syncthreads();
     float* x = reinterpret_cast<float*>(lds) + wave % KB * (2 * NDB * 1024) + lane;
@@ -458,7 +494,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_d
     }
     return;
   }
-  store_row<T>(p.dk + b * p.dks.b + key * p.dks.l + g * p.dks.h, on, dk, p.scale * kUnshift, h, p.D);
+  store_row<T>(p.dk + b * p.dks.b + key * p.dks.l + g * p.dks.h, on, dk, T::kScaled ? p.scale : p.scale * kUnshift, h,
+               p.D);
   store_row<T>(p.dv + b * p.dvs.b + key * p.dvs.l + g * p.dvs.h, on, dv, kUnshift, h, p.D);
 }
 
@@ -492,7 +529,8 @@ __global__ __launch_bounds__(256) void xattn_sum_kernel(const Args p) {
   } else {
     dst = p.dk + b * p.dks.b + x * p.dks.l + g * p.dks.h;
   }
-  const float f = (is_v ? 1.f : p.scale) / (1 << T::kShift);
+  constexpr float kUnshift = 1.f / (1 << T::kShift);
+  const float f = is_v ? kUnshift : T::kScaled ? p.scale : p.scale * kUnshift;
   *reinterpret_cast<uint4*>(dst + d0) = uint4{T::pack(o[0] * f, o[1] * f), T::pack(o[2] * f, o[3] * f),
                                               T::pack(o[4] * f, o[5] * f), T::pack(o[6] * f, o[7] * f)};
 }

@@ -39,6 +39,30 @@ __device__ __forceinline__ uint32_t resident_keys(const Args& p, int b, int g, u
   return act;
 }
 
+// |x|^2 of 8 elements added to n
+template <class T>
+__device__ __forceinline__ float length2(uint4 x, float n) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    n = __builtin_fmaf(T::lo(w[i]), T::lo(w[i]), n);
+    n = __builtin_fmaf(T::hi(w[i]), T::hi(w[i]), n);
+  }
+  return n;
+}
+// (a row that is not finite takes no part in a maximum: its dS is not finite either)
+__device__ __forceinline__ float finite(float n) { return n < __builtin_inff() ? n : 0.f; }
+// the maximum over a wave, of nothing negative: halves, rows of 16 lanes, then within a row
+__device__ __forceinline__ float wave_max(float x) {
+  x = max_halves(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false)));  // row_ror:8
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x124, 0xf, 0xf, false)));
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x122, 0xf, 0xf, false)));
+  return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x121, 0xf, 0xf, false)));
+}
+
 // ---------------------------------------------------------------------------------------
 // Forward: four waves, each with its own 32 rows of every tile of 128; the next tile's queries load
 // while this one's are at work. Layouts and products as in xattn_fwd.hip.
@@ -195,6 +219,21 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_short_bwd_kernel
   for (int x = 0; x < 4; ++x) ps_at[x] = opaque(l0 + kPS + wave * 2048 + col * 64 + ((x ^ swz<32>(col)) << 4) + 8 * h);
   const TrAt<32, 1> ps_tr(lane, l0 + kPS + mat * 8192 + part * 4096);
   const TrAt<DP, NT> qg_tr(lane, l0 + kQG + mat * kTile + part * 2 * kBlock, db0, 2);
+
+  // dS's scale 2^-down with T::kScaled (the workgroup's, as its sums over rows are): |dP - D| <=
+  // 2 max |v| max |dO|, lengths of the rows of the tiles so far, so that 2^(kShift - down) dS is at most
+  // 2^15. It moves one way only. The waves leave their parts of the maxima in LDS. (fp16, one
+  // barrier a tile more: 128 x 256 queries of 64 dims over 77 keys 24.2 -> 25.6 us, 512 x 1 80 -> 88.)
+  int down = 0;
+  float* most = bias + 128;  // [2: tile t & 1][4 waves] of |dO|^2, then [4] of |v|^2
+  if constexpr (T::kScaled) {
+    float n = 0.f;  // (of 8 dims: a row's is at most DP / 8 times the largest)
+#pragma unroll
+    for (uint32_t at = 0; at < kV; at += 4096)
+      if (at + tid * 16 < kV) n = fmaxf(n, finite(length2<T>(__builtin_bit_cast(uint4, lds_ld16(l0 + kV + at + tid * 16)), 0.f)));
+    n = wave_max(n) * (DP / 8);
+    if (lane == 0) most[8 + wave] = n;
+  }
   // one tile over the first N blocks of keys
   auto tile = [&](int t, auto blocks) __attribute__((always_inline)) {
     constexpr int N = decltype(blocks)::value;
@@ -210,6 +249,35 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_short_bwd_kernel
         lds_st16(row_at.a[k] + my_rows + kTile, gf[k]);
       }
       const float nlse2 = lse == -__builtin_inff() ? -__builtin_inff() : (float)T::kShift - lse * kLog2e;
+      if constexpr (T::kScaled) {  // (before the scores: they fill the registers)
+        float n = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) n = length2<T>(gf[k], n);
+        n = wave_max(finite(sum_halves(n)));
+        if (lane == 0) most[4 * (t & 1) + wave] = n;
+        wait_lgkmcnt0();
+        lds_barrier();
+        const float* g = most + 4 * (t & 1);
+        const float n2 = fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3])) *
+                         fmaxf(fmaxf(most[8], most[9]), fmaxf(most[10], most[11]));
+        // (n2 < 2^frexp, so max |v| max |dO| < 2^half of it, rounded up; 0 gives 2^0)
+        const int ex = __builtin_amdgcn_readfirstlane((__builtin_amdgcn_frexp_expf(n2) + 1) >> 1);
+        if (t == t_lo) {
+          down = ex;
+        } else if (ex > down) {
+          if (mat == 0) {
+            const float f = ldexpf(1.f, down - ex);
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+              for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] *= f;
+          }
+          down = ex;
+        }
+      }
+      const float up = T::kScaled ? ldexpf(1.f, -down) : 1.f;
       v16f s[N], dp[N];  // (s: then P)
       float nd = 0.f;
 #pragma unroll
@@ -229,7 +297,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_short_bwd_kernel
         __builtin_amdgcn_sched_barrier(0);
       }
       if (DP == 32) load(t + 1);
-      nd = sum_halves(nd) * kUnshift;
+      nd = sum_halves(nd) * (T::kScaled ? kUnshift * up : kUnshift);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
 #pragma unroll
@@ -239,7 +307,11 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_short_bwd_kernel
           for (int r = 0; r < 8; r += 2) {
             const float p0 = s[i][8 * s2 + r], p1 = s[i][8 * s2 + r + 1];
             pw[r / 2] = T::pack(p0, p1);
-            sw[r / 2] = T::pack(p0 * (dp[i][8 * s2 + r] + nd), p1 * (dp[i][8 * s2 + r + 1] + nd));
+            const float d0 = dp[i][8 * s2 + r], d1 = dp[i][8 * s2 + r + 1];
+            if constexpr (T::kScaled)
+              sw[r / 2] = T::pack(p0 * __builtin_fmaf(d0, up, nd), p1 * __builtin_fmaf(d1, up, nd));
+            else
+              sw[r / 2] = T::pack(p0 * (d0 + nd), p1 * (d1 + nd));
           }
 #pragma unroll
           for (int x = 0; kKeys && x < 2; ++x) {
@@ -269,7 +341,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_short_bwd_kernel
     const int row = t * 128 + mine;
     const bool on = row < p.rows;
     const uint32_t hg = fdiv(on ? row : 0, p.by_lq), tok = (on ? row : 0) - hg * p.Lq;
-    store_row<T>(p.dq + (((int64_t)b * p.Lq + tok) * p.H + g * p.G + hg) * p.D, on, dq, p.scale * kUnshift, h, p.D);
+    store_row<T>(p.dq + (((int64_t)b * p.Lq + tok) * p.H + g * p.G + hg) * p.D, on, dq,
+                 T::kScaled ? p.scale * ldexpf(kUnshift, down) : p.scale * kUnshift, h, p.D);
   };
   // (a loop for each number of blocks up to the last with a visible key)
   auto walk = [&](auto blocks) __attribute__((always_inline)) {
@@ -303,14 +376,18 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void xattn_short_bwd_kernel
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int dim = 32 * (db0 + 2 * j);
-      const v16f a[1] = {vis ? acc[i][j] : zero16()};
+      v16f a[1] = {vis ? acc[i][j] : zero16()};
+      if (T::kScaled && mat == 0)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) a[0][r] *= ldexpf(kUnshift, down);
       if (p.splits > 1) {
         const int64_t at = (split * 2 + mat) * n + (int64_t)bkv * p.Lk + key;
         if (on) store_part(p.part + at * p.D + dim, a, h, p.D - dim);
       } else {
         uint16_t* dst = mat == 0 ? p.dk + b * p.dks.b + key * p.dks.l + g * p.dks.h
                                  : p.dv + b * p.dvs.b + key * p.dvs.l + g * p.dvs.h;
-        store_row<T>(dst + dim, on, a, (mat == 0 ? p.scale : 1.f) * kUnshift, h, p.D - dim);
+        const float f = mat == 0 ? T::kScaled ? p.scale : p.scale * kUnshift : kUnshift;
+        store_row<T>(dst + dim, on, a, f, h, p.D - dim);
       }
     }
   }
