@@ -446,8 +446,7 @@ def embedding_bwd(dout: torch.Tensor, tokens: torch.Tensor, num_embeddings: int,
     """The gradient [num_embeddings, C] of ``embedding_fwd``'s weight in dtype (dout's by default):
     per row the fp32 sum over its tokens in order, rounded once; zeros for padding_idx. Tokens
     outside the table add nothing. Deterministic."""
-    dw = _fast().embedding_bwd(dout, tokens, num_embeddings, scale,
-                               -1 if padding_idx is None else padding_idx, p_drop, seed, dtype)
+    dw = _fast().embedding_bwd(dout, tokens, num_embeddings, scale, padding_idx, p_drop, seed, dtype)
     if dw is not None:
         return dw
     if dout.ndim < 1 or dout.shape[:-1] != tokens.shape or dout.shape[-1] == 0 or num_embeddings <= 0:

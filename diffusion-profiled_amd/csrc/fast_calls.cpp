@@ -256,7 +256,7 @@ PyObject* embedding_fwd(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (dout, tokens, num_embeddings, scale, padding_idx or -1, p, seed, dtype) -> dweight
+// (dout, tokens, num_embeddings, scale, padding_idx or None, p, seed, dtype) -> dweight
 PyObject* embedding_bwd(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 8) return none();
@@ -264,16 +264,16 @@ PyObject* embedding_bwd(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const at::Tensor *g = plain(o[0], &device), *t = plain(o[1], &device), *seed;
   float p;
   if (!g || !t || !tokens_ok(*t) || !g->is_contiguous() || g->dim() != t->dim() + 1 || !PyLong_CheckExact(o[2]) ||
-      !PyFloat_CheckExact(o[3]) || !PyLong_CheckExact(o[4]) || !embed_drop(o[5], o[6], &device, &p, &seed))
+      !PyFloat_CheckExact(o[3]) || (o[4] != Py_None && !PyLong_CheckExact(o[4])) || !embed_drop(o[5], o[6], &device, &p, &seed))
     return none();
   at::ScalarType type = g->scalar_type();
   if (dtype_of(type) < 0 || !dtype_arg(o[7], &type) || dtype_of(type) < 0) return none();
-  const int64_t v = PyLong_AsLongLong(o[2]), pad = PyLong_AsLongLong(o[4]), c = g->size(-1);
+  const int64_t v = PyLong_AsLongLong(o[2]), pad = o[4] == Py_None ? -1 : PyLong_AsLongLong(o[4]), c = g->size(-1);
   if (PyErr_Occurred()) {
     PyErr_Clear();
     return none();
   }
-  if (v <= 0 || pad < -1 || pad >= v || c <= 0 || c > 1 << 20 || t->numel() == 0 || g->sizes().slice(0, t->dim()) != t->sizes())
+  if (v <= 0 || (o[4] != Py_None && pad < 0) || pad >= v || c <= 0 || c > 1 << 20 || t->numel() == 0 || g->sizes().slice(0, t->dim()) != t->sizes())
     return none();
   at::Tensor dw = at::empty({v, c}, g->options().dtype(type));
   const int64_t bytes = emb_bwd_bytes(t->numel(), (int)c);
