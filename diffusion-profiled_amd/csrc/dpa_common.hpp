@@ -418,6 +418,10 @@ inline int launch_status() {
   return e == hipSuccess ? DPA_OK : (int)e;
 }
 
+// Workgroups of 256 in a launch: a grid has less than 2^32 threads along an axis. A launch of more gives no
+// error: the number wraps and work is left out.
+constexpr int64_t kMaxGroups256 = (1 << 24) - 1;
+
 // CUs of the device (256 where there is none to ask)
 int num_cus();
 

@@ -154,15 +154,16 @@ __global__ __launch_bounds__(256) void embed_units_kernel(const Args p) {
 template <int WT, int OT, int TB>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const Args p) {
   const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (row >= p.n) return;
-  const int64_t t = token_at<TB>(p.tokens, row);
-  const bool in = t >= 0 && t < (int64_t)p.V;
   const uint64_t seed = p.seed ? *p.seed : 0;
-  for (int c = lane; c < p.C; c += 64) {
-    float v[1] = {0.f};
-    if (in) load<WT, 1>(p.src, t * p.C + c, v);
-    embed_store<WT, OT, 1>(p, seed, in, row * p.C + c, v);
+  for (int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < p.n;
+       row += (int64_t)gridDim.x * 4) {
+    const int64_t t = token_at<TB>(p.tokens, row);
+    const bool in = t >= 0 && t < (int64_t)p.V;
+    for (int c = lane; c < p.C; c += 64) {
+      float v[1] = {0.f};
+      if (in) load<WT, 1>(p.src, t * p.C + c, v);
+      embed_store<WT, OT, 1>(p, seed, in, row * p.C + c, v);
+    }
   }
 }
 
@@ -641,7 +642,8 @@ static void launch_fwd(Args& a, int token_bytes, hipStream_t s) {
     else embed_units_kernel<WT, OT, 4><<<grid, 256, 0, s>>>(a);
     return;
   }
-  const unsigned grid = (unsigned)ceil_div(a.n, 4);
+  const int64_t groups = ceil_div(a.n, 4);
+  const unsigned grid = (unsigned)(groups < 1 << 22 ? groups : 1 << 22);
   if (token_bytes == 8) embed_rows_kernel<WT, OT, 8><<<grid, 256, 0, s>>>(a);
   else embed_rows_kernel<WT, OT, 4><<<grid, 256, 0, s>>>(a);
 }
@@ -728,6 +730,8 @@ extern "C" int dpa_embedding_bwd(const void* dout, int dout_dtype, const void* t
                                  int64_t workspace_bytes, void* stream) {
   int st = check(n, V, C, token_bytes, dout_dtype, weight_dtype, drop_seed, drop_p);
   if (st != DPA_OK) return st;
+  // (a workgroup of 256 for 32 places: the join's grid)
+  if (ceil_div(n, kPiece) > kMaxGroups256) return DPA_ERR_SIZE;
   if (!dweight || (n > 0 && (!dout || !tokens))) return DPA_ERR_NULL;
   if (!aligned(dweight, 16) || !aligned(tokens, token_bytes) || !aligned(dout, dtype_size(dout_dtype)))
     return DPA_ERR_ALIGN;

@@ -835,7 +835,8 @@ int dpa_dropout(const void* x, const void* residual, void* y, int dtype, int64_t
  * i C + c. A token outside [0, V) gives a row of NaN.
  * bwd: dweight [V][C], all of it written: scale times the sum, in order of i and in fp32, of
  * (dropped) dout[i] over the tokens of a row; zeros for rows without tokens and for padding_idx
- * (-1: none). Tokens outside [0, V) add nothing. Deterministic. dweight 16-B aligned. */
+ * (-1: none). Tokens outside [0, V) add nothing. Deterministic. dweight 16-B aligned.
+ * n < 2^31 forward, below 2^29 backward; C at most 2^20. */
 int dpa_embedding_fwd(const void* tokens, int token_bytes, const void* weight, int weight_dtype,
                       void* out, int out_dtype, int64_t n, int64_t V, int C, float scale,
                       const void* drop_seed, float drop_p, void* stream);
