@@ -524,6 +524,10 @@ inline void set_grid(Args& p, int64_t total, int64_t per_head) {
   p.grid = (uint32_t)(ceil_div(total, 8 * unit) * 8 * unit);
 }
 
+// Every kernel's workgroups have 256 threads. (The launches behind a split have fewer: it is made where few
+// workgroups run.)
+inline bool grid_ok(const Args& p) { return p.grid <= kMaxGroups256; }
+
 inline int dim_pad(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 // The forward's and dQ's forms: four waves of 32 rows that share tiles of keys, or four waves that

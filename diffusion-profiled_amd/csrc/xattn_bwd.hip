@@ -627,6 +627,7 @@ extern "C" int dpa_cross_attention_bwd(const DpaCrossAttention* a, void* workspa
   hipStream_t s = (hipStream_t)stream;
   if (short_keys_bwd(k)) {
     plan_short(k, true);
+    if (!grid_ok(k)) return DPA_ERR_SIZE;
     if (!workspace || workspace_bytes < short_workspace(k)) return DPA_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return DPA_ERR_ALIGN;
     k.part = (float*)workspace;
@@ -636,6 +637,7 @@ extern "C" int dpa_cross_attention_bwd(const DpaCrossAttention* a, void* workspa
   }
   plan_rows(r, few_rows_dq(r));
   plan_keys(k);
+  if (!grid_ok(r) || (a->dk && !grid_ok(k))) return DPA_ERR_SIZE;
   const int64_t need = bwd_workspace(r, k);
   if (need) {
     if (!workspace || workspace_bytes < need) return DPA_ERR_WORKSPACE;

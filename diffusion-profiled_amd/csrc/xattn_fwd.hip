@@ -492,9 +492,11 @@ extern "C" int dpa_cross_attention_fwd(const DpaCrossAttention* a, void* workspa
   hipStream_t s = (hipStream_t)stream;
   if (short_keys_fwd(p)) {
     plan_short(p, false);
+    if (!grid_ok(p)) return DPA_ERR_SIZE;
     return short_fwd(p, a->dtype, s);
   }
   plan_rows(p, few_rows_fwd(p));
+  if (!grid_ok(p)) return DPA_ERR_SIZE;
   const int64_t need = fwd_workspace(p);
   if (need) {
     if (!workspace || workspace_bytes < need) return DPA_ERR_WORKSPACE;

@@ -1,8 +1,10 @@
 """What the conditioning operators refuse at the edges of what they take (nothing is launched)."""
 from __future__ import annotations
 
+import pytest
+
 from conftest import dpa_mod
-from test_conditioning_cpu import FAKE
+from test_conditioning_cpu import FAKE, _desc
 
 L = dpa_mod("_lib")
 
@@ -12,3 +14,21 @@ def test_embedding_gradient_refuses_more_tokens_than_a_grid_has():
     f = L.load().dpa_embedding_bwd
     for n, status in ((1 << 29, -2), ((1 << 31) - 65, -2), ((1 << 29) - 32, -5)):     # (-5: no workspace)
         assert f(FAKE, 0, FAKE, 8, FAKE, 0, n, 10, 8, 1.0, -1, None, 0.0, None, 0, None) == status
+
+
+@pytest.mark.parametrize("kw", [
+    dict(b=1 << 20, h=16, g=16, lq=1, lk=8),            # keys in LDS: a workgroup per head
+    dict(b=1 << 20, h=16, g=16, lq=40, lk=8),
+    dict(b=1 << 20, h=16, g=16, lq=1, lk=200),          # few rows
+    dict(b=1 << 10, h=16, g=16, lq=(1 << 17) + 1, lk=200),
+])
+def test_attention_refuses_more_workgroups_than_a_grid_has(kw):
+    lib = L.load()
+    room = 1 << 62
+    assert lib.dpa_cross_attention_fwd(_desc(**kw), FAKE, room, None) == -2
+    assert lib.dpa_cross_attention_bwd(_desc(**kw), FAKE, room, None) == -2
+
+
+def test_attention_refuses_more_workgroups_of_keys_than_a_grid_has():
+    kw = dict(b=1 << 10, h=16, g=16, lq=1, lk=1 << 17)
+    assert L.load().dpa_cross_attention_bwd(_desc(**kw), FAKE, 1 << 62, None) == -2
