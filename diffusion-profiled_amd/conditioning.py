@@ -27,6 +27,7 @@ from .gn_silu import DROPOUT_SEEDS
 
 _DT = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}     # DPA_DTYPE_*
 _MAX_HEAD_DIM = 128
+_MAX_WIDTH = 1 << 20        # of a row of the embedding
 
 # DpaCrossAttention of include/dpa_fp8.h: 11 pointers, the mask's stride, 6 x 3 strides, 7 sizes,
 # the scale
@@ -427,8 +428,8 @@ def embedding_fwd(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 
     out = _fast().embedding_fwd(tokens, weight, scale, p_drop, seed, out_dtype)
     if out is not None:
         return out
-    if weight.ndim != 2 or weight.numel() == 0:
-        raise ValueError(f"embedding: the weight is [V, C], got {tuple(weight.shape)}")
+    if weight.ndim != 2 or weight.numel() == 0 or weight.shape[1] > _MAX_WIDTH:
+        raise ValueError(f"embedding: the weight is [V, C], C up to {_MAX_WIDTH}, got {tuple(weight.shape)}")
     out_dtype = weight.dtype if out_dtype is None else out_dtype
     p_drop = _check_embedding(tokens, weight.dtype, out_dtype, p_drop, seed, weight)
     v, c = weight.shape
@@ -452,6 +453,8 @@ def embedding_bwd(dout: torch.Tensor, tokens: torch.Tensor, num_embeddings: int,
     if dout.ndim < 1 or dout.shape[:-1] != tokens.shape or dout.shape[-1] == 0 or num_embeddings <= 0:
         raise ValueError(f"embedding: dout {tuple(dout.shape)} does not go with tokens "
                          f"{tuple(tokens.shape)} and {num_embeddings} rows")
+    if dout.shape[-1] > _MAX_WIDTH:
+        raise ValueError(f"embedding: rows of up to {_MAX_WIDTH}, got {dout.shape[-1]}")
     dtype = dout.dtype if dtype is None else dtype
     p_drop = _check_embedding(tokens, dout.dtype, dtype, p_drop, seed, dout)
     if padding_idx is None:

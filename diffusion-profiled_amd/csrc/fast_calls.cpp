@@ -240,7 +240,7 @@ PyObject* embedding_fwd(PyObject*, PyObject* const* o, Py_ssize_t n) {
   int device = -1;
   const at::Tensor *t = plain(o[0], &device), *w = plain(o[1], &device), *seed;
   float p;
-  if (!t || !w || !tokens_ok(*t) || w->dim() != 2 || w->numel() == 0 || !w->is_contiguous() || !PyFloat_CheckExact(o[2]) ||
+  if (!t || !w || !tokens_ok(*t) || w->dim() != 2 || w->numel() == 0 || w->size(1) > 1 << 20 || !w->is_contiguous() || !PyFloat_CheckExact(o[2]) ||
       !embed_drop(o[3], o[4], &device, &p, &seed))
     return none();
   at::ScalarType type = w->scalar_type();

@@ -2,10 +2,12 @@
 from __future__ import annotations
 
 import pytest
+import torch
 
 from conftest import dpa_mod
 from test_conditioning_cpu import FAKE, _desc
 
+C = dpa_mod("conditioning")
 L = dpa_mod("_lib")
 
 
@@ -32,3 +34,15 @@ def test_attention_refuses_more_workgroups_than_a_grid_has(kw):
 def test_attention_refuses_more_workgroups_of_keys_than_a_grid_has():
     kw = dict(b=1 << 10, h=16, g=16, lq=1, lk=1 << 17)
     assert L.load().dpa_cross_attention_bwd(_desc(**kw), FAKE, 1 << 62, None) == -2
+
+
+@pytest.mark.parametrize("c", [(1 << 20) + 1, (1 << 32) + 8])
+def test_embedding_refuses_wide_rows(c):
+    """A width past 32 bits would reach the entry as its lowest 32."""
+    wide, tokens = torch.zeros(1).expand(1, c), torch.zeros(1, dtype=torch.int64)
+    with pytest.raises(ValueError, match="C up to"):
+        C.embedding_fwd(tokens, wide)
+    with pytest.raises(ValueError, match="C up to"):
+        C.embedding(tokens, wide)
+    with pytest.raises(ValueError, match="rows of up to"):
+        C.embedding_bwd(wide, tokens, 5)
