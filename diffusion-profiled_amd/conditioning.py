@@ -127,8 +127,8 @@ def _scale_of(scale: float | None, head_dim: int) -> float:
     if scale is None:
         return 1.0 / math.sqrt(head_dim)
     scale = float(scale)
-    if not 0.0 < scale < 3.4e38:
-        raise ValueError(f"cross attention: scale {scale} is not positive and finite")
+    if not 0.0 < scale < 2.3e38:        # (scale log2(e) is finite in fp32)
+        raise ValueError(f"cross attention: scale {scale} is not positive and below 2.3e38")
     return scale
 
 

@@ -93,7 +93,7 @@ bool describe(DpaCrossAttention& a, const at::Tensor& q, const at::Tensor& k, co
     a.scale = (float)(1.0 / std::sqrt((double)d));
   } else if (PyFloat_CheckExact(scale)) {
     const double s = PyFloat_AS_DOUBLE(scale);
-    if (!(s > 0.0 && s < 3.4e38)) return false;
+    if (!(s > 0.0 && s < 2.3e38)) return false;
     a.scale = (float)s;
   } else {
     return false;

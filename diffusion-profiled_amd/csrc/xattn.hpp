@@ -464,7 +464,7 @@ inline int check_shape(const DpaCrossAttention& a) {
   if (a.dtype != DPA_DTYPE_BF16 && a.dtype != DPA_DTYPE_F16) return DPA_ERR_SHAPE;
   if (a.batch < 0 || a.q_len < 0 || a.kv_len < 0 || a.heads <= 0 || a.kv_heads <= 0) return DPA_ERR_SIZE;
   if (a.heads % a.kv_heads || a.head_dim <= 0 || a.head_dim > 128 || a.head_dim % 8) return DPA_ERR_SHAPE;
-  if (!(a.scale > 0.f) || !(a.scale <= 3.4e38f)) return DPA_ERR_SIZE;
+  if (!(a.scale > 0.f) || !(a.scale * kLog2e <= 3.4e38f)) return DPA_ERR_SIZE;
   const int64_t most = 1ll << 30;
   const int64_t rows = (int64_t)a.heads / a.kv_heads * a.q_len;
   if (rows >= most || a.kv_len >= most || (int64_t)a.batch * a.kv_heads >= most) return DPA_ERR_SIZE;

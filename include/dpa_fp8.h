@@ -797,7 +797,7 @@ int dpa_conv3x3_thin_wgrad(const void* x, int x_dtype, const void* dy, float* dw
  * q, out, dout, dq: [batch][q_len][heads][head_dim]; k, v, dk, dv: [batch][kv_len][kv_heads]
  * [head_dim]; lse: [batch][heads][q_len]. out and dq are dense; the others have element strides
  * {batch, token, head} (multiples of 8; 0 repeats k and v over the batch) and dense head_dim;
- * pointers 16-B aligned. scale > 0. Lengths may be 0. Sizes that would take 2^24 workgroups
+ * pointers 16-B aligned. scale > 0, its product with log2(e) finite. Lengths may be 0. Sizes that would take 2^24 workgroups
  * (of up to 128 query rows or 64 keys of a key/value head) are refused. The descriptor is host memory,
  * read at the call.
  * ---------------------------------------------------------------------------------------- */

@@ -46,3 +46,12 @@ def test_embedding_refuses_wide_rows(c):
         C.embedding(tokens, wide)
     with pytest.raises(ValueError, match="rows of up to"):
         C.embedding_bwd(wide, tokens, 5)
+
+
+def test_attention_refuses_scales_that_overflow_in_base_2():
+    """The kernels work on scale log2(e): infinite, a score of 0 would be NaN."""
+    for s in (2.5e38, 3.3e38):
+        with pytest.raises(ValueError, match="scale"):
+            C._scale_of(s, 64)
+        assert L.load().dpa_cross_attention_fwd(_desc(scale=s), None, 0, None) == -2
+    assert C._scale_of(2.2e38, 64) == 2.2e38
