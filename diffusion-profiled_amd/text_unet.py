@@ -39,10 +39,10 @@ class TextEmbedding(nn.Module):
         with torch.no_grad():
             self.weight[text.padding_idx].zero_()
 
-    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
+    def forward(self, tokens: torch.Tensor, dropout: bool = True) -> torch.Tensor:
         return C.embedding(tokens, self.weight, scale=math.sqrt(self.text.width),
                            padding_idx=self.text.padding_idx, p_drop=self.text.p_drop,
-                           training=self.training, out_dtype=torch.bfloat16)
+                           training=self.training and dropout, out_dtype=torch.bfloat16)
 
 
 class CrossAttentionBlock(nn.Module):
@@ -115,19 +115,21 @@ class TextUNet(UNet):
 
     @torch.no_grad()
     def keep_prompt(self, tokens: torch.Tensor | None) -> None:
-        """For sampling: every block's keys and values of these prompts, formed once and used by the
-        calls without a prompt of their own until the next ``keep_prompt`` (None: no longer). They are
-        of the weights as they are now."""
+        """For sampling: every block's keys and values of these prompts, formed once (without dropout) and
+        used by the calls without a prompt of their own until the next ``keep_prompt`` (None: no longer).
+        They are of the weights as they are now, and carry no gradient: training steps (calls in training
+        mode that record one) take ``prompt``."""
         self._kept = None
         if tokens is not None:
             with torch.autocast("cuda", dtype=torch.bfloat16):
-                states = self.text(tokens)
+                states = self.text(tokens, dropout=False)
                 self._kept = ({name: block.project(states) for name, block in self.cross.items()},
                               tokens != self.text.text.padding_idx)
 
     def _forward(self, x: torch.Tensor, t: torch.Tensor) -> torch.Tensor:
         tokens = self._tokens if self._tokens is not None else self.prompt
-        if self._tokens is None and self._kept is not None:
+        training = self.training and torch.is_grad_enabled()
+        if self._tokens is None and self._kept is not None and not training:
             kept, self._seen = self._kept
             self._kv = kept.__getitem__
         elif tokens is not None:
