@@ -3,7 +3,8 @@
 The library has a plain C ABI (``include/dpa_fp8.h``) and does not link against torch.
 Sources compile in parallel (one ``hipcc -c`` per file) and link with ``hipcc -shared``. Beside it
 ``lib/dpa_fast_calls.so`` (``csrc/fast_calls.cpp``, host code only) is a Python module for the torch
-of this interpreter.
+of this interpreter; without torch, its headers or g++ the library is built alone, with a warning, and the
+module's calls take the general way through Python.
 """
 from __future__ import annotations
 
@@ -11,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sysconfig
+import warnings
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -77,8 +79,11 @@ def build_library(verbose: bool = False) -> Path:
         if verbose:
             print(" ".join(cmd), flush=True)
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
-    fast = subprocess.Popen(_fast_calls_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
-    procs.append((CSRC_DIR / "fast_calls.cpp", fast))
+    fast, why = None, ""
+    try:
+        fast = subprocess.Popen(_fast_calls_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+    except (ImportError, OSError) as e:     # no torch, no g++
+        why = str(e)
     errors = []
     for src, p in procs:
         out, _ = p.communicate()
@@ -89,6 +94,9 @@ def build_library(verbose: bool = False) -> Path:
             errors.append(f"{src.name}:\n" + "\n".join(lines))
         elif verbose and lines:
             print("\n".join(lines), flush=True)
+    if fast is not None:
+        out, _ = fast.communicate()
+        why = out.decode(errors="replace") if fast.returncode != 0 else ""
     if errors:
         raise RuntimeError("hipcc failed:\n" + "\n\n".join(errors))
     tmp = LIB_PATH.with_suffix(".so.tmp")
@@ -99,7 +107,11 @@ def build_library(verbose: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError("hipcc link failed:\n" + r.stdout.decode(errors="replace"))
     os.replace(tmp, LIB_PATH)
-    os.replace(FAST_PATH.with_suffix(".so.tmp"), FAST_PATH)
+    if why:
+        FAST_PATH.unlink(missing_ok=True)       # (one of another build would not fit this library)
+        warnings.warn(f"{FAST_PATH.name} was not built, its calls go through Python: {why}")
+    else:
+        os.replace(FAST_PATH.with_suffix(".so.tmp"), FAST_PATH)
     return LIB_PATH
 
 
