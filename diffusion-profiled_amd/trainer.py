@@ -33,9 +33,13 @@ def save_checkpoint(model: torch.nn.Module, step: int, config: dict, filename: s
     """train.py:85-91: ``{"model_state_dict": model.state_dict(), "step": step, "config":
     config}`` written with torch.save. The reference passes its EMA model and
     ``UNetConfig.as_dict()`` plus ``hparams.*`` entries; the keys of this build's state dict
-    are the reference's (module tree, parameter and FP8 window buffer names)."""
-    torch.save({"model_state_dict": model.state_dict(), "step": int(step), "config": config},
-               filename)
+    are the reference's (module tree, parameter and FP8 window buffer names). A
+    ``text_unet.TextUNet``'s file has its ``TextConfig`` as "text" beside them."""
+    ck = {"model_state_dict": model.state_dict(), "step": int(step), "config": config}
+    plain = getattr(model, "_orig_mod", model)      # (of a torch.compile'd module)
+    if isinstance(plain, TextUNet):
+        ck["text"] = dataclasses.asdict(plain.text.text)
+    torch.save(ck, filename)
 
 
 def config_from_dict(config: dict) -> UNetConfig:
@@ -51,8 +55,8 @@ def load_checkpoint(filename: str | os.PathLike, model: torch.nn.Module | None =
     (tensors, numbers, strings and containers only; nothing in the file is executed).
     State dicts saved from a torch.compile'd module (the reference compiles its model and
     its EMA copy, train.py:251, diffusion/ddpm.py:16) carry an ``_orig_mod.`` prefix, which
-    is removed. Loads into ``model`` (built from the checkpoint's config when None) and
-    returns ``(model, step, config)``."""
+    is removed. Loads into ``model`` (built from the checkpoint's config when None: a
+    ``text_unet.TextUNet`` where the file names its text, else a ``UNet``) and returns ``(model, step, config)``."""
     ck = torch.load(filename, map_location=map_location, weights_only=True)
     if not isinstance(ck, dict) or any(k not in ck for k in CHECKPOINT_KEYS):
         raise KeyError(f"{filename}: not a checkpoint with keys {CHECKPOINT_KEYS}")
@@ -60,7 +64,8 @@ def load_checkpoint(filename: str | os.PathLike, model: torch.nn.Module | None =
           for k, v in ck["model_state_dict"].items()}
     config = ck["config"]
     if model is None:
-        model = UNet(config_from_dict(config))
+        model = UNet(config_from_dict(config)) if ck.get("text") is None else TextUNet(
+            config_from_dict(config), TextConfig(**ck["text"]))
     model.load_state_dict(sd, strict=strict)
     return model, int(ck["step"]), config
 
