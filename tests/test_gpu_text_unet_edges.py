@@ -1,11 +1,11 @@
-"""The text-conditioned U-Net: prompts kept for sampling against training."""
+"""The text-conditioned U-Net: prompts kept for sampling against training, and the captured step."""
 from __future__ import annotations
 
 import pytest
 import torch
 
 from conftest import dpa_mod
-from test_gpu_text_unet import _images, _model, _text, _tokens
+from test_gpu_text_unet import _config, _images, _model, _text, _tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,37 @@ def test_a_prompt_kept_in_training_mode_is_kept_without_dropout():
         m.train().keep_prompt(tokens)
         assert m.training and m.text.training
         assert torch.equal(_loss(m.eval(), x, t), want)
+
+
+@pytest.mark.parametrize("scaling", ["current", "delayed"])
+def test_captured_steps_are_the_eager_ones_to_the_bit(scaling):
+    g = torch.Generator().manual_seed(11)
+    data = [(_images(8, g), torch.randint(0, 100, (8,), generator=g).cuda(), _images(8, g), _tokens(8, 12, g))
+            for _ in range(4)]
+
+    def state():
+        s = T.TrainState(_config(fp8_scaling_type=scaling), 8, max_t=100, text=_text(), prompt_length=12,
+                         fixed_noise=True, ema_beta=0.9, seed=1)
+        s.set_batch(*data[0])
+        return s
+
+    def walk(s, step):
+        losses = []
+        for i in range(6):
+            s.set_batch(*data[i % 4])
+            s.loss_acc.zero_()
+            step()
+            torch.cuda.synchronize()
+            losses.append(float(s.loss_acc))
+        return losses
+    a, b = state(), state()
+    before = a.model.text.weight.detach().clone()
+    a.capture(warmup=3)
+    for _ in range(3):
+        b.eager_step()
+    assert walk(a, a.replay) == walk(b, b.eager_step)
+    for (n, p), q in zip(a.model.named_parameters(), b.model.parameters()):
+        assert torch.equal(p, q), n
+    dw = a.model.text.weight.grad
+    assert dw is not None and bool(dw.isfinite().all()) and bool(dw.any()) and not dw[0].any()
+    assert bool((a.model.text.weight[1:] != before[1:]).any())
