@@ -193,7 +193,7 @@ def cross_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     [B], clamped to [0, Lk]) and where key_mask ([B, Lk], bool or uint8) is true; keys that do not
     are never read. A query without any gets 0, and -inf as its log sum exp. scale: 1 / sqrt(D) by
     default, positive. Returns (out [B, Lq, H, D], lse [B, H, Lq] fp32)."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_dynamo_compiling():
         return _between_graphs(cross_attention_fwd, q, k, v, key_lengths=key_lengths, key_mask=key_mask, scale=scale)
     done = _fast().attention_fwd(q, k, v, key_lengths, key_mask, scale)
     if done is not None:
@@ -213,7 +213,7 @@ def cross_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
 
 def _attention_bwd(dout, q, k, v, out, lse, key_lengths, key_mask, scale, dk, dv):
     """(dq, dk, dv); dk and dv: None (not formed), True (a new dense tensor) or where to write them."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_dynamo_compiling():
         return _between_graphs(_attention_bwd, dout, q, k, v, out, lse, key_lengths, key_mask, scale, dk, dv)
     done = _fast().attention_bwd(dout, q, k, v, out, lse, key_lengths, key_mask, scale, dk, dv)
     if done is not None:
@@ -309,7 +309,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
                     scale: float | None = None) -> torch.Tensor:
     """Differentiable ``cross_attention_fwd`` (its first output). Under autocast fp32 operands are
     rounded to the autocast dtype first."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_dynamo_compiling():
         return _between_graphs(cross_attention, q, k, v, key_lengths=key_lengths, key_mask=key_mask, scale=scale)
     q, k, v = _autocast(q, k, v)
     return apply(CrossAttention, q, k, v, key_lengths, key_mask, scale)
@@ -322,7 +322,7 @@ def cross_attention_kv(q: torch.Tensor, kv: torch.Tensor, *,
     """``cross_attention`` over keys and values side by side, kv [B, Lk, 2, G, D] (a projection of
     the encoder's states to 2 G D columns). A sampler projects them once and keeps kv over its
     steps."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_dynamo_compiling():
         return _between_graphs(cross_attention_kv, q, kv, key_lengths=key_lengths, key_mask=key_mask, scale=scale)
     if kv.ndim != 5 or kv.shape[2] != 2:
         raise ValueError(f"cross attention: kv is [batch, tokens, 2, heads, head_dim], got {tuple(kv.shape)}")
@@ -363,7 +363,7 @@ def dropout_fwd(x: torch.Tensor, p: float, seed: torch.Tensor, *,
     fp32 and rounded once. x is bf16, fp16 or fp32. An element's place in memory is its index for
     the mask (dense or channels-last tensors as they are, others as their dense copy); the result
     has x's layout. A dropped element counts as 0 whatever it holds."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_dynamo_compiling():
         return _between_graphs(dropout_fwd, x, p, seed, residual=residual)
     y = _fast().dropout(x, p, seed, residual)
     if y is not None:
@@ -414,7 +414,7 @@ def dropout(x: torch.Tensor, p: float = 0.5, *, training: bool = True,
             residual: torch.Tensor | None = None, seed: torch.Tensor | None = None) -> torch.Tensor:
     """Differentiable ``dropout_fwd``. seed: drawn from torch's generator when not given (a captured
     graph draws a new one each replay). Without training, or with p = 0, x (+ residual)."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_dynamo_compiling():
         return _between_graphs(dropout, x, p, training=training, residual=residual, seed=seed)
     p = _check_p(p, "dropout")
     if not training or p == 0.0:
@@ -444,7 +444,7 @@ def embedding_fwd(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 
     """scale weight[tokens] in out_dtype (weight's by default), with p_drop > 0 followed by dropout
     (index: the element's place in the output; seed as in ``dropout_fwd``). tokens int32 or int64
     of any shape, weight [V, C] bf16, fp16 or fp32. A token outside [0, V) gives a row of NaN."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_dynamo_compiling():
         return _between_graphs(embedding_fwd, tokens, weight, scale=scale, p_drop=p_drop, seed=seed,
                                out_dtype=out_dtype)
     out = _fast().embedding_fwd(tokens, weight, scale, p_drop, seed, out_dtype)
@@ -469,7 +469,7 @@ def embedding_bwd(dout: torch.Tensor, tokens: torch.Tensor, num_embeddings: int,
     """The gradient [num_embeddings, C] of ``embedding_fwd``'s weight in dtype (dout's by default):
     per row the fp32 sum over its tokens in order, rounded once; zeros for padding_idx. Tokens
     outside the table add nothing. Deterministic."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_dynamo_compiling():
         return _between_graphs(embedding_bwd, dout, tokens, num_embeddings, scale=scale, padding_idx=padding_idx,
                                p_drop=p_drop, seed=seed, dtype=dtype)
     dw = _fast().embedding_bwd(dout, tokens, num_embeddings, scale, padding_idx, p_drop, seed, dtype)
@@ -521,7 +521,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
               seed: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """Differentiable ``embedding_fwd``; the weight's gradient comes in its own dtype. Dropout only
     with training; seed as in ``dropout``."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_dynamo_compiling():
         return _between_graphs(embedding, tokens, weight, scale=scale, padding_idx=padding_idx, p_drop=p_drop,
                                training=training, seed=seed, out_dtype=out_dtype)
     p_drop = _check_p(p_drop, "embedding") if training else 0.0
