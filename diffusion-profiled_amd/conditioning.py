@@ -190,9 +190,9 @@ def cross_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     H (query head h reads key head h // (H / G)). Any strides with dense heads are read in place
     when they are multiples of 8 elements -- halves of a packed projection, ``expand`` over the
     batch -- others through a dense copy. A key takes part below key_lengths[b] (int32 or int64
-    [B], clamped to [0, Lk]) and where key_mask ([B, Lk], bool or uint8) is true; keys that do not
-    are never read. A query without any gets 0, and -inf as its log sum exp. scale: 1 / sqrt(D) by
-    default, positive. Returns (out [B, Lq, H, D], lse [B, H, Lq] fp32)."""
+    [B], clamped to [0, Lk]) and where key_mask ([B, Lk], bool or uint8) is true; what keys hold
+    that do not changes nothing (rows from the length on are not read, rows that the mask hides may be). A
+    query without any gets 0, and -inf as its log sum exp. scale: 1 / sqrt(D) by default, positive. Returns (out [B, Lq, H, D], lse [B, H, Lq] fp32)."""
     if torch.compiler.is_dynamo_compiling():
         return _between_graphs(cross_attention_fwd, q, k, v, key_lengths=key_lengths, key_mask=key_mask, scale=scale)
     done = _fast().attention_fwd(q, k, v, key_lengths, key_mask, scale)
@@ -467,8 +467,9 @@ def embedding_bwd(dout: torch.Tensor, tokens: torch.Tensor, num_embeddings: int,
                   scale: float = 1.0, padding_idx: int | None = None, p_drop: float = 0.0,
                   seed: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
     """The gradient [num_embeddings, C] of ``embedding_fwd``'s weight in dtype (dout's by default):
-    per row the fp32 sum over its tokens in order, rounded once; zeros for padding_idx. Tokens
-    outside the table add nothing. Deterministic."""
+    per row the fp32 sum over its tokens, rounded once; zeros for padding_idx. Tokens outside the table
+    add nothing. A row's tokens are summed by position, many in pieces of up to 32 whose sums are then
+    added: always in the same order."""
     if torch.compiler.is_dynamo_compiling():
         return _between_graphs(embedding_bwd, dout, tokens, num_embeddings, scale=scale, padding_idx=padding_idx,
                                p_drop=p_drop, seed=seed, dtype=dtype)

@@ -1,7 +1,7 @@
 // Token embedding, out[i] = keep scale / (1 - p) W[token i] (keep and p: an optional dropout by
 // counter hash, element index i C + c), and the gradient of W,
-//   dW[v] = scale / (1 - p) sum over i with token i = v of keep dout[i], in order of i,
-// without atomics: the tokens are sorted, and every run of equal ones has one writer.
+//   dW[v] = scale / (1 - p) sum over i with token i = v of keep dout[i], in a fixed order,
+// without atomics: the tokens are sorted (stable), and every run of equal ones has one writer.
 #include "dpa_common.hpp"
 
 namespace dpa {
@@ -292,8 +292,8 @@ __global__ __launch_bounds__(kChunk) void embed_sort_kernel(const SortArgs p) {
 // Up to kSmall tokens: the whole gradient in one launch, for whose others a small call would wait (512
 // tokens, 663 rows of 768: 12.2 us; with 1000 tokens it would be 17.9, and the three launches of the
 // form for more 14.7).
-// `slices` workgroups of 64 channels sort the tokens, each for itself, and sum: a wave takes 16, 32,
-// 48 or 64 sorted places; a run that goes on in the next wave is finished, in order, by the wave in which it
+// `slices` workgroups of 64 channels sort the tokens, each for itself, and sum: a wave takes 16 or
+// 32 sorted places; a run that goes on in the next wave is finished, in order, by the wave in which it
 // starts, from what the others leave in LDS. The other workgroups clear the rows that no token names
 // (a bit per row in LDS).
 // ---------------------------------------------------------------------------------------
@@ -337,6 +337,7 @@ __global__ __launch_bounds__(kChunk) void embed_small_kernel(const Args p, const
   if (tid < n) s.sort.key[tid] = key_of<TB>(tokens, tid, p.V, p.pad);
   const uint16_t* order = sort_chunk(s.sort, n, passes, tid);
   const int per = (n + kSortWaves * kBatch - 1) / (kSortWaves * kBatch) * kBatch;  // a wave's places
+  static_assert(kSmall <= 2 * kSortWaves * kBatch, "16 or 32 places");
   const int place = wave * per + lane;
   const bool on = lane < per && place < n;
   const uint32_t at = on ? order[place] : 0;

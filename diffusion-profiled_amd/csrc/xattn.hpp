@@ -4,8 +4,9 @@
 // token r % Lq):
 //   S = c Q K^T over the visible keys, P = softmax(S), O = P V, lse = log sum exp S.
 // A key is visible below its batch's length and where its mask byte is not 0. Rows of keys and
-// values that are not visible are never read (they may hold NaN): zeros take their place in LDS,
-// and their scores are -inf. A row without a visible key gives O = 0 and lse = -inf.
+// values that are not visible change nothing (they may hold NaN): zeros take their place in LDS,
+// and their scores are -inf. Those from the length on are not read; those that the mask hides below it
+// may be, where a tile goes as a whole, and are cleared in LDS. A row without a visible key gives O = 0 and lse = -inf.
 //
 // Products run on v_mfma_f32_32x32x16 (bf16 or fp16 operands, fp32 sums): against the 16x16x32
 // form it needs half the LDS reads per product, and one query per lane column, so a row's

@@ -789,8 +789,9 @@ int dpa_conv3x3_thin_wgrad(const void* x, int x_dtype, const void* dy, float* dw
  * key/value head h / (heads / kv_heads); head_dim a multiple of 8 up to 128; operands bf16 or
  * fp16 (dtype DPA_DTYPE_BF16 / DPA_DTYPE_F16), sums and softmax in fp32. A key takes part when
  * its index is below key_lengths[b] (NULL: all of kv_len; values are clamped to [0, kv_len]) and
- * key_mask[b * mask_stride + key] is not 0 (NULL: all). Keys and values that take no part are
- * not read. Without any: out = 0, lse = -inf, no gradient from that query.
+ * key_mask[b * mask_stride + key] is not 0 (NULL: all). What keys and values hold that take no part
+ * changes nothing; from the length on they are not read, those that key_mask hides may be. Without
+ * any: out = 0, lse = -inf, no gradient from that query.
  *   fwd: out = softmax(scale q k^T) v, lse = log sum exp(scale q k^T)  (natural logarithm)
  *   bwd: dq, dk, dv (dk and dv summed over the query heads that share them; zeros for keys that
  *        take no part) from dout, out and lse; deterministic. dk and dv both NULL: not formed.
@@ -834,9 +835,10 @@ int dpa_dropout(const void* x, const void* residual, void* y, int dtype, int64_t
  * or 8: int32 or int64), weight [V][C] and out [n][C] dense, each bf16, fp16 or fp32; with
  * drop_seed (a uint64 in device memory, NULL for none) followed by dropout of the element index
  * i C + c. A token outside [0, V) gives a row of NaN.
- * bwd: dweight [V][C], all of it written: scale times the sum, in order of i and in fp32, of
- * (dropped) dout[i] over the tokens of a row; zeros for rows without tokens and for padding_idx
- * (-1: none). Tokens outside [0, V) add nothing. Deterministic. dweight 16-B aligned.
+ * bwd: dweight [V][C], all of it written: scale times the fp32 sum of (dropped)
+ * dout[i] over the tokens of a row, by position, of many tokens in pieces of up to 32 whose sums are
+ * then added; zeros for rows without tokens and for padding_idx (-1: none). Tokens outside [0, V)
+ * add nothing. The order of sums is fixed: the same bits every time. dweight 16-B aligned.
  * n < 2^31 forward, below 2^29 backward; C at most 2^20. */
 int dpa_embedding_fwd(const void* tokens, int token_bytes, const void* weight, int weight_dtype,
                       void* out, int out_dtype, int64_t n, int64_t V, int C, float scale,
