@@ -192,7 +192,8 @@ def cross_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     batch -- others through a dense copy. A key takes part below key_lengths[b] (int32 or int64
     [B], clamped to [0, Lk]) and where key_mask ([B, Lk], bool or uint8) is true; what keys hold
     that do not changes nothing (rows from the length on are not read, rows that the mask hides may be). A
-    query without any gets 0, and -inf as its log sum exp. scale: 1 / sqrt(D) by default, positive. Returns (out [B, Lq, H, D], lse [B, H, Lq] fp32)."""
+    query without any gets 0, and -inf as its log sum exp. scale: 1 / sqrt(D) by default, positive.
+    Returns (out [B, Lq, H, D], lse [B, H, Lq] fp32)."""
     if torch.compiler.is_dynamo_compiling():
         return _between_graphs(cross_attention_fwd, q, k, v, key_lengths=key_lengths, key_mask=key_mask, scale=scale)
     done = _fast().attention_fwd(q, k, v, key_lengths, key_mask, scale)

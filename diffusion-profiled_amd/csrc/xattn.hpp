@@ -20,7 +20,6 @@ namespace xattn {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -56,7 +55,7 @@ struct Args {
 // bits of probabilities down to 2^-28.
 // kScaled: dS is scaled by a power of 2 that follows its size (in fp16: P (dP - D) over 4096 keys with
 // gradients of 1e-5 is mostly below its subnormals, and beyond 65504 with a large loss scale).
-struct Bf16 {
+struct Bf16 : Elem<DPA_DTYPE_BF16> {
   static constexpr int kShift = 24;
   static constexpr bool kScaled = false;
   template <class A>
@@ -64,27 +63,15 @@ struct Bf16 {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
-  static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
-  static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 };
 
-struct F16 {
+struct F16 : Elem<DPA_DTYPE_F16> {
   static constexpr int kShift = 14;
   static constexpr bool kScaled = true;
   template <class A>
   static __device__ __forceinline__ v16f mfma(A a, uint4 b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, f16x2));
-  }
-  static __device__ __forceinline__ float lo(uint32_t w) {
-    return (float)__builtin_bit_cast(f16x2, w).x;
-  }
-  static __device__ __forceinline__ float hi(uint32_t w) {
-    return (float)__builtin_bit_cast(f16x2, w).y;
   }
 };
 
