@@ -377,30 +377,50 @@ __device__ __forceinline__ float sum_halves(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// the maximum over a wave, of nothing negative: halves, rows of 16 lanes, then within a row
+__device__ __forceinline__ float wave_max(float x) {
+  x = max_halves(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false)));  // row_ror:8
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x124, 0xf, 0xf, false)));
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x122, 0xf, 0xf, false)));
+  return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x121, 0xf, 0xf, false)));
+}
+
 // The power of 2, `up`, at which a lane's column of 2^kShift dS stands (fp16): moved down only when a
 // |dP - D| passes what the type holds, and then so far that values 2^4 larger fit too, so that nearly every
-// tile goes without moving the sums. Costs half a vector instruction per score and an exchange (dK's one
-// more): the fp16 backward of 16 x 1024 queries of 8 heads over 512 keys of 2, 128 dims, 168 -> 175 us, of 16 x 1
-// of 16 heads over 4097 keys of 4 133 -> 145, of 8 x 4096 of 64 dims over 1024 as before (293, 288).
+// tile goes without moving the sums. In the kernel of dK and dV a wave's columns share it, in a scalar
+// register: at 128 dims it has no vector register left (175 us with one, 171 without, at 16 x 1024 below). Numbers
+// down to 2^-25 of the largest that fits stay normal, so smaller columns lose nothing.
+// Half a vector instruction per score, in dK one more. The fp16 backward without and with it: 16 x 1024 queries of
+// 8 heads over 512 keys of 2, 128 dims, 168, 171 us; 16 x 1 of 16 heads over 4097 keys of 4 133, 142; 8 x 4096 of 64
+// dims over 1024 keys 293, 298; 128 x 1024 of 32 dims over 200 keys 98, 106.
 struct DsScale {
   static constexpr int kFirst = 46;  // (nothing passes before it is 2^-45)
   float up = __uint_as_float((127u + kFirst) << 23);
-  // the largest of these 16 of the column's values (and the 16 of lane ^ 32)
+  // the largest of these 16 of the column's values (lane ^ 32 has as many more of them)
   static __device__ __forceinline__ float largest(const v16f& dp) {
-    float t = 0.f;
+    float t[2] = {0.f, 0.f};
 #pragma unroll
-    for (int r = 0; r < 16; ++r) t = fmaxf(t, fabsf(dp[r]));
-    return max_halves(t);
+    for (int r = 0; r < 16; ++r) t[r & 1] = fmaxf(t[r & 1], fabsf(dp[r]));
+    return fmaxf(t[0], t[1]);
   }
   // 2^kShift dS up stays below 2^15 (P is at most 1, but for its rounding)
   __device__ __forceinline__ bool passes(float top) const { return top * up > 2.f; }
-  // the binary exponent by which it moves, 0 if top does not pass
+  // the binary exponent by which it moves for the column's `top`, 0 if that does not pass
   __device__ __forceinline__ int move(float top) {
     if (!passes(top)) return 0;
     const int was = __builtin_amdgcn_frexp_expf(up) - 1;
     const int k = min(was, -3 - __builtin_amdgcn_frexp_expf(top));  // (top < 2^its exponent)
     up = ldexpf(1.f, k);
     return k - was;
+  }
+  // the same for all of the wave's columns, from its lanes' largest
+  __device__ __forceinline__ int move_wave(float top) {
+    const int by = move(wave_max(top));
+    up = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(up)));
+    return __builtin_amdgcn_readfirstlane(by);
   }
 };
 

@@ -73,7 +73,7 @@ template <int NDB>
 __device__ __forceinline__ void follow(DsScale& ds, const v16f& dp, v16f (&dq)[NDB], float& nlse2) {
   const float top = DsScale::largest(dp);
   if (!__any(ds.passes(top))) return;
-  const int by = ds.move(top);
+  const int by = ds.move(max_halves(top));
   times(dq, ldexpf(1.f, by));
   nlse2 += (float)by;
 }
@@ -407,7 +407,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_d
   v16f dk[NDB], dv[NDB];
 #pragma unroll
   for (int i = 0; i < NDB; ++i) dk[i] = dv[i] = zero16();
-  DsScale ds;  // (of the key in the lane)
+  DsScale ds;  // (of the wave's keys)
   auto step = [&](int t, auto buffer) __attribute__((always_inline)) {
     constexpr int buf = decltype(buffer)::value;
     wait_vmcnt<0>();
@@ -426,9 +426,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_d
         }
         if constexpr (T::kScaled) {
           const float top = DsScale::largest(dp);
-          if (__any(ds.passes(top))) times(dk, ldexpf(1.f, ds.move(top)));
-#pragma unroll
-          for (int r = 0; r < 16; ++r) dp[r] *= ds.up;
+          if (__any(ds.passes(top))) times(dk, ldexpf(1.f, ds.move_wave(top)));
         }
         const v16f e = start_at(stat_at + st);
 #pragma unroll
@@ -439,7 +437,10 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : DP == 64 ? 3 : 4) void xattn_d
             const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c2, e[r]));
             const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], p.c2, e[r + 1]));
             pw[(r & 7) / 2] = T::pack(p0, p1);
-            sw[(r & 7) / 2] = T::pack(p0 * dp[r], p1 * dp[r + 1]);
+            if constexpr (T::kScaled)
+              sw[(r & 7) / 2] = T::pack(p0 * (dp[r] * ds.up), p1 * (dp[r + 1] * ds.up));
+            else
+              sw[(r & 7) / 2] = T::pack(p0 * dp[r], p1 * dp[r + 1]);
           }
           const uint4 pf = {pw[0], pw[1], pw[2], pw[3]}, sf = {sw[0], sw[1], sw[2], sw[3]};
 #pragma unroll

@@ -52,16 +52,6 @@ __device__ __forceinline__ float length2(uint4 x, float n) {
 }
 // (a row that is not finite takes no part in a maximum: its dS is not finite either)
 __device__ __forceinline__ float finite(float n) { return n < __builtin_inff() ? n : 0.f; }
-// the maximum over a wave, of nothing negative: halves, rows of 16 lanes, then within a row
-__device__ __forceinline__ float wave_max(float x) {
-  x = max_halves(x);
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false)));  // row_ror:8
-  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x124, 0xf, 0xf, false)));
-  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x122, 0xf, 0xf, false)));
-  return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x121, 0xf, 0xf, false)));
-}
 
 // ---------------------------------------------------------------------------------------
 // Forward: four waves, each with its own 32 rows of every tile of 128; the next tile's queries load
