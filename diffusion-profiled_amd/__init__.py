@@ -6,8 +6,17 @@ from ``csrc/*.hip`` by ``build.build_library()``.
 """
 from . import _lib, attention, build, conditioning, fp8_kernels, gn_silu  # noqa: F401
 from . import ddpm, unet, trainer  # noqa: F401
-from . import text_unet  # noqa: F401
+from . import mxfp4, text_unet  # noqa: F401
 from .conditioning import cross_attention, cross_attention_kv, dropout, embedding  # noqa: F401
+from .mxfp4 import (  # noqa: F401
+    MXFP4,
+    LinearMXFP4,
+    cross_attention_mxfp4,
+    dequantize_mxfp4,
+    linear_mxfp4,
+    mxfp4_operand,
+    quantize_mxfp4,
+)
 from .fp8_kernels import (  # noqa: F401
     FP8_DTYPE,
     FP8_MAX_E4M3,

@@ -248,6 +248,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_int, c_float,
                 c_int64, c_void_p, c_float, c_void_p, c_int64, c_void_p],
     ),
+    "dpa_mxfp4_quantize": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p]),
+    "dpa_mxfp4_dequantize": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p]),
+    "dpa_mxfp4_operand_data_bytes": (c_int64, [c_int64, c_int64]),
+    "dpa_mxfp4_operand_scale_bytes": (c_int64, [c_int64, c_int64]),
+    "dpa_mxfp4_operands": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64] + [c_void_p] * 6),
+    "dpa_mxfp4_gemm_workspace_bytes": (c_int64, [c_int64] * 3),
+    "dpa_mxfp4_gemm": (c_int, [c_void_p] * 6 + [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
+    "dpa_column_sum_workspace_bytes": (c_int64, [c_int64, c_int64]),
+    "dpa_column_sum": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
+    "dpa_cross_attention_mxfp4_workspace_bytes": (c_int64, [c_void_p]),
+    "dpa_cross_attention_mxfp4": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
 }
 
 _lock = threading.Lock()

@@ -849,6 +849,63 @@ int dpa_embedding_bwd(const void* dout, int dout_dtype, const void* tokens, int 
                       int64_t padding_idx, const void* drop_seed, float drop_p, void* workspace,
                       int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * MXFP4 (csrc/mxfp4*): blocks of 32 elements in e2m1 with one power of two each, its exponent + 127 in a
+ * byte. A block of largest magnitude amax gets 2^max(floor(log2 amax) - 2, -127) and elements to nearest
+ * even, those beyond 6 of it as 6; a block with a NaN or an infinity gets byte 255 and stands for NaN.
+ * Dense: a tensor whose last dim is a multiple of 32, n elements in n / 2 bytes (the first of two in the
+ * low half) and n / 32 scale bytes, in order. x and y are bf16, fp16 or fp32, 16-B aligned.
+ * ---------------------------------------------------------------------------------------- */
+int dpa_mxfp4_quantize(const void* x, int dtype, int64_t n, void* data, void* scales, void* stream);
+int dpa_mxfp4_dequantize(const void* data, const void* scales, void* y, int dtype, int64_t n,
+                         void* stream);
+
+/* Operands of dpa_mxfp4_gemm: a matrix whose contraction runs along its rows, cols long, any number of
+ * them: data of ceil(cols / 256) * 128 B a row, scales of ceil(cols / 512) * 16 B a row (buffers of
+ * *_bytes, 16-B aligned, opaque). dpa_mxfp4_operands lays out x [rows][cols] (row_stride elements apart)
+ * from one read: as it is (row_*: blocks along the rows) and transposed (col_*: an operand of `cols` rows,
+ * blocks down the columns); NULL for the one that is not wanted. With seed (a uint64 in device
+ * memory) elements are rounded up or down at random so that their mean is the element, the scale one power
+ * higher where amax would pass 6 of it: 16 bits a element of splitmix64(seed + i / 4 * golden ratio),
+ * i = row * (cols rounded up to 32) + col, for both arrangements. */
+int64_t dpa_mxfp4_operand_data_bytes(int64_t rows, int64_t cols);
+int64_t dpa_mxfp4_operand_scale_bytes(int64_t rows, int64_t cols);
+int dpa_mxfp4_operands(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride,
+                       void* row_data, void* row_scales, void* col_data, void* col_scales,
+                       const void* seed, void* stream);
+
+/* y [M][N] (bf16, fp16 or fp32) = a b^T + bias over operands a of M rows and b of N rows, K columns each;
+ * bias fp32 [N] or NULL. fp32 sums in a fixed order. */
+int64_t dpa_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int dpa_mxfp4_gemm(const void* a_data, const void* a_scales, const void* b_data, const void* b_scales,
+                   const float* bias, void* y, int dtype, int64_t M, int64_t N, int64_t K,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/* y [cols] fp32 = sums down the columns of x [rows][cols] (bf16, fp16 or fp32, rows row_stride elements
+ * apart), in fp32, in a fixed order. */
+int64_t dpa_column_sum_workspace_bytes(int64_t rows, int64_t cols);
+int dpa_column_sum(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, void* y,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The forward of dpa_cross_attention_fwd over keys and values in MXFP4, head_dim a multiple of 32 up to
+ * 128: elements of a head dense, 16-B aligned, strides of data and scales (batch, token, head) in bytes, those of
+ * data multiples of 16. With fp16 queries a value of the cache is rounded to fp16. */
+typedef struct DpaCrossAttentionMxfp4 {
+  const void *q, *k_data, *k_scales, *v_data, *v_scales;
+  void* out;
+  float* lse;
+  const int32_t* key_lengths;
+  const uint8_t* key_mask;
+  int64_t mask_stride;
+  int64_t q_stride[3], k_data_stride[3], k_scale_stride[3], v_data_stride[3], v_scale_stride[3];
+  int32_t dtype, batch, q_len, kv_len, heads, kv_heads, head_dim;
+  float scale;
+} DpaCrossAttentionMxfp4;
+
+int64_t dpa_cross_attention_mxfp4_workspace_bytes(const DpaCrossAttentionMxfp4* a);
+int dpa_cross_attention_mxfp4(const DpaCrossAttentionMxfp4* a, void* workspace, int64_t workspace_bytes,
+                              void* stream);
+
 #ifdef __cplusplus
 }
 #endif
