@@ -250,11 +250,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "dpa_mxfp4_quantize": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p]),
     "dpa_mxfp4_dequantize": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p]),
-    "dpa_mxfp4_operand_data_bytes": (c_int64, [c_int64, c_int64]),
-    "dpa_mxfp4_operand_scale_bytes": (c_int64, [c_int64, c_int64]),
-    "dpa_mxfp4_operands": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64] + [c_void_p] * 6),
+    "dpa_mxfp4_operand_bytes": (c_int64, [c_int64, c_int64]),
+    "dpa_mxfp4_operands": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64] + [c_void_p] * 4),
     "dpa_mxfp4_gemm_workspace_bytes": (c_int64, [c_int64] * 3),
-    "dpa_mxfp4_gemm": (c_int, [c_void_p] * 6 + [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
+    "dpa_mxfp4_gemm": (c_int, [c_void_p] * 4 + [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
+    "dpa_mxfp4_linear_workspace_bytes": (c_int64, [c_int64] * 3),
+    "dpa_mxfp4_linear": (
+        c_int, [c_void_p, c_int, c_int64] + [c_void_p] * 3 + [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p],
+    ),
     "dpa_column_sum_workspace_bytes": (c_int64, [c_int64, c_int64]),
     "dpa_column_sum": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
     "dpa_cross_attention_mxfp4_workspace_bytes": (c_int64, [c_void_p]),
@@ -315,7 +318,10 @@ def query(name: str, *args) -> int:
 _FAST_ENTRIES = ("dpa_cross_attention_fwd", "dpa_cross_attention_fwd_workspace_bytes",
                  "dpa_cross_attention_bwd", "dpa_cross_attention_bwd_workspace_bytes", "dpa_dropout",
                  "dpa_embedding_fwd", "dpa_embedding_bwd", "dpa_embedding_bwd_workspace_bytes",
-                 "dpa_status_string")
+                 "dpa_status_string", "dpa_mxfp4_quantize", "dpa_mxfp4_dequantize", "dpa_mxfp4_operand_bytes",
+                 "dpa_mxfp4_operands", "dpa_mxfp4_gemm", "dpa_mxfp4_gemm_workspace_bytes", "dpa_mxfp4_linear",
+                 "dpa_mxfp4_linear_workspace_bytes", "dpa_column_sum", "dpa_column_sum_workspace_bytes",
+                 "dpa_cross_attention_mxfp4", "dpa_cross_attention_mxfp4_workspace_bytes")
 
 
 def fast_calls():

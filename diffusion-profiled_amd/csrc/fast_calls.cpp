@@ -1,10 +1,10 @@
-// The conditioning operators' Python calls where nothing has to be converted: checks, allocation and
+// The conditioning and MXFP4 operators' Python calls where nothing has to be converted: checks, allocation and
 // the C entry in one native call. An eager call on small operands waits for its host side, of which
 // Python code and its arguments' conversion were two thirds: 4 x 1 queries over 77 keys 9.6 us in
 // Python, 3.4 us of it the launch.
 //
 // Every function returns None for a call that it does not take -- operands that need a copy, are
-// refused, or are anything but plain strided GPU tensors; conditioning.py then goes the general way,
+// refused, or are anything but plain strided GPU tensors; conditioning.py and mxfp4.py then go the general way,
 // which copies or raises. A module of the CPython API; the kernels' library is not linked but handed
 // over as addresses (init).
 #include <Python.h>
@@ -27,6 +27,18 @@ decltype(&dpa_dropout) drop;
 decltype(&dpa_embedding_fwd) emb_fwd;
 decltype(&dpa_embedding_bwd) emb_bwd;
 decltype(&dpa_embedding_bwd_workspace_bytes) emb_bwd_bytes;
+decltype(&dpa_mxfp4_quantize) mx_quant;
+decltype(&dpa_mxfp4_dequantize) mx_dequant;
+decltype(&dpa_mxfp4_operand_bytes) mx_operand_bytes;
+decltype(&dpa_mxfp4_operands) mx_operands;
+decltype(&dpa_mxfp4_gemm) mx_gemm;
+decltype(&dpa_mxfp4_gemm_workspace_bytes) mx_gemm_bytes;
+decltype(&dpa_mxfp4_linear) mx_linear;
+decltype(&dpa_mxfp4_linear_workspace_bytes) mx_linear_bytes;
+decltype(&dpa_column_sum) column_sum;
+decltype(&dpa_column_sum_workspace_bytes) column_sum_bytes;
+decltype(&dpa_cross_attention_mxfp4) mx_attn;
+decltype(&dpa_cross_attention_mxfp4_workspace_bytes) mx_attn_bytes;
 decltype(&dpa_status_string) status_string;
 
 // A plain strided tensor on a GPU (device: the first one's), or null
@@ -71,18 +83,13 @@ bool strides_of(const at::Tensor& t, int64_t* s) {
   return aligned16(t);
 }
 
-// What forward and backward describe alike. Sizes past 32 bits and the rest that the entry refuses
-// are left to it, and so to the general way's message.
-bool describe(DpaCrossAttention& a, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-              const at::Tensor* lengths, const at::Tensor* mask, PyObject* scale) {
-  if (q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || q.scalar_type() != k.scalar_type() ||
-      q.scalar_type() != v.scalar_type() || (q.scalar_type() != at::kBFloat16 && q.scalar_type() != at::kHalf) ||
-      k.sizes() != v.sizes() || k.size(0) != q.size(0) || k.size(3) != q.size(3))
-    return false;
-  const int64_t b = q.size(0), lq = q.size(1), h = q.size(2), d = q.size(3), lk = k.size(1), g = k.size(2);
-  const int64_t most = INT32_MAX;
-  if (b <= 0 || lq <= 0 || lk <= 0 || h <= 0 || g <= 0 || d <= 0 || d % 8 || d > 128 || h % g || b > most || lq > most ||
-      lk > most || h > most)
+// What a call over keys of any kind describes: queries, masks over lk keys, the scale. Sizes past 32 bits and
+// the rest that the entries refuse are left to them, and so to the general way's message.
+bool describe_queries(DpaCrossAttention& a, const at::Tensor& q, int64_t lk, const at::Tensor* lengths,
+                      const at::Tensor* mask, PyObject* scale) {
+  const int64_t b = q.size(0), lq = q.size(1), h = q.size(2), d = q.size(3), most = INT32_MAX;
+  if ((q.scalar_type() != at::kBFloat16 && q.scalar_type() != at::kHalf) || b <= 0 || lq <= 0 || h <= 0 || b > most ||
+      lq > most || h > most)
     return false;
   if (lengths && (lengths->dim() != 1 || lengths->size(0) != b || lengths->scalar_type() != at::kInt || !lengths->is_contiguous()))
     return false;
@@ -98,14 +105,27 @@ bool describe(DpaCrossAttention& a, const at::Tensor& q, const at::Tensor& k, co
   } else {
     return false;
   }
-  if (!strides_of(q, a.q_stride) || !strides_of(k, a.k_stride) || !strides_of(v, a.v_stride)) return false;
-  a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr();
+  if (!strides_of(q, a.q_stride)) return false;
+  a.q = q.data_ptr();
   a.key_lengths = lengths ? (const int32_t*)lengths->data_ptr() : nullptr;
   a.key_mask = mask ? (const uint8_t*)mask->data_ptr() : nullptr;
   a.mask_stride = mask ? mask->stride(0) : 0;
   a.dtype = dtype_of(q.scalar_type());
-  a.batch = (int32_t)b, a.q_len = (int32_t)lq, a.kv_len = (int32_t)lk;
-  a.heads = (int32_t)h, a.kv_heads = (int32_t)g, a.head_dim = (int32_t)d;
+  a.batch = (int32_t)b, a.q_len = (int32_t)lq, a.heads = (int32_t)h;
+  return true;
+}
+
+// What forward and backward describe alike
+bool describe(DpaCrossAttention& a, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+              const at::Tensor* lengths, const at::Tensor* mask, PyObject* scale) {
+  if (q.dim() != 4 || k.dim() != 4 || v.dim() != 4 || q.scalar_type() != k.scalar_type() ||
+      q.scalar_type() != v.scalar_type() || k.sizes() != v.sizes() || k.size(0) != q.size(0) || k.size(3) != q.size(3))
+    return false;
+  const int64_t h = q.size(2), d = q.size(3), lk = k.size(1), g = k.size(2), most = INT32_MAX;
+  if (lk <= 0 || g <= 0 || d <= 0 || d % 8 || d > 128 || h % g || lk > most) return false;
+  if (!describe_queries(a, q, lk, lengths, mask, scale) || !strides_of(k, a.k_stride) || !strides_of(v, a.v_stride)) return false;
+  a.k = k.data_ptr(), a.v = v.data_ptr();
+  a.kv_len = (int32_t)lk, a.kv_heads = (int32_t)g, a.head_dim = (int32_t)d;
   return true;
 }
 
@@ -286,25 +306,256 @@ PyObject* embedding_bwd(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// init(addresses of the library's entries, in the order of the pointers above)
-PyObject* init(PyObject*, PyObject* args) {
-  unsigned long long f[9];
-  if (!PyArg_ParseTuple(args, "KKKKKKKKK", f, f + 1, f + 2, f + 3, f + 4, f + 5, f + 6, f + 7, f + 8)) return nullptr;
-  attn_fwd = reinterpret_cast<decltype(attn_fwd)>(f[0]);
-  attn_fwd_bytes = reinterpret_cast<decltype(attn_fwd_bytes)>(f[1]);
-  attn_bwd = reinterpret_cast<decltype(attn_bwd)>(f[2]);
-  attn_bwd_bytes = reinterpret_cast<decltype(attn_bwd_bytes)>(f[3]);
-  drop = reinterpret_cast<decltype(drop)>(f[4]);
-  emb_fwd = reinterpret_cast<decltype(emb_fwd)>(f[5]);
-  emb_bwd = reinterpret_cast<decltype(emb_bwd)>(f[6]);
-  emb_bwd_bytes = reinterpret_cast<decltype(emb_bwd_bytes)>(f[7]);
-  status_string = reinterpret_cast<decltype(status_string)>(f[8]);
+// ---- MXFP4 (mxfp4.py) ----
+at::Tensor bytes_like(const at::Tensor& t, int64_t n) { return at::empty({n}, t.options().dtype(at::kByte)); }
+
+// the 16-B aligned beginning of the next part of a workspace
+int64_t round256(int64_t n) { return (n + 255) & ~255ll; }
+
+PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
+  PyObject* r = PyTuple_New((Py_ssize_t)ts.size());
+  if (!r) return nullptr;
+  Py_ssize_t i = 0;
+  for (const at::Tensor& t : ts) {
+    if (t.defined()) {
+      PyTuple_SET_ITEM(r, i++, THPVariable_Wrap(t));
+    } else {
+      Py_INCREF(Py_None);
+      PyTuple_SET_ITEM(r, i++, Py_None);
+    }
+  }
+  return r;
+}
+
+// x -> (data, scales)
+PyObject* mxfp4_quantize(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 1) return none();
+  int device = -1;
+  const at::Tensor* x = plain(o[0], &device);
+  if (!x || dtype_of(x->scalar_type()) < 0 || x->dim() < 1 || x->numel() == 0 || x->size(-1) % 32 || !x->is_contiguous() ||
+      !aligned16(*x))
+    return none();
+  at::DimVector shape(x->sizes().begin(), x->sizes().end());
+  shape.back() = x->size(-1) / 2;
+  at::Tensor data = at::empty(shape, x->options().dtype(at::kByte));
+  shape.back() = x->size(-1) / 32;
+  at::Tensor scales = at::empty(shape, x->options().dtype(at::kByte));
+  const int status = mx_quant(x->data_ptr(), dtype_of(x->scalar_type()), x->numel(), data.data_ptr(), scales.data_ptr(),
+                              stream_of(device));
+  if (status) return failed("dpa_mxfp4_quantize", status);
+  return tuple_of({data, scales});
+  END_HANDLE_TH_ERRORS
+}
+
+bool mxfp4_ok(const at::Tensor& d, const at::Tensor& s) {
+  const int64_t k = d.dim();
+  return d.scalar_type() == at::kByte && s.scalar_type() == at::kByte && k >= 1 && s.dim() == k &&
+         d.sizes().slice(0, k - 1) == s.sizes().slice(0, k - 1) && d.size(-1) == 16 * s.size(-1);
+}
+
+// (data, scales, dtype) -> y
+PyObject* mxfp4_dequantize(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 3) return none();
+  int device = -1;
+  const at::Tensor *d = plain(o[0], &device), *s = plain(o[1], &device);
+  at::ScalarType type = at::kBFloat16;
+  if (!d || !s || !mxfp4_ok(*d, *s) || !dtype_arg(o[2], &type) || dtype_of(type) < 0 || d->numel() == 0 || !d->is_contiguous() ||
+      !s->is_contiguous() || !aligned16(*d))
+    return none();
+  at::DimVector shape(d->sizes().begin(), d->sizes().end());
+  shape.back() *= 2;
+  at::Tensor y = at::empty(shape, d->options().dtype(type));
+  const int status = mx_dequant(d->data_ptr(), s->data_ptr(), y.data_ptr(), dtype_of(type), y.numel(), stream_of(device));
+  if (status) return failed("dpa_mxfp4_dequantize", status);
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// x [..., K] as a matrix of dense rows; its rows
+bool matrix_of(const at::Tensor& x, int64_t k, int64_t* rows) {
+  if (dtype_of(x.scalar_type()) < 0 || x.dim() < 1 || k <= 0 || x.size(-1) != k || x.numel() == 0 || !x.is_contiguous()) return false;
+  *rows = x.numel() / k;
+  return true;
+}
+
+bool bias_ok(const at::Tensor* b, int64_t n) {
+  return !b || (b->scalar_type() == at::kFloat && b->dim() == 1 && b->size(0) == n && b->is_contiguous());
+}
+
+// (x, operand, rows, cols, bias, out_dtype) -> y
+PyObject* mxfp4_linear(PyObject*, PyObject* const* o, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 6 || !PyLong_CheckExact(o[2]) || !PyLong_CheckExact(o[3])) return none();
+  int device = -1;
+  const at::Tensor *x = plain(o[0], &device), *w = plain(o[1], &device), *bias;
+  if (!x || !w || !maybe(o[4], &device, &bias)) return none();
+  const int64_t n = PyLong_AsLongLong(o[2]), k = PyLong_AsLongLong(o[3]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return none();
+  }
+  int64_t m;
+  at::ScalarType type = x->scalar_type();
+  if (!dtype_arg(o[5], &type) || dtype_of(type) < 0 || n <= 0 || !matrix_of(*x, k, &m) || !bias_ok(bias, n) ||
+      w->scalar_type() != at::kByte || !w->is_contiguous() || !aligned16(*w) || w->numel() != mx_operand_bytes(n, k))
+    return none();
+  const int64_t bytes = mx_linear_bytes(m, n, k);
+  if (bytes == 0) return none();
+  at::DimVector shape(x->sizes().begin(), x->sizes().end());
+  shape.back() = n;
+  at::Tensor y = at::empty(shape, x->options().dtype(type)), ws = bytes_like(*x, bytes);
+  const int status = mx_linear(x->data_ptr(), dtype_of(x->scalar_type()), k, w->data_ptr(),
+                               bias ? (const float*)bias->data_ptr() : nullptr, y.data_ptr(), dtype_of(type), m, n, k,
+                               ws.data_ptr(), bytes, stream_of(device));
+  if (status) return failed("dpa_mxfp4_linear", status);
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, weight, bias, out_dtype) -> (y, operand of x^T, operand of weight^T)
+PyObject* mxfp4_train_fwd(PyObject*, PyObject* const* o, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 4) return none();
+  int device = -1;
+  const at::Tensor *x = plain(o[0], &device), *w = plain(o[1], &device), *bias;
+  if (!x || !w || !maybe(o[2], &device, &bias) || w->dim() != 2) return none();
+  const int64_t n = w->size(0), k = w->size(1);
+  int64_t m, rows;
+  at::ScalarType type = x->scalar_type();
+  if (!dtype_arg(o[3], &type) || dtype_of(type) < 0 || n <= 0 || !matrix_of(*x, k, &m) || !matrix_of(*w, k, &rows) ||
+      !bias_ok(bias, n))
+    return none();
+  const int64_t xr = mx_operand_bytes(m, k), xc = mx_operand_bytes(k, m), wr = mx_operand_bytes(n, k), wc = mx_operand_bytes(k, n);
+  if (!xr || !xc || !wr || !wc) return none();
+  const int64_t gemm = mx_gemm_bytes(m, n, k), at_w = round256(xr), at_ws = at_w + round256(wr);
+  at::DimVector shape(x->sizes().begin(), x->sizes().end());
+  shape.back() = n;
+  at::Tensor y = at::empty(shape, x->options().dtype(type)), xo = bytes_like(*x, xc), wo = bytes_like(*x, wc),
+             ws = bytes_like(*x, at_ws + gemm);
+  uint8_t* p = (uint8_t*)ws.data_ptr();
+  void* s = stream_of(device);
+  int status = mx_operands(x->data_ptr(), dtype_of(x->scalar_type()), m, k, k, p, xo.data_ptr(), nullptr, s);
+  if (!status) status = mx_operands(w->data_ptr(), dtype_of(w->scalar_type()), n, k, k, p + at_w, wo.data_ptr(), nullptr, s);
+  if (status) return failed("dpa_mxfp4_operands", status);
+  status = mx_gemm(p, p + at_w, bias ? (const float*)bias->data_ptr() : nullptr, y.data_ptr(), dtype_of(type), m, n, k, p + at_ws,
+                   gemm, s);
+  if (status) return failed("dpa_mxfp4_gemm", status);
+  return tuple_of({y, xo, wo});
+  END_HANDLE_TH_ERRORS
+}
+
+// (dy, operand of x^T, operand of weight^T, n, k, dx dtype, dw dtype, whether dbias, seed) -> (dx, dw, db)
+PyObject* mxfp4_bwd(PyObject*, PyObject* const* o, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 9 || !PyLong_CheckExact(o[3]) || !PyLong_CheckExact(o[4])) return none();
+  int device = -1;
+  const at::Tensor *dy = plain(o[0], &device), *xo = plain(o[1], &device), *wo = plain(o[2], &device), *seed;
+  if (!dy || !xo || !wo || !maybe(o[8], &device, &seed) || (seed && !seed_ok(seed))) return none();
+  const int64_t n = PyLong_AsLongLong(o[3]), k = PyLong_AsLongLong(o[4]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return none();
+  }
+  int64_t m;
+  at::ScalarType dxt = at::kFloat, dwt = at::kFloat;
+  if (o[5] == Py_None || o[6] == Py_None || !dtype_arg(o[5], &dxt) || !dtype_arg(o[6], &dwt) || dtype_of(dxt) < 0 ||
+      dtype_of(dwt) < 0 || !matrix_of(*dy, n, &m))
+    return none();
+  const int64_t xc = mx_operand_bytes(k, m), wc = mx_operand_bytes(k, n), dr = mx_operand_bytes(m, n), dc = mx_operand_bytes(n, m);
+  if (!xc || !wc || !dr || !dc || xo->numel() != xc || wo->numel() != wc || xo->scalar_type() != at::kByte ||
+      wo->scalar_type() != at::kByte || !xo->is_contiguous() || !wo->is_contiguous() || !aligned16(*xo) || !aligned16(*wo))
+    return none();
+  const bool bias = o[7] == Py_True;
+  const int64_t g1 = mx_gemm_bytes(m, k, n), g2 = mx_gemm_bytes(n, k, m), sums = bias ? column_sum_bytes(m, n) : 0;
+  const int64_t at_c = round256(dr), at_ws = at_c + round256(dc), most = std::max(std::max(g1, g2), sums);
+  at::DimVector shape(dy->sizes().begin(), dy->sizes().end());
+  shape.back() = k;
+  at::Tensor dx = at::empty(shape, dy->options().dtype(dxt)), dw = at::empty({n, k}, dy->options().dtype(dwt)), db,
+             ws = bytes_like(*dy, at_ws + most);
+  if (bias) db = at::empty({n}, dy->options().dtype(at::kFloat));
+  uint8_t* p = (uint8_t*)ws.data_ptr();
+  void* s = stream_of(device);
+  const int type = dtype_of(dy->scalar_type());
+  int status = mx_operands(dy->data_ptr(), type, m, n, n, p, p + at_c, seed ? seed->data_ptr() : nullptr, s);
+  if (status) return failed("dpa_mxfp4_operands", status);
+  status = mx_gemm(p, wo->data_ptr(), nullptr, dx.data_ptr(), dtype_of(dxt), m, k, n, p + at_ws, g1, s);
+  if (!status) status = mx_gemm(p + at_c, xo->data_ptr(), nullptr, dw.data_ptr(), dtype_of(dwt), n, k, m, p + at_ws, g2, s);
+  if (status) return failed("dpa_mxfp4_gemm", status);
+  if (bias) status = column_sum(dy->data_ptr(), type, m, n, n, db.data_ptr(), p + at_ws, sums, s);
+  if (status) return failed("dpa_column_sum", status);
+  return tuple_of({dx, dw, db});
+  END_HANDLE_TH_ERRORS
+}
+
+// Byte strides of a cache's part [batch, tokens, 2, heads, width] in the order batch, token, head
+void part_strides(const at::Tensor& t, int64_t* s) {
+  s[0] = t.size(0) > 1 ? t.stride(0) : 0, s[1] = t.size(1) > 1 ? t.stride(1) : 0, s[2] = t.size(3) > 1 ? t.stride(3) : 0;
+}
+
+// (q, data, scales, key_lengths, key_mask, scale) -> (out, lse)
+PyObject* mxfp4_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6) return none();
+  int device = -1;
+  const at::Tensor *q = plain(o[0], &device), *d = plain(o[1], &device), *x = plain(o[2], &device), *lengths, *mask;
+  if (!q || !d || !x || !maybe(o[3], &device, &lengths) || !maybe(o[4], &device, &mask)) return none();
+  if (q->dim() != 4 || d->dim() != 5 || !mxfp4_ok(*d, *x) || d->size(2) != 2 || d->stride(4) != 1 ||
+      (x->stride(4) != 1 && x->size(4) > 1) || !aligned16(*d) || d->stride(2) % 16 || d->size(4) * 2 % 32)
+    return none();
+  // (shapes, masks and the scale as over keys of that shape: strides of k and v are those of q there)
+  DpaCrossAttention c{};
+  const int64_t b = q->size(0), lk = d->size(1), g = d->size(3), dim = 2 * d->size(4), most = INT32_MAX;
+  if (d->size(0) != b || q->size(3) != dim || g <= 0 || lk <= 0 || lk > most || g > most || q->size(2) % g || dim > 128 || dim <= 0 ||
+      !describe_queries(c, *q, lk, lengths, mask, o[5]))
+    return none();
+  DpaCrossAttentionMxfp4 a{};
+  part_strides(*d, a.k_data_stride), part_strides(*x, a.k_scale_stride);
+  for (int i = 0; i < 3; ++i) {
+    if (a.k_data_stride[i] % 16) return none();
+    a.q_stride[i] = c.q_stride[i], a.v_data_stride[i] = a.k_data_stride[i], a.v_scale_stride[i] = a.k_scale_stride[i];
+  }
+  at::Tensor out = at::empty(q->sizes(), q->options());
+  at::Tensor lse = at::empty({b, q->size(2), q->size(1)}, q->options().dtype(at::kFloat)), ws;
+  a.q = c.q, a.key_lengths = c.key_lengths, a.key_mask = c.key_mask, a.mask_stride = c.mask_stride;
+  a.k_data = d->data_ptr(), a.v_data = (uint8_t*)d->data_ptr() + d->stride(2);
+  a.k_scales = x->data_ptr(), a.v_scales = (uint8_t*)x->data_ptr() + x->stride(2);
+  a.out = out.data_ptr(), a.lse = (float*)lse.data_ptr();
+  a.dtype = c.dtype, a.batch = c.batch, a.q_len = c.q_len, a.kv_len = (int32_t)lk;
+  a.heads = c.heads, a.kv_heads = (int32_t)g, a.head_dim = (int32_t)dim, a.scale = c.scale;
+  const int64_t bytes = mx_attn_bytes(&a);
+  if (bytes) ws = bytes_like(*q, bytes);
+  const int status = mx_attn(&a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(device));
+  if (status) return failed("dpa_cross_attention_mxfp4", status);
+  return tuple_of({out, lse});
+  END_HANDLE_TH_ERRORS
+}
+
+// init(addresses of the library's entries, in this order)
+PyObject* init(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  void** const to[] = {(void**)&attn_fwd, (void**)&attn_fwd_bytes, (void**)&attn_bwd, (void**)&attn_bwd_bytes, (void**)&drop,
+                       (void**)&emb_fwd, (void**)&emb_bwd, (void**)&emb_bwd_bytes, (void**)&status_string,
+                       (void**)&mx_quant, (void**)&mx_dequant, (void**)&mx_operand_bytes, (void**)&mx_operands,
+                       (void**)&mx_gemm, (void**)&mx_gemm_bytes, (void**)&mx_linear, (void**)&mx_linear_bytes,
+                       (void**)&column_sum, (void**)&column_sum_bytes, (void**)&mx_attn, (void**)&mx_attn_bytes};
+  if (n != (Py_ssize_t)(sizeof(to) / sizeof(to[0]))) {
+    PyErr_Format(PyExc_TypeError, "init takes %d addresses, got %d", (int)(sizeof(to) / sizeof(to[0])), (int)n);
+    return nullptr;
+  }
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    void* const address = PyLong_AsVoidPtr(o[i]);
+    if (PyErr_Occurred()) return nullptr;
+    *to[i] = address;
+  }
   Py_RETURN_NONE;
 }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {{"init", init, METH_VARARGS, nullptr}, FAST(attention_fwd), FAST(attention_bwd), FAST(dropout),
-                         FAST(embedding_fwd), FAST(embedding_bwd), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {FAST(init), FAST(attention_fwd), FAST(attention_bwd), FAST(dropout),
+                         FAST(embedding_fwd), FAST(embedding_bwd), FAST(mxfp4_quantize),
+                         FAST(mxfp4_dequantize), FAST(mxfp4_linear), FAST(mxfp4_train_fwd), FAST(mxfp4_bwd),
+                         FAST(mxfp4_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "dpa_fast_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -12,8 +12,8 @@
 //   dense    a tensor [..., C], C a multiple of 32: its bytes in order, the first of two elements in the low
 //            half, and its scale bytes in order.
 //   operand  a matrix [rows][cols] as the product reads it, whose contraction runs over cols: rows of
-//            ceil(cols / 256) * 128 B, zeros behind cols; scales [ceil(cols / 512)][rows][16], block
-//            8 s + 2 q + t of a row's 16 at byte 4 q + 2 s + t. Lane (row, q) of a matrix instruction then
+//            ceil(cols / 256) * 128 B, zeros behind cols; behind them scales [ceil(cols / 512)][rows][16],
+//            block 8 s + 2 q + t of a row's 16 at byte 4 q + 2 s + t. Lane (row, q) of a matrix instruction then
 //            has the scales of its four 32-element pieces of 512 columns in one word, and takes pieces
 //            2 q, 2 q + 1 of each 256 (the order of a contraction is free as long as both operands keep it).
 #pragma once
@@ -22,14 +22,23 @@
 namespace dpa {
 namespace mx {
 
-typedef int v4i __attribute__((ext_vector_type(4)));
-
 constexpr int kBlock = 32;
 constexpr int kStep = 256;   // columns of an operand's padding and of a step of the product
 constexpr int kGroup = 512;  // columns of a group of scales
 
 __host__ __device__ inline int64_t pitch_of(int64_t cols) { return (cols + kStep - 1) / kStep * (kStep / 2); }
 __host__ __device__ inline int64_t groups_of(int64_t cols) { return (cols + kGroup - 1) / kGroup; }
+
+inline int64_t operand_data_bytes(int64_t rows, int64_t cols) { return rows * pitch_of(cols); }
+inline int64_t operand_bytes(int64_t rows, int64_t cols) {
+  return operand_data_bytes(rows, cols) + groups_of(cols) * rows * 16;
+}
+
+// Sizes of a matrix that the kernels take: 32-bit numbers of 8-element groups and workgroups, and of scales
+inline bool matrix_ok(int64_t rows, int64_t cols) {
+  if (rows < 0 || cols <= 0 || rows >= (1 << 26) || cols >= (1 << 26)) return false;
+  return rows * (pitch_of(cols) / 4) < (1ll << 31) && cols * (pitch_of(rows) / 4) < (1ll << 31);
+}
 
 // place of block b of a row within the 16 B of its group
 __host__ __device__ inline int scale_at(int b) { return 4 * ((b >> 1) & 3) + 2 * ((b >> 3) & 1) + (b & 1); }
@@ -39,52 +48,56 @@ template <bool SR>
 __device__ __forceinline__ uint32_t scale_byte(uint32_t m) {
   const int e = (int)(m >> 23);
   int k = e - 2;
-  if (SR && (m & 0x7fffffu) > 0x400000u) ++k;
-  if (e < 2) k = 0;
+  if (SR && (m & 0x7fffffu) > 0x400000u && e >= 2) ++k;
   return e == 255 ? 255u : (uint32_t)(k < 0 ? 0 : k);
 }
-// 2^-(byte - 127): a normal number for every byte of a finite block (at most 253)
-__device__ __forceinline__ float inverse_of(uint32_t byte) { return __uint_as_float((254u - min(byte, 253u)) << 23); }
-// 2^(byte - 127); NaN for 255
-__device__ __forceinline__ float scale_of(uint32_t byte) {
-  return __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7fc00000u : byte << 23);
+
+// The conversions v_cvt_scalef32_* take a scale by its exponent bits: every byte below 255 stands as
+// byte << 23, 0 for 2^-127 too, which the tests check over all bytes. A block of byte 255 gets codes of no
+// meaning.
+__device__ __forceinline__ float scale_bits(uint32_t byte) { return __uint_as_float(byte << 23); }
+// for the way back: NaN for 255
+__device__ __forceinline__ float scale_back(uint32_t byte) { return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23); }
+
+typedef __bf16 pk_bf16 __attribute__((ext_vector_type(2)));
+
+// Byte I of r: the codes of two numbers over the scale, to nearest even, beyond 6 to 6. w: a pair of a
+// 16-bit type.
+template <int DT, int I>
+__device__ __forceinline__ uint32_t encode_pair(uint32_t r, uint32_t w, float scale) {
+  if constexpr (DT == DPA_DTYPE_BF16)
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(pk_bf16, w), scale, I);
+  else
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, w), scale, I);
+}
+template <int I>
+__device__ __forceinline__ uint32_t encode_pair(uint32_t r, float a, float b, float scale) {
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, a, b, scale, I);
 }
 
-// Eight numbers, scaled already, to eight codes: to nearest even, beyond 6 to 6 (v_cvt_scalef32_pk_fp4_f32
-// at scale 1).
-__device__ __forceinline__ uint32_t encode8(const float (&v)[8]) {
-  uint32_t r = 0;
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], 1.0f, 0);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], 1.0f, 1);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], 1.0f, 2);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], 1.0f, 3);
-  return r;
+// The lowest 4 bits: the code of v over the scale, magnitude rounded up where its place between two codes, in
+// units of 2^-16 and rounded down, plus the 16 random bits reaches 2^16 (bits: those 16 in the upper half,
+// zeros below: the instruction adds them to what it cuts off). What lies above the 4 bits is of no meaning: the
+// instruction's second number, which would share the bits, and three bytes that it leaves.
+__device__ __forceinline__ uint32_t encode_sr(float v, uint32_t bits, float scale) {
+  return __builtin_amdgcn_cvt_scalef32_sr_pk_fp4_f32(0u, v2f{v, __builtin_nondeterministic_value(v)}, bits, scale, 0);
 }
-__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
-  uint32_t r = 0;
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, a, b, 1.0f, 0);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, c, d, 1.0f, 1);
-  return r;
-}
-
-// One number of magnitude up to 6 to its code, up where its place between two codes, in units of 2^-16 and
-// rounded down, plus the 16 random bits reaches 2^16. From 1 on the place is the 22 bits behind a code's
-// mantissa bit, below it the fraction of v / 0.5.
-__device__ __forceinline__ uint32_t encode_sr(float v, uint32_t bits16) {
-  const uint32_t u = __float_as_uint(v), a = u & 0x7fffffffu;
-  const uint32_t big = ((a + (bits16 << 6)) >> 22) - 252u;
-  const uint32_t small = ((uint32_t)(__uint_as_float(a) * 131072.0f) + bits16) >> 16;
-  return (a >= 0x3f800000u ? big : small) | ((u >> 28) & 8u);
+// a byte of two codes, the lower bits first
+__device__ __forceinline__ uint32_t two_codes(uint32_t a, uint32_t b) { return (a & 0xfu) | (b << 4); }
+// the lowest bytes of a, b, c and d
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b) { return perm_b32(b, a, 0x0c0c0400u); }
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return perm_b32(perm_b32(d, c, 0x0c0c0400u), perm_b32(b, a, 0x0c0c0400u), 0x05040100u);
 }
 
 // The random bits of elements 4 i .. 4 i + 3: splitmix64(seed + i * golden ratio), 16 bits each. Elements are
 // numbered in rows of whole blocks: row * (cols rounded up to 32) + col.
-__device__ __forceinline__ uint64_t bits_of(uint64_t seed, uint64_t i) {
-  uint64_t z = seed + i * kDropGolden;
+__device__ __forceinline__ uint64_t mix(uint64_t z) {
   z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
   z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
   return z ^ (z >> 31);
 }
+__device__ __forceinline__ uint64_t bits_of(uint64_t seed, uint64_t i) { return mix(seed + i * kDropGolden); }
 
 // D(16 x 16) += A(16 x 128) B(128 x 16) over blocks of 32: lane l supplies 32 elements of row (column of B)
 // l & 15 with byte SA (SB) of its scale word, and receives D[4 (l >> 4) + t][l & 15], t = 0 .. 3.

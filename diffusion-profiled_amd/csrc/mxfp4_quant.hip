@@ -18,41 +18,73 @@ struct RowArgs {
   FastDiv per_row;       // groups to a padded row
 };
 
+// Eight neighbours of a row as they lie in memory
 template <int DT>
-__device__ __forceinline__ void load8(float (&v)[8], const void* p, int64_t at) {
-  if constexpr (DT == DPA_DTYPE_F32) {
+struct Eight {
+  uint4 w;
+  __device__ __forceinline__ float get(int i) const {
+    const uint32_t u = i < 2 ? w.x : i < 4 ? w.y : i < 6 ? w.z : w.w;
+    return i & 1 ? Elem<DT>::hi(u) : Elem<DT>::lo(u);
+  }
+  __device__ __forceinline__ void load(const void* p, int64_t at) {
+    w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+  }
+  __device__ __forceinline__ void load_some(const void* p, int64_t at, int64_t left) {
+    const uint16_t* s = static_cast<const uint16_t*>(p) + at;
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = i < left ? s[i] : 0u;
+    w = uint4{u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16};
+  }
+  // bits of the largest magnitude, as fp32's
+  __device__ __forceinline__ uint32_t amax() const {
+    const us2 a = absmax8(us2{0, 0}, w);
+    const uint32_t m = a.x > a.y ? a.x : a.y;
+    return DT == DPA_DTYPE_BF16 ? m << 16 : __float_as_uint(Elem<DT>::lo(m));
+  }
+  __device__ __forceinline__ uint32_t codes(float scale) const {
+    uint32_t r = encode_pair<DT, 0>(0u, w.x, scale);
+    r = encode_pair<DT, 1>(r, w.y, scale);
+    r = encode_pair<DT, 2>(r, w.z, scale);
+    return encode_pair<DT, 3>(r, w.w, scale);
+  }
+};
+template <>
+struct Eight<DPA_DTYPE_F32> {
+  float v[8];
+  __device__ __forceinline__ float get(int i) const { return v[i]; }
+  __device__ __forceinline__ void load(const void* p, int64_t at) {
     const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
     const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4);
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = Elem<DT>::lo(w[i]), v[2 * i + 1] = Elem<DT>::hi(w[i]);
   }
-}
+  __device__ __forceinline__ void load_some(const void* p, int64_t at, int64_t left) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? static_cast<const float*>(p)[at + i] : 0.f;
+  }
+  __device__ __forceinline__ uint32_t amax() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m;
+  }
+  __device__ __forceinline__ uint32_t codes(float scale) const {
+    uint32_t r = encode_pair<0>(0u, v[0], v[1], scale);
+    r = encode_pair<1>(r, v[2], v[3], scale);
+    r = encode_pair<2>(r, v[4], v[5], scale);
+    return encode_pair<3>(r, v[6], v[7], scale);
+  }
+};
 
 __device__ __forceinline__ uint32_t quad_max(uint32_t m) {
   m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, false));  // lane ^ 1
   return max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4e, 0xf, 0xf, false));  // lane ^ 2
 }
 
-// 8 elements of a block, its largest magnitude m -> their codes; idx4: the number of the first, over 4
-template <bool SR>
-__device__ __forceinline__ uint32_t codes8(const float (&v)[8], uint32_t byte, uint64_t seed, uint64_t idx4) {
-  const float inv = inverse_of(byte);
-  float s[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[i] = v[i] * inv;
-  if constexpr (!SR) return encode8(s);
-  uint32_t r = 0;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const uint64_t z = bits_of(seed, idx4 + j);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r |= encode_sr(s[4 * j + i], (uint32_t)(z >> (16 * i)) & 0xffffu) << (4 * (4 * j + i));
-  }
-  return r;
+// The random bits of four elements as the conversion takes them
+__device__ __forceinline__ void bits4(uint32_t (&b)[4], uint64_t z) {
+  const uint32_t lo = (uint32_t)z, hi = (uint32_t)(z >> 32);
+  b[0] = lo << 16, b[1] = lo & 0xffff0000u, b[2] = hi << 16, b[3] = hi & 0xffff0000u;
 }
 
 // kOperand: an operand's rows, else dense. kWide: rows of whole aligned 8-element groups.
@@ -63,23 +95,29 @@ __global__ __launch_bounds__(256) void mxfp4_rows_kernel(const RowArgs p) {
   int64_t row = 0, in_row = g;
   if constexpr (kOperand) row = fdiv((uint32_t)g, p.per_row), in_row = g - row * p.per_row.d;
   const int64_t c0 = in_row * 8, at = row * p.ld + c0;
-  float v[8];
-  if constexpr (!kOperand) {
-    load8<DT>(v, p.x, at);
-  } else {
-    if (kWide && c0 + 8 <= p.cols) {
-      load8<DT>(v, p.x, at);
-    } else {
+  Eight<DT> v;
+  if (!kOperand || (kWide && c0 + 8 <= p.cols))
+    v.load(p.x, at);
+  else
+    v.load_some(p.x, at, p.cols - c0);
+  const uint32_t byte = scale_byte<SR>(quad_max(v.amax()));
+  const float scale = scale_bits(byte);
+  uint32_t r;
+  if constexpr (SR) {
+    const uint64_t i4 = (uint64_t)row * (uint64_t)((p.cols + kBlock - 1) / kBlock * (kBlock / 4)) + (uint64_t)in_row * 2;
+    uint32_t a[4], b[4];
+    bits4(a, bits_of(*p.seed, i4));
+    bits4(b, bits_of(*p.seed, i4 + 1));
+    uint32_t c[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = c0 + i < p.cols ? load1<DT>(p.x, at + i) : 0.f;
+    for (int i = 0; i < 2; ++i) {
+      c[i] = two_codes(encode_sr(v.get(2 * i), a[2 * i], scale), encode_sr(v.get(2 * i + 1), a[2 * i + 1], scale));
+      c[2 + i] = two_codes(encode_sr(v.get(4 + 2 * i), b[2 * i], scale), encode_sr(v.get(5 + 2 * i), b[2 * i + 1], scale));
     }
+    r = low_bytes(c[0], c[1], c[2], c[3]);
+  } else {
+    r = v.codes(scale);
   }
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  const uint32_t byte = scale_byte<SR>(quad_max(m));
-  const uint64_t pitch4 = kOperand ? (uint64_t)((p.cols + kBlock - 1) / kBlock) * (kBlock / 4) : 0;
-  const uint32_t r = codes8<SR>(v, byte, SR ? *p.seed : 0, row * pitch4 + (uint64_t)in_row * 2);
   reinterpret_cast<uint32_t*>(p.data)[g] = r;
   if ((threadIdx.x & 3) == 0) {
     if constexpr (kOperand) {
@@ -93,9 +131,11 @@ __global__ __launch_bounds__(256) void mxfp4_rows_kernel(const RowArgs p) {
 
 // ---------------------------------------------------------------------------------------
 // Both operands of a matrix from one read of it: its rows, and its columns (blocks down the columns, the
-// matrix transposed). A thread holds 4 columns of 32 rows in registers: a column's block is its own, a
-// row's block the 8 lanes beside it. W waves below each other; their codes of a column meet in LDS,
-// so that they leave in pieces of 16 W B.
+// matrix transposed). Eight waves take 64 rows of 256 columns at a time, `iters` times down the matrix, the next
+// 64 rows' loads out before these are worked on. A thread holds 4 columns of 8 rows: a row's block is the 8
+// lanes beside each other, a column's the 4 waves below each other, which trade their largest magnitudes
+// through LDS. The columns' codes gather in LDS and leave at the end, 32 iters B to a column (a whole
+// line of 128 B with 4).
 // ---------------------------------------------------------------------------------------
 struct BothArgs {
   const void* x;
@@ -105,13 +145,7 @@ struct BothArgs {
   int col_tiles;
 };
 
-template <int DT>
-struct Quad;  // 4 neighbours of a row
-template <>
-struct Quad<DPA_DTYPE_F32> {
-  float4 w;
-  __device__ __forceinline__ float get(int i) const { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
-};
+// Four neighbours of a row
 template <int DT>
 struct Quad {
   uint2 w;
@@ -119,6 +153,11 @@ struct Quad {
     const uint32_t u = i < 2 ? w.x : w.y;
     return i & 1 ? Elem<DT>::hi(u) : Elem<DT>::lo(u);
   }
+};
+template <>
+struct Quad<DPA_DTYPE_F32> {
+  float4 w;
+  __device__ __forceinline__ float get(int i) const { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
 };
 
 template <int DT>
@@ -139,97 +178,190 @@ __device__ __forceinline__ Quad<DT> quad_at(const void* x, int64_t at, int64_t l
   return q;
 }
 
-template <int DT, int W, bool kRows, bool SR>
-__global__ __launch_bounds__(64 * W) void mxfp4_both_kernel(const BothArgs p, bool wide) {
-  constexpr int kPitch = 16 * W + 16;  // (lanes then lie in 16 different places of the banks)
-  __shared__ __attribute__((aligned(16))) uint8_t lds[256 * kPitch];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t tr = blockIdx.x / (uint32_t)p.col_tiles, tc = blockIdx.x - tr * p.col_tiles;
-  const int64_t block = tr * W + wave, r0 = block * 32, c0 = tc * 256 + 4 * lane, left = p.cols - c0;
-  Quad<DT> x[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i)
-    x[i] = quad_at<DT>(p.x, (r0 + i) * p.ld + c0, r0 + i < p.rows ? left : 0, wide);
-  const uint64_t seed = SR ? *p.seed : 0;
-  const uint64_t pitch4 = (uint64_t)((p.cols + kBlock - 1) / kBlock) * (kBlock / 4);
-  auto bits = [&](int i) { return bits_of(seed, (uint64_t)(r0 + i) * pitch4 + (uint64_t)c0 / 4); };
-
-  if constexpr (kRows) {
-    const int64_t pitch = pitch_of(p.cols);
-    const int b = (int)(c0 >> 5);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      float v[4];
-      uint32_t m = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = x[i].get(j), m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-      m = quad_max(m);
-      m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, false));  // 7 - lane of 8
-      const uint32_t byte = scale_byte<SR>(m);
-      const float inv = inverse_of(byte);
-      uint32_t r;
-      if constexpr (SR) {
-        const uint64_t z = bits(i);
-        r = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r |= encode_sr(v[j] * inv, (uint32_t)(z >> (16 * j)) & 0xffffu) << (4 * j);
-      } else {
-        r = encode4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-      }
-      if (r0 + i < p.rows) {
-        *reinterpret_cast<uint16_t*>(p.row_data + (r0 + i) * pitch + c0 / 2) = (uint16_t)r;
-        if ((lane & 7) == 0)
-          p.row_scales[((int64_t)(b >> 4) * p.rows + r0 + i) * 16 + scale_at(b & 15)] = (uint8_t)byte;
-      }
-    }
+// Magnitudes of four columns: a word each in fp32, a half each (two columns to a word) of 16-bit types
+template <int DT>
+struct ColMax {
+  us2 a = {0, 0}, b = {0, 0};
+  __device__ __forceinline__ void take(const Quad<DT>& q) {
+    a = __builtin_elementwise_max(a, __builtin_bit_cast(us2, q.w.x & 0x7fff7fffu));
+    b = __builtin_elementwise_max(b, __builtin_bit_cast(us2, q.w.y & 0x7fff7fffu));
   }
-
+  static constexpr int kWords = 2;
+  __device__ __forceinline__ void put(uint32_t* lds) const {
+    *reinterpret_cast<uint2*>(lds) = uint2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+  }
+  __device__ __forceinline__ void join(const uint32_t* lds) {
+    const uint2 v = *reinterpret_cast<const uint2*>(lds);
+    a = __builtin_elementwise_max(a, __builtin_bit_cast(us2, v.x));
+    b = __builtin_elementwise_max(b, __builtin_bit_cast(us2, v.y));
+  }
+  __device__ __forceinline__ uint32_t get(int j) const {
+    const uint32_t m = j == 0 ? a.x : j == 1 ? a.y : j == 2 ? b.x : b.y;
+    return DT == DPA_DTYPE_BF16 ? m << 16 : __float_as_uint(Elem<DT>::lo(m));
+  }
+};
+template <>
+struct ColMax<DPA_DTYPE_F32> {
   uint32_t m[4] = {0, 0, 0, 0};
+  __device__ __forceinline__ void take(const Quad<DPA_DTYPE_F32>& q) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
+    for (int j = 0; j < 4; ++j) m[j] = max(m[j], __float_as_uint(q.get(j)) & 0x7fffffffu);
+  }
+  static constexpr int kWords = 4;
+  __device__ __forceinline__ void put(uint32_t* lds) const {
+    *reinterpret_cast<uint4*>(lds) = uint4{m[0], m[1], m[2], m[3]};
+  }
+  __device__ __forceinline__ void join(const uint32_t* lds) {
+    const uint4 v = *reinterpret_cast<const uint4*>(lds);
+    m[0] = max(m[0], v.x), m[1] = max(m[1], v.y), m[2] = max(m[2], v.z), m[3] = max(m[3], v.w);
+  }
+  __device__ __forceinline__ uint32_t get(int j) const { return m[j]; }
+};
+
+// largest magnitude of a row's four, as fp32's bits
+template <int DT>
+__device__ __forceinline__ uint32_t row_max(const Quad<DT>& q) {
+  if constexpr (DT == DPA_DTYPE_F32) {
+    return max(max(__float_as_uint(q.w.x) & 0x7fffffffu, __float_as_uint(q.w.y) & 0x7fffffffu),
+               max(__float_as_uint(q.w.z) & 0x7fffffffu, __float_as_uint(q.w.w) & 0x7fffffffu));
+  } else {
+    const us2 a = __builtin_elementwise_max(__builtin_bit_cast(us2, q.w.x & 0x7fff7fffu),
+                                            __builtin_bit_cast(us2, q.w.y & 0x7fff7fffu));
+    const uint32_t m = a.x > a.y ? a.x : a.y;
+    return DT == DPA_DTYPE_BF16 ? m << 16 : __float_as_uint(Elem<DT>::lo(m));
+  }
+}
+
+// Rows i and i + 1 of column j as a pair
+template <int DT>
+__device__ __forceinline__ uint32_t down_pair(const Quad<DT>& a, const Quad<DT>& b, int j) {
+  return perm_b32(j < 2 ? b.w.x : b.w.y, j < 2 ? a.w.x : a.w.y, j & 1 ? 0x07060302u : 0x05040100u);
+}
+
+template <int DT, int kIters, bool SR>
+__global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p, bool wide) {
+  constexpr int kLine = 32 * kIters;   // bytes of a column
+  constexpr int kPitch = kLine + 16;   // (lanes then lie in different places of the banks)
+  constexpr int kW = ColMax<DT>::kWords;
+  __shared__ __attribute__((aligned(16))) uint8_t out[256 * kPitch];
+  __shared__ __attribute__((aligned(16))) uint32_t tops[2][8][64 * kW];
+  __shared__ __attribute__((aligned(8))) uint8_t bytes[2 * kIters][256];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = wave >> 2, sub = wave & 3;
+  const int64_t tr = blockIdx.x / (uint32_t)p.col_tiles, tc = blockIdx.x - tr * p.col_tiles;
+  const int64_t c0 = tc * 256 + 4 * lane, left = p.cols - c0;
+  const int64_t first = tr * 64 * kIters + 8 * wave;  // of this wave's rows in the first iteration
+  const int64_t pitch = pitch_of(p.cols);
+  Quad<DT> x[8], next[8];
+  auto load = [&](Quad<DT>(&q)[8], int it) __attribute__((always_inline)) {
+    const int64_t r0 = first + 64 * it;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m[j] = max(m[j], __float_as_uint(x[i].get(j)) & 0x7fffffffu);
-  uint32_t byte[4];
-  float inv[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    byte[j] = scale_byte<SR>(m[j]), inv[j] = inverse_of(byte[j]);
-    if (j < left)
-      p.col_scales[((block >> 4) * p.cols + c0 + j) * 16 + scale_at((int)(block & 15))] = (uint8_t)byte[j];
+    for (int i = 0; i < 8; ++i)
+      q[i] = quad_at<DT>(p.x, (r0 + i) * p.ld + c0, r0 + i < p.rows ? left : 0, wide);
+  };
+  load(x, 0);
+  uint64_t z = 0, z_row = 0;
+  if constexpr (SR) {
+    z_row = (uint64_t)((p.cols + kBlock - 1) / kBlock) * (kBlock / 4) * kDropGolden;
+    z = *p.seed + (uint64_t)first * z_row + (uint64_t)(c0 / 4) * kDropGolden;
   }
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {  // 8 rows: a word of each column
-    uint32_t r[4] = {0, 0, 0, 0};
+  for (int it = 0; it < kIters; ++it) {
+    const int64_t r0 = first + 64 * it;
+    if (it + 1 < kIters) load(next, it + 1);
+    ColMax<DT> top;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top.take(x[i]);
+    top.put(&tops[it & 1][wave][lane * kW]);
+    uint32_t rnd[SR ? 8 : 1][4];
     if constexpr (SR) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint64_t z = bits(8 * q + i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          r[j] |= encode_sr(x[8 * q + i].get(j) * inv[j], (uint32_t)(z >> (16 * j)) & 0xffffu) << (4 * i);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = x[8 * q + i].get(j) * inv[j];
-        r[j] = encode8(v);
-      }
+      for (int i = 0; i < 8; ++i) bits4(rnd[i], mix(z + (uint64_t)i * z_row));
+      z += 64 * z_row;
     }
+    // rows
+    if (p.row_data) {
+      uint32_t mine = 0;  // lane 8 b + i: the scale of row i, block b
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<uint32_t*>(lds + (j * 64 + lane) * kPitch + wave * 16 + 4 * q) = r[j];
+      for (int i = 0; i < 8; ++i) {
+        uint32_t m = quad_max(row_max<DT>(x[i]));
+        m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, false));  // 7 - lane of 8
+        const uint32_t byte = scale_byte<SR>(m);
+        const float scale = scale_bits(byte);
+        mine = (lane & 7) == i ? byte : mine;
+        uint32_t r;
+        if constexpr (SR) {
+          r = low_bytes(two_codes(encode_sr(x[i].get(0), rnd[i][0], scale), encode_sr(x[i].get(1), rnd[i][1], scale)),
+                        two_codes(encode_sr(x[i].get(2), rnd[i][2], scale), encode_sr(x[i].get(3), rnd[i][3], scale)));
+        } else if constexpr (DT == DPA_DTYPE_F32) {
+          r = encode_pair<1>(encode_pair<0>(0u, x[i].w.x, x[i].w.y, scale), x[i].w.z, x[i].w.w, scale);
+        } else {
+          r = encode_pair<DT, 1>(encode_pair<DT, 0>(0u, x[i].w.x, scale), x[i].w.y, scale);
+        }
+        if (r0 + i < p.rows) *reinterpret_cast<uint16_t*>(p.row_data + (r0 + i) * pitch + c0 / 2) = (uint16_t)r;
+      }
+      const int64_t row = r0 + (lane & 7);
+      const int b = (int)(tc * 8) + (lane >> 3);
+      if (row < p.rows) p.row_scales[((int64_t)(b >> 4) * p.rows + row) * 16 + scale_at(b & 15)] = (uint8_t)mine;
+    }
+    wait_lgkmcnt0();
+    lds_barrier();
+    // columns: word `sub` of block 2 it + half
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top.join(&tops[it & 1][4 * half + w][lane * kW]);
+    uint32_t r[4], some = 0;
+    float scale[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t byte = scale_byte<SR>(top.get(j));
+      some |= byte << (8 * j);
+      scale[j] = scale_bits(byte);
+    }
+    if (sub == 0) *reinterpret_cast<uint32_t*>(&bytes[2 * it + half][4 * lane]) = some;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (SR) {
+        uint32_t c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          c[i] = two_codes(encode_sr(x[2 * i].get(j), rnd[2 * i][j], scale[j]),
+                           encode_sr(x[2 * i + 1].get(j), rnd[2 * i + 1][j], scale[j]));
+        r[j] = low_bytes(c[0], c[1], c[2], c[3]);
+      } else if constexpr (DT == DPA_DTYPE_F32) {
+        r[j] = encode_pair<0>(0u, x[0].get(j), x[1].get(j), scale[j]);
+        r[j] = encode_pair<1>(r[j], x[2].get(j), x[3].get(j), scale[j]);
+        r[j] = encode_pair<2>(r[j], x[4].get(j), x[5].get(j), scale[j]);
+        r[j] = encode_pair<3>(r[j], x[6].get(j), x[7].get(j), scale[j]);
+      } else {
+        r[j] = encode_pair<DT, 0>(0u, down_pair<DT>(x[0], x[1], j), scale[j]);
+        r[j] = encode_pair<DT, 1>(r[j], down_pair<DT>(x[2], x[3], j), scale[j]);
+        r[j] = encode_pair<DT, 2>(r[j], down_pair<DT>(x[4], x[5], j), scale[j]);
+        r[j] = encode_pair<DT, 3>(r[j], down_pair<DT>(x[6], x[7], j), scale[j]);
+      }
+      *reinterpret_cast<uint32_t*>(out + (j * 64 + lane) * kPitch + (2 * it + half) * 16 + 4 * sub) = r[j];
+    }
+    if (it + 1 < kIters)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = next[i];
   }
   __syncthreads();
-  const int64_t pitch = pitch_of(p.rows);
+  const int64_t col_pitch = pitch_of(p.rows);
 #pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    const int id = it * 64 * W + threadIdx.x, line = id / W, chunk = id % W;
+  for (int it = 0; it < kIters; ++it) {
+    const int id = it * 512 + threadIdx.x, line = id / (2 * kIters), chunk = id % (2 * kIters);
     const int64_t col = tc * 256 + 4 * (line & 63) + (line >> 6);
     if (col < p.cols)
-      *reinterpret_cast<uint4*>(p.col_data + col * pitch + tr * (16 * W) + chunk * 16) =
-          *reinterpret_cast<const uint4*>(lds + line * kPitch + chunk * 16);
+      *reinterpret_cast<uint4*>(p.col_data + col * col_pitch + tr * kLine + chunk * 16) =
+          *reinterpret_cast<const uint4*>(out + line * kPitch + chunk * 16);
+  }
+  // pairs of blocks 2 q, 2 q + 1 lie together in a group of scales
+#pragma unroll
+  for (int it = 0; it < (kIters + 1) / 2; ++it) {
+    const int id = it * 512 + threadIdx.x, pair = id >> 8;
+    const int64_t col = tc * 256 + (id & 255), block = tr * 2 * kIters + 2 * pair;
+    if (pair < kIters && col < p.cols)
+      *reinterpret_cast<uint16_t*>(p.col_scales + ((block >> 4) * p.cols + col) * 16 + scale_at((int)(block & 15))) =
+          (uint16_t)(bytes[2 * pair][id & 255] | bytes[2 * pair + 1][id & 255] << 8);
   }
 }
 
@@ -242,46 +374,40 @@ __global__ __launch_bounds__(256) void mxfp4_values_kernel(const uint32_t* data,
   const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (g >= groups) return;
   const uint32_t w = data[g];
-  const float s = scale_of(scales[g >> 2]);
-  const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1),
-            c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+  const float s = scale_back(scales[g >> 2]);
+  const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1),
+            c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
   if constexpr (DT == DPA_DTYPE_F32) {
     float4* o = reinterpret_cast<float4*>(y) + 2 * g;
-    o[0] = float4{a.x * s, a.y * s, b.x * s, b.y * s};
-    o[1] = float4{c.x * s, c.y * s, d.x * s, d.y * s};
+    o[0] = float4{a.x, a.y, b.x, b.y};
+    o[1] = float4{c.x, c.y, d.x, d.y};
   } else {
-    reinterpret_cast<uint4*>(y)[g] = uint4{Elem<DT>::pack(a.x * s, a.y * s), Elem<DT>::pack(b.x * s, b.y * s),
-                                           Elem<DT>::pack(c.x * s, c.y * s), Elem<DT>::pack(d.x * s, d.y * s)};
+    reinterpret_cast<uint4*>(y)[g] =
+        uint4{Elem<DT>::pack(a.x, a.y), Elem<DT>::pack(b.x, b.y), Elem<DT>::pack(c.x, c.y), Elem<DT>::pack(d.x, d.y)};
   }
 }
 
 // ---------------------------------------------------------------------------------------
-// Column sums in fp32, in a fixed order: a workgroup's 256 columns of kSumRows rows, then the pieces
+// Column sums in fp32, in a fixed order: a workgroup takes 64 columns of `span` rows, its four waves every fourth
+// row; then the pieces
 // ---------------------------------------------------------------------------------------
-constexpr int kSumRows = 128;
-
 template <int DT>
-__global__ __launch_bounds__(256) void column_sum_kernel(const void* x, float* part, int64_t rows, int64_t cols, int64_t ld) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
-  const int64_t r0 = (int64_t)blockIdx.y * kSumRows, r1 = min(rows, r0 + kSumRows);
+__global__ __launch_bounds__(256) void column_sum_kernel(const void* x, float* part, int64_t rows, int64_t cols,
+                                                         int64_t ld, int span) {
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  const int64_t r0 = (int64_t)blockIdx.y * span, r1 = min(rows, r0 + span);
   float s[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t r = r0; r < r1; r += 4)
+  if (c < cols)
+    for (int64_t r = r0 + wave; r < r1; r += 16)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (r + i < r1) s[i] += load1<DT>(x, (r + i) * ld + c);
-  part[blockIdx.y * cols + c] = (s[0] + s[1]) + (s[2] + s[3]);
-}
-
-__global__ __launch_bounds__(256) void column_join_kernel(const float* part, float* y, int64_t pieces, int64_t cols) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t r = 0; r < pieces; r += 4)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (r + i < pieces) s[i] += part[(r + i) * cols + c];
-  y[c] = (s[0] + s[1]) + (s[2] + s[3]);
+      for (int i = 0; i < 4; ++i)
+        if (r + 4 * i < r1) s[i] += load1<DT>(x, (r + 4 * i) * ld + c);
+  sums[wave][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (wave == 0 && c < cols)
+    part[blockIdx.y * cols + c] = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
 }
 
 template <int DT, bool SR>
@@ -296,36 +422,36 @@ static int run_rows(const RowArgs& p, bool operand, bool wide, hipStream_t s) {
   return launch_status();
 }
 
-template <int DT, int W>
+template <int DT, int kIters>
 static int run_both(const BothArgs& p, bool wide, hipStream_t s) {
-  const int64_t row_tiles = ceil_div(p.rows, 256) * (8 / W);
-  const unsigned grid = (unsigned)(row_tiles * p.col_tiles);
-  if (p.row_data && p.seed)
-    mxfp4_both_kernel<DT, W, true, true><<<grid, 64 * W, 0, s>>>(p, wide);
-  else if (p.row_data)
-    mxfp4_both_kernel<DT, W, true, false><<<grid, 64 * W, 0, s>>>(p, wide);
-  else if (p.seed)
-    mxfp4_both_kernel<DT, W, false, true><<<grid, 64 * W, 0, s>>>(p, wide);
+  const unsigned grid = (unsigned)(ceil_div(p.rows, 256) * (4 / kIters) * p.col_tiles);
+  if (p.seed)
+    mxfp4_both_kernel<DT, kIters, true><<<grid, 512, 0, s>>>(p, wide);
   else
-    mxfp4_both_kernel<DT, W, false, false><<<grid, 64 * W, 0, s>>>(p, wide);
+    mxfp4_both_kernel<DT, kIters, false><<<grid, 512, 0, s>>>(p, wide);
   return launch_status();
 }
 
 template <int DT>
 static int run_operands(const RowArgs& r, const BothArgs& b, bool wide, hipStream_t s) {
   if (!b.col_data) return r.seed ? run_rows<DT, true>(r, true, wide, s) : run_rows<DT, false>(r, true, wide, s);
-  // Waves below each other: fewer where the workgroups would leave CUs idle
+  // rows to a workgroup: whole lines of the columns where there are enough workgroups
   const int64_t tiles = ceil_div(b.rows, 256) * b.col_tiles;
-  if (tiles >= 2 * num_cus()) return run_both<DT, 8>(b, wide, s);
-  return run_both<DT, 2>(b, wide, s);
+  if (tiles >= 2 * num_cus()) return run_both<DT, 4>(b, wide, s);
+  return run_both<DT, 1>(b, wide, s);
 }
 
-// Sizes of a matrix that the kernels take: 32-bit numbers of 8-element groups and workgroups
-static int check_matrix(int64_t rows, int64_t cols) {
-  if (rows < 0 || cols <= 0) return DPA_ERR_SIZE;
-  if (rows >= (1ll << 30) || cols >= (1ll << 30)) return DPA_ERR_SIZE;
-  if (rows * (pitch_of(cols) / 4) >= (1ll << 31) || cols * (pitch_of(rows) / 4) >= (1ll << 31)) return DPA_ERR_SIZE;
-  return DPA_OK;
+// rows of x to a workgroup of column_sum_kernel
+static int sum_span(int64_t rows, int64_t cols) {
+  int64_t pieces = 4 * num_cus() / ceil_div(cols, 64);
+  if (pieces > rows / 32) pieces = rows / 32;
+  if (pieces < 1) pieces = 1;
+  return (int)ceil_div(rows, pieces);
+}
+
+template <int DT>
+static void run_sum(const void* x, float* part, int64_t rows, int64_t cols, int64_t ld, int span, hipStream_t s) {
+  column_sum_kernel<DT><<<dim3((unsigned)ceil_div(cols, 64), (unsigned)ceil_div(rows, span)), 256, 0, s>>>(x, part, rows, cols, ld, span);
 }
 
 }  // namespace mx
@@ -367,39 +493,30 @@ extern "C" int dpa_mxfp4_dequantize(const void* data, const void* scales, void* 
   return launch_status();
 }
 
-extern "C" int64_t dpa_mxfp4_operand_data_bytes(int64_t rows, int64_t cols) {
-  return check_matrix(rows, cols) == DPA_OK ? rows * pitch_of(cols) : 0;
-}
-
-extern "C" int64_t dpa_mxfp4_operand_scale_bytes(int64_t rows, int64_t cols) {
-  return check_matrix(rows, cols) == DPA_OK ? groups_of(cols) * rows * 16 : 0;
+extern "C" int64_t dpa_mxfp4_operand_bytes(int64_t rows, int64_t cols) {
+  return matrix_ok(rows, cols) ? operand_bytes(rows, cols) : 0;
 }
 
 extern "C" int dpa_mxfp4_operands(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride,
-                                  void* row_data, void* row_scales, void* col_data, void* col_scales,
-                                  const void* seed, void* stream) {
+                                  void* by_rows, void* by_cols, const void* seed, void* stream) {
   if (!dtype_ok(dtype)) return DPA_ERR_SHAPE;
-  const int st = check_matrix(rows, cols);
-  if (st != DPA_OK) return st;
-  if (row_stride < cols && rows > 1) return DPA_ERR_SIZE;
-  if ((!row_data) != (!row_scales) || (!col_data) != (!col_scales) || (!row_data && !col_data)) return DPA_ERR_NULL;
+  if (!matrix_ok(rows, cols) || (row_stride < cols && rows > 1)) return DPA_ERR_SIZE;
+  if (!by_rows && !by_cols) return DPA_ERR_NULL;
   if (rows == 0) return DPA_OK;
   if (!x) return DPA_ERR_NULL;
-  if (!aligned(x, size_of(dtype)) || !aligned(row_data, 16) || !aligned(row_scales, 16) || !aligned(col_data, 16) ||
-      !aligned(col_scales, 16) || !aligned(seed, 8))
-    return DPA_ERR_ALIGN;
+  if (!aligned(x, size_of(dtype)) || !aligned(by_rows, 16) || !aligned(by_cols, 16) || !aligned(seed, 8)) return DPA_ERR_ALIGN;
   RowArgs r{};
-  r.x = x, r.data = (uint8_t*)row_data, r.scales = (uint8_t*)row_scales, r.seed = (const uint64_t*)seed;
+  r.x = x, r.data = (uint8_t*)by_rows, r.scales = r.data + operand_data_bytes(rows, cols), r.seed = (const uint64_t*)seed;
   r.rows = rows, r.cols = cols, r.ld = row_stride;
   r.groups = rows * (pitch_of(cols) / 4);
   r.per_row = make_fastdiv((uint32_t)(pitch_of(cols) / 4));
   BothArgs b{};
   b.x = x, b.row_data = r.data, b.row_scales = r.scales, b.seed = r.seed;
-  b.col_data = (uint8_t*)col_data, b.col_scales = (uint8_t*)col_scales;
+  b.col_data = (uint8_t*)by_cols, b.col_scales = b.col_data + operand_data_bytes(cols, rows);
   b.rows = rows, b.cols = cols, b.ld = row_stride;
   b.col_tiles = (int)ceil_div(cols, 256);
   // whole aligned vectors: 16 B of 8 elements (8 B of 4) of a 16-bit type, 16 B of 4 of fp32
-  const int vec = col_data || dtype == DPA_DTYPE_F32 ? 4 : 8;
+  const int vec = by_cols || dtype == DPA_DTYPE_F32 ? 4 : 8;
   const bool wide = row_stride % vec == 0 && aligned(x, vec * size_of(dtype));
   hipStream_t s = (hipStream_t)stream;
   if (dtype == DPA_DTYPE_BF16) return run_operands<DPA_DTYPE_BF16>(r, b, wide, s);
@@ -408,28 +525,28 @@ extern "C" int dpa_mxfp4_operands(const void* x, int dtype, int64_t rows, int64_
 }
 
 extern "C" int64_t dpa_column_sum_workspace_bytes(int64_t rows, int64_t cols) {
-  return rows > 0 && cols > 0 ? ceil_div(rows, kSumRows) * cols * 4 : 0;
+  return rows > 0 && cols > 0 ? ceil_div(rows, sum_span(rows, cols)) * cols * 4 : 0;
 }
 
 extern "C" int dpa_column_sum(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, void* y,
                               void* workspace, int64_t workspace_bytes, void* stream) {
   if (!dtype_ok(dtype)) return DPA_ERR_SHAPE;
-  if (rows <= 0 || cols <= 0 || cols >= (1ll << 30) || ceil_div(rows, kSumRows) > 65535 || (row_stride < cols && rows > 1))
-    return DPA_ERR_SIZE;
+  if (rows <= 0 || cols <= 0 || rows >= (1 << 30) || cols >= (1 << 30) || (row_stride < cols && rows > 1)) return DPA_ERR_SIZE;
   if (!x || !y) return DPA_ERR_NULL;
   if (!workspace || workspace_bytes < dpa_column_sum_workspace_bytes(rows, cols)) return DPA_ERR_WORKSPACE;
   if (!aligned(x, size_of(dtype)) || !aligned(y, 4) || !aligned(workspace, 4)) return DPA_ERR_ALIGN;
   hipStream_t s = (hipStream_t)stream;
-  const unsigned cb = (unsigned)ceil_div(cols, 256), rb = (unsigned)ceil_div(rows, kSumRows);
-  float* part = (float*)workspace;
+  const int span = sum_span(rows, cols);
+  const int64_t pieces = ceil_div(rows, span);
+  float* part = pieces > 1 ? (float*)workspace : (float*)y;
   if (dtype == DPA_DTYPE_BF16)
-    column_sum_kernel<DPA_DTYPE_BF16><<<dim3(cb, rb), 256, 0, s>>>(x, part, rows, cols, row_stride);
+    run_sum<DPA_DTYPE_BF16>(x, part, rows, cols, row_stride, span, s);
   else if (dtype == DPA_DTYPE_F16)
-    column_sum_kernel<DPA_DTYPE_F16><<<dim3(cb, rb), 256, 0, s>>>(x, part, rows, cols, row_stride);
+    run_sum<DPA_DTYPE_F16>(x, part, rows, cols, row_stride, span, s);
   else
-    column_sum_kernel<DPA_DTYPE_F32><<<dim3(cb, rb), 256, 0, s>>>(x, part, rows, cols, row_stride);
+    run_sum<DPA_DTYPE_F32>(x, part, rows, cols, row_stride, span, s);
   const int st = launch_status();
-  if (st != DPA_OK) return st;
-  column_join_kernel<<<cb, 256, 0, s>>>(part, (float*)y, rb, cols);
+  if (st != DPA_OK || pieces <= 1) return st;
+  run_sum<DPA_DTYPE_F32>(part, (float*)y, pieces, cols, cols, (int)pieces, s);
   return launch_status();
 }

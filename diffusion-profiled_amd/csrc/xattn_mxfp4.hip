@@ -45,7 +45,7 @@ __device__ __forceinline__ RawBlock raw_block(const uint8_t* data, const uint8_t
 // A block's 32 values as granules 4 blk .. 4 blk + 3 of row `row` of the array at `at`
 template <class T, int DP>
 __device__ __forceinline__ void put_block(uint32_t at, int row, int blk, const RawBlock& raw) {
-  const float s = mx::scale_of(raw.byte);
+  const float s = mx::scale_back(raw.byte);
   const uint32_t w[4] = {raw.w.x, raw.w.y, raw.w.z, raw.w.w};
 #pragma unroll
   for (int g = 0; g < 4; ++g)
@@ -329,7 +329,7 @@ __global__ __launch_bounds__(256, 2) void xattn_mxfp4_few_kernel(const MxArgs p)
     u32x4 kf[KS];
 #pragma unroll
     for (int k = 0; k < KS; ++k)
-      kf[k] = __builtin_bit_cast(u32x4, eight_of<T>(kw[k], mx::scale_of(ksc[NB > 1 ? k / 4 : 0])));
+      kf[k] = __builtin_bit_cast(u32x4, eight_of<T>(kw[k], mx::scale_back(ksc[NB > 1 ? k / 4 : 0])));
     asm volatile("" ::: "memory");  // (behind the reads of the tile before)
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {

@@ -24,7 +24,7 @@ import torch.nn as nn
 from torch.amp.autocast_mode import custom_bwd, custom_fwd
 
 from . import _lib
-from .conditioning import (_DT, _between_graphs, _check_masks, _check_seed, _on_one_gpu, _ptr, _rows,
+from .conditioning import (_DT, _between_graphs, _check_masks, _check_seed, _fast, _on_one_gpu, _ptr, _rows,
                            _scale_of, _strides, _workspace)
 from .eager import apply
 from .gn_silu import DROPOUT_SEEDS
@@ -48,7 +48,6 @@ class MXFP4Operand(NamedTuple):
     """A matrix [rows, cols] for a product that sums over its cols: any sizes, blocks along the rows, laid
     out by ``mxfp4_operand`` (include/dpa_fp8.h has the sizes; the order is the kernels')."""
     data: torch.Tensor
-    scales: torch.Tensor
     rows: int
     cols: int
 
@@ -64,6 +63,9 @@ def quantize_mxfp4(x: torch.Tensor) -> MXFP4:
     """x [..., C] (bf16, fp16 or fp32; C a multiple of 32) in MXFP4, blocks along the last dimension."""
     if torch.compiler.is_dynamo_compiling():
         return _between_graphs(quantize_mxfp4, x)
+    done = _fast().mxfp4_quantize(x)
+    if done is not None:
+        return MXFP4(*done)
     _check_dtype("quantize_mxfp4", x.dtype)
     if x.ndim < 1 or x.shape[-1] == 0 or x.shape[-1] % BLOCK:
         raise ValueError(f"quantize_mxfp4: the last dimension is a multiple of {BLOCK}, got {tuple(x.shape)}")
@@ -92,6 +94,9 @@ def dequantize_mxfp4(q: MXFP4, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
     """The values of q in dtype: exact in bf16 and fp32, rounded once in fp16."""
     if torch.compiler.is_dynamo_compiling():
         return _between_graphs(dequantize_mxfp4, q, dtype)
+    y = _fast().mxfp4_dequantize(q.data, q.scales, dtype)
+    if y is not None:
+        return y
     _check_dtype("dequantize_mxfp4", dtype)
     _check_mxfp4(q, "dequantize_mxfp4")
     data, scales = q.data.contiguous(), q.scales.contiguous()
@@ -105,12 +110,10 @@ def dequantize_mxfp4(q: MXFP4, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
 
 # ---- operands ----------------------------------------------------------------------------
 def _new_operand(rows: int, cols: int, device) -> MXFP4Operand:
-    nd = _lib.query("dpa_mxfp4_operand_data_bytes", rows, cols)
-    ns = _lib.query("dpa_mxfp4_operand_scale_bytes", rows, cols)
-    if nd == 0 and rows and cols:
+    nbytes = _lib.query("dpa_mxfp4_operand_bytes", rows, cols)
+    if nbytes == 0 and rows and cols:
         raise ValueError(f"mxfp4 operand: {rows} x {cols} is beyond what the kernels take")
-    return MXFP4Operand(torch.empty(nd, device=device, dtype=torch.uint8),
-                        torch.empty(ns, device=device, dtype=torch.uint8), rows, cols)
+    return MXFP4Operand(torch.empty(nbytes, device=device, dtype=torch.uint8), rows, cols)
 
 
 def _matrix(x: torch.Tensor) -> torch.Tensor:
@@ -132,8 +135,7 @@ def _operands(x: torch.Tensor, rows: bool, cols: bool, seed: torch.Tensor | None
     c = _new_operand(k, m, x.device) if cols else None
     if m:
         _lib.call("dpa_mxfp4_operands", x.data_ptr(), _DT[x.dtype], m, k, x.stride(0) if m > 1 else k,
-                  _ptr(r and r.data), _ptr(r and r.scales), _ptr(c and c.data), _ptr(c and c.scales),
-                  _ptr(seed), _lib.current_stream(x))
+                  _ptr(r and r.data), _ptr(c and c.data), _ptr(seed), _lib.current_stream(x))
     return r, c
 
 
@@ -159,19 +161,17 @@ def _product(a: MXFP4Operand, b: MXFP4Operand, bias: torch.Tensor | None, dtype:
     if m and n:
         nbytes = _lib.query("dpa_mxfp4_gemm_workspace_bytes", m, n, k)
         ws = _workspace(nbytes, a.data.device)
-        _lib.call("dpa_mxfp4_gemm", a.data.data_ptr(), a.scales.data_ptr(), b.data.data_ptr(), b.scales.data_ptr(),
-                  _ptr(bias), y.data_ptr(), _DT[dtype], m, n, k, _ptr(ws), nbytes, _lib.current_stream(a.data))
+        _lib.call("dpa_mxfp4_gemm", a.data.data_ptr(), b.data.data_ptr(), _ptr(bias), y.data_ptr(), _DT[dtype], m, n, k,
+                  _ptr(ws), nbytes, _lib.current_stream(a.data))
     return y
 
 
 # ---- the linear layer --------------------------------------------------------------------
 def _check_operand(w: MXFP4Operand) -> None:
-    nd = _lib.query("dpa_mxfp4_operand_data_bytes", w.rows, w.cols)
-    ns = _lib.query("dpa_mxfp4_operand_scale_bytes", w.rows, w.cols)
-    for t, n in ((w.data, nd), (w.scales, ns)):
-        if t.dtype != torch.uint8 or t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"linear_mxfp4: not an operand of {w.rows} x {w.cols}: {t.dtype} {tuple(t.shape)}")
-    _on_one_gpu(w.data, w.scales)
+    if (w.data.dtype != torch.uint8 or not w.data.is_contiguous() or w.data.data_ptr() % 16
+            or w.data.numel() != _lib.query("dpa_mxfp4_operand_bytes", w.rows, w.cols)):
+        raise ValueError(f"linear_mxfp4: not an operand of {w.rows} x {w.cols}: {w.data.dtype} {tuple(w.data.shape)}")
+    _on_one_gpu(w.data)
 
 
 def _check_linear(x: torch.Tensor, n: int, k: int, bias: torch.Tensor | None, out_dtype: torch.dtype | None):
@@ -197,6 +197,9 @@ def linear_mxfp4_fwd(x: torch.Tensor, weight: torch.Tensor | MXFP4Operand, bias:
     if torch.compiler.is_dynamo_compiling():
         return _between_graphs(linear_mxfp4_fwd, x, weight, bias, out_dtype=out_dtype)
     if isinstance(weight, MXFP4Operand):
+        y = _fast().mxfp4_linear(x, weight.data, weight.rows, weight.cols, bias, out_dtype)
+        if y is not None:
+            return y
         _check_operand(weight)
         _on_one_gpu(x, weight.data)
         n, k = weight.rows, weight.cols
@@ -207,7 +210,15 @@ def linear_mxfp4_fwd(x: torch.Tensor, weight: torch.Tensor | MXFP4Operand, bias:
         n, k = weight.shape
     x2, b32, dtype = _check_linear(x, n, k, bias, out_dtype)
     w = weight if isinstance(weight, MXFP4Operand) else _operands(weight, True, False, None)[0]
-    y = _product(_operands(x2, True, False, None)[0], w, b32, dtype)
+    x2 = _matrix(x2)
+    m = x2.shape[0]
+    y = torch.empty((m, n), device=x.device, dtype=dtype)
+    if m and n:
+        _new_operand(m, k, "meta")      # (refuses sizes beyond the kernels')
+        nbytes = _lib.query("dpa_mxfp4_linear_workspace_bytes", m, n, k)
+        ws = _workspace(nbytes, x.device)
+        _lib.call("dpa_mxfp4_linear", x2.data_ptr(), _DT[x2.dtype], x2.stride(0) if m > 1 else k, w.data.data_ptr(),
+                  _ptr(b32), y.data_ptr(), _DT[dtype], m, n, k, _ptr(ws), nbytes, _lib.current_stream(x2))
     return y.view(*x.shape[:-1], n)
 
 
@@ -241,6 +252,11 @@ def linear_mxfp4_train_fwd(x: torch.Tensor, weight: torch.Tensor, bias: torch.Te
     the weight)."""
     if torch.compiler.is_dynamo_compiling():
         return _between_graphs(linear_mxfp4_train_fwd, x, weight, bias, out_dtype=out_dtype)
+    done = _fast().mxfp4_train_fwd(x, weight, bias, out_dtype)
+    if done is not None:
+        (y, xc, wc), (n, k) = done, weight.shape
+        return y, LinearKept(MXFP4Operand(xc, k, x.numel() // k), MXFP4Operand(wc, k, n), x.shape, n, x.dtype,
+                             weight.dtype, bias is not None)
     return _train_fwd(x, weight, bias, out_dtype, True, True)
 
 
@@ -263,6 +279,10 @@ def linear_mxfp4_bwd(dy: torch.Tensor, kept: LinearKept, *, seed: torch.Tensor |
     if torch.compiler.is_dynamo_compiling():
         return _between_graphs(linear_mxfp4_bwd, dy, kept, seed=seed)
     n, k = kept.out_features, kept.shape[-1]
+    if kept.x is not None and kept.weight is not None and dy.shape[:-1] == kept.shape[:-1]:
+        done = _fast().mxfp4_bwd(dy, kept.x.data, kept.weight.data, n, k, kept.dtype, kept.weight_dtype, kept.bias, seed)
+        if done is not None:
+            return done
     _check_dtype("linear_mxfp4", dy.dtype)
     if dy.shape != (*kept.shape[:-1], n):
         raise ValueError(f"linear_mxfp4: dy {tuple(dy.shape)} is not the output's {(*kept.shape[:-1], n)}")
@@ -292,11 +312,10 @@ class LinearMXFP4Function(torch.autograd.Function):
     def forward(ctx: Any, x, weight, bias, out_dtype, seed):
         want_dx, want_dw = getattr(ctx, "needs_input_grad", (False, False))[:2]
         y, kept = _train_fwd(x, weight, bias, out_dtype, want_dx, want_dw)
-        tensors = [t for o in (kept.x, kept.weight) if o is not None for t in (o.data, o.scales)]
-        ctx.save_for_backward(seed, *tensors)
-        # (the operands' tensors are kept by autograd, their sizes here)
-        ctx.kept = kept._replace(x=kept.x and (kept.x.rows, kept.x.cols),
-                                 weight=kept.weight and (kept.weight.rows, kept.weight.cols))
+        ctx.save_for_backward(seed, kept.x and kept.x.data, kept.weight and kept.weight.data)
+        # (the operands' tensors are kept by autograd, the rest here)
+        ctx.kept = kept._replace(x=kept.x and kept.x._replace(data=None),
+                                 weight=kept.weight and kept.weight._replace(data=None))
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
@@ -304,13 +323,10 @@ class LinearMXFP4Function(torch.autograd.Function):
     @custom_bwd(device_type="cuda")
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, dy):
-        seed, *tensors = ctx.saved_tensors
+        seed, x, weight = ctx.saved_tensors
         kept = ctx.kept
-        if kept.weight is not None:
-            kept = kept._replace(weight=MXFP4Operand(*tensors[-2:], *kept.weight))
-        if kept.x is not None:
-            kept = kept._replace(x=MXFP4Operand(*tensors[:2], *kept.x))
-        kept = kept._replace(bias=ctx.needs_input_grad[2])
+        kept = kept._replace(x=kept.x and kept.x._replace(data=x), bias=ctx.needs_input_grad[2],
+                             weight=kept.weight and kept.weight._replace(data=weight))
         dx, dw, db = linear_mxfp4_bwd(dy, kept, seed=seed)
         return dx, dw, None if db is None else db.to(ctx.bias_dtype), None, None
 
@@ -377,6 +393,9 @@ def cross_attention_mxfp4_fwd(q: torch.Tensor, kv: MXFP4, *, key_lengths: torch.
     if torch.compiler.is_dynamo_compiling():
         return _between_graphs(cross_attention_mxfp4_fwd, q, kv, key_lengths=key_lengths, key_mask=key_mask,
                                scale=scale)
+    done = _fast().mxfp4_attention(q, kv.data, kv.scales, key_lengths, key_mask, scale)
+    if done is not None:
+        return done
     _check_mxfp4(kv, "cross attention")
     if q.ndim != 4 or kv.data.ndim != 5 or kv.data.shape[2] != 2:
         raise ValueError("cross attention: q is [batch, tokens, heads, head_dim], kv [batch, tokens, 2, heads, "

@@ -861,25 +861,29 @@ int dpa_mxfp4_dequantize(const void* data, const void* scales, void* y, int dtyp
                          void* stream);
 
 /* Operands of dpa_mxfp4_gemm: a matrix whose contraction runs along its rows, cols long, any number of
- * them: data of ceil(cols / 256) * 128 B a row, scales of ceil(cols / 512) * 16 B a row (buffers of
- * *_bytes, 16-B aligned, opaque). dpa_mxfp4_operands lays out x [rows][cols] (row_stride elements apart)
- * from one read: as it is (row_*: blocks along the rows) and transposed (col_*: an operand of `cols` rows,
- * blocks down the columns); NULL for the one that is not wanted. With seed (a uint64 in device
+ * them, in a buffer of *_bytes (16-B aligned, its order the kernels': rows of ceil(cols / 256) * 128 B, then
+ * ceil(cols / 512) * 16 scales a row). dpa_mxfp4_operands lays out x [rows][cols] (row_stride elements
+ * apart) from one read: as it is (by_rows: blocks along the rows) and transposed (by_cols: an operand of `cols`
+ * rows, blocks down the columns of x); NULL for the one that is not wanted. With seed (a uint64 in device
  * memory) elements are rounded up or down at random so that their mean is the element, the scale one power
  * higher where amax would pass 6 of it: 16 bits a element of splitmix64(seed + i / 4 * golden ratio),
  * i = row * (cols rounded up to 32) + col, for both arrangements. */
-int64_t dpa_mxfp4_operand_data_bytes(int64_t rows, int64_t cols);
-int64_t dpa_mxfp4_operand_scale_bytes(int64_t rows, int64_t cols);
+int64_t dpa_mxfp4_operand_bytes(int64_t rows, int64_t cols);
 int dpa_mxfp4_operands(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride,
-                       void* row_data, void* row_scales, void* col_data, void* col_scales,
-                       const void* seed, void* stream);
+                       void* by_rows, void* by_cols, const void* seed, void* stream);
 
 /* y [M][N] (bf16, fp16 or fp32) = a b^T + bias over operands a of M rows and b of N rows, K columns each;
  * bias fp32 [N] or NULL. fp32 sums in a fixed order. */
 int64_t dpa_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
-int dpa_mxfp4_gemm(const void* a_data, const void* a_scales, const void* b_data, const void* b_scales,
-                   const float* bias, void* y, int dtype, int64_t M, int64_t N, int64_t K,
-                   void* workspace, int64_t workspace_bytes, void* stream);
+int dpa_mxfp4_gemm(const void* a, const void* b, const float* bias, void* y, int dtype, int64_t M, int64_t N,
+                   int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The same from x [M][K] itself (rows row_stride elements apart), rounded to nearest: for few rows within the
+ * product's launch, else laid out in the workspace first. */
+int64_t dpa_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int dpa_mxfp4_linear(const void* x, int x_dtype, int64_t row_stride, const void* weight, const float* bias,
+                     void* y, int dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+                     int64_t workspace_bytes, void* stream);
 
 /* y [cols] fp32 = sums down the columns of x [rows][cols] (bf16, fp16 or fp32, rows row_stride elements
  * apart), in fp32, in a fixed order. */

@@ -133,20 +133,30 @@ def test_operands_hold_the_rounded_values(M, dtype, shape, seed):
     assert torch.equal(operand_values(M, t), want_r)
 
 
-def test_large_operands_take_the_wide_form(M):
-    """Enough tiles for eight waves to a workgroup."""
-    x = randn((8192, 4352), 6, torch.bfloat16).cuda()
-    rows, cols = M.mxfp4_operands(x)
-    t = M.mxfp4_operands(x.t().contiguous())
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_large_operands_take_the_wide_form(M, dtype):
+    """Enough tiles for whole lines of the columns: the bytes of the small form, which is checked above, on the same
+    rows, and of the transpose the other way round."""
+    x = randn((16384, 2100), 6, dtype).cuda()
     n, k = x.shape
-    # rows by the forms that are checked above: what the transpose gives the other way round
-    for got, want, cols_ in ((rows, t[1], k), (cols, t[0], n)):
-        assert torch.equal(got.data, want.data)
-        full = cols_ // 512 * got.rows * 16
-        assert torch.equal(got.scales[:full], want.scales[:full])
-    pick = torch.tensor([0, 31, 257, 4000, 8191])
-    small = M.mxfp4_operand(x[pick.cuda()].contiguous())
-    assert torch.equal(small.data.view(5, -1), rows.data.view(n, -1)[pick.cuda()])
+    rows, cols = M.mxfp4_operands(x)
+    t_rows, t_cols = M.mxfp4_operands(x.t().contiguous())
+    nd = n * (-(-k // 256) * 128)
+    assert torch.equal(rows.data[:nd], t_cols.data[:nd])
+    nd = k * (-(-n // 256) * 128)
+    assert torch.equal(cols.data, t_rows.data)      # (whole groups: 16384 is a multiple of 512)
+    pick = torch.tensor([0, 31, 257, 4000, 16383], device="cuda")
+    small = M.mxfp4_operand(x[pick].contiguous())
+    y = M.mxfp4_operand(randn((40, k), 7, dtype).cuda())
+    assert torch.equal(M._product(small, y, None, torch.float32), M._product(rows, y, None, torch.float32)[pick])
+    s = seed_of(77)
+    r1, c1 = M.mxfp4_operands(x, seed=s)
+    r2 = M.mxfp4_operand(x, seed=s)
+    assert torch.equal(r1.data[:n * 128 * 9], r2.data[:n * 128 * 9])
+    few = M.mxfp4_operands(x[:300], seed=s)
+    assert torch.equal(operand_values(M, few[1]), R.rounded(x[:300].cpu(), 0, 77).t())
+    line = c1.data[:nd].view(k, -1)
+    assert torch.equal(line[:, :128], few[1].data[:k * 256].view(k, -1)[:, :128])
 
 
 def test_stochastic_rounding_keeps_the_mean(M):

@@ -80,38 +80,47 @@ def test_c_entries_refuse_before_launch(lib):
     assert d(fake, nul, fake, 0, 32, nul) == -1 and d(fake, fake, odd, 0, 32, nul) == -3
     assert d(fake, fake, fake, 0, 16, nul) == -2 and d(fake, fake, fake, 7, 32, nul) == -4
     o = lib.dpa_mxfp4_operands
-    assert o(fake, 0, 4, 40, 40, nul, nul, nul, nul, nul, nul) == -1          # neither wanted
-    assert o(fake, 0, 4, 40, 40, fake, nul, nul, nul, nul, nul) == -1
-    assert o(nul, 0, 4, 40, 40, fake, fake, nul, nul, nul, nul) == -1
-    assert o(fake, 0, 4, 40, 39, fake, fake, nul, nul, nul, nul) == -2        # rows that overlap
-    assert o(fake, 0, 4, 0, 40, fake, fake, nul, nul, nul, nul) == -2
-    assert o(fake, 0, -1, 40, 40, fake, fake, nul, nul, nul, nul) == -2
-    assert o(fake, 0, 1 << 26, 1 << 12, 1 << 12, fake, fake, nul, nul, nul, nul) == -2
-    assert o(fake, 5, 4, 40, 40, fake, fake, nul, nul, nul, nul) == -4
-    assert o(fake, 0, 4, 40, 40, odd, fake, nul, nul, nul, nul) == -3
-    assert o(fake, 0, 4, 40, 40, fake, fake, nul, nul, odd, nul) == -3        # the seed
+    assert o(fake, 0, 4, 40, 40, nul, nul, nul, nul) == -1          # neither wanted
+    assert o(nul, 0, 4, 40, 40, fake, nul, nul, nul) == -1
+    assert o(fake, 0, 4, 40, 39, fake, nul, nul, nul) == -2         # rows that overlap
+    assert o(fake, 0, 4, 0, 40, fake, nul, nul, nul) == -2
+    assert o(fake, 0, -1, 40, 40, fake, nul, nul, nul) == -2
+    assert o(fake, 0, 1 << 25, 1 << 12, 1 << 12, fake, nul, nul, nul) == -2
+    assert o(fake, 5, 4, 40, 40, fake, nul, nul, nul) == -4
+    assert o(fake, 0, 4, 40, 40, odd, nul, nul, nul) == -3
+    assert o(fake, 0, 4, 40, 40, nul, odd, nul, nul) == -3
+    assert o(fake, 0, 4, 40, 40, fake, nul, odd, nul) == -3         # the seed
+    assert o(nul, 0, 0, 40, 40, fake, nul, nul, nul) == 0
     g = lib.dpa_mxfp4_gemm
-    assert g(fake, fake, fake, nul, nul, fake, 0, 4, 4, 32, nul, 0, nul) == -1
-    assert g(fake, fake, fake, fake, nul, fake, 0, 4, 4, 0, nul, 0, nul) == -2
-    assert g(fake, fake, fake, fake, nul, fake, 0, 1 << 27, 4, 32, nul, 0, nul) == -2
-    assert g(fake, fake, fake, fake, nul, fake, 9, 4, 4, 32, nul, 0, nul) == -4
-    assert g(odd, fake, fake, fake, nul, fake, 0, 4, 4, 32, nul, 0, nul) == -3
-    assert lib.dpa_mxfp4_gemm_workspace_bytes(16, 64, 16384) > 0
-    assert g(fake, fake, fake, fake, nul, fake, 0, 16, 64, 16384, nul, 0, nul) == -5
-    assert g(fake, fake, fake, fake, nul, fake, 0, 16, 64, 16384, fake, 16, nul) == -5
-    assert g(nul, nul, nul, nul, nul, nul, 0, 0, 4, 32, nul, 0, nul) == 0
+    assert g(fake, nul, nul, fake, 0, 4, 4, 32, nul, 0, nul) == -1
+    assert g(fake, fake, nul, fake, 0, 4, 4, 0, nul, 0, nul) == -2
+    assert g(fake, fake, nul, fake, 0, 1 << 27, 4, 32, nul, 0, nul) == -2
+    assert g(fake, fake, nul, fake, 9, 4, 4, 32, nul, 0, nul) == -4
+    assert g(odd, fake, nul, fake, 0, 4, 4, 32, nul, 0, nul) == -3
+    assert lib.dpa_mxfp4_gemm_workspace_bytes(100, 64, 16384) > 0
+    assert g(fake, fake, nul, fake, 0, 100, 64, 16384, nul, 0, nul) == -5
+    assert g(fake, fake, nul, fake, 0, 100, 64, 16384, fake, 16, nul) == -5
+    assert g(nul, nul, nul, nul, 0, 0, 4, 32, nul, 0, nul) == 0
+    li = lib.dpa_mxfp4_linear
+    need = lib.dpa_mxfp4_linear_workspace_bytes(20, 64, 512)
+    assert need >= lib.dpa_mxfp4_operand_bytes(20, 512) > 0
+    assert li(fake, 0, 512, fake, nul, fake, 0, 20, 64, 512, fake, need - 1, nul) == -5
+    assert li(fake, 0, 511, fake, nul, fake, 0, 20, 64, 512, fake, need, nul) == -2
+    assert li(fake, 0, 512, nul, nul, fake, 0, 20, 64, 512, fake, need, nul) == -1
+    assert li(fake, 4, 512, fake, nul, fake, 0, 20, 64, 512, fake, need, nul) == -4
+    assert li(fake, 0, 512, odd, nul, fake, 0, 20, 64, 512, fake, need, nul) == -3
+    assert li(fake, 0, 512, fake, nul, fake, 0, 0, 64, 512, nul, 0, nul) == 0
     c = lib.dpa_column_sum
     assert c(fake, 0, 0, 4, 4, fake, fake, 64, nul) == -2 and c(nul, 0, 4, 4, 4, fake, fake, 64, nul) == -1
     assert c(fake, 0, 4, 4, 4, fake, fake, 15, nul) == -5 and c(fake, 4, 4, 4, 4, fake, fake, 64, nul) == -4
-    assert lib.dpa_column_sum_workspace_bytes(129, 10) == 2 * 10 * 4
+    assert lib.dpa_column_sum_workspace_bytes(129, 10) == 4 * 10 * 4
 
 
 def test_operand_sizes(lib):
-    data, scales = lib.dpa_mxfp4_operand_data_bytes, lib.dpa_mxfp4_operand_scale_bytes
-    assert data(3, 1) == 3 * 128 and scales(3, 1) == 3 * 16
-    assert data(3, 256) == 3 * 128 and data(3, 257) == 3 * 256
-    assert scales(3, 512) == 3 * 16 and scales(3, 513) == 2 * 3 * 16
-    assert data(0, 40) == 0 and data(-1, 40) == 0 and data(3, 0) == 0 and data(1 << 40, 32) == 0
+    size = lib.dpa_mxfp4_operand_bytes
+    assert size(3, 1) == 3 * 128 + 3 * 16 and size(3, 256) == 3 * 128 + 3 * 16
+    assert size(3, 257) == 3 * 256 + 3 * 16 and size(3, 513) == 3 * 384 + 2 * 3 * 16
+    assert size(0, 40) == 0 and size(-1, 40) == 0 and size(3, 0) == 0 and size(1 << 40, 32) == 0
 
 
 def test_attention_entry_refuses_before_launch(lib, M):
