@@ -29,9 +29,12 @@ constexpr int kGroup = 512;  // columns of a group of scales
 __host__ __device__ inline int64_t pitch_of(int64_t cols) { return (cols + kStep - 1) / kStep * (kStep / 2); }
 __host__ __device__ inline int64_t groups_of(int64_t cols) { return (cols + kGroup - 1) / kGroup; }
 
-inline int64_t operand_data_bytes(int64_t rows, int64_t cols) { return rows * pitch_of(cols); }
+// (Rows come to the product eight at a time, scales of up to 256: the buffer holds as many behind the last,
+// which hold anything.)
+__host__ __device__ inline int64_t padded_rows(int64_t rows) { return (rows + 7) & ~7ll; }
+inline int64_t operand_data_bytes(int64_t rows, int64_t cols) { return padded_rows(rows) * pitch_of(cols); }
 inline int64_t operand_bytes(int64_t rows, int64_t cols) {
-  return operand_data_bytes(rows, cols) + groups_of(cols) * rows * 16;
+  return operand_data_bytes(rows, cols) + (groups_of(cols) * rows + 256) * 16;
 }
 
 // Sizes of a matrix that the kernels take: 32-bit numbers of 8-element groups and workgroups, and of scales

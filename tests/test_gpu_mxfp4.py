@@ -144,7 +144,9 @@ def test_large_operands_take_the_wide_form(M, dtype):
     nd = n * (-(-k // 256) * 128)
     assert torch.equal(rows.data[:nd], t_cols.data[:nd])
     nd = k * (-(-n // 256) * 128)
-    assert torch.equal(cols.data, t_rows.data)      # (whole groups: 16384 is a multiple of 512)
+    assert torch.equal(cols.data[:nd], t_rows.data[:nd])
+    y = M.mxfp4_operand(randn((40, n), 8, dtype).cuda())
+    assert torch.equal(M._product(cols, y, None, torch.float32), M._product(t_rows, y, None, torch.float32))
     pick = torch.tensor([0, 31, 257, 4000, 16383], device="cuda")
     small = M.mxfp4_operand(x[pick].contiguous())
     y = M.mxfp4_operand(randn((40, k), 7, dtype).cuda())
