@@ -401,14 +401,14 @@ PyObject* mxfp4_linear(PyObject*, PyObject* const* o, Py_ssize_t count) {
   if (!dtype_arg(o[5], &type) || dtype_of(type) < 0 || n <= 0 || !matrix_of(*x, k, &m) || !bias_ok(bias, n) ||
       w->scalar_type() != at::kByte || !w->is_contiguous() || !aligned16(*w) || w->numel() != mx_operand_bytes(n, k))
     return none();
-  const int64_t bytes = mx_linear_bytes(m, n, k);
-  if (bytes == 0) return none();
+  const int64_t bytes = mx_linear_bytes(x->data_ptr(), dtype_of(x->scalar_type()), k, m, n, k);
   at::DimVector shape(x->sizes().begin(), x->sizes().end());
   shape.back() = n;
-  at::Tensor y = at::empty(shape, x->options().dtype(type)), ws = bytes_like(*x, bytes);
+  at::Tensor y = at::empty(shape, x->options().dtype(type)), ws;
+  if (bytes) ws = bytes_like(*x, bytes);
   const int status = mx_linear(x->data_ptr(), dtype_of(x->scalar_type()), k, w->data_ptr(),
                                bias ? (const float*)bias->data_ptr() : nullptr, y.data_ptr(), dtype_of(type), m, n, k,
-                               ws.data_ptr(), bytes, stream_of(device));
+                               bytes ? ws.data_ptr() : nullptr, bytes, stream_of(device));
   if (status) return failed("dpa_mxfp4_linear", status);
   return THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS

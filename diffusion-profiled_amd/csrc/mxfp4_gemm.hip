@@ -18,31 +18,28 @@ struct GemmArgs {
   int M, N, K;
   int steps, per_split, splits;  // of 256 columns; per_split is even
   int tiles_m, tiles_n;
-  bool large;  // tiles of 256 x 256, else 128 x 128
+  int form;  // of the tiles
 };
 
-// v[0 .. 7] to columns n0 .. n0 + 7 of a row
+// v[0 .. 7] to columns n .. n + 7 of a row, by whole vectors
 template <int DT>
-__device__ __forceinline__ void store8(void* y, int64_t row, int n0, int N, bool vec, const float (&v)[8]) {
-  const int64_t at = row * N + n0;
-  if (vec && n0 + 8 <= N) {
-    if constexpr (DT == DPA_DTYPE_F32) {
-      float4* o = reinterpret_cast<float4*>(static_cast<float*>(y) + at);
-      o[0] = float4{v[0], v[1], v[2], v[3]}, o[1] = float4{v[4], v[5], v[6], v[7]};
-    } else {
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + at) =
-          uint4{Elem<DT>::pack(v[0], v[1]), Elem<DT>::pack(v[2], v[3]), Elem<DT>::pack(v[4], v[5]), Elem<DT>::pack(v[6], v[7])};
-    }
-    return;
+__device__ __forceinline__ void store8(void* y, int64_t row, int n, int N, const float (&v)[8]) {
+  const int64_t at = row * N + n;
+  if constexpr (DT == DPA_DTYPE_F32) {
+    float4* o = reinterpret_cast<float4*>(static_cast<float*>(y) + at);
+    o[0] = float4{v[0], v[1], v[2], v[3]};
+    if (n + 4 < N) o[1] = float4{v[4], v[5], v[6], v[7]};
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + at) =
+        uint4{Elem<DT>::pack(v[0], v[1]), Elem<DT>::pack(v[2], v[3]), Elem<DT>::pack(v[4], v[5]), Elem<DT>::pack(v[6], v[7])};
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (n0 + i < N) store1<DT>(y, at + i, v[i]);
 }
 
 // ---------------------------------------------------------------------------------------
 // Tiles of WM x WN waves of 16 FM x 16 FN each, steps of 256 columns (128 B of a row) through LDS by
-// DMA, double-buffered. b's rows are the A operand (rows of D), in the order that gives a lane 8 columns of y in
+// DMA, NS of them on their way, and their scales by the same way. (The scales straight to registers, a word to a
+// lane and fragment for every second step: 4096 x 8192 of 8192 156 us against 128.) Workgroups stay and take tile
+// after tile, the next one's first steps out before this one's stores. b's rows are the A operand (rows of D), in the order that gives a lane 8 columns of y in
 // a row and four lanes 64 B: row r of fragment i is row 32 (i / 2) + 8 (r / 4) + 4 (i % 2) + r % 4 of the
 // wave's. The 16-B piece c of a row lies at c ^ swz(row): the 16 lanes that LDS serves together (rows 0-3 and 12-15 at one piece,
 // 4-11 at the piece two further) then lie in 16 different places of the banks.
@@ -67,21 +64,14 @@ __device__ __forceinline__ void dma16_from(const void* base, uint32_t off, uint3
 // live at once, and gives results other registers than the sums had (207 registers spilled of the 128 x 64
 // wave, 0.7 PFLOP/s). It does not know these for matrix instructions, so the waits are here: s_nop before a product
 // whose scales a vector instruction may just have written, and results_ready before the sums are read.
-template <int AT, bool kAgpr>
+template <int AT>
 __device__ __forceinline__ void mfma_in_place(v4f& acc, u32x4 a, u32x4 b, uint32_t sa, uint32_t sb) {
-#define DPA_MFMA(C, SEL) \
-  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " SEL " cbsz:4 blgp:4" : C(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb))
-#define DPA_MFMA_AT(C)                                            \
-  if constexpr (AT == 0) DPA_MFMA(C, "op_sel_hi:[0,0,0]");        \
-  if constexpr (AT == 1) DPA_MFMA(C, "op_sel:[1,1,0] op_sel_hi:[0,0,0]"); \
-  if constexpr (AT == 2) DPA_MFMA(C, "op_sel_hi:[1,1,0]");        \
-  if constexpr (AT == 3) DPA_MFMA(C, "op_sel:[1,1,0] op_sel_hi:[1,1,0]")
-  if constexpr (kAgpr) {
-    DPA_MFMA_AT("+a");
-  } else {
-    DPA_MFMA_AT("+v");
-  }
-#undef DPA_MFMA_AT
+#define DPA_MFMA(SEL) \
+  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " SEL " cbsz:4 blgp:4" : "+v"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb))
+  if constexpr (AT == 0) DPA_MFMA("op_sel_hi:[0,0,0]");
+  if constexpr (AT == 1) DPA_MFMA("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
+  if constexpr (AT == 2) DPA_MFMA("op_sel_hi:[1,1,0]");
+  if constexpr (AT == 3) DPA_MFMA("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
 #undef DPA_MFMA
 }
 // 16 passes and more after the last product
@@ -91,18 +81,23 @@ __device__ __forceinline__ void results_ready() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-template <int WM, int WN, int FM, int FN, int DT>
+template <int WM, int WN, int FM, int FN, int NS, int DT>
 __global__ __launch_bounds__(64 * WM * WN) void mxfp4_gemm_kernel(const GemmArgs p, bool vec) {
   constexpr int kWaves = WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN;
-  // two buffers of b's rows, then two of a's: a read's place in them is an immediate offset
-  constexpr uint32_t kBytesB = BN * 128, kBytesA = BM * 128, kA = 2 * kBytesB;
-  constexpr int kXferB = BN / 8 / kWaves, kXferA = BM / 8 / kWaves;
+  // NS buffers of b's rows, NS of a's (a read's place in them is an immediate offset), NS / 2 of their scales
+  constexpr uint32_t kBytesB = BN * 128, kBytesA = BM * 128, kA = NS * kBytesB, kS = kA + NS * kBytesA;
+  constexpr uint32_t kBytesS = (BM + BN) * 16;
+  constexpr int kXferB = BN / 8 / kWaves, kXferA = BM / 8 / kWaves, kXfer = kXferB + kXferA;
   static_assert(BN % (8 * kWaves) == 0 && BM % (8 * kWaves) == 0, "transfers of 8 rows");
   static_assert(FN % 2 == 0 && kWaves % 4 == 0, "pairs of fragments; a swizzle of the row's place among 32");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kA + 2 * kBytesA];
+  static_assert(NS % 2 == 0 && (BM + BN) / 64 <= kWaves, "two steps to a group of scales, at most a transfer to a wave");
+  // 8 rows of a wave's columns in turn, granule g of 4 columns of row r at g ^ r
+  constexpr int kCols = 16 * FN;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kS + NS / 2 * kBytesS + kWaves * 8 * kCols * 4];
   const uint32_t l0 = LDS_ADDR(lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM, r = lane & 15, q = lane >> 4;
+  float* turn = reinterpret_cast<float*>(lds + kS + NS / 2 * kBytesS) + wave * 8 * kCols;
   const uint32_t tiles = p.tiles_m * p.tiles_n, total = tiles * p.splits;
   struct Tile {
     int m0, n0, split, s_lo, s_hi;
@@ -130,12 +125,19 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_gemm_kernel(const GemmArgs
   if (!there(blockIdx.x)) return;
   Tile c = tile_of(blockIdx.x);
 
-  // A transfer is 8 rows of a wave; its first row is the same for all lanes
+  // A transfer is 8 rows of a wave; its first row is the same for all lanes. Transfer 0 of an even step is the
+  // scales of its group, 64 rows to a wave (waves beyond those repeat them).
   const int lr = lane >> 3;
   const uint32_t off_b = opaque(lr * (uint32_t)p.pitch + (((lane & 7) ^ swz_b(8 * wave + lr)) << 4));
   const uint32_t off_a = opaque(lr * (uint32_t)p.pitch + (((lane & 7) ^ swz_a(8 * wave + lr)) << 4));
   const int last_a = ((p.M + 7) & ~7) - 8, last_b = ((p.N + 7) & ~7) - 8;
-  constexpr int kXfer = kXferB + kXferA;
+  const int part = wave % ((BM + BN) / 64);
+  auto fetch_scales = [&](int step, int slot) __attribute__((always_inline)) {
+    const int64_t group = step >> 1;
+    const uint8_t* from = part < BN / 64 ? p.bs + (group * p.N + c.n0 + 64 * part) * 16
+                                         : p.as + (group * p.M + c.m0 + 64 * (part - BN / 64)) * 16;
+    dma16_from(from, (uint32_t)lane * 16, l0 + kS + slot * kBytesS + part * 1024);
+  };
   auto fetch1 = [&](int i, int step, int buf) __attribute__((always_inline)) {
     const uint32_t at = l0 + wave * 1024;
     if (i < kXferB)
@@ -145,29 +147,15 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_gemm_kernel(const GemmArgs
       dma16_from(p.a + min(c.m0 + 8 * ((i - kXferB) * kWaves + wave), last_a) * p.pitch + step * 128ll, off_a,
                  at + kA + buf * kBytesA + (i - kXferB) * kWaves * 1024);
   };
-  auto fetch = [&](int step, int buf) __attribute__((always_inline)) {
+  // all NS first steps of a tile, or as many as there are
+  auto begin = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kXfer; ++i) fetch1(i, step, buf);
-  };
-  // scales of this lane's rows, by fragment (of rows behind the last too: what comes there is not used)
-  const uint32_t at_b = (16 * FN * wn + 8 * (r >> 2) + (r & 3)) * 16 + 4 * q;
-  const uint32_t at_a = (16 * FM * wm + r) * 16 + 4 * q;
-  uint32_t sa[FM], sb[FN], sa_next[FM], sb_next[FN];
-  auto fetch_scales1 = [&](int j, int group) __attribute__((always_inline)) {  // of FM parts
-    const uint8_t *ga = p.as + ((int64_t)group * p.M + c.m0) * 16, *gb = p.bs + ((int64_t)group * p.N + c.n0) * 16;
-    sa_next[j] = *reinterpret_cast<const uint32_t*>(ga + at_a + 256 * j);
+    for (int k = 0; k < NS; ++k)
+      if (c.s_lo + k < c.s_hi) {
+        if (k % 2 == 0) fetch_scales(c.s_lo + k, k / 2);
 #pragma unroll
-    for (int i = j; i < FN; i += FM) sb_next[i] = *reinterpret_cast<const uint32_t*>(gb + at_b + 512 * (i / 2) + 64 * (i % 2));
-  };
-  auto fetch_scales = [&](int group) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < FM; ++j) fetch_scales1(j, group);
-  };
-  auto take_scales = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < FN; ++i) sb[i] = sb_next[i];
-#pragma unroll
-    for (int j = 0; j < FM; ++j) sa[j] = sa_next[j];
+        for (int i = 0; i < kXfer; ++i) fetch1(i, c.s_lo + k, k);
+      }
   };
 
   const int rb = 16 * FN * wn + 8 * (r >> 2) + (r & 3), ra = 16 * FM * wm + r;
@@ -177,84 +165,116 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_gemm_kernel(const GemmArgs
     read_b[t] = opaque(l0 + rb * 128 + (((2 * q + t) ^ swz_b(rb)) << 4));
     read_a[t] = opaque(l0 + kA + ra * 128 + (((2 * q + t) ^ swz_a(ra)) << 4));
   }
+  const uint32_t read_s = opaque(l0 + kS + rb * 16 + 4 * q), read_sa = opaque(l0 + kS + BN * 16 + ra * 16 + 4 * q);
+  auto lds4 = [](uint32_t a) { return *(const __attribute__((address_space(3))) uint32_t*)(a); };
 
   v4f acc[FN][FM];
   u32x4 fa[FM], fb[2][FN];
-  auto read_b4 = [&](int i, auto buffer, auto piece) __attribute__((always_inline)) {
-    return lds16(read_b[decltype(piece)::value] + decltype(buffer)::value * kBytesB + 4096 * (i / 2) + 512 * (i % 2));
+  uint32_t sa[FM], sb[FN], sa_next[FM], sb_next[FN];
+  auto read_b4 = [&](int i, int buf, int t) __attribute__((always_inline)) {
+    return lds16(read_b[t] + buf * kBytesB + 4096 * (i / 2) + 512 * (i % 2));
   };
-  auto read_a4 = [&](int j, auto buffer, auto piece) __attribute__((always_inline)) {
-    return lds16(read_a[decltype(piece)::value] + decltype(buffer)::value * kBytesA + 2048 * j);
+  auto read_a4 = [&](int j, int buf, int t) __attribute__((always_inline)) { return lds16(read_a[t] + buf * kBytesA + 2048 * j); };
+  auto read_scales = [&](int j, int slot) __attribute__((always_inline)) {  // of FM parts
+    sa_next[j] = lds4(read_sa + slot * kBytesS + 256 * j);
+#pragma unroll
+    for (int i = j; i < FN; i += FM) sb_next[i] = lds4(read_s + slot * kBytesS + 512 * (i / 2) + 64 * (i % 2));
   };
-  constexpr bool kAgpr = FM * FN > 32;
+  auto take_scales = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i) sb[i] = sb_next[i];
+#pragma unroll
+    for (int j = 0; j < FM; ++j) sa[j] = sa_next[j];
+  };
   // The products of a half step, whose fragments are in fa and fb[piece]; the next half's take their places
   auto half = [&](auto buffer, auto piece, auto next_buffer, auto next_piece, auto between) __attribute__((always_inline)) {
-    constexpr int t = decltype(piece)::value, at = 2 * decltype(buffer)::value + t;
+    constexpr int t = decltype(piece)::value, at = 2 * (decltype(buffer)::value % 2) + t;
 #pragma unroll
-    for (int i = 0; i < FN; ++i) fb[1 - t][i] = read_b4(i, next_buffer, next_piece);
+    for (int i = 0; i < FN; ++i) fb[1 - t][i] = read_b4(i, decltype(next_buffer)::value, decltype(next_piece)::value);
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_nop 3");
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
 #pragma unroll
-      for (int i = 0; i < FN; ++i) mfma_in_place<at, kAgpr>(acc[i][j], fb[t][i], fa[j], sb[i], sa[j]);
-      fa[j] = read_a4(j, next_buffer, next_piece);
+      for (int i = 0; i < FN; ++i) mfma_in_place<at>(acc[i][j], fb[t][i], fa[j], sb[i], sa[j]);
+      fa[j] = read_a4(j, decltype(next_buffer)::value, decltype(next_piece)::value);
       between(j);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto nothing = [](int) __attribute__((always_inline)) {};
   typedef std::integral_constant<int, 0> Zero;
   typedef std::integral_constant<int, 1> One;
-  // Step s, whose first half's fragments are there. Transfers and scales go out between its products: all at once
-  // they hold both waves of a SIMD up together.
-  auto step = [&](int s, auto buffer, auto other) __attribute__((always_inline)) {
-    constexpr int buf = decltype(buffer)::value;
-    half(buffer, Zero(), buffer, One(), nothing);
+  // Step s in buffer k = (s - s_lo) % NS, whose first half's fragments are there. Transfers and scales go out between
+  // its products: all at once they hold both waves of a SIMD up together.
+  auto step = [&](int s, auto buffer) __attribute__((always_inline)) {
+    constexpr int k = decltype(buffer)::value;
+    typedef std::integral_constant<int, (k + 1) % NS> Next;
+    if constexpr (k % 2 == 0) take_scales();
+    half(buffer, Zero(), buffer, One(), [](int) __attribute__((always_inline)) {});
     wait_lgkmcnt0();
-    wait_vmcnt<0>();
-    lds_barrier();  // step s + 1 is there, and every wave has read step s
-    const bool more = s + 2 < c.s_hi;
-    half(buffer, One(), other, Zero(), [&](int j) __attribute__((always_inline)) {
-      if constexpr (buf == 0) fetch_scales1(j, min(s + 2, c.s_hi - 1) >> 1);
-      if (more)
+    // step s + 1 is there, and every wave has read step s; steps s + 2 .. s + NS - 1 are on their way
+    if (s + NS - 1 < c.s_hi)
+      wait_vmcnt<(NS - 2) * kXfer + (NS - 2) / 2>();
+    else
+      wait_vmcnt<0>();
+    lds_barrier();
+    const bool more = s + NS < c.s_hi;
+    half(buffer, One(), Next(), Zero(), [&](int j) __attribute__((always_inline)) {
+      if constexpr (k % 2 == 1) read_scales(j, (k + 1) % NS / 2);
+      if (more) {
+        if (k % 2 == 0 && j == 0) fetch_scales(s + NS, k / 2);
 #pragma unroll
-        for (int i = j; i < kXfer; i += FM) fetch1(i, s + 2, buf);
+        for (int i = j; i < kXfer; i += FM) fetch1(i, s + NS, k);
+      }
     });
   };
-  auto begin = [&]() __attribute__((always_inline)) {
-    fetch(c.s_lo, 0);
-    if (c.s_lo + 1 < c.s_hi) fetch(c.s_lo + 1, 1);
-    fetch_scales(c.s_lo >> 1);
-  };
   constexpr int kStores = FN / 2 * FM * Elem<DT>::size / 2;
+  constexpr int kAhead = (NS - 1) * kXfer + NS / 2 - 1;  // transfers behind a tile's first step
+  static_assert(kAhead + kStores < 64, "vmcnt");
   bool counted = false;
   begin();
   for (uint32_t id = blockIdx.x;;) {
-    // the tile's first steps, behind which come only the stores of the tile before
-    if (counted)
-      wait_vmcnt<kStores>();
-    else
+    // the tile's first step, behind which come its next ones and the stores of the tile before
+    if (c.s_lo + NS > c.s_hi)
       wait_vmcnt<0>();
+    else if (counted)
+      wait_vmcnt<kAhead + kStores>();
+    else
+      wait_vmcnt<kAhead>();
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll
       for (int j = 0; j < FM; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < FN; ++i) fb[0][i] = read_b4(i, Zero(), Zero());
+    for (int j = 0; j < FM; ++j) read_scales(j, 0);
 #pragma unroll
-    for (int j = 0; j < FM; ++j) fa[j] = read_a4(j, Zero(), Zero());
+    for (int i = 0; i < FN; ++i) fb[0][i] = read_b4(i, 0, 0);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) fa[j] = read_a4(j, 0, 0);
     int s = c.s_lo;
-    for (; s + 1 < c.s_hi; s += 2) {
-      take_scales();
-      step(s, Zero(), One());
-      step(s + 1, One(), Zero());
-    }
-    if (s < c.s_hi) {  // (an odd number of steps: the last, there already)
-      take_scales();
-      half(Zero(), Zero(), Zero(), One(), nothing);
-      half(Zero(), One(), Zero(), Zero(), nothing);
+    if constexpr (NS == 2) {
+      for (; s + 2 <= c.s_hi; s += 2) {
+        step(s, Zero());
+        step(s + 1, One());
+      }
+      if (s < c.s_hi) step(s, Zero());
+    } else {
+      typedef std::integral_constant<int, 2> Two;
+      typedef std::integral_constant<int, 3> Three;
+      for (; s + 4 <= c.s_hi; s += 4) {
+        step(s, Zero());
+        step(s + 1, One());
+        step(s + 2, Two());
+        step(s + 3, Three());
+      }
+      if (s < c.s_hi) {
+        step(s, Zero());
+        if (s + 1 < c.s_hi) {
+          step(s + 1, One());
+          if (s + 2 < c.s_hi) step(s + 2, Two());
+        }
+      }
     }
     results_ready();
     const Tile done = c;
@@ -268,23 +288,54 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_gemm_kernel(const GemmArgs
       __builtin_amdgcn_sched_barrier(0);
       counted = done.whole;
     }
+    if (vec) {
 #pragma unroll
-    for (int u = 0; u < FN / 2; ++u) {
-      const int n = done.n0 + 16 * FN * wn + 32 * u + 8 * q;
-      float bias[8];
+      for (int u = 0; u < FN / 2; ++u) {
+        const int n = done.n0 + 16 * FN * wn + 32 * u + 8 * q;
+        float bias[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) bias[i] = p.bias && p.splits == 1 && n + i < p.N ? p.bias[n + i] : 0.f;
+        for (int i = 0; i < 8; ++i) bias[i] = p.bias && p.splits == 1 && n + i < p.N ? p.bias[n + i] : 0.f;
 #pragma unroll
-      for (int j = 0; j < FM; ++j) {
-        const int m = done.m0 + 16 * FM * wm + 16 * j + r;
-        float v[8];
+        for (int j = 0; j < FM; ++j) {
+          const int m = done.m0 + 16 * FM * wm + 16 * j + r;
+          float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = acc[2 * u + i / 4][j][i % 4] + bias[i];
-        if (!done.whole && m >= p.M) continue;
-        if (p.splits > 1)
-          store8<DPA_DTYPE_F32>(p.part, (int64_t)done.split * p.M + m, n, p.N, vec, v);
-        else
-          store8<DT>(p.y, m, n, p.N, vec, v);
+          for (int i = 0; i < 8; ++i) v[i] = acc[2 * u + i / 4][j][i % 4] + bias[i];
+          if (!done.whole && (m >= p.M || n >= p.N)) continue;  // (whole vectors: N is a multiple of them)
+          if (p.splits > 1)
+            store8<DPA_DTYPE_F32>(p.part, (int64_t)done.split * p.M + m, n, p.N, v);
+          else
+            store8<DT>(p.y, m, n, p.N, v);
+        }
+      }
+    } else {
+      // Rows that no vector fits: 8 of them turn in LDS, so that neighbouring lanes store neighbours (each lane its
+      // 8 one by one: 3850 x 1023 of 513 in fp32 22.5 us, against 16.3)
+      const int col = lane % kCols, n = done.n0 + 16 * FN * wn + col;
+      const float bias = p.bias && p.splits == 1 && n < p.N ? p.bias[n] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 2 * FM; ++j) {
+        if ((r >> 3) == (j & 1)) {
+#pragma unroll
+          for (int i = 0; i < FN; ++i) {
+            const v4f v = acc[i][j / 2];
+            *reinterpret_cast<float4*>(turn + (r & 7) * kCols + (((8 * (i / 2) + 2 * q + i % 2) ^ (r & 7)) << 2)) =
+                float4{v[0], v[1], v[2], v[3]};
+          }
+        }
+        asm volatile("" ::: "memory");
+        const int m0 = done.m0 + 16 * FM * wm + 8 * j;
+#pragma unroll
+        for (int i = 0; i < 8 * kCols / 64; ++i) {
+          const int row = i * (64 / kCols) + lane / kCols, m = m0 + row;
+          const float v = turn[row * kCols + (((col >> 2) ^ row) << 2) + (col & 3)] + bias;
+          if (m >= p.M || n >= p.N) continue;
+          if (p.splits > 1)
+            p.part[((int64_t)done.split * p.M + m) * p.N + n] = v;
+          else
+            store1<DT>(p.y, (int64_t)m * p.N + n, v);
+        }
+        asm volatile("" ::: "memory");
       }
     }
     if (!more) break;
@@ -544,39 +595,48 @@ static int check_gemm(int64_t M, int64_t N, int64_t K) {
   return DPA_OK;
 }
 
-// How often tiles of `rows` x `cols` run and over how much of the contraction, by what they cost: a round of
-// workgroups `tile_us` and `step_us` for each step of 256 columns, a split's sums their bytes twice and a launch.
-struct Plan {
-  int tiles_m, tiles_n, per_split, splits;
-  double us;
+// The forms of the product: 256 x 256 tiles by 8 waves, one workgroup to a CU; 128 x 128 by 4, two to a CU; 64 x 64
+// by 4 with four steps on their way, two to a CU, for little work, whose time is that of the loads' way. And how
+// often the contraction is split. All by what they cost, in us: a round of workgroups tile_us and step_us for each
+// step of 256 columns (step_few_us where a CU has one workgroup), a split's sums their bytes twice and a launch.
+// Measured (us, 256 / 128 / 64): 4096 x 8192 of 8192 128, 179, 227; 8192 x 4096 of 4096 74, 81, 127; 32768 x 768
+// of 256 18.2, 16.9, 23.9; 2048 x 2048 of 2048 18.9, 11.2, 12.8; 512 x 4096 of 4096 27.5, 13.8, 11.1; 1024 x 1024
+// of 1024 13.3, 7.9, 5.9; 3840 x 1024 of 512 11.9, 7.8, 7.5.
+struct Form {
+  int side, per_cu;
+  double tile_us, step_us, step_few_us;
 };
-static Plan plan_tiles(int64_t M, int64_t N, int64_t steps, int rows, int cols, int64_t slots, double tile_us, double step_us) {
-  Plan best{};
-  const int64_t tm = ceil_div(M, rows), tn = ceil_div(N, cols), tiles = tm * tn;
-  const int64_t most = std::min<int64_t>(std::max<int64_t>(1, 2 * slots / std::max<int64_t>(1, tiles)), ceil_div(steps, 4));
-  for (int64_t n = 1; n <= most; ++n) {
-    const int64_t per = ceil_div(ceil_div(steps, n), 2) * 2, splits = ceil_div(steps, per);
-    if (splits < n && n > 1) continue;
-    const double us = (double)ceil_div(tiles * splits, slots) * (tile_us + (double)std::min(per, steps) * step_us) +
-                      (splits > 1 ? 4.0 + 2.0 * (double)(splits * M * N * 4) * 2.5e-7 : 0.0);
-    if (n == 1 || us < best.us) best = Plan{(int)tm, (int)tn, (int)per, (int)splits, us};
+constexpr Form kForms[3] = {{256, 1, 8.5, 1.65, 1.3}, {128, 2, 3.0, 1.15, 0.7}, {64, 2, 2.2, 0.43, 0.4}};
+constexpr int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64};
+
+static void plan_tiles(GemmArgs& p) {
+  double best = 0.0;
+  for (int f = 0; f < 3; ++f) {
+    const Form& form = kForms[f];
+    const int tm = (int)ceil_div(p.M, form.side), tn = (int)ceil_div(p.N, form.side);
+    const int64_t tiles = (int64_t)tm * tn, cus = num_cus(), slots = cus * form.per_cu;
+    for (const int n : kSplits) {
+      if (n > 1 && (n * 4 > p.steps || n * tiles > slots)) break;
+      const int per = (p.steps + 2 * n - 1) / (2 * n) * 2, splits = (p.steps + per - 1) / per;
+      const int64_t rounds = (tiles * splits + slots - 1) / slots;
+      double us = (double)rounds * (form.tile_us + std::min(per, p.steps) * (tiles * splits > cus ? form.step_us : form.step_few_us));
+      if (splits > 1) us += 2.5 + (double)splits * p.M * p.N * 4 * 2 * 2e-7;
+      if (best == 0.0 || us < best) {
+        best = us;
+        p.form = f, p.tiles_m = tm, p.tiles_n = tn, p.per_split = per, p.splits = splits;
+      }
+    }
   }
-  return best;
 }
 
-// The operand a laid out, or x itself (`token`). Tiles of 256 x 256, one to a CU, against 128 x 128, two to a
-// CU, by the costs that they measured (4096 x 8192 of 8192 156 and 214 us, 32768 x 768 of 256 20.9 and 18.7).
+// The operand a laid out, or x itself (`token`)
 static GemmArgs plan(int64_t M, int64_t N, int64_t K, bool token) {
   GemmArgs p{};
   p.M = (int)M, p.N = (int)N, p.K = (int)K;
   p.pitch = pitch_of(K);
   p.steps = (int)(p.pitch / 128);
   if (!token && M > kFewRows) {
-    const Plan large = plan_tiles(M, N, p.steps, 256, 256, num_cus(), 4.5, 2.35);
-    const Plan small = plan_tiles(M, N, p.steps, 128, 128, 2 * num_cus(), 3.5, 1.6);
-    const Plan& best = large.us < small.us ? large : small;
-    p.large = large.us < small.us;
-    p.tiles_m = best.tiles_m, p.tiles_n = best.tiles_n, p.per_split = best.per_split, p.splits = best.splits;
+    plan_tiles(p);
     return p;
   }
   p.tiles_m = 1;
@@ -619,10 +679,13 @@ static int run_gemm(const GemmArgs& p, hipStream_t s) {
       mxfp4_few_kernel<4, DT><<<grid, 512, 0, s>>>(p);
   } else {
     const int64_t items = ceil_div((int64_t)p.tiles_m * p.tiles_n * p.splits, 8) * 8;
-    if (p.large)
-      mxfp4_gemm_kernel<2, 4, 8, 4, DT><<<(unsigned)std::min<int64_t>(items, num_cus()), 512, 0, s>>>(p, vec);
+    const unsigned grid = (unsigned)std::min<int64_t>(items, kForms[p.form].per_cu * num_cus());
+    if (p.form == 0)
+      mxfp4_gemm_kernel<2, 4, 8, 4, 2, DT><<<grid, 512, 0, s>>>(p, vec);
+    else if (p.form == 1)
+      mxfp4_gemm_kernel<2, 2, 4, 4, 2, DT><<<grid, 256, 0, s>>>(p, vec);
     else
-      mxfp4_gemm_kernel<2, 2, 4, 4, DT><<<(unsigned)std::min<int64_t>(items, 2 * num_cus()), 256, 0, s>>>(p, vec);
+      mxfp4_gemm_kernel<2, 2, 2, 2, 4, DT><<<grid, 256, 0, s>>>(p, vec);
   }
   return join<DT>(p, s);
 }
@@ -687,11 +750,11 @@ extern "C" int dpa_mxfp4_gemm(const void* a, const void* b, const float* bias, v
   return run(p, dtype, (hipStream_t)stream);
 }
 
-extern "C" int64_t dpa_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (check_gemm(M, N, K) != DPA_OK || M == 0) return 0;
-  const int64_t two = align256(operand_bytes(M, K)) + part_bytes(plan(M, N, K, false));
-  const int64_t one = M <= 16 ? part_bytes(plan(M, N, K, true)) : 0;
-  return one > two ? one : two;
+extern "C" int64_t dpa_mxfp4_linear_workspace_bytes(const void* x, int x_dtype, int64_t row_stride, int64_t M, int64_t N,
+                                                    int64_t K) {
+  if (!dtype_ok(x_dtype) || check_gemm(M, N, K) != DPA_OK || M == 0) return 0;
+  if (takes_token(x, x_dtype, row_stride, M, K)) return part_bytes(plan(M, N, K, true));
+  return align256(operand_bytes(M, K)) + part_bytes(plan(M, N, K, false));
 }
 
 extern "C" int dpa_mxfp4_linear(const void* x, int x_dtype, int64_t row_stride, const void* weight, const float* bias,
@@ -705,7 +768,8 @@ extern "C" int dpa_mxfp4_linear(const void* x, int x_dtype, int64_t row_stride, 
   if (!x || !weight || !y) return DPA_ERR_NULL;
   if (!aligned(x, size_of(x_dtype)) || !aligned(weight, 16) || !aligned(bias, 4) || !aligned(y, size_of(dtype)))
     return DPA_ERR_ALIGN;
-  if (!workspace || workspace_bytes < dpa_mxfp4_linear_workspace_bytes(M, N, K)) return DPA_ERR_WORKSPACE;
+  const int64_t need = dpa_mxfp4_linear_workspace_bytes(x, x_dtype, row_stride, M, N, K);
+  if (need && (!workspace || workspace_bytes < need)) return DPA_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return DPA_ERR_ALIGN;
   uint8_t* ws = (uint8_t*)workspace;
   hipStream_t s = (hipStream_t)stream;

@@ -215,10 +215,11 @@ def linear_mxfp4_fwd(x: torch.Tensor, weight: torch.Tensor | MXFP4Operand, bias:
     y = torch.empty((m, n), device=x.device, dtype=dtype)
     if m and n:
         _new_operand(m, k, "meta")      # (refuses sizes beyond the kernels')
-        nbytes = _lib.query("dpa_mxfp4_linear_workspace_bytes", m, n, k)
+        ld = x2.stride(0) if m > 1 else k
+        nbytes = _lib.query("dpa_mxfp4_linear_workspace_bytes", x2.data_ptr(), _DT[x2.dtype], ld, m, n, k)
         ws = _workspace(nbytes, x.device)
-        _lib.call("dpa_mxfp4_linear", x2.data_ptr(), _DT[x2.dtype], x2.stride(0) if m > 1 else k, w.data.data_ptr(),
-                  _ptr(b32), y.data_ptr(), _DT[dtype], m, n, k, _ptr(ws), nbytes, _lib.current_stream(x2))
+        _lib.call("dpa_mxfp4_linear", x2.data_ptr(), _DT[x2.dtype], ld, w.data.data_ptr(), _ptr(b32), y.data_ptr(),
+                  _DT[dtype], m, n, k, _ptr(ws), nbytes, _lib.current_stream(x2))
     return y.view(*x.shape[:-1], n)
 
 

@@ -879,8 +879,9 @@ int dpa_mxfp4_gemm(const void* a, const void* b, const float* bias, void* y, int
                    int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* The same from x [M][K] itself (rows row_stride elements apart), rounded to nearest: for few rows within the
- * product's launch, else laid out in the workspace first. */
-int64_t dpa_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+ * product's launch, else laid out in the workspace first (x's alignment has a say in it; the query reads
+ * nothing). */
+int64_t dpa_mxfp4_linear_workspace_bytes(const void* x, int x_dtype, int64_t row_stride, int64_t M, int64_t N, int64_t K);
 int dpa_mxfp4_linear(const void* x, int x_dtype, int64_t row_stride, const void* weight, const float* bias,
                      void* y, int dtype, int64_t M, int64_t N, int64_t K, void* workspace,
                      int64_t workspace_bytes, void* stream);

@@ -102,8 +102,10 @@ def test_c_entries_refuse_before_launch(lib):
     assert g(fake, fake, nul, fake, 0, 100, 64, 16384, fake, 16, nul) == -5
     assert g(nul, nul, nul, nul, 0, 0, 4, 32, nul, 0, nul) == 0
     li = lib.dpa_mxfp4_linear
-    need = lib.dpa_mxfp4_linear_workspace_bytes(20, 64, 512)
+    need = lib.dpa_mxfp4_linear_workspace_bytes(fake, 0, 512, 20, 64, 512)
     assert need >= lib.dpa_mxfp4_operand_bytes(20, 512) > 0
+    assert lib.dpa_mxfp4_linear_workspace_bytes(fake, 0, 512, 2, 64, 512) == 0          # within the launch
+    assert lib.dpa_mxfp4_linear_workspace_bytes(odd, 0, 512, 2, 64, 512) > 0            # not by vectors
     assert li(fake, 0, 512, fake, nul, fake, 0, 20, 64, 512, fake, need - 1, nul) == -5
     assert li(fake, 0, 511, fake, nul, fake, 0, 20, 64, 512, fake, need, nul) == -2
     assert li(fake, 0, 512, nul, nul, fake, 0, 20, 64, 512, fake, need, nul) == -1
