@@ -2,6 +2,7 @@
 // xattn_fwd.hip, with values of the operands' type made from the 4-bit ones on the way to the products.
 // The products stay those of bf16 or fp16: queries and probabilities in 4 bits would lose what the cache
 // keeps. A value of the cache is exact in bf16; in fp16 it is one that fp16 holds if it was quantised from fp16.
+#include <algorithm>
 #include <type_traits>
 
 #include "mxfp4.hpp"
@@ -58,7 +59,7 @@ __device__ __forceinline__ void put_block(uint32_t at, int row, int blk, const R
 constexpr float kSlack = 8.f;
 
 template <class T, int DP>
-__global__ __launch_bounds__(256, 2) void xattn_mxfp4_fwd_kernel(const MxArgs p) {
+__global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_mxfp4_fwd_kernel(const MxArgs p) {
   constexpr int KT = 64;
   constexpr int KS = DP / 16, NDB = DP / 32, NB = DP / 32;
   constexpr int kItems = 2 * KT * NB / 256 > 0 ? 2 * KT * NB / 256 : 1;  // blocks to a thread
@@ -438,6 +439,265 @@ __global__ __launch_bounds__(256, 2) void xattn_mxfp4_few_kernel(const MxArgs p)
           uint2{T::pack(acc[i] * il, acc[i + 1] * il), T::pack(acc[i + 2] * il, acc[i + 3] * il)};
 }
 
+// ---------------------------------------------------------------------------------------
+// Up to 16 rows of a key head (single tokens, their heads sharing keys): as above, on v_mfma_f32_16x16x32, whose
+// columns are the rows. Bound by the bytes of the cache, so made for bytes in flight: half the registers, two tiles
+// of 32 keys a wave on their way, and as many waves as fit at once.
+//   S^T (16 keys x 16 rows) = K Q^T: lane (key l & 15, q = l >> 4) takes dims [q D / 4, (q + 1) D / 4) of its key, 8 to
+//   a product. It receives the scores of row l & 15 at keys 4 q + t of each 16, which packed are the B operand of
+//   O^T += V^T P^T if the sum over 32 keys runs over {4 q + t, 16 + 4 q + t} in lane q: so the values' transpose
+//   reads fetch rows 4 q .. and 16 + 4 q ...
+// ---------------------------------------------------------------------------------------
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+template <class T>
+__device__ __forceinline__ v4f mfma16(uint4 a, uint4 b, v4f c) {
+  if constexpr (std::is_same_v<T, Bf16>)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// maximum and sum over the four lanes of a row
+__device__ __forceinline__ float max_quarters(float x) {
+  x = max_halves(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_quarters(float x) {
+  x = sum_halves(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(256, 3) void xattn_mxfp4_token_kernel(const MxArgs p) {
+  constexpr int KT = 32;
+  constexpr int DP = D == 96 ? 128 : D;   // of the values' rows in LDS
+  constexpr int NB = D / 32;              // blocks to a row, words of 8 dims to a lane's quarter of it
+  constexpr int ND = D / 16;              // tiles of dims of O
+  constexpr int kItems = NB > 1 ? (NB + 1) / 2 : 1;  // blocks of values to a lane
+  constexpr uint32_t kBytes = KT * DP * 2, kJoin = 4 * D * 16 * 4;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kBytes > kJoin ? 4 * kBytes : kJoin];
+  __shared__ uint32_t seen[kMaxRange / 32];
+  const uint32_t l0 = LDS_ADDR(lds);
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, q = lane >> 4;
+  const uint32_t id = work_item(p);
+  if (id >= p.total) return;
+  // the heads of a batch's keys beside each other: their pieces of a token share cache lines
+  const uint32_t bs = id / (uint32_t)p.KVH;
+  const int g = id - bs * p.KVH, b = bs / (uint32_t)p.splits, split = bs - b * p.splits, bkv = b * p.KVH + g;
+
+  const int klen = __builtin_amdgcn_readfirstlane(keys_of(p, b));
+  const int nt = (klen + KT - 1) / KT;
+  const int t_lo = split * p.per_split + wave;
+  int t_hi = split + 1 == p.splits ? nt : min(nt, (split + 1) * p.per_split);
+  const KeyBits bits(p, b, klen, split * p.per_split * KT, t_hi * KT, seen, tid);
+  t_hi = bits.tiles_to<KT>(t_hi);
+
+  const bool has_row = col < p.rows;
+  const uint32_t head = fdiv(has_row ? col : 0, p.by_lq), tok = (has_row ? col : 0) - head * p.Lq;
+
+  const uint8_t* kd = p.kd + b * p.kds.b + g * p.kds.h + q * (D / 8);
+  const uint8_t* kx = p.kx + b * p.kxs.b + g * p.kxs.h + q * NB / 4;
+  const uint8_t* vd = p.vd + b * p.vds.b + g * p.vds.h;
+  const uint8_t* vx = p.vx + b * p.vxs.b + g * p.vxs.h;
+  struct Raw {
+    uint32_t k[2][NB], kb[2][2];
+    RawBlock v[kItems];
+    uint32_t word;
+  };
+  // A tile's loads go out together, without branches: rows behind the length are its last row, and what is not
+  // visible is cleared before its use.
+  auto load = [&](Raw& raw, int t) __attribute__((always_inline)) {
+    raw.word = (uint32_t)bits.template word<KT>(t);
+    const int last = klen - 1 - t * KT;
+    const uint8_t *kt = kd + (int64_t)t * KT * p.kds.l, *kxt = kx + (int64_t)t * KT * p.kxs.l;
+    const uint8_t *vt = vd + (int64_t)t * KT * p.vds.l, *vxt = vx + (int64_t)t * KT * p.vxs.l;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t row = min(16 * h + col, last);
+      const uint8_t *s = kt + (uint64_t)row * (uint32_t)p.kds.l, *x = kxt + (uint64_t)row * (uint32_t)p.kxs.l;
+      if constexpr (NB == 4) {
+        const uint4 w = *reinterpret_cast<const uint4*>(s);
+        raw.k[h][0] = w.x, raw.k[h][1] = w.y, raw.k[h][2] = w.z, raw.k[h][3] = w.w;
+      } else if constexpr (NB == 2) {
+        const uint2 w = *reinterpret_cast<const uint2*>(s);
+        raw.k[h][0] = w.x, raw.k[h][1] = w.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) raw.k[h][i] = reinterpret_cast<const uint32_t*>(s)[i];
+      }
+      raw.kb[h][0] = raw.kb[h][1] = x[0];
+      if constexpr (NB == 3) raw.kb[h][1] = x[q == 1 || q == 2 ? 1 : 0];
+    }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int at = min(lane + 64 * i, KT * NB - 1), blk = at % NB;  // (lanes behind the last block: that one)
+      const uint32_t row = min(at / NB, last);
+      raw.v[i].w = *reinterpret_cast<const uint4*>(vt + (uint64_t)row * (uint32_t)p.vds.l + 16 * blk);
+      raw.v[i].byte = vxt[(uint64_t)row * (uint32_t)p.vxs.l + blk];
+    }
+  };
+  auto clear_hidden = [&](Raw& raw) __attribute__((always_inline)) {
+    if (raw.word == ~0u) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (!((raw.word >> (16 * h + col)) & 1)) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) raw.k[h][i] = 0;
+        raw.kb[h][0] = raw.kb[h][1] = 127;
+      }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i)
+      if (!((raw.word >> (((lane + 64 * i) / NB) & 31)) & 1)) raw.v[i] = RawBlock{uint4{0u, 0u, 0u, 0u}, 127u};
+  };
+  Raw r0, r1;
+  if (t_lo < t_hi) load(r0, t_lo);
+  uint4 qf[NB];
+  {
+    const uint16_t* s = p.q + b * p.qs.b + (int64_t)tok * p.qs.l + (g * p.G + head) * p.qs.h + q * (D / 4);
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      qf[i] = *static_cast<const uint4*>(has_row ? static_cast<const void*>(s + 8 * i) : g_zero16);
+  }
+  if (t_lo + 4 < t_hi) load(r1, t_lo + 4);
+  const uint32_t v0 = l0 + wave * kBytes;
+  // transpose reads: lane k of a quarter addresses 4 dims of row 4 q + (k >> 2) (and of the row 16 further)
+  uint32_t tr[ND][2];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int row = 4 * q + (col >> 2) + 16 * x, gr = 2 * d + ((col & 3) >> 1);
+      tr[d][x] = v0 + row * DP * 2 + ((gr ^ swz<DP>(row)) << 4) + 8 * (col & 1);
+    }
+
+  v4f o[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
+  float m = -__builtin_inff(), l = 0.f;
+
+  auto tile = [&](Raw& raw, int t) __attribute__((always_inline)) {
+    // the tile out of its registers, then the loads of the one after the next into them
+    clear_hidden(raw);
+    uint4 kf[2][NB];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        // word i of quarter q lies in block (q NB + i) / 4, the first of the quarter's or the one behind it
+        const bool second = NB == 3 && (3 * q + i) / 4 != 3 * q / 4;
+        kf[h][i] = eight_of<T>(raw.k[h][i], mx::scale_back(second ? raw.kb[h][1] : raw.kb[h][0]));
+      }
+    asm volatile("" ::: "memory");  // (behind the reads of the tile before)
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int at = lane + 64 * i;
+      if (at < KT * NB) put_block<T, DP>(v0, at / NB, at % NB, raw.v[i]);
+    }
+    asm volatile("" ::: "memory");
+    const uint32_t word = raw.word;
+    if (t + 8 < t_hi) load(raw, t + 8);
+    if (word == 0) return;
+    v4f s[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[h][i] = (word >> (16 * h + 4 * q + i)) & 1 ? 0.f : -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < NB; ++i) s[h] = mfma16<T>(kf[h][i], qf[i], s[h]);
+    }
+    float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    top = max_quarters(top) * p.c2;
+    if (__any(top > m + kSlack)) {
+      const float mn = fmaxf(top, m);
+      const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] *= f;
+    }
+    const float ms = m == -__builtin_inff() ? 0.f : m;
+    uint32_t pk[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], p.c2, -ms));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i + 1], p.c2, -ms));
+        l += e0 + e1;
+        pk[2 * h + i / 2] = T::pack(e0, e1);
+      }
+    const uint4 pf = {pk[0], pk[1], pk[2], pk[3]};
+    wait_lgkmcnt0();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      typedef v4s __attribute__((address_space(3))) * LP;
+      const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(tr[d][0])));
+      const uint2 c = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(tr[d][1])));
+      o[d] = mfma16<T>(uint4{a.x, a.y, c.x, c.y}, pf, o[d]);
+    }
+  };
+  for (int t = t_lo; t < t_hi; t += 8) {
+    tile(r0, t);
+    if (t + 4 < t_hi) tile(r1, t + 4);
+  }
+  l = sum_quarters(l);
+
+  // wave w leaves its (m, l) and O; a thread adds up D / 16 dims of a row
+  __syncthreads();
+  float* ox = reinterpret_cast<float*>(lds);  // [4][D][16]
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ox[(wave * D + 16 * d + 4 * q + i) * 16 + col] = o[d][i];
+  __shared__ float ml[2][4][16];
+  if (q == 0) {
+    ml[0][wave][col] = m;
+    ml[1][wave][col] = l;
+  }
+  __syncthreads();
+  m = fmaxf(fmaxf(ml[0][0][col], ml[0][1][col]), fmaxf(ml[0][2][col], ml[0][3][col]));
+  const float ms = m == -__builtin_inff() ? 0.f : m;
+  float f[4];
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = __builtin_amdgcn_exp2f(ml[0][w][col] - ms);
+    l += f[w] * ml[1][w][col];
+  }
+  if (!has_row) return;
+  const int part = tid >> 4;  // dims [part ND, (part + 1) ND)
+  float acc[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    acc[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) acc[i] += f[w] * ox[(w * D + part * ND + i) * 16 + col];
+  }
+  if (p.splits > 1) {
+    const int64_t at = ((int64_t)split * p.B * p.KVH + bkv) * p.rows + col;
+    if (part == 0) p.stat[at] = float2{m, l};
+#pragma unroll
+    for (int i = 0; i < ND; i += 2)
+      *reinterpret_cast<float2*>(p.part + at * D + part * ND + i) = float2{acc[i], acc[i + 1]};
+    return;
+  }
+  const int64_t orow = ((int64_t)b * p.Lq + tok) * p.H + g * p.G + head;
+  if (part == 0)
+    p.lse[((int64_t)b * p.H + g * p.G + head) * p.Lq + tok] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+  const float il = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < ND; i += 2)
+    *reinterpret_cast<uint32_t*>(p.out + orow * D + part * ND + i) = T::pack(acc[i] * il, acc[i + 1] * il);
+}
+
 // ---- host ------------------------------------------------------------------------------
 static DpaCrossAttention shape_of(const DpaCrossAttentionMxfp4& a) {
   DpaCrossAttention c{};
@@ -457,6 +717,29 @@ static int check_mx(const DpaCrossAttentionMxfp4& a) {
 
 static bool strides16(const int64_t* s) { return s[0] % 16 == 0 && s[1] % 16 == 0 && s[2] % 16 == 0; }
 
+// Up to 16 rows of a key head have a form of their own
+static bool token_rows(const Args& p) { return p.rows <= 16; }
+
+static void plan_mx(Args& p) {
+  if (!token_rows(p)) {
+    plan_rows(p, few_rows_fwd(p));
+    return;
+  }
+  p.tiles = 1;
+  const int64_t groups = (int64_t)p.B * p.KVH;
+  // four workgroups to a CU, of which three are there at once and the others take the place of those whose keys
+  // end early; what fills the CUs without is not split, and no row into more than 64 parts, which the join would
+  // wait for
+  const int64_t want = groups >= 2 * num_cus() ? groups : std::min<int64_t>(4 * num_cus(), 64 * groups);
+  choose_splits(p, groups, ceil_div(p.Lk, 32), want, 8, kMaxRange / 32, 4);
+  // A head's piece of a token is 16 to 64 B and its scales 1 to 4, so that cache lines hold those of several: the
+  // heads of a split go to one XCD; splits are dealt out in turn, since lengths differ.
+  p.total = (uint32_t)(groups * p.splits);
+  p.unit = (uint32_t)p.KVH;
+  p.by_unit = make_fastdiv(p.unit);
+  p.grid = (uint32_t)(ceil_div(groups * p.splits, 8 * (int64_t)p.KVH) * 8 * p.KVH);
+}
+
 template <class T, int DP>
 static void launch_mx(const MxArgs& p, hipStream_t s) {
   if (few_rows_fwd(p))
@@ -467,10 +750,19 @@ static void launch_mx(const MxArgs& p, hipStream_t s) {
 
 template <class T>
 static int run_mx(const MxArgs& p, hipStream_t s) {
-  switch (dim_pad(p.D)) {
-    case 32: launch_mx<T, 32>(p, s); break;
-    case 64: launch_mx<T, 64>(p, s); break;
-    default: launch_mx<T, 128>(p, s); break;
+  if (token_rows(p)) {
+    switch (p.D) {
+      case 32: xattn_mxfp4_token_kernel<T, 32><<<p.grid, 256, 0, s>>>(p); break;
+      case 64: xattn_mxfp4_token_kernel<T, 64><<<p.grid, 256, 0, s>>>(p); break;
+      case 96: xattn_mxfp4_token_kernel<T, 96><<<p.grid, 256, 0, s>>>(p); break;
+      default: xattn_mxfp4_token_kernel<T, 128><<<p.grid, 256, 0, s>>>(p); break;
+    }
+  } else {
+    switch (dim_pad(p.D)) {
+      case 32: launch_mx<T, 32>(p, s); break;
+      case 64: launch_mx<T, 64>(p, s); break;
+      default: launch_mx<T, 128>(p, s); break;
+    }
   }
   const int st = launch_status();
   return st != DPA_OK || p.splits <= 1 ? st : join_splits<T>(p, s);
@@ -485,7 +777,7 @@ using namespace dpa::xattn;
 extern "C" int64_t dpa_cross_attention_mxfp4_workspace_bytes(const DpaCrossAttentionMxfp4* a) {
   if (!a || check_mx(*a) != DPA_OK) return 0;
   Args p = make_args(shape_of(*a));
-  plan_rows(p, few_rows_fwd(p));
+  plan_mx(p);
   return fwd_workspace(p);
 }
 
@@ -508,7 +800,7 @@ extern "C" int dpa_cross_attention_mxfp4(const DpaCrossAttentionMxfp4* a, void* 
   p.kds = stride_of(a->k_data_stride), p.kxs = stride_of(a->k_scale_stride);
   p.vds = stride_of(a->v_data_stride), p.vxs = stride_of(a->v_scale_stride);
   hipStream_t s = (hipStream_t)stream;
-  plan_rows(p, few_rows_fwd(p));
+  plan_mx(p);
   if (!grid_ok(p)) return DPA_ERR_SIZE;
   const int64_t need = fwd_workspace(p);
   if (need) {
