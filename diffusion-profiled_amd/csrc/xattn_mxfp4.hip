@@ -7,6 +7,7 @@
 
 #include "mxfp4.hpp"
 #include "xattn_join.hpp"
+#include "xattn_short.hpp"
 
 namespace dpa {
 namespace xattn {
@@ -698,6 +699,41 @@ __global__ __launch_bounds__(256, 3) void xattn_mxfp4_token_kernel(const MxArgs 
     *reinterpret_cast<uint32_t*>(p.out + orow * D + part * ND + i) = T::pack(acc[i] * il, acc[i + 1] * il);
 }
 
+// ---------------------------------------------------------------------------------------
+// Up to 128 keys: xattn_short.hpp over the values that a workgroup makes of them once. 128 x 1024 queries of 4 heads of
+// 64 dims over 77 keys 40 us by tiles of keys.
+// ---------------------------------------------------------------------------------------
+template <class T, int DP, int NB>
+__global__ __launch_bounds__(256, short_waves(DP)) void xattn_mxfp4_short_kernel(const MxArgs p) {
+  short_forward<T, DP, NB>(p, [&](int b, int g, uint32_t kl, uint32_t vl, float* bias, int tid, int wave, int lane)
+                               __attribute__((always_inline)) {
+    constexpr int kRow = DP / 32;  // blocks to a row
+    const int klen = keys_of(p, b);
+    const uint8_t* mb = p.kmask ? p.kmask + b * p.mask_b : nullptr;
+    auto visible = [&](int key) __attribute__((always_inline)) { return key < klen && (!mb || mb[key] != 0); };
+    const uint8_t *kd = p.kd + b * p.kds.b + g * p.kds.h, *kx = p.kx + b * p.kxs.b + g * p.kxs.h;
+    const uint8_t *vd = p.vd + b * p.vds.b + g * p.vds.h, *vx = p.vx + b * p.vxs.b + g * p.vxs.h;
+    constexpr int kAll = 2 * NB * 32 * kRow;
+    RawBlock raw[(kAll + 255) / 256];
+#pragma unroll
+    for (int i = 0; i < (kAll + 255) / 256; ++i) {
+      const int at = tid + 256 * i, in = at % (kAll / 2), key = in / kRow, blk = in % kRow;
+      const bool value = at >= kAll / 2, on = at < kAll && blk * 32 < p.D && visible(key);
+      raw[i] = raw_block((value ? vd + key * p.vds.l : kd + key * p.kds.l) + 16 * blk,
+                         (value ? vx + key * p.vxs.l : kx + key * p.kxs.l) + blk, on);
+    }
+#pragma unroll
+    for (int i = 0; i < (kAll + 255) / 256; ++i) {
+      const int at = tid + 256 * i, in = at % (kAll / 2);
+      if (at < kAll) put_block<T, DP>(at >= kAll / 2 ? vl : kl, in / kRow, in % kRow, raw[i]);
+    }
+    put_bias<NB>(bias, tid, visible);
+    wait_lgkmcnt0();
+    lds_barrier();
+    return active_blocks<NB>(bias, lane);
+  });
+}
+
 // ---- host ------------------------------------------------------------------------------
 static DpaCrossAttention shape_of(const DpaCrossAttentionMxfp4& a) {
   DpaCrossAttention c{};
@@ -722,7 +758,10 @@ static bool token_rows(const Args& p) { return p.rows <= 16; }
 
 static void plan_mx(Args& p) {
   if (!token_rows(p)) {
-    plan_rows(p, few_rows_fwd(p));
+    if (short_keys_fwd(p))
+      plan_short(p, false);
+    else
+      plan_rows(p, few_rows_fwd(p));
     return;
   }
   p.tiles = 1;
@@ -740,9 +779,17 @@ static void plan_mx(Args& p) {
   p.grid = (uint32_t)(ceil_div(groups * p.splits, 8 * (int64_t)p.KVH) * 8 * p.KVH);
 }
 
+// Whether the keys of a row are split (the short form's splits are of the rows)
+static bool has_parts(const Args& p) { return p.splits > 1 && (token_rows(p) || !short_keys_fwd(p)); }
+
 template <class T, int DP>
 static void launch_mx(const MxArgs& p, hipStream_t s) {
-  if (few_rows_fwd(p))
+  if (short_keys_fwd(p)) {
+    if (p.Lk <= 96)
+      xattn_mxfp4_short_kernel<T, DP, 3><<<p.grid, 256, 0, s>>>(p);
+    else
+      xattn_mxfp4_short_kernel<T, DP, 4><<<p.grid, 256, 0, s>>>(p);
+  } else if (few_rows_fwd(p))
     xattn_mxfp4_few_kernel<T, DP><<<p.grid, 256, 0, s>>>(p);
   else
     xattn_mxfp4_fwd_kernel<T, DP><<<p.grid, 256, 0, s>>>(p);
@@ -765,7 +812,7 @@ static int run_mx(const MxArgs& p, hipStream_t s) {
     }
   }
   const int st = launch_status();
-  return st != DPA_OK || p.splits <= 1 ? st : join_splits<T>(p, s);
+  return st != DPA_OK || !has_parts(p) ? st : join_splits<T>(p, s);
 }
 
 }  // namespace xattn
@@ -778,7 +825,7 @@ extern "C" int64_t dpa_cross_attention_mxfp4_workspace_bytes(const DpaCrossAtten
   if (!a || check_mx(*a) != DPA_OK) return 0;
   Args p = make_args(shape_of(*a));
   plan_mx(p);
-  return fwd_workspace(p);
+  return has_parts(p) ? fwd_workspace(p) : 0;
 }
 
 extern "C" int dpa_cross_attention_mxfp4(const DpaCrossAttentionMxfp4* a, void* workspace, int64_t workspace_bytes,
@@ -802,7 +849,7 @@ extern "C" int dpa_cross_attention_mxfp4(const DpaCrossAttentionMxfp4* a, void* 
   hipStream_t s = (hipStream_t)stream;
   plan_mx(p);
   if (!grid_ok(p)) return DPA_ERR_SIZE;
-  const int64_t need = fwd_workspace(p);
+  const int64_t need = has_parts(p) ? fwd_workspace(p) : 0;
   if (need) {
     if (!workspace || workspace_bytes < need) return DPA_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return DPA_ERR_ALIGN;
