@@ -131,11 +131,11 @@ __global__ __launch_bounds__(256) void mxfp4_rows_kernel(const RowArgs p) {
 
 // ---------------------------------------------------------------------------------------
 // Both operands of a matrix from one read of it: its rows, and its columns (blocks down the columns, the
-// matrix transposed). Eight waves take 64 rows of 256 columns at a time, `iters` times down the matrix, the next
-// 64 rows' loads out before these are worked on. A thread holds 4 columns of 8 rows: a row's block is the 8
-// lanes beside each other, a column's the 4 waves below each other, which trade their largest magnitudes
-// through LDS. The columns' codes gather in LDS and leave at the end, 32 iters B to a column (a whole
-// line of 128 B with 4).
+// matrix transposed). Eight waves take 64 rows of 256 columns; a thread holds 4 columns of 8 rows: a row's block is
+// the 8 lanes beside each other, a column's the 4 waves below each other, which trade their largest magnitudes
+// through LDS. The columns' codes turn in LDS and leave as 32 B of a column; the four tiles of a line of 128 B
+// go to one XCD, whose L2 joins them. (Two or four tiles to a workgroup, the next one's loads ahead, is slower,
+// from cold caches: 8192 x 4096 of bf16 37.7 and 36.2 us against 34.2, 768 x 256 of fp32 10.8 and 16.8 against 7.6.)
 // ---------------------------------------------------------------------------------------
 struct BothArgs {
   const void* x;
@@ -143,6 +143,7 @@ struct BothArgs {
   const uint64_t* seed;
   int64_t rows, cols, ld;
   int col_tiles;
+  uint32_t lines;  // of 256 rows x 256 columns
 };
 
 // Four neighbours of a row
@@ -160,20 +161,35 @@ struct Quad<DPA_DTYPE_F32> {
   __device__ __forceinline__ float get(int i) const { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
 };
 
-template <int DT>
-__device__ __forceinline__ Quad<DT> quad_at(const void* x, int64_t at, int64_t left, bool wide) {
+// Columns c0 .. c0 + 3 of a row, zeros outside of the matrix: from inside it all the same, so that loads go out
+// together, without branches.
+template <int DT, bool kWide>
+__device__ __forceinline__ Quad<DT> quad_at(const BothArgs& p, int64_t row, int64_t c0) {
   Quad<DT> q;
-  if (wide && left >= 4) {
-    q.w = *reinterpret_cast<const decltype(q.w)*>(static_cast<const uint8_t*>(x) + at * Elem<DT>::size);
+  const int64_t at = min(row, p.rows - 1) * p.ld;
+  const bool in = row < p.rows;
+  if constexpr (kWide) {  // (cols is a multiple of 4)
+    const bool on = in && c0 < p.cols;
+    q.w = *reinterpret_cast<const decltype(q.w)*>(static_cast<const uint8_t*>(p.x) + (at + (c0 < p.cols ? c0 : 0)) * Elem<DT>::size);
+    if (!on) q.w = decltype(q.w){};
     return q;
   }
   if constexpr (DT == DPA_DTYPE_F32) {
-    const float* s = static_cast<const float*>(x) + at;
-    q.w = float4{left > 0 ? s[0] : 0.f, left > 1 ? s[1] : 0.f, left > 2 ? s[2] : 0.f, left > 3 ? s[3] : 0.f};
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = static_cast<const float*>(p.x)[at + min(c0 + i, p.cols - 1)];
+      if (!in || c0 + i >= p.cols) v[i] = 0.f;
+    }
+    q.w = float4{v[0], v[1], v[2], v[3]};
   } else {
-    const uint16_t* s = static_cast<const uint16_t*>(x) + at;
-    const uint32_t a = left > 0 ? s[0] : 0, b = left > 1 ? s[1] : 0, c = left > 2 ? s[2] : 0, d = left > 3 ? s[3] : 0;
-    q.w = uint2{a | b << 16, c | d << 16};
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = static_cast<const uint16_t*>(p.x)[at + min(c0 + i, p.cols - 1)];
+      if (!in || c0 + i >= p.cols) v[i] = 0u;
+    }
+    q.w = uint2{v[0] | v[1] << 16, v[2] | v[3] << 16};
   }
   return q;
 }
@@ -238,131 +254,112 @@ __device__ __forceinline__ uint32_t down_pair(const Quad<DT>& a, const Quad<DT>&
   return perm_b32(j < 2 ? b.w.x : b.w.y, j < 2 ? a.w.x : a.w.y, j & 1 ? 0x07060302u : 0x05040100u);
 }
 
-template <int DT, int kIters, bool SR>
-__global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p, bool wide) {
-  constexpr int kLine = 32 * kIters;   // bytes of a column
-  constexpr int kPitch = kLine + 16;   // (lanes then lie in different places of the banks)
+template <int DT, bool kWide, bool SR>
+__global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p) {
+  constexpr int kPitch = 36;  // bytes of a column in LDS (lanes then lie in different banks)
   constexpr int kW = ColMax<DT>::kWords;
   __shared__ __attribute__((aligned(16))) uint8_t out[256 * kPitch];
-  __shared__ __attribute__((aligned(16))) uint32_t tops[2][8][64 * kW];
-  __shared__ __attribute__((aligned(8))) uint8_t bytes[2 * kIters][256];
+  __shared__ __attribute__((aligned(16))) uint32_t tops[8][64 * kW];
+  __shared__ __attribute__((aligned(8))) uint8_t bytes[2][256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = wave >> 2, sub = wave & 3;
-  const int64_t tr = blockIdx.x / (uint32_t)p.col_tiles, tc = blockIdx.x - tr * p.col_tiles;
-  const int64_t c0 = tc * 256 + 4 * lane, left = p.cols - c0;
-  const int64_t first = tr * 64 * kIters + 8 * wave;  // of this wave's rows in the first iteration
+  // workgroups i, i + 8, i + 16, i + 24 of 32 (on one XCD): the tiles below each other of a line
+  const uint32_t line = (blockIdx.x >> 5) * 8 + (blockIdx.x & 7);
+  if (line >= p.lines) return;
+  const int64_t tl = line / (uint32_t)p.col_tiles, tc = line - tl * p.col_tiles, tr = 4 * tl + ((blockIdx.x >> 3) & 3);
+  const int64_t c0 = tc * 256 + 4 * lane;
+  const int64_t r0 = tr * 64 + 8 * wave;
   const int64_t pitch = pitch_of(p.cols);
-  Quad<DT> x[8], next[8];
-  auto load = [&](Quad<DT>(&q)[8], int it) __attribute__((always_inline)) {
-    const int64_t r0 = first + 64 * it;
+  Quad<DT> x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      q[i] = quad_at<DT>(p.x, (r0 + i) * p.ld + c0, r0 + i < p.rows ? left : 0, wide);
-  };
-  load(x, 0);
-  uint64_t z = 0, z_row = 0;
+  for (int i = 0; i < 8; ++i) x[i] = quad_at<DT, kWide>(p, r0 + i, c0);
+  uint32_t rnd[SR ? 8 : 1][4];
   if constexpr (SR) {
-    z_row = (uint64_t)((p.cols + kBlock - 1) / kBlock) * (kBlock / 4) * kDropGolden;
-    z = *p.seed + (uint64_t)first * z_row + (uint64_t)(c0 / 4) * kDropGolden;
+    const uint64_t z_row = (uint64_t)((p.cols + kBlock - 1) / kBlock) * (kBlock / 4) * kDropGolden;
+    const uint64_t z = *p.seed + (uint64_t)r0 * z_row + (uint64_t)(c0 / 4) * kDropGolden;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bits4(rnd[i], mix(z + (uint64_t)i * z_row));
   }
+  ColMax<DT> top;
 #pragma unroll
-  for (int it = 0; it < kIters; ++it) {
-    const int64_t r0 = first + 64 * it;
-    if (it + 1 < kIters) load(next, it + 1);
-    ColMax<DT> top;
+  for (int i = 0; i < 8; ++i) top.take(x[i]);
+  top.put(&tops[wave][lane * kW]);
+  // rows
+  if (p.row_data) {
+    uint32_t mine = 0;  // lane 8 b + i: the scale of row i, block b
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top.take(x[i]);
-    top.put(&tops[it & 1][wave][lane * kW]);
-    uint32_t rnd[SR ? 8 : 1][4];
-    if constexpr (SR) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) bits4(rnd[i], mix(z + (uint64_t)i * z_row));
-      z += 64 * z_row;
-    }
-    // rows
-    if (p.row_data) {
-      uint32_t mine = 0;  // lane 8 b + i: the scale of row i, block b
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint32_t m = quad_max(row_max<DT>(x[i]));
-        m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, false));  // 7 - lane of 8
-        const uint32_t byte = scale_byte<SR>(m);
-        const float scale = scale_bits(byte);
-        mine = (lane & 7) == i ? byte : mine;
-        uint32_t r;
-        if constexpr (SR) {
-          r = low_bytes(two_codes(encode_sr(x[i].get(0), rnd[i][0], scale), encode_sr(x[i].get(1), rnd[i][1], scale)),
-                        two_codes(encode_sr(x[i].get(2), rnd[i][2], scale), encode_sr(x[i].get(3), rnd[i][3], scale)));
-        } else if constexpr (DT == DPA_DTYPE_F32) {
-          r = encode_pair<1>(encode_pair<0>(0u, x[i].w.x, x[i].w.y, scale), x[i].w.z, x[i].w.w, scale);
-        } else {
-          r = encode_pair<DT, 1>(encode_pair<DT, 0>(0u, x[i].w.x, scale), x[i].w.y, scale);
-        }
-        if (r0 + i < p.rows) *reinterpret_cast<uint16_t*>(p.row_data + (r0 + i) * pitch + c0 / 2) = (uint16_t)r;
-      }
-      const int64_t row = r0 + (lane & 7);
-      const int b = (int)(tc * 8) + (lane >> 3);
-      if (row < p.rows) p.row_scales[((int64_t)(b >> 4) * p.rows + row) * 16 + scale_at(b & 15)] = (uint8_t)mine;
-    }
-    wait_lgkmcnt0();
-    lds_barrier();
-    // columns: word `sub` of block 2 it + half
-#pragma unroll
-    for (int w = 0; w < 4; ++w) top.join(&tops[it & 1][4 * half + w][lane * kW]);
-    uint32_t r[4], some = 0;
-    float scale[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t byte = scale_byte<SR>(top.get(j));
-      some |= byte << (8 * j);
-      scale[j] = scale_bits(byte);
-    }
-    if (sub == 0) *reinterpret_cast<uint32_t*>(&bytes[2 * it + half][4 * lane]) = some;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int i = 0; i < 8; ++i) {
+      uint32_t m = quad_max(row_max<DT>(x[i]));
+      m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, false));  // 7 - lane of 8
+      const uint32_t byte = scale_byte<SR>(m);
+      const float scale = scale_bits(byte);
+      mine = (lane & 7) == i ? byte : mine;
+      uint32_t r;
       if constexpr (SR) {
-        uint32_t c[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          c[i] = two_codes(encode_sr(x[2 * i].get(j), rnd[2 * i][j], scale[j]),
-                           encode_sr(x[2 * i + 1].get(j), rnd[2 * i + 1][j], scale[j]));
-        r[j] = low_bytes(c[0], c[1], c[2], c[3]);
+        r = low_bytes(two_codes(encode_sr(x[i].get(0), rnd[i][0], scale), encode_sr(x[i].get(1), rnd[i][1], scale)),
+                      two_codes(encode_sr(x[i].get(2), rnd[i][2], scale), encode_sr(x[i].get(3), rnd[i][3], scale)));
       } else if constexpr (DT == DPA_DTYPE_F32) {
-        r[j] = encode_pair<0>(0u, x[0].get(j), x[1].get(j), scale[j]);
-        r[j] = encode_pair<1>(r[j], x[2].get(j), x[3].get(j), scale[j]);
-        r[j] = encode_pair<2>(r[j], x[4].get(j), x[5].get(j), scale[j]);
-        r[j] = encode_pair<3>(r[j], x[6].get(j), x[7].get(j), scale[j]);
+        r = encode_pair<1>(encode_pair<0>(0u, x[i].w.x, x[i].w.y, scale), x[i].w.z, x[i].w.w, scale);
       } else {
-        r[j] = encode_pair<DT, 0>(0u, down_pair<DT>(x[0], x[1], j), scale[j]);
-        r[j] = encode_pair<DT, 1>(r[j], down_pair<DT>(x[2], x[3], j), scale[j]);
-        r[j] = encode_pair<DT, 2>(r[j], down_pair<DT>(x[4], x[5], j), scale[j]);
-        r[j] = encode_pair<DT, 3>(r[j], down_pair<DT>(x[6], x[7], j), scale[j]);
+        r = encode_pair<DT, 1>(encode_pair<DT, 0>(0u, x[i].w.x, scale), x[i].w.y, scale);
       }
-      *reinterpret_cast<uint32_t*>(out + (j * 64 + lane) * kPitch + (2 * it + half) * 16 + 4 * sub) = r[j];
+      if (r0 + i < p.rows) *reinterpret_cast<uint16_t*>(p.row_data + (r0 + i) * pitch + c0 / 2) = (uint16_t)r;
     }
-    if (it + 1 < kIters)
+    const int64_t row = r0 + (lane & 7);
+    const int b = (int)(tc * 8) + (lane >> 3);
+    if (row < p.rows) p.row_scales[((int64_t)(b >> 4) * p.rows + row) * 16 + scale_at(b & 15)] = (uint8_t)mine;
+  }
+  wait_lgkmcnt0();
+  lds_barrier();
+  // columns: word `sub` of block `half`
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = next[i];
+  for (int w = 0; w < 4; ++w) top.join(&tops[4 * half + w][lane * kW]);
+  uint32_t some = 0;
+  float scale[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t byte = scale_byte<SR>(top.get(j));
+    some |= byte << (8 * j);
+    scale[j] = scale_bits(byte);
+  }
+  if (sub == 0) *reinterpret_cast<uint32_t*>(&bytes[half][4 * lane]) = some;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t r;
+    if constexpr (SR) {
+      uint32_t c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        c[i] = two_codes(encode_sr(x[2 * i].get(j), rnd[2 * i][j], scale[j]),
+                         encode_sr(x[2 * i + 1].get(j), rnd[2 * i + 1][j], scale[j]));
+      r = low_bytes(c[0], c[1], c[2], c[3]);
+    } else if constexpr (DT == DPA_DTYPE_F32) {
+      r = encode_pair<0>(0u, x[0].get(j), x[1].get(j), scale[j]);
+      r = encode_pair<1>(r, x[2].get(j), x[3].get(j), scale[j]);
+      r = encode_pair<2>(r, x[4].get(j), x[5].get(j), scale[j]);
+      r = encode_pair<3>(r, x[6].get(j), x[7].get(j), scale[j]);
+    } else {
+      r = encode_pair<DT, 0>(0u, down_pair<DT>(x[0], x[1], j), scale[j]);
+      r = encode_pair<DT, 1>(r, down_pair<DT>(x[2], x[3], j), scale[j]);
+      r = encode_pair<DT, 2>(r, down_pair<DT>(x[4], x[5], j), scale[j]);
+      r = encode_pair<DT, 3>(r, down_pair<DT>(x[6], x[7], j), scale[j]);
+    }
+    *reinterpret_cast<uint32_t*>(out + (j * 64 + lane) * kPitch + half * 16 + 4 * sub) = r;
   }
   __syncthreads();
   const int64_t col_pitch = pitch_of(p.rows);
-#pragma unroll
-  for (int it = 0; it < kIters; ++it) {
-    const int id = it * 512 + threadIdx.x, line = id / (2 * kIters), chunk = id % (2 * kIters);
-    const int64_t col = tc * 256 + 4 * (line & 63) + (line >> 6);
+  {
+    const int at = threadIdx.x >> 1, chunk = threadIdx.x & 1;
+    const int64_t col = tc * 256 + 4 * (at & 63) + (at >> 6);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(out + at * kPitch + chunk * 16);
     if (col < p.cols)
-      *reinterpret_cast<uint4*>(p.col_data + col * col_pitch + tr * kLine + chunk * 16) =
-          *reinterpret_cast<const uint4*>(out + line * kPitch + chunk * 16);
+      *reinterpret_cast<uint4*>(p.col_data + col * col_pitch + tr * 32 + chunk * 16) = uint4{w[0], w[1], w[2], w[3]};
   }
-  // pairs of blocks 2 q, 2 q + 1 lie together in a group of scales
-#pragma unroll
-  for (int it = 0; it < (kIters + 1) / 2; ++it) {
-    const int id = it * 512 + threadIdx.x, pair = id >> 8;
-    const int64_t col = tc * 256 + (id & 255), block = tr * 2 * kIters + 2 * pair;
-    if (pair < kIters && col < p.cols)
-      *reinterpret_cast<uint16_t*>(p.col_scales + ((block >> 4) * p.cols + col) * 16 + scale_at((int)(block & 15))) =
-          (uint16_t)(bytes[2 * pair][id & 255] | bytes[2 * pair + 1][id & 255] << 8);
-  }
+  // the two blocks' scales of a column lie together
+  const int64_t col = tc * 256 + threadIdx.x, block = tr * 2;
+  if (threadIdx.x < 256 && col < p.cols)
+    *reinterpret_cast<uint16_t*>(p.col_scales + ((block >> 4) * p.cols + col) * 16 + scale_at((int)(block & 15))) =
+        (uint16_t)(bytes[0][threadIdx.x] | bytes[1][threadIdx.x] << 8);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -422,23 +419,20 @@ static int run_rows(const RowArgs& p, bool operand, bool wide, hipStream_t s) {
   return launch_status();
 }
 
-template <int DT, int kIters>
-static int run_both(const BothArgs& p, bool wide, hipStream_t s) {
-  const unsigned grid = (unsigned)(ceil_div(p.rows, 256) * (4 / kIters) * p.col_tiles);
+template <int DT, bool kWide>
+static int run_both(const BothArgs& p, hipStream_t s) {
+  const unsigned grid = (unsigned)(ceil_div(p.lines, 8) * 32);
   if (p.seed)
-    mxfp4_both_kernel<DT, kIters, true><<<grid, 512, 0, s>>>(p, wide);
+    mxfp4_both_kernel<DT, kWide, true><<<grid, 512, 0, s>>>(p);
   else
-    mxfp4_both_kernel<DT, kIters, false><<<grid, 512, 0, s>>>(p, wide);
+    mxfp4_both_kernel<DT, kWide, false><<<grid, 512, 0, s>>>(p);
   return launch_status();
 }
 
 template <int DT>
 static int run_operands(const RowArgs& r, const BothArgs& b, bool wide, hipStream_t s) {
-  if (!b.col_data) return r.seed ? run_rows<DT, true>(r, true, wide, s) : run_rows<DT, false>(r, true, wide, s);
-  // rows to a workgroup: whole lines of the columns where there are enough workgroups
-  const int64_t tiles = ceil_div(b.rows, 256) * b.col_tiles;
-  if (tiles >= 2 * num_cus()) return run_both<DT, 4>(b, wide, s);
-  return run_both<DT, 1>(b, wide, s);
+  if (b.col_data) return wide ? run_both<DT, true>(b, s) : run_both<DT, false>(b, s);
+  return r.seed ? run_rows<DT, true>(r, true, wide, s) : run_rows<DT, false>(r, true, wide, s);
 }
 
 // rows of x to a workgroup of column_sum_kernel
@@ -515,9 +509,10 @@ extern "C" int dpa_mxfp4_operands(const void* x, int dtype, int64_t rows, int64_
   b.col_data = (uint8_t*)by_cols, b.col_scales = b.col_data + operand_data_bytes(cols, rows);
   b.rows = rows, b.cols = cols, b.ld = row_stride;
   b.col_tiles = (int)ceil_div(cols, 256);
+  b.lines = (uint32_t)(ceil_div(rows, 256) * b.col_tiles);
   // whole aligned vectors: 16 B of 8 elements (8 B of 4) of a 16-bit type, 16 B of 4 of fp32
   const int vec = by_cols || dtype == DPA_DTYPE_F32 ? 4 : 8;
-  const bool wide = row_stride % vec == 0 && aligned(x, vec * size_of(dtype));
+  const bool wide = row_stride % vec == 0 && (!by_cols || cols % 4 == 0) && aligned(x, vec * size_of(dtype));
   hipStream_t s = (hipStream_t)stream;
   if (dtype == DPA_DTYPE_BF16) return run_operands<DPA_DTYPE_BF16>(r, b, wide, s);
   if (dtype == DPA_DTYPE_F16) return run_operands<DPA_DTYPE_F16>(r, b, wide, s);
