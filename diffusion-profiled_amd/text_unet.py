@@ -17,6 +17,7 @@ import torch.nn as nn
 from . import conditioning as C
 from .layer_norm import layer_norm_bf16
 from .layer_norm import supported as ln_supported
+from .mxfp4 import BLOCK, MXFP4, LinearMXFP4, cross_attention_mxfp4, quantize_mxfp4
 from .unet import UNet, UNetConfig
 
 
@@ -26,6 +27,7 @@ class TextConfig:
     width: int
     p_drop: float = 0.1         # of the embeddings and of the blocks' outputs
     padding_idx: int = 0        # takes no part in attention and learns nothing
+    mxfp4: bool = False         # the blocks' projections multiply 4-bit operands (``mxfp4.LinearMXFP4``)
 
 
 class TextEmbedding(nn.Module):
@@ -54,9 +56,10 @@ class CrossAttentionBlock(nn.Module):
             raise ValueError(f"cross attention block: {channels} channels over {heads} heads")
         self.heads, self.p_drop = heads, text.p_drop
         self.norm = nn.LayerNorm(channels)
-        self.q = nn.Linear(channels, channels, bias=False)
-        self.kv = nn.Linear(text.width, 2 * channels, bias=False)
-        self.out = nn.Linear(channels, channels, bias=False)
+        linear = LinearMXFP4 if text.mxfp4 else nn.Linear
+        self.q = linear(channels, channels, bias=False)
+        self.kv = linear(text.width, 2 * channels, bias=False)
+        self.out = linear(channels, channels, bias=False)
         nn.init.zeros_(self.out.weight)
 
     def project(self, states: torch.Tensor) -> torch.Tensor:
@@ -65,12 +68,12 @@ class CrossAttentionBlock(nn.Module):
         b, l, _ = states.shape
         return self.kv(states).view(b, l, 2, self.heads, -1)
 
-    def forward(self, x: torch.Tensor, kv: torch.Tensor, key_mask: torch.Tensor | None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, kv: torch.Tensor | MXFP4, key_mask: torch.Tensor | None) -> torch.Tensor:
         b, c, h, w = x.shape
         seq = x.permute(0, 2, 3, 1).reshape(b, h * w, c)
         y = layer_norm_bf16(seq, self.norm) if ln_supported(c) else self.norm(seq)
         q = self.q(y).view(b, h * w, self.heads, -1)
-        o = C.cross_attention_kv(q, kv, key_mask=key_mask)
+        o = (cross_attention_mxfp4 if isinstance(kv, MXFP4) else C.cross_attention_kv)(q, kv, key_mask=key_mask)
         o = self.out(o.view(b, h * w, c)).to(seq.dtype)
         y = C.dropout(o, self.p_drop, training=self.training, residual=seq)
         return y.reshape(b, h, w, c).permute(0, 3, 1, 2)
@@ -103,6 +106,8 @@ class TextUNet(UNet):
         n = super()._dropouts()
         if self.training and self.text.text.p_drop > 0.0:
             n += 1 + len(self.cross)
+        if self.text.text.mxfp4 and torch.is_grad_enabled():       # stochastic rounding of gradients
+            n += sum(isinstance(m, LinearMXFP4) for m in self.cross.modules())
         return n
 
     def _after_stage(self, name: str, act: torch.Tensor) -> torch.Tensor:
@@ -114,17 +119,31 @@ class TextUNet(UNet):
     _seen: torch.Tensor | None = None
 
     @torch.no_grad()
-    def keep_prompt(self, tokens: torch.Tensor | None) -> None:
+    def keep_prompt(self, tokens: torch.Tensor | None, bits: int = 16) -> None:
         """For sampling: every block's keys and values of these prompts, formed once (without dropout) and
         used by the calls without a prompt of their own until the next ``keep_prompt`` (None: no longer).
         They are of the weights as they are now, and carry no gradient: training steps (calls in training
-        mode that record one) take ``prompt``."""
+        mode that record one) take ``prompt``. bits=4: in MXFP4 (heads of a multiple of 32), for calls that
+        record no gradient."""
+        if bits not in (16, 4):
+            raise ValueError(f"keep_prompt: keys and values in 16 or 4 bits, got {bits}")
+        if bits == 4 and any(b.norm.weight.numel() // b.heads % BLOCK for b in self.cross.values()):
+            raise ValueError(f"keep_prompt: 4 bits need heads of a multiple of {BLOCK}")
         self._kept = None
         if tokens is not None:
             with torch.autocast("cuda", dtype=torch.bfloat16):
                 states = self.text(tokens, dropout=False)
-                self._kept = ({name: block.project(states) for name, block in self.cross.items()},
-                              tokens != self.text.text.padding_idx)
+                kept = {name: block.project(states) for name, block in self.cross.items()}
+                if bits == 4:
+                    kept = {name: quantize_mxfp4(kv) for name, kv in kept.items()}
+                self._kept = kept, tokens != self.text.text.padding_idx
+
+    def keep_weights(self, keep: bool = True) -> None:
+        """For sampling with ``TextConfig.mxfp4``: the blocks' weights as they are now, laid out once for the calls
+        that record no gradient, until ``keep_weights(False)``."""
+        for m in self.cross.modules():
+            if isinstance(m, LinearMXFP4):
+                m.keep_weight(keep)
 
     def _forward(self, x: torch.Tensor, t: torch.Tensor) -> torch.Tensor:
         tokens = self._tokens if self._tokens is not None else self.prompt

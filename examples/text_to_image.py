@@ -61,6 +61,7 @@ def main(argv: list[str] | None = None) -> list[float]:
     ap.add_argument("--batch", type=int, default=64)
     ap.add_argument("--size", type=int, default=16)
     ap.add_argument("--max-t", type=int, default=200)
+    ap.add_argument("--mxfp4", action="store_true", help="4-bit projections, keys and values of the text")
     ap.add_argument("--prompts", nargs="*", default=["red square", "blue disc"])
     args = ap.parse_args(argv)
     trainer = importlib.import_module(f"{PKG}.trainer")
@@ -69,7 +70,7 @@ def main(argv: list[str] | None = None) -> list[float]:
 
     config = unet.UNetConfig(in_channels=3, base_hidden=64, scales=[1, 2], n_heads=2, p_drop=0.1,
                              attn_resolutions=[args.size], in_resolution=args.size, n_resblocks=2)
-    text = text_unet.TextConfig(vocab=len(WORDS), width=64)
+    text = text_unet.TextConfig(vocab=len(WORDS), width=64, mxfp4=args.mxfp4)
     state = trainer.TrainState(config, args.batch, lr=1e-3, max_t=args.max_t, text=text,
                                prompt_length=LENGTH, ema_beta=0.99)
     g = torch.Generator().manual_seed(0)
@@ -88,9 +89,11 @@ def main(argv: list[str] | None = None) -> list[float]:
             state.loss_acc.zero_()
             print(f"step {i + 1}: mean loss {losses[-1]:.4f}", flush=True)
     model = state.ema_ddpm.model.model
-    model.keep_prompt(tokenize(args.prompts).cuda())
+    model.keep_prompt(tokenize(args.prompts).cuda(), bits=4 if args.mxfp4 else 16)
+    model.keep_weights()
     samples = state.ema_ddpm.generate_samples(len(args.prompts))
     model.keep_prompt(None)
+    model.keep_weights(False)
     for prompt, image in zip(args.prompts, samples):
         spread = image.flatten(1).amax(1) - image.flatten(1).amin(1)
         print(f"{prompt!r}: channel means {image.mean((1, 2)).tolist()}, spreads {spread.tolist()}")

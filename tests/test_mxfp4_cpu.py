@@ -144,3 +144,29 @@ def test_attention_entry_refuses_before_launch(lib, M):
     assert lib.dpa_cross_attention_mxfp4_workspace_bytes(many) > 0
     assert f(many, None, 0, None) == -5
     assert f(desc(b=0), None, 0, None) == 0
+
+
+def test_text_model_in_four_bits_on_the_cpu(tmp_path):
+    """Its parameters are those of the 16-bit one, its file says which it is, and older files still load."""
+    T, U, X = (dpa_mod(n) for n in ("trainer", "unet", "text_unet"))
+    config = U.UNetConfig(in_channels=3, base_hidden=64, scales=[1, 2], n_heads=2, p_drop=0.1, attn_resolutions=[16],
+                          in_resolution=16, n_resblocks=2)
+    m = X.TextUNet(config, X.TextConfig(vocab=11, width=24, mxfp4=True))
+    plain = X.TextUNet(config, X.TextConfig(vocab=11, width=24))
+    plain.load_state_dict(m.state_dict())
+    path = tmp_path / "four.pt"
+    T.save_checkpoint(m, 2, config.as_dict(), str(path))
+    assert T.load_checkpoint(path)[0].text.text.mxfp4
+    old = torch.load(path, weights_only=True)
+    del old["text"]["mxfp4"]
+    torch.save(old, path)
+    back = T.load_checkpoint(path)[0]
+    assert not back.text.text.mxfp4 and type(back.cross["mid"].q) is torch.nn.Linear
+    tokens = torch.zeros(1, 4, dtype=torch.int64)
+    with pytest.raises(ValueError, match="16 or 4 bits"):
+        m.keep_prompt(tokens, bits=8)
+    odd = X.TextUNet(U.UNetConfig(in_channels=3, base_hidden=64, scales=[1, 2], n_heads=4, p_drop=0.1,
+                                  attn_resolutions=[16], in_resolution=16, n_resblocks=2),
+                     X.TextConfig(vocab=11, width=24))
+    with pytest.raises(ValueError, match="multiple of 32"):
+        odd.keep_prompt(tokens, bits=4)
