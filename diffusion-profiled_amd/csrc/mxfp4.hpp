@@ -11,11 +11,11 @@
 // Two arrangements:
 //   dense    a tensor [..., C], C a multiple of 32: its bytes in order, the first of two elements in the low
 //            half, and its scale bytes in order.
-//   operand  a matrix [rows][cols] as the product reads it, whose contraction runs over cols: rows of
-//            ceil(cols / 256) * 128 B, zeros behind cols; behind them scales [ceil(cols / 512)][rows][16],
-//            block 8 s + 2 q + t of a row's 16 at byte 4 q + 2 s + t. Lane (row, q) of a matrix instruction then
-//            has the scales of its four 32-element pieces of 512 columns in one word, and takes pieces
-//            2 q, 2 q + 1 of each 256 (the order of a contraction is free as long as both operands keep it).
+//   operand  a matrix [rows][cols] as the product reads it, whose contraction runs over cols: panels of 128
+//            columns, 2 ceil(cols / 256) of them, zeros behind cols, 64 B of a row after the other (what the product
+//            takes at a time is then whole lines: 64 B of rows further apart cost its loads 1.7 times the time);
+//            behind them scales [ceil(cols / 512)][rows][16], block 4 t + q of a row's 16 at byte 4 q + t. Lane (row, q) of a matrix instruction over columns
+//            128 t .. 128 t + 127 then has the scales of its four blocks of 512 columns in one word.
 #pragma once
 #include "dpa_common.hpp"
 
@@ -29,9 +29,10 @@ constexpr int kGroup = 512;  // columns of a group of scales
 __host__ __device__ inline int64_t pitch_of(int64_t cols) { return (cols + kStep - 1) / kStep * (kStep / 2); }
 __host__ __device__ inline int64_t groups_of(int64_t cols) { return (cols + kGroup - 1) / kGroup; }
 
-// (Rows come to the product eight at a time, scales of up to 256: the buffer holds as many behind the last,
+// (Rows come to the product 16 at a time, scales of up to 256: the buffer holds as many behind the last,
 // which hold anything.)
-__host__ __device__ inline int64_t padded_rows(int64_t rows) { return (rows + 7) & ~7ll; }
+__host__ __device__ inline int64_t padded_rows(int64_t rows) { return (rows + 15) & ~15ll; }
+__host__ __device__ inline int64_t panel_of(int64_t rows) { return padded_rows(rows) * 64; }
 inline int64_t operand_data_bytes(int64_t rows, int64_t cols) { return padded_rows(rows) * pitch_of(cols); }
 inline int64_t operand_bytes(int64_t rows, int64_t cols) {
   return operand_data_bytes(rows, cols) + (groups_of(cols) * rows + 256) * 16;
@@ -40,11 +41,11 @@ inline int64_t operand_bytes(int64_t rows, int64_t cols) {
 // Sizes of a matrix that the kernels take: 32-bit numbers of 8-element groups and workgroups, and of scales
 inline bool matrix_ok(int64_t rows, int64_t cols) {
   if (rows < 0 || cols <= 0 || rows >= (1 << 26) || cols >= (1 << 26)) return false;
-  return rows * (pitch_of(cols) / 4) < (1ll << 31) && cols * (pitch_of(rows) / 4) < (1ll << 31);
+  return padded_rows(rows) * (groups_of(cols) * 64) < (1ll << 31) && padded_rows(cols) * (groups_of(rows) * 64) < (1ll << 31);
 }
 
 // place of block b of a row within the 16 B of its group
-__host__ __device__ inline int scale_at(int b) { return 4 * ((b >> 1) & 3) + 2 * ((b >> 3) & 1) + (b & 1); }
+__host__ __device__ inline int scale_at(int b) { return 4 * (b & 3) + (b >> 2); }
 
 // scale byte from the largest magnitude's bits
 template <bool SR>

@@ -12,7 +12,7 @@ struct GemmArgs {
   const float* bias;
   void* y;
   float* part;  // [splits][M][N] where the contraction is split
-  int64_t pitch;
+  int64_t panel_a, panel_b;  // bytes
   const void* x;  // a before its rounding, where the kernel does that, rows ld elements apart
   int64_t ld;
   int M, N, K;
@@ -21,31 +21,17 @@ struct GemmArgs {
   int form;  // of the tiles
 };
 
-// v[0 .. 7] to columns n .. n + 7 of a row, by whole vectors
-template <int DT>
-__device__ __forceinline__ void store8(void* y, int64_t row, int n, int N, const float (&v)[8]) {
-  const int64_t at = row * N + n;
-  if constexpr (DT == DPA_DTYPE_F32) {
-    float4* o = reinterpret_cast<float4*>(static_cast<float*>(y) + at);
-    o[0] = float4{v[0], v[1], v[2], v[3]};
-    if (n + 4 < N) o[1] = float4{v[4], v[5], v[6], v[7]};
-  } else {
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + at) =
-        uint4{Elem<DT>::pack(v[0], v[1]), Elem<DT>::pack(v[2], v[3]), Elem<DT>::pack(v[4], v[5]), Elem<DT>::pack(v[6], v[7])};
-  }
-}
-
 // ---------------------------------------------------------------------------------------
-// Tiles of WM x WN waves of 16 FM x 16 FN each, steps of 256 columns (128 B of a row) through LDS by
-// DMA, NS of them on their way, and their scales by the same way. (The scales straight to registers, a word to a
-// lane and fragment for every second step: 4096 x 8192 of 8192 156 us against 128.) Workgroups stay and take tile
-// after tile, the next one's first steps out before this one's stores. b's rows are the A operand (rows of D), in the order that gives a lane 8 columns of y in
-// a row and four lanes 64 B: row r of fragment i is row 32 (i / 2) + 8 (r / 4) + 4 (i % 2) + r % 4 of the
-// wave's. The 16-B piece c of a row lies at c ^ swz(row): the 16 lanes that LDS serves together (rows 0-3 and 12-15 at one piece,
-// 4-11 at the piece two further) then lie in 16 different places of the banks.
+// Tiles of WM x WN waves of 16 FM x 16 FN each, a panel of 128 columns (64 B of a row) at a time through a ring of NH buffers
+// in LDS by DMA, and their scales by the same way. Workgroups stay and take tile after tile, the next one's first
+// transfers out before this one's stores. b's rows are the A operand (rows of D), in the order that gives a lane 8
+// columns of y in a row and four lanes 64 B: row r of fragment i is row 32 (i / 2) + 8 (r / 4) + 4 (i % 2) + r % 4 of
+// the wave's. The 16-B piece c of a row lies at c ^ turned(its r / 4): the 16 lanes that LDS serves together (rows
+// 0-3 and 12-15 at one piece, 4-11 at the one beside it) then lie in 16 different places of the banks.
 // ---------------------------------------------------------------------------------------
-__device__ __forceinline__ int swz_b(int r) { return ((r >> 1) & 1) | ((r >> 3) & 2) | (((r >> 1) ^ (r >> 2)) & 4); }
-__device__ __forceinline__ int swz_a(int r) { return ((r >> 1) & 1) | ((r >> 2) & 2) | ((r ^ (r >> 1)) & 4); }
+__device__ __forceinline__ int turned(int x) { return ((x ^ (x >> 1)) & 1) << 1 | x >> 1; }  // 0 2 3 1
+__device__ __forceinline__ int place_b(int row) { return turned((row >> 3) & 3); }
+__device__ __forceinline__ int place_a(int row) { return turned((row >> 2) & 3); }
 
 // (else the compiler keeps a register for every sum with an address)
 __device__ __forceinline__ uint32_t opaque(uint32_t x) {
@@ -64,14 +50,17 @@ __device__ __forceinline__ void dma16_from(const void* base, uint32_t off, uint3
 // live at once, and gives results other registers than the sums had (207 registers spilled of the 128 x 64
 // wave, 0.7 PFLOP/s). It does not know these for matrix instructions, so the waits are here: s_nop before a product
 // whose scales a vector instruction may just have written, and results_ready before the sums are read.
-template <int AT>
+template <int AT, bool kAcc>
 __device__ __forceinline__ void mfma_in_place(v4f& acc, u32x4 a, u32x4 b, uint32_t sa, uint32_t sb) {
-#define DPA_MFMA(SEL) \
-  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " SEL " cbsz:4 blgp:4" : "+v"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb))
-  if constexpr (AT == 0) DPA_MFMA("op_sel_hi:[0,0,0]");
-  if constexpr (AT == 1) DPA_MFMA("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
-  if constexpr (AT == 2) DPA_MFMA("op_sel_hi:[1,1,0]");
-  if constexpr (AT == 3) DPA_MFMA("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
+#define DPA_MFMA(SEL)                                                                                                     \
+  if constexpr (kAcc)                                                                                                     \
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " SEL " cbsz:4 blgp:4" : "+a"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb)); \
+  else                                                                                                                    \
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " SEL " cbsz:4 blgp:4" : "+v"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb))
+  if constexpr (AT == 0) { DPA_MFMA("op_sel_hi:[0,0,0]"); }
+  if constexpr (AT == 1) { DPA_MFMA("op_sel:[1,1,0] op_sel_hi:[0,0,0]"); }
+  if constexpr (AT == 2) { DPA_MFMA("op_sel_hi:[1,1,0]"); }
+  if constexpr (AT == 3) { DPA_MFMA("op_sel:[1,1,0] op_sel_hi:[1,1,0]"); }
 #undef DPA_MFMA
 }
 // 16 passes and more after the last product
@@ -81,27 +70,33 @@ __device__ __forceinline__ void results_ready() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-template <int WM, int WN, int FM, int FN, int NS, int DT>
-__global__ __launch_bounds__(64 * WM * WN) void mxfp4_gemm_kernel(const GemmArgs p, bool vec) {
+constexpr int kBufferFlags = 0x00020000;     // of a buffer of bytes
+constexpr uint32_t kNowhere = 0x80000000u;   // behind the end of every buffer here (check_gemm)
+
+// (DT: of y, or fp32 for the sums of a split, which y then is. vec: N in whole vectors, y aligned to them)
+template <int WM, int WN, int FM, int FN, int NH, int DT, bool vec>
+__global__ __launch_bounds__(64 * WM * WN) void mxfp4_gemm_kernel(const GemmArgs p) {
   constexpr int kWaves = WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN;
-  // NS buffers of b's rows, NS of a's (a read's place in them is an immediate offset), NS / 2 of their scales
-  constexpr uint32_t kBytesB = BN * 128, kBytesA = BM * 128, kA = NS * kBytesB, kS = kA + NS * kBytesA;
+  // NH buffers of b's rows, NH of a's (a read's place in them is an immediate offset), and scales, 16 B a row and
+  // 512 columns, a group more than the ring holds
+  constexpr uint32_t kBytesB = BN * 64, kBytesA = BM * 64, kA = NH * kBytesB, kS = kA + NH * kBytesA;
   constexpr uint32_t kBytesS = (BM + BN) * 16;
-  constexpr int kXferB = BN / 8 / kWaves, kXferA = BM / 8 / kWaves, kXfer = kXferB + kXferA;
-  static_assert(BN % (8 * kWaves) == 0 && BM % (8 * kWaves) == 0, "transfers of 8 rows");
-  static_assert(FN % 2 == 0 && kWaves % 4 == 0, "pairs of fragments; a swizzle of the row's place among 32");
-  static_assert(NS % 2 == 0 && (BM + BN) / 64 <= kWaves, "two steps to a group of scales, at most a transfer to a wave");
-  // 8 rows of a wave's columns in turn, granule g of 4 columns of row r at g ^ r
-  constexpr int kCols = 16 * FN;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kS + NS / 2 * kBytesS + kWaves * 8 * kCols * 4];
+  constexpr int kSlots = NH / 4 + 1;
+  constexpr int kXferB = BN / 16 / kWaves, kXferA = BM / 16 / kWaves, kXfer = kXferB + kXferA;
+  static_assert(BN % (16 * kWaves) == 0 && BM % (16 * kWaves) == 0, "transfers of 16 rows");
+  static_assert(FN % 2 == 0 && kWaves % 2 == 0 && NH % 4 == 0, "pairs of fragments; a row's place among 32; groups");
+  constexpr int kPieces = (BM + BN) / 64, kXferS = (kPieces + kWaves - 1) / kWaves;
+  constexpr bool kAcc = FM * FN >= 64;  // sums of 256 registers are the accumulation registers
+  // 8 rows of up to 64 of a wave's columns in turn, granule g of 4 columns of row r at g ^ r
+  constexpr int kCols = FN > 4 ? 64 : 16 * FN, kParts = 16 * FN / kCols;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kS + kSlots * kBytesS + (vec ? 0 : kWaves * 8 * kCols * 4)];
   const uint32_t l0 = LDS_ADDR(lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM, r = lane & 15, q = lane >> 4;
-  float* turn = reinterpret_cast<float*>(lds + kS + NS / 2 * kBytesS) + wave * 8 * kCols;
+  float* turn = reinterpret_cast<float*>(lds + kS + kSlots * kBytesS) + wave * 8 * kCols;
   const uint32_t tiles = p.tiles_m * p.tiles_n, total = tiles * p.splits;
   struct Tile {
-    int m0, n0, split, s_lo, s_hi;
-    bool whole;  // no row or column behind the last, stores by vectors
+    int m0, n0, split, lo, hi;  // its 128 columns lo .. hi - 1
   };
   // Workgroup i goes to XCD i % 8, whose L2 holds the rows that its tiles share: an XCD takes an eighth of the
   // tiles in their order, kBand tiles of rows beside each other.
@@ -117,227 +112,308 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_gemm_kernel(const GemmArgs
     id -= band * kBand * p.tiles_n;
     const uint32_t tn = id / rows;
     c.m0 = (band * kBand + id - tn * rows) * BM, c.n0 = tn * BN;
-    c.s_lo = c.split * p.per_split, c.s_hi = min(p.steps, c.s_lo + p.per_split);
-    c.whole = vec && c.m0 + BM <= p.M && c.n0 + BN <= p.N;
+    c.lo = 2 * c.split * p.per_split, c.hi = min(2 * p.steps, c.lo + 2 * p.per_split);
     return c;
   };
   auto there = [&](uint32_t id) { return (id >> 3) < share && place(id) < total; };
   if (!there(blockIdx.x)) return;
   Tile c = tile_of(blockIdx.x);
 
-  // A transfer is 8 rows of a wave; its first row is the same for all lanes. Transfer 0 of an even step is the
-  // scales of its group, 64 rows to a wave (waves beyond those repeat them).
-  const int lr = lane >> 3;
-  const uint32_t off_b = opaque(lr * (uint32_t)p.pitch + (((lane & 7) ^ swz_b(8 * wave + lr)) << 4));
-  const uint32_t off_a = opaque(lr * (uint32_t)p.pitch + (((lane & 7) ^ swz_a(8 * wave + lr)) << 4));
-  const int last_a = ((p.M + 7) & ~7) - 8, last_b = ((p.N + 7) & ~7) - 8;
-  const int part = wave % ((BM + BN) / 64);
-  auto fetch_scales = [&](int step, int slot) __attribute__((always_inline)) {
-    const int64_t group = step >> 1;
-    const uint8_t* from = part < BN / 64 ? p.bs + (group * p.N + c.n0 + 64 * part) * 16
-                                         : p.as + (group * p.M + c.m0 + 64 * (part - BN / 64)) * 16;
-    dma16_from(from, (uint32_t)lane * 16, l0 + kS + slot * kBytesS + part * 1024);
+  // A transfer is 16 rows of a wave; its first row is the same for all lanes. Before the first of a group's go the
+  // group's scales, 64 rows to a wave (waves beyond those repeat them).
+  const int lr = lane >> 2;
+  const uint32_t off_b = opaque(lr * 64 + (((lane & 3) ^ place_b(16 * wave + lr)) << 4));
+  const uint32_t off_a = opaque(lr * 64 + (((lane & 3) ^ place_a(lr)) << 4));
+  const int last_a = (int)padded_rows(p.M) - 16, last_b = (int)padded_rows(p.N) - 16;
+  auto fetch_scales = [&](int group, int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < kXferS; ++k) {
+      const int part = (k * kWaves + wave) % kPieces;
+      const uint8_t* from = part < BN / 64 ? p.bs + ((int64_t)group * p.N + c.n0 + 64 * part) * 16
+                                           : p.as + ((int64_t)group * p.M + c.m0 + 64 * (part - BN / 64)) * 16;
+      dma16_from(from, (uint32_t)lane * 16, l0 + kS + slot * kBytesS + part * 1024);
+    }
   };
-  auto fetch1 = [&](int i, int step, int buf) __attribute__((always_inline)) {
+  const uint8_t* from[kXfer];  // where each transfer goes on
+  auto fetch1 = [&](int i, int buf) __attribute__((always_inline)) {
     const uint32_t at = l0 + wave * 1024;
-    if (i < kXferB)
-      dma16_from(p.b + min(c.n0 + 8 * (i * kWaves + wave), last_b) * p.pitch + step * 128ll, off_b,
-                 at + buf * kBytesB + i * kWaves * 1024);
-    else
-      dma16_from(p.a + min(c.m0 + 8 * ((i - kXferB) * kWaves + wave), last_a) * p.pitch + step * 128ll, off_a,
-                 at + kA + buf * kBytesA + (i - kXferB) * kWaves * 1024);
+    if (i < kXferB) {
+      dma16_from(from[i], off_b, at + buf * kBytesB + i * kWaves * 1024);
+      from[i] += p.panel_b;
+    } else {
+      dma16_from(from[i], off_a, at + kA + buf * kBytesA + (i - kXferB) * kWaves * 1024);
+      from[i] += p.panel_a;
+    }
   };
-  // all NS first steps of a tile, or as many as there are
+  // the first NH of a tile, or as many as there are
   auto begin = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < NS; ++k)
-      if (c.s_lo + k < c.s_hi) {
-        if (k % 2 == 0) fetch_scales(c.s_lo + k, k / 2);
+    for (int i = 0; i < kXfer; ++i)
+      from[i] = i < kXferB ? p.b + c.lo * p.panel_b + min(c.n0 + 16 * (i * kWaves + wave), last_b) * 64ll
+                           : p.a + c.lo * p.panel_a + min(c.m0 + 16 * ((i - kXferB) * kWaves + wave), last_a) * 64ll;
 #pragma unroll
-        for (int i = 0; i < kXfer; ++i) fetch1(i, c.s_lo + k, k);
+    for (int k = 0; k < NH; ++k)
+      if (c.lo + k < c.hi) {
+        if (k % 4 == 0) fetch_scales((c.lo + k) >> 2, k / 4);
+#pragma unroll
+        for (int i = 0; i < kXfer; ++i) fetch1(i, k);
       }
   };
 
   const int rb = 16 * FN * wn + 8 * (r >> 2) + (r & 3), ra = 16 * FM * wm + r;
-  uint32_t read_b[2], read_a[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    read_b[t] = opaque(l0 + rb * 128 + (((2 * q + t) ^ swz_b(rb)) << 4));
-    read_a[t] = opaque(l0 + kA + ra * 128 + (((2 * q + t) ^ swz_a(ra)) << 4));
-  }
+  const uint32_t read_b = opaque(l0 + rb * 64 + ((q ^ place_b(rb)) << 4));
+  const uint32_t read_a = opaque(l0 + kA + ra * 64 + ((q ^ place_a(ra)) << 4));
   const uint32_t read_s = opaque(l0 + kS + rb * 16 + 4 * q), read_sa = opaque(l0 + kS + BN * 16 + ra * 16 + 4 * q);
   auto lds4 = [](uint32_t a) { return *(const __attribute__((address_space(3))) uint32_t*)(a); };
 
   v4f acc[FN][FM];
   u32x4 fa[FM], fb[2][FN];
   uint32_t sa[FM], sb[FN], sa_next[FM], sb_next[FN];
-  auto read_b4 = [&](int i, int buf, int t) __attribute__((always_inline)) {
-    return lds16(read_b[t] + buf * kBytesB + 4096 * (i / 2) + 512 * (i % 2));
+  auto read_b4 = [&](int i, int buf) __attribute__((always_inline)) {
+    return lds16(read_b + buf * kBytesB + 2048 * (i / 2) + 256 * (i % 2));
   };
-  auto read_a4 = [&](int j, int buf, int t) __attribute__((always_inline)) { return lds16(read_a[t] + buf * kBytesA + 2048 * j); };
-  auto read_scales = [&](int j, int slot) __attribute__((always_inline)) {  // of FM parts
-    sa_next[j] = lds4(read_sa + slot * kBytesS + 256 * j);
+  auto read_a4 = [&](int j, int buf) __attribute__((always_inline)) { return lds16(read_a + buf * kBytesA + 1024 * j); };
+  auto read_scales = [&](int j, uint32_t slot) __attribute__((always_inline)) {  // of FM parts
+    sa_next[j] = lds4(read_sa + slot + 256 * j);
 #pragma unroll
-    for (int i = j; i < FN; i += FM) sb_next[i] = lds4(read_s + slot * kBytesS + 512 * (i / 2) + 64 * (i % 2));
+    for (int i = j; i < FN; i += FM) sb_next[i] = lds4(read_s + slot + 512 * (i / 2) + 64 * (i % 2));
   };
-  auto take_scales = [&]() __attribute__((always_inline)) {
+  constexpr int kStores = FN / 2 * FM * Elem<DT>::size / 2;
+  constexpr auto at_most = [](int n) { return n < 64 ? n : 63; };
+  // Whether stores of the tile before went out behind this one's first transfers
+  bool behind = false;
+  uint32_t slot = 0;  // of the next group's scales
+  // The products of panel h, in buffer k = (h - lo) % NH, whose fragments are there. After the first of them the wave
+  // meets the others: h + 1 is there then, and every wave has read h, whose buffer takes h + NH. Fragments of
+  // h + 1, transfers and scales go out between the other products (all at once they hold both waves of a SIMD up).
+  // steady: NH more come after the four of this call's, and no stores are on their way.
+  auto panel = [&](int h, auto number, auto steady) __attribute__((always_inline)) {
+    constexpr int k = decltype(number)::value, next = (k + 1) % NH, t = k & 1;
+    constexpr int kMeet = FM / 4;
+    if constexpr (k % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < FN; ++i) sb[i] = sb_next[i];
+      for (int i = 0; i < FN; ++i) sb[i] = sb_next[i];
 #pragma unroll
-    for (int j = 0; j < FM; ++j) sa[j] = sa_next[j];
-  };
-  // The products of a half step, whose fragments are in fa and fb[piece]; the next half's take their places
-  auto half = [&](auto buffer, auto piece, auto next_buffer, auto next_piece, auto between) __attribute__((always_inline)) {
-    constexpr int t = decltype(piece)::value, at = 2 * (decltype(buffer)::value % 2) + t;
-#pragma unroll
-    for (int i = 0; i < FN; ++i) fb[1 - t][i] = read_b4(i, decltype(next_buffer)::value, decltype(next_piece)::value);
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_nop 3");
+      for (int j = 0; j < FM; ++j) sa[j] = sa_next[j];
+      slot = slot + 1 == kSlots ? 0 : slot + 1;
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_nop 3");
+    }
+    const bool more = decltype(steady)::value || h + NH < c.hi;
+    // transfers behind those of h + 1
+    constexpr int kGroups = [](int k) {
+      int n = 0;
+      for (int i = 1; i <= NH - 2; ++i) n += (k + NH - i) % 4 == 0;
+      return n;
+    }(k);
+    constexpr int kBehind = (NH - 2) * kXfer + kGroups * kXferS;
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
 #pragma unroll
-      for (int i = 0; i < FN; ++i) mfma_in_place<at>(acc[i][j], fb[t][i], fa[j], sb[i], sa[j]);
-      fa[j] = read_a4(j, decltype(next_buffer)::value, decltype(next_piece)::value);
-      between(j);
+      for (int i = 0; i < FN; ++i) mfma_in_place<k % 4, kAcc>(acc[i][j], fb[t][i], fa[j], sb[i], sa[j]);
+      if (j < kMeet) continue;
+      if (j == kMeet) {
+        __builtin_amdgcn_sched_barrier(0);
+        wait_lgkmcnt0();
+        if (decltype(steady)::value) {
+          wait_vmcnt<kBehind>();
+        } else if (h + NH <= c.hi) {
+          if (k < NH - 1 && behind && h == c.lo + k)
+            wait_vmcnt<at_most(kBehind + kStores)>();
+          else
+            wait_vmcnt<kBehind>();
+        } else if (behind && c.hi - c.lo <= NH) {
+          wait_vmcnt<at_most(kStores)>();
+        } else {
+          wait_vmcnt<0>();
+        }
+        lds_barrier();
+#pragma unroll
+        for (int i = 0; i < FN; ++i) fb[1 - t][i] = read_b4(i, next);
+#pragma unroll
+        for (int i = 0; i < kMeet; ++i) fa[i] = read_a4(i, next);
+      }
+      fa[j] = read_a4(j, next);
+      if constexpr (k % 4 == 3) {
+        read_scales(j, slot * kBytesS);
+        if (j == kMeet)
+#pragma unroll
+          for (int i = 0; i < kMeet; ++i) read_scales(i, slot * kBytesS);
+      }
+      if (more) {
+        if (k % 4 == 0 && j == kMeet) fetch_scales((h + NH) >> 2, slot + NH / 4 - 1 < kSlots ? slot + NH / 4 - 1 : slot + NH / 4 - 1 - kSlots);
+#pragma unroll
+        for (int i = j - kMeet; i < kXfer; i += FM - kMeet) fetch1(i, k);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  typedef std::integral_constant<int, 0> Zero;
-  typedef std::integral_constant<int, 1> One;
-  // Step s in buffer k = (s - s_lo) % NS, whose first half's fragments are there. Transfers and scales go out between
-  // its products: all at once they hold both waves of a SIMD up together.
-  auto step = [&](int s, auto buffer) __attribute__((always_inline)) {
-    constexpr int k = decltype(buffer)::value;
-    typedef std::integral_constant<int, (k + 1) % NS> Next;
-    if constexpr (k % 2 == 0) take_scales();
-    half(buffer, Zero(), buffer, One(), [](int) __attribute__((always_inline)) {});
-    wait_lgkmcnt0();
-    // step s + 1 is there, and every wave has read step s; steps s + 2 .. s + NS - 1 are on their way
-    if (s + NS - 1 < c.s_hi)
-      wait_vmcnt<(NS - 2) * kXfer + (NS - 2) / 2>();
-    else
-      wait_vmcnt<0>();
-    lds_barrier();
-    const bool more = s + NS < c.s_hi;
-    half(buffer, One(), Next(), Zero(), [&](int j) __attribute__((always_inline)) {
-      if constexpr (k % 2 == 1) read_scales(j, (k + 1) % NS / 2);
-      if (more) {
-        if (k % 2 == 0 && j == 0) fetch_scales(s + NS, k / 2);
+  // Sums and bias to y (16 rows of it, or 8, to a buffer whose end is theirs: what lies behind y's last row or column
+  // is not stored, without a branch)
+  float bias[FN / 2][8];
+  const __amdgpu_buffer_rsrc_t biases = __builtin_amdgcn_make_buffer_rsrc((void*)p.bias, 0, p.N * 4, kBufferFlags);
+  auto load_bias = [&](const Tile& c) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = j; i < kXfer; i += FM) fetch1(i, s + NS, k);
-      }
-    });
+    for (int u = 0; u < FN / 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) bias[u][i] = 0.f;
+    if (!p.bias || p.splits > 1) return;
+#pragma unroll
+    for (int u = 0; u < FN / 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        bias[u][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(biases, (c.n0 + 16 * FN * wn + 32 * u + 8 * q + i) * 4, 0, 0));
+#pragma unroll
+    for (int u = 0; u < FN / 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(bias[u][i]));  // there before the transfers behind them
   };
-  constexpr int kStores = FN / 2 * FM * Elem<DT>::size / 2;
-  constexpr int kAhead = (NS - 1) * kXfer + NS / 2 - 1;  // transfers behind a tile's first step
-  static_assert(kAhead + kStores < 64, "vmcnt");
-  bool counted = false;
+  auto save = [&](const Tile& c) __attribute__((always_inline)) {
+    constexpr int kSize = Elem<DT>::size;
+    uint8_t* y = static_cast<uint8_t*>(p.y) + (int64_t)c.split * p.M * p.N * kSize;
+    const int n = c.n0 + 16 * FN * wn, m = c.m0 + 16 * FM * wm;
+    auto rows_at = [&](int row, int rows) __attribute__((always_inline)) {
+      const uint64_t from = (uint64_t)(y + (int64_t)min(row, p.M) * p.N * kSize);
+      const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(from >> 32)) << 32 |
+                            (uint32_t)__builtin_amdgcn_readfirstlane((int)from);
+      return __builtin_amdgcn_make_buffer_rsrc(
+          (void*)base, 0, __builtin_amdgcn_readfirstlane(max(0, min(rows, p.M - row)) * p.N * kSize), kBufferFlags);
+    };
+    if constexpr (vec) {
+      uint32_t off[FN / 2][kSize / 2];
+#pragma unroll
+      for (int u = 0; u < FN / 2; ++u)
+#pragma unroll
+        for (int k = 0; k < kSize / 2; ++k) {
+          const int col = n + 32 * u + 8 * q + 4 * k;
+          off[u][k] = col < p.N ? (uint32_t)(r * p.N + col) * kSize : kNowhere;
+        }
+#pragma unroll
+      for (int j = 0; j < FM; ++j) {
+        const __amdgpu_buffer_rsrc_t rows = rows_at(m + 16 * j, 16);
+#pragma unroll
+        for (int u = 0; u < FN / 2; ++u) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = acc[2 * u + i / 4][j][i % 4] + bias[u][i];
+          if constexpr (DT == DPA_DTYPE_F32) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              __builtin_amdgcn_raw_buffer_store_b128(u32x4{__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]),
+                                                           __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3])},
+                                                     rows, off[u][k], 0, 0);
+          } else {
+            __builtin_amdgcn_raw_buffer_store_b128(u32x4{Elem<DT>::pack(v[0], v[1]), Elem<DT>::pack(v[2], v[3]),
+                                                         Elem<DT>::pack(v[4], v[5]), Elem<DT>::pack(v[6], v[7])},
+                                                   rows, off[u][0], 0, 0);
+          }
+        }
+      }
+      return;
+    }
+    // Rows that no vector fits: 8 of them turn in LDS, so that neighbouring lanes store neighbours (each lane its
+    // 8 one by one: 3850 x 1023 of 513 in fp32 22.5 us, against 16.3)
+#pragma unroll
+    for (int h = 0; h < kParts; ++h) {
+      const int col = lane % kCols, at = n + h * kCols + col;
+      const uint32_t off = at < p.N ? (uint32_t)(lane / kCols * p.N + at) * kSize : kNowhere;
+#pragma unroll
+      for (int j = 0; j < 2 * FM; ++j) {
+        if ((r >> 3) == (j & 1)) {
+#pragma unroll
+          for (int i = 0; i < kCols / 16; ++i) {
+            v4f v = acc[h * (kCols / 16) + i][j / 2];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += bias[h * (kCols / 32) + i / 2][4 * (i % 2) + e];
+            *reinterpret_cast<float4*>(turn + (r & 7) * kCols + (((8 * (i / 2) + 2 * q + i % 2) ^ (r & 7)) << 2)) =
+                float4{v[0], v[1], v[2], v[3]};
+          }
+        }
+        asm volatile("" ::: "memory");
+        const __amdgpu_buffer_rsrc_t rows = rows_at(m + 8 * j, 8);
+#pragma unroll
+        for (int i = 0; i < 8 * kCols / 64; ++i) {
+          const int row = i * (64 / kCols) + lane / kCols;
+          const float v = turn[row * kCols + (((col >> 2) ^ row) << 2) + (col & 3)];
+          const uint32_t from = off == kNowhere ? off : off + (uint32_t)(i * (64 / kCols) * p.N) * kSize;
+          if constexpr (DT == DPA_DTYPE_F32)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rows, from, 0, 0);
+          else
+            __builtin_amdgcn_raw_buffer_store_b16((uint16_t)Elem<DT>::pack(v, v), rows, from, 0, 0);
+        }
+        asm volatile("" ::: "memory");
+      }
+    }
+  };
+  constexpr int kAhead = (NH - 1) * kXfer + (NH / 4 - 1) * kXferS;  // transfers behind a tile's first
+  static_assert(kAhead < 64, "vmcnt");
   begin();
   for (uint32_t id = blockIdx.x;;) {
-    // the tile's first step, behind which come its next ones and the stores of the tile before
-    if (c.s_lo + NS > c.s_hi)
+    if (c.lo + NH <= c.hi) {
+      if (behind)
+        wait_vmcnt<at_most(kAhead + kStores)>();
+      else
+        wait_vmcnt<kAhead>();
+    } else if (behind) {
+      wait_vmcnt<at_most(kStores)>();
+    } else {
       wait_vmcnt<0>();
-    else if (counted)
-      wait_vmcnt<kAhead + kStores>();
-    else
-      wait_vmcnt<kAhead>();
+    }
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll
       for (int j = 0; j < FM; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    slot = 0;
 #pragma unroll
     for (int j = 0; j < FM; ++j) read_scales(j, 0);
 #pragma unroll
-    for (int i = 0; i < FN; ++i) fb[0][i] = read_b4(i, 0, 0);
+    for (int i = 0; i < FN; ++i) fb[0][i] = read_b4(i, 0);
 #pragma unroll
-    for (int j = 0; j < FM; ++j) fa[j] = read_a4(j, 0, 0);
-    int s = c.s_lo;
-    if constexpr (NS == 2) {
-      for (; s + 2 <= c.s_hi; s += 2) {
-        step(s, Zero());
-        step(s + 1, One());
+    for (int j = 0; j < FM; ++j) fa[j] = read_a4(j, 0);
+    int h = c.lo;
+    auto four = [&](auto first, auto steady) __attribute__((always_inline)) {  // or two, where the columns end
+      constexpr int f = decltype(first)::value;
+      panel(h, std::integral_constant<int, f>(), steady);
+      panel(h + 1, std::integral_constant<int, f + 1>(), steady);
+      if (decltype(steady)::value || h + 2 < c.hi) {
+        panel(h + 2, std::integral_constant<int, f + 2>(), steady);
+        panel(h + 3, std::integral_constant<int, f + 3>(), steady);
       }
-      if (s < c.s_hi) step(s, Zero());
+      h += 4;
+    };
+    typedef std::integral_constant<int, 0> First;
+    typedef std::integral_constant<int, 4> Fifth;
+    if constexpr (NH == 4) {
+      if (behind) four(First(), std::false_type());
+      while (h + 4 + NH <= c.hi) four(First(), std::true_type());
+      while (h < c.hi) four(First(), std::false_type());
     } else {
-      typedef std::integral_constant<int, 2> Two;
-      typedef std::integral_constant<int, 3> Three;
-      for (; s + 4 <= c.s_hi; s += 4) {
-        step(s, Zero());
-        step(s + 1, One());
-        step(s + 2, Two());
-        step(s + 3, Three());
+      static_assert(NH == 8, "");
+      if (behind) {
+        four(First(), std::false_type());
+        if (h < c.hi) four(Fifth(), std::false_type());
       }
-      if (s < c.s_hi) {
-        step(s, Zero());
-        if (s + 1 < c.s_hi) {
-          step(s + 1, One());
-          if (s + 2 < c.s_hi) step(s + 2, Two());
-        }
+      while (h + 8 + NH <= c.hi) four(First(), std::true_type()), four(Fifth(), std::true_type());
+      while (h < c.hi) {
+        four(First(), std::false_type());
+        if (h < c.hi) four(Fifth(), std::false_type());
       }
     }
     results_ready();
     const Tile done = c;
     id += gridDim.x;
     const bool more = there(id);
+    load_bias(done);
     if (more) {  // the next tile's first steps, before this one's stores
       wait_lgkmcnt0();
       lds_barrier();  // every wave is past its reads
       c = tile_of(id);
       begin();
       __builtin_amdgcn_sched_barrier(0);
-      counted = done.whole;
+      behind = vec;
     }
-    if (vec) {
-#pragma unroll
-      for (int u = 0; u < FN / 2; ++u) {
-        const int n = done.n0 + 16 * FN * wn + 32 * u + 8 * q;
-        float bias[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) bias[i] = p.bias && p.splits == 1 && n + i < p.N ? p.bias[n + i] : 0.f;
-#pragma unroll
-        for (int j = 0; j < FM; ++j) {
-          const int m = done.m0 + 16 * FM * wm + 16 * j + r;
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = acc[2 * u + i / 4][j][i % 4] + bias[i];
-          if (!done.whole && (m >= p.M || n >= p.N)) continue;  // (whole vectors: N is a multiple of them)
-          if (p.splits > 1)
-            store8<DPA_DTYPE_F32>(p.part, (int64_t)done.split * p.M + m, n, p.N, v);
-          else
-            store8<DT>(p.y, m, n, p.N, v);
-        }
-      }
-    } else {
-      // Rows that no vector fits: 8 of them turn in LDS, so that neighbouring lanes store neighbours (each lane its
-      // 8 one by one: 3850 x 1023 of 513 in fp32 22.5 us, against 16.3)
-      const int col = lane % kCols, n = done.n0 + 16 * FN * wn + col;
-      const float bias = p.bias && p.splits == 1 && n < p.N ? p.bias[n] : 0.f;
-#pragma unroll
-      for (int j = 0; j < 2 * FM; ++j) {
-        if ((r >> 3) == (j & 1)) {
-#pragma unroll
-          for (int i = 0; i < FN; ++i) {
-            const v4f v = acc[i][j / 2];
-            *reinterpret_cast<float4*>(turn + (r & 7) * kCols + (((8 * (i / 2) + 2 * q + i % 2) ^ (r & 7)) << 2)) =
-                float4{v[0], v[1], v[2], v[3]};
-          }
-        }
-        asm volatile("" ::: "memory");
-        const int m0 = done.m0 + 16 * FM * wm + 8 * j;
-#pragma unroll
-        for (int i = 0; i < 8 * kCols / 64; ++i) {
-          const int row = i * (64 / kCols) + lane / kCols, m = m0 + row;
-          const float v = turn[row * kCols + (((col >> 2) ^ row) << 2) + (col & 3)] + bias;
-          if (m >= p.M || n >= p.N) continue;
-          if (p.splits > 1)
-            p.part[((int64_t)done.split * p.M + m) * p.N + n] = v;
-          else
-            store1<DT>(p.y, (int64_t)m * p.N + n, v);
-        }
-        asm volatile("" ::: "memory");
-      }
-    }
+    save(done);
     if (!more) break;
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -357,14 +433,14 @@ __global__ __launch_bounds__(512, MT > 2 ? 2 : 4) void mxfp4_few_kernel(const Ge
   const int n0 = tn * 16;
   const int s_lo = split * p.per_split, s_hi = min(p.steps, s_lo + p.per_split);
   const int nb = min(n0 + r, p.N - 1);
-  const uint8_t* b = p.b + nb * p.pitch + 32 * q;
+  const uint8_t* b = p.b + nb * 64ll + 16 * q;
   const uint8_t* bs = p.bs + nb * 16 + 4 * q;
   const uint8_t *a[MT], *as[MT];
   v4f acc[MT];
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
     const int m = min(16 * j + r, p.M - 1);
-    a[j] = p.a + m * p.pitch + 32 * q;
+    a[j] = p.a + m * 64ll + 16 * q;
     as[j] = p.as + m * 16 + 4 * q;
     acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
   }
@@ -375,10 +451,10 @@ __global__ __launch_bounds__(512, MT > 2 ? 2 : 4) void mxfp4_few_kernel(const Ge
   auto load = [&](Group& g, int s) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int64_t at = (t < 2 || s + 1 < p.steps ? s + t / 2 : s) * 128ll + 16 * (t & 1);
-      g.b[t] = *reinterpret_cast<const u32x4*>(b + at);
+      const int64_t panel = 2 * s + (t < 2 || s + 1 < p.steps ? t : t - 2);
+      g.b[t] = *reinterpret_cast<const u32x4*>(b + panel * p.panel_b);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) g.a[j][t] = *reinterpret_cast<const u32x4*>(a[j] + at);
+      for (int j = 0; j < MT; ++j) g.a[j][t] = *reinterpret_cast<const u32x4*>(a[j] + panel * p.panel_a);
     }
     g.sb = *reinterpret_cast<const uint32_t*>(bs + (int64_t)(s >> 1) * p.N * 16);
 #pragma unroll
@@ -495,7 +571,7 @@ __global__ __launch_bounds__(512, 2) void mxfp4_token_kernel(const GemmArgs p) {
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     const int row = min(n0 + 16 * i + r, p.N - 1);
-    b[i] = p.b + row * p.pitch + 32 * q;
+    b[i] = p.b + row * 64ll + 16 * q;
     bs[i] = p.bs + row * 16 + 4 * q;
     acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
   }
@@ -507,7 +583,7 @@ __global__ __launch_bounds__(512, 2) void mxfp4_token_kernel(const GemmArgs p) {
     for (int i = 0; i < NT; ++i) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
-        f[i][t] = *reinterpret_cast<const u32x4*>(b[i] + (t < 2 || s + 1 < p.steps ? s + t / 2 : s) * 128ll + 16 * (t & 1));
+        f[i][t] = *reinterpret_cast<const u32x4*>(b[i] + (2 * s + (t < 2 || s + 1 < p.steps ? t : t - 2)) * p.panel_b);
       sc[i] = *reinterpret_cast<const uint32_t*>(bs[i] + (int64_t)(s >> 1) * p.N * 16);
     }
   };
@@ -517,7 +593,7 @@ __global__ __launch_bounds__(512, 2) void mxfp4_token_kernel(const GemmArgs p) {
     XBlock<DX> xb[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int col = s * 256 + 256 * (t >> 1) + 64 * q + 32 * (t & 1);
+      const int col = s * 256 + 128 * t + 32 * q;
       xb[t] = load_block<DX>(x + (int64_t)col * Elem<DX>::size, p.K - col);
     }
     if (s + 16 < s_hi) fetch(s + 16, sb_next, fb_next);
@@ -589,8 +665,8 @@ constexpr int kFewRows = 64;
 
 // Scales are addressed by 32-bit offsets of 16 B a row, tiles' rows by offsets of 256 rows
 static int check_gemm(int64_t M, int64_t N, int64_t K) {
-  const int64_t most = 1ll << 26;
-  if (M < 0 || N < 0 || K <= 0 || M >= most || N >= most || K > 1 << 24) return DPA_ERR_SIZE;
+  // (16 rows of N columns are within the 2^31 bytes of a buffer)
+  if (M < 0 || N < 0 || K <= 0 || M >= 1 << 26 || N >= 1 << 25 || K > 1 << 24) return DPA_ERR_SIZE;
   if (M * N >= 1ll << 36 || ceil_div(M, 128) * ceil_div(N, 16) >= kMaxGroups256 / 2) return DPA_ERR_SIZE;
   return DPA_OK;
 }
@@ -633,8 +709,8 @@ static void plan_tiles(GemmArgs& p) {
 static GemmArgs plan(int64_t M, int64_t N, int64_t K, bool token) {
   GemmArgs p{};
   p.M = (int)M, p.N = (int)N, p.K = (int)K;
-  p.pitch = pitch_of(K);
-  p.steps = (int)(p.pitch / 128);
+  p.panel_a = panel_of(M), p.panel_b = panel_of(N);
+  p.steps = (int)(pitch_of(K) / 128);
   if (!token && M > kFewRows) {
     plan_tiles(p);
     return p;
@@ -666,9 +742,25 @@ static int join(const GemmArgs& p, hipStream_t s) {
 }
 
 template <int DT>
+static int run_tiles(GemmArgs p, hipStream_t s) {
+  const bool vec = p.N % (16 / Elem<DT>::size) == 0 && aligned(p.y, 16);
+  if (!vec && p.form == 0) {  // (the largest tiles leave no registers to turn rows)
+    p.form = 1;
+    p.tiles_m = (int)ceil_div(p.M, kForms[1].side), p.tiles_n = (int)ceil_div(p.N, kForms[1].side);
+  }
+  const int64_t items = ceil_div((int64_t)p.tiles_m * p.tiles_n * p.splits, 8) * 8;
+  const unsigned grid = (unsigned)std::min<int64_t>(items, kForms[p.form].per_cu * num_cus());
+  if (p.form == 0)
+    mxfp4_gemm_kernel<2, 4, 8, 4, 4, DT, true><<<grid, 512, 0, s>>>(p);
+  else if (p.form == 1)
+    vec ? mxfp4_gemm_kernel<2, 2, 4, 4, 4, DT, true><<<grid, 256, 0, s>>>(p) : mxfp4_gemm_kernel<2, 2, 4, 4, 4, DT, false><<<grid, 256, 0, s>>>(p);
+  else
+    vec ? mxfp4_gemm_kernel<2, 2, 2, 2, 8, DT, true><<<grid, 256, 0, s>>>(p) : mxfp4_gemm_kernel<2, 2, 2, 2, 8, DT, false><<<grid, 256, 0, s>>>(p);
+  return launch_status();
+}
+
+template <int DT>
 static int run_gemm(const GemmArgs& p, hipStream_t s) {
-  const int elems = p.splits > 1 || DT == DPA_DTYPE_F32 ? 4 : 8;
-  const bool vec = p.N % elems == 0 && (p.splits > 1 || aligned(p.y, 16));
   if (p.M <= kFewRows) {
     const unsigned grid = (unsigned)(p.tiles_n * p.splits);
     if (p.M <= 16)
@@ -678,14 +770,10 @@ static int run_gemm(const GemmArgs& p, hipStream_t s) {
     else
       mxfp4_few_kernel<4, DT><<<grid, 512, 0, s>>>(p);
   } else {
-    const int64_t items = ceil_div((int64_t)p.tiles_m * p.tiles_n * p.splits, 8) * 8;
-    const unsigned grid = (unsigned)std::min<int64_t>(items, kForms[p.form].per_cu * num_cus());
-    if (p.form == 0)
-      mxfp4_gemm_kernel<2, 4, 8, 4, 2, DT><<<grid, 512, 0, s>>>(p, vec);
-    else if (p.form == 1)
-      mxfp4_gemm_kernel<2, 2, 4, 4, 2, DT><<<grid, 256, 0, s>>>(p, vec);
-    else
-      mxfp4_gemm_kernel<2, 2, 2, 2, 4, DT><<<grid, 256, 0, s>>>(p, vec);
+    GemmArgs g = p;
+    if (p.splits > 1) g.y = p.part;
+    const int st = p.splits > 1 ? run_tiles<DPA_DTYPE_F32>(g, s) : run_tiles<DT>(g, s);
+    if (st != DPA_OK) return st;
   }
   return join<DT>(p, s);
 }

@@ -13,9 +13,9 @@ struct RowArgs {
   const void* x;
   uint8_t *data, *scales;
   const uint64_t* seed;  // null: to nearest
-  int64_t groups;        // of 8 elements
+  int64_t groups;      // of 8 elements, of a dense tensor
   int64_t rows, cols, ld;
-  FastDiv per_row;       // groups to a padded row
+  FastDiv per_rows;    // workgroups (of 512 columns) to four rows
 };
 
 // Eight neighbours of a row as they lie in memory
@@ -91,9 +91,15 @@ __device__ __forceinline__ void bits4(uint32_t (&b)[4], uint64_t z) {
 template <int DT, bool kOperand, bool kWide, bool SR>
 __global__ __launch_bounds__(256) void mxfp4_rows_kernel(const RowArgs p) {
   const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (g >= p.groups) return;  // (whole blocks: a quad ends together)
   int64_t row = 0, in_row = g;
-  if constexpr (kOperand) row = fdiv((uint32_t)g, p.per_row), in_row = g - row * p.per_row.d;
+  if constexpr (kOperand) {  // a wave takes 512 columns, a workgroup four rows of them: whole lines of the panels
+    const uint32_t four = fdiv(blockIdx.x, p.per_rows);
+    row = 4 * (int64_t)four + (threadIdx.x >> 6);
+    in_row = (int64_t)(blockIdx.x - four * p.per_rows.d) * 64 + (threadIdx.x & 63);
+    if (row >= p.rows || in_row * 4 >= pitch_of(p.cols)) return;
+  } else if (g >= p.groups) {
+    return;  // (whole blocks: a quad ends together)
+  }
   const int64_t c0 = in_row * 8, at = row * p.ld + c0;
   Eight<DT> v;
   if (!kOperand || (kWide && c0 + 8 <= p.cols))
@@ -118,7 +124,10 @@ __global__ __launch_bounds__(256) void mxfp4_rows_kernel(const RowArgs p) {
   } else {
     r = v.codes(scale);
   }
-  reinterpret_cast<uint32_t*>(p.data)[g] = r;
+  if constexpr (kOperand)
+    *reinterpret_cast<uint32_t*>(p.data + (in_row >> 4) * panel_of(p.rows) + row * 64 + (in_row & 15) * 4) = r;
+  else
+    reinterpret_cast<uint32_t*>(p.data)[g] = r;
   if ((threadIdx.x & 3) == 0) {
     if constexpr (kOperand) {
       const int b = (int)(in_row >> 2);
@@ -133,8 +142,8 @@ __global__ __launch_bounds__(256) void mxfp4_rows_kernel(const RowArgs p) {
 // Both operands of a matrix from one read of it: its rows, and its columns (blocks down the columns, the
 // matrix transposed). Eight waves take 64 rows of 256 columns; a thread holds 4 columns of 8 rows: a row's block is
 // the 8 lanes beside each other, a column's the 4 waves below each other, which trade their largest magnitudes
-// through LDS. The columns' codes turn in LDS and leave as 32 B of a column; the four tiles of a line of 128 B
-// go to one XCD, whose L2 joins them. (Two or four tiles to a workgroup, the next one's loads ahead, is slower,
+// through LDS. The columns' codes turn in LDS and leave as 32 B of a column; the tiles below each other, which fill
+// a line of 128 B, go to one XCD, whose L2 joins them. (Two or four tiles to a workgroup, the next one's loads ahead, is slower,
 // from cold caches: 8192 x 4096 of bf16 37.7 and 36.2 us against 34.2, 768 x 256 of fp32 10.8 and 16.8 against 7.6.)
 // ---------------------------------------------------------------------------------------
 struct BothArgs {
@@ -269,7 +278,6 @@ __global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p) {
   const int64_t tl = line / (uint32_t)p.col_tiles, tc = line - tl * p.col_tiles, tr = 4 * tl + ((blockIdx.x >> 3) & 3);
   const int64_t c0 = tc * 256 + 4 * lane;
   const int64_t r0 = tr * 64 + 8 * wave;
-  const int64_t pitch = pitch_of(p.cols);
   Quad<DT> x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = quad_at<DT, kWide>(p, r0 + i, c0);
@@ -287,6 +295,7 @@ __global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p) {
   // rows
   if (p.row_data) {
     uint32_t mine = 0;  // lane 8 b + i: the scale of row i, block b
+    uint8_t* rows_at = p.row_data + (c0 >> 7) * panel_of(p.rows) + r0 * 64 + (c0 & 127) / 2;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       uint32_t m = quad_max(row_max<DT>(x[i]));
@@ -303,7 +312,7 @@ __global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p) {
       } else {
         r = encode_pair<DT, 1>(encode_pair<DT, 0>(0u, x[i].w.x, scale), x[i].w.y, scale);
       }
-      if (r0 + i < p.rows) *reinterpret_cast<uint16_t*>(p.row_data + (r0 + i) * pitch + c0 / 2) = (uint16_t)r;
+      if (r0 + i < p.rows) *reinterpret_cast<uint16_t*>(rows_at + 64 * i) = (uint16_t)r;
     }
     const int64_t row = r0 + (lane & 7);
     const int b = (int)(tc * 8) + (lane >> 3);
@@ -347,19 +356,17 @@ __global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p) {
     *reinterpret_cast<uint32_t*>(out + (j * 64 + lane) * kPitch + half * 16 + 4 * sub) = r;
   }
   __syncthreads();
-  const int64_t col_pitch = pitch_of(p.rows);
   {
     const int at = threadIdx.x >> 1, chunk = threadIdx.x & 1;
     const int64_t col = tc * 256 + 4 * (at & 63) + (at >> 6);
     const uint32_t* w = reinterpret_cast<const uint32_t*>(out + at * kPitch + chunk * 16);
     if (col < p.cols)
-      *reinterpret_cast<uint4*>(p.col_data + col * col_pitch + tr * 32 + chunk * 16) = uint4{w[0], w[1], w[2], w[3]};
+      *reinterpret_cast<uint4*>(p.col_data + (tr >> 1) * panel_of(p.cols) + col * 64 + (tr & 1) * 32 + chunk * 16) =
+          uint4{w[0], w[1], w[2], w[3]};
   }
-  // the two blocks' scales of a column lie together
-  const int64_t col = tc * 256 + threadIdx.x, block = tr * 2;
-  if (threadIdx.x < 256 && col < p.cols)
-    *reinterpret_cast<uint16_t*>(p.col_scales + ((block >> 4) * p.cols + col) * 16 + scale_at((int)(block & 15))) =
-        (uint16_t)(bytes[0][threadIdx.x] | bytes[1][threadIdx.x] << 8);
+  const int64_t col = tc * 256 + (threadIdx.x >> 1), block = tr * 2 + (threadIdx.x & 1);
+  if (col < p.cols)
+    p.col_scales[((block >> 4) * p.cols + col) * 16 + scale_at((int)(block & 15))] = bytes[threadIdx.x & 1][threadIdx.x >> 1];
 }
 
 // ---------------------------------------------------------------------------------------
@@ -409,7 +416,7 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const void* x, float* p
 
 template <int DT, bool SR>
 static int run_rows(const RowArgs& p, bool operand, bool wide, hipStream_t s) {
-  const unsigned grid = (unsigned)ceil_div(p.groups, 256);
+  const unsigned grid = (unsigned)(operand ? ceil_div(p.rows, 4) * groups_of(p.cols) : ceil_div(p.groups, 256));
   if (!operand)
     mxfp4_rows_kernel<DT, false, true, SR><<<grid, 256, 0, s>>>(p);
   else if (wide)
@@ -502,8 +509,7 @@ extern "C" int dpa_mxfp4_operands(const void* x, int dtype, int64_t rows, int64_
   RowArgs r{};
   r.x = x, r.data = (uint8_t*)by_rows, r.scales = r.data + operand_data_bytes(rows, cols), r.seed = (const uint64_t*)seed;
   r.rows = rows, r.cols = cols, r.ld = row_stride;
-  r.groups = rows * (pitch_of(cols) / 4);
-  r.per_row = make_fastdiv((uint32_t)(pitch_of(cols) / 4));
+  r.per_rows = make_fastdiv((uint32_t)groups_of(cols));
   BothArgs b{};
   b.x = x, b.row_data = r.data, b.row_scales = r.scales, b.seed = r.seed;
   b.col_data = (uint8_t*)by_cols, b.col_scales = b.col_data + operand_data_bytes(cols, rows);

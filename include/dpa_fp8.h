@@ -861,8 +861,8 @@ int dpa_mxfp4_dequantize(const void* data, const void* scales, void* y, int dtyp
                          void* stream);
 
 /* Operands of dpa_mxfp4_gemm: a matrix whose contraction runs along its rows, cols long, any number of
- * them, in a buffer of *_bytes (16-B aligned, its order the kernels': rows of ceil(cols / 256) * 128 B, then
- * ceil(cols / 512) * 16 scales a row). dpa_mxfp4_operands lays out x [rows][cols] (row_stride elements
+ * them, in a buffer of *_bytes (16-B aligned, its order the kernels': ceil(cols / 256) * 128 B of data
+ * a row, then ceil(cols / 512) * 16 scales a row). dpa_mxfp4_operands lays out x [rows][cols] (row_stride elements
  * apart) from one read: as it is (by_rows: blocks along the rows) and transposed (by_cols: an operand of `cols`
  * rows, blocks down the columns of x); NULL for the one that is not wanted. With seed (a uint64 in device
  * memory) elements are rounded up or down at random so that their mean is the element, the scale one power

@@ -120,9 +120,9 @@ def test_c_entries_refuse_before_launch(lib):
 
 def test_operand_sizes(lib):
     size = lib.dpa_mxfp4_operand_bytes
-    # whole eights of rows, and scales of 256 rows behind the last
-    assert size(3, 1) == 8 * 128 + (3 + 256) * 16 and size(8, 256) == 8 * 128 + (8 + 256) * 16
-    assert size(9, 257) == 16 * 256 + (9 + 256) * 16 and size(3, 513) == 8 * 384 + (2 * 3 + 256) * 16
+    # whole sixteens of rows, and scales of 256 rows behind the last
+    assert size(3, 1) == 16 * 128 + (3 + 256) * 16 and size(16, 256) == 16 * 128 + (16 + 256) * 16
+    assert size(17, 257) == 32 * 256 + (17 + 256) * 16 and size(3, 513) == 16 * 384 + (2 * 3 + 256) * 16
     assert size(0, 40) == 256 * 16 and size(-1, 40) == 0 and size(3, 0) == 0 and size(1 << 40, 32) == 0
 
 
