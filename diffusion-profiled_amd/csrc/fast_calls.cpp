@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -307,6 +308,12 @@ PyObject* embedding_bwd(PyObject*, PyObject* const* o, Py_ssize_t n) {
 }
 
 // ---- MXFP4 (mxfp4.py) ----
+// A plain tensor on the current device (the general way makes another one current first)
+const at::Tensor* local(PyObject* o, int* device) {
+  const at::Tensor* t = plain(o, device);
+  return t && *device == c10::hip::current_device() ? t : nullptr;
+}
+
 at::Tensor bytes_like(const at::Tensor& t, int64_t n) { return at::empty({n}, t.options().dtype(at::kByte)); }
 
 // the 16-B aligned beginning of the next part of a workspace
@@ -332,7 +339,7 @@ PyObject* mxfp4_quantize(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 1) return none();
   int device = -1;
-  const at::Tensor* x = plain(o[0], &device);
+  const at::Tensor* x = local(o[0], &device);
   if (!x || dtype_of(x->scalar_type()) < 0 || x->dim() < 1 || x->numel() == 0 || x->size(-1) % 32 || !x->is_contiguous() ||
       !aligned16(*x))
     return none();
@@ -359,7 +366,7 @@ PyObject* mxfp4_dequantize(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 3) return none();
   int device = -1;
-  const at::Tensor *d = plain(o[0], &device), *s = plain(o[1], &device);
+  const at::Tensor *d = local(o[0], &device), *s = local(o[1], &device);
   at::ScalarType type = at::kBFloat16;
   if (!d || !s || !mxfp4_ok(*d, *s) || !dtype_arg(o[2], &type) || dtype_of(type) < 0 || d->numel() == 0 || !d->is_contiguous() ||
       !s->is_contiguous() || !aligned16(*d))
@@ -389,7 +396,7 @@ PyObject* mxfp4_linear(PyObject*, PyObject* const* o, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   if (count != 6 || !PyLong_CheckExact(o[2]) || !PyLong_CheckExact(o[3])) return none();
   int device = -1;
-  const at::Tensor *x = plain(o[0], &device), *w = plain(o[1], &device), *bias;
+  const at::Tensor *x = local(o[0], &device), *w = local(o[1], &device), *bias;
   if (!x || !w || !maybe(o[4], &device, &bias)) return none();
   const int64_t n = PyLong_AsLongLong(o[2]), k = PyLong_AsLongLong(o[3]);
   if (PyErr_Occurred()) {
@@ -419,7 +426,7 @@ PyObject* mxfp4_train_fwd(PyObject*, PyObject* const* o, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   if (count != 4) return none();
   int device = -1;
-  const at::Tensor *x = plain(o[0], &device), *w = plain(o[1], &device), *bias;
+  const at::Tensor *x = local(o[0], &device), *w = local(o[1], &device), *bias;
   if (!x || !w || !maybe(o[2], &device, &bias) || w->dim() != 2) return none();
   const int64_t n = w->size(0), k = w->size(1);
   int64_t m, rows;
@@ -451,7 +458,7 @@ PyObject* mxfp4_bwd(PyObject*, PyObject* const* o, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   if (count != 9 || !PyLong_CheckExact(o[3]) || !PyLong_CheckExact(o[4])) return none();
   int device = -1;
-  const at::Tensor *dy = plain(o[0], &device), *xo = plain(o[1], &device), *wo = plain(o[2], &device), *seed;
+  const at::Tensor *dy = local(o[0], &device), *xo = local(o[1], &device), *wo = local(o[2], &device), *seed;
   if (!dy || !xo || !wo || !maybe(o[8], &device, &seed) || (seed && !seed_ok(seed))) return none();
   const int64_t n = PyLong_AsLongLong(o[3]), k = PyLong_AsLongLong(o[4]);
   if (PyErr_Occurred()) {
@@ -499,7 +506,7 @@ PyObject* mxfp4_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 6) return none();
   int device = -1;
-  const at::Tensor *q = plain(o[0], &device), *d = plain(o[1], &device), *x = plain(o[2], &device), *lengths, *mask;
+  const at::Tensor *q = local(o[0], &device), *d = local(o[1], &device), *x = local(o[2], &device), *lengths, *mask;
   if (!q || !d || !x || !maybe(o[3], &device, &lengths) || !maybe(o[4], &device, &mask)) return none();
   if (q->dim() != 4 || d->dim() != 5 || !mxfp4_ok(*d, *x) || d->size(2) != 2 || d->stride(4) != 1 ||
       (x->stride(4) != 1 && x->size(4) > 1) || !aligned16(*d) || d->stride(2) % 16 || d->size(4) * 2 % 32)

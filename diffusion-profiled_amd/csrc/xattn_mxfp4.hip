@@ -748,7 +748,11 @@ static DpaCrossAttention shape_of(const DpaCrossAttentionMxfp4& a) {
 static int check_mx(const DpaCrossAttentionMxfp4& a) {
   const int st = check_shape(shape_of(a));
   if (st != DPA_OK) return st;
-  return a.head_dim % 32 ? DPA_ERR_SHAPE : DPA_OK;
+  if (a.head_dim % 32) return DPA_ERR_SHAPE;
+  // (a row's place in a tile is its number times 32 bits)
+  for (const int64_t tokens : {a.k_data_stride[1], a.k_scale_stride[1], a.v_data_stride[1], a.v_scale_stride[1]})
+    if (tokens < 0 || tokens >= 1ll << 32) return DPA_ERR_SIZE;
+  return DPA_OK;
 }
 
 static bool strides16(const int64_t* s) { return s[0] % 16 == 0 && s[1] % 16 == 0 && s[2] % 16 == 0; }

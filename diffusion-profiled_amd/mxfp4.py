@@ -58,6 +58,17 @@ def _check_dtype(what: str, *dtypes: torch.dtype) -> None:
             raise ValueError(f"{what}: bf16, fp16 or fp32, got {dt}")
 
 
+def _call(entry: str, *args) -> None:
+    """An entry of the library on the current stream of the last argument's device, which is the current one for the
+    launch."""
+    *args, on = args
+    if on.get_device() == torch.cuda.current_device():
+        _lib.call(entry, *args, _lib.current_stream(on))
+    else:
+        with torch.cuda.device(on.device):
+            _lib.call(entry, *args, _lib.current_stream(on))
+
+
 # ---- quantisation ------------------------------------------------------------------------
 def quantize_mxfp4(x: torch.Tensor) -> MXFP4:
     """x [..., C] (bf16, fp16 or fp32; C a multiple of 32) in MXFP4, blocks along the last dimension."""
@@ -76,8 +87,8 @@ def quantize_mxfp4(x: torch.Tensor) -> MXFP4:
     lead, c = x.shape[:-1], x.shape[-1]
     data = torch.empty((*lead, c // 2), device=x.device, dtype=torch.uint8)
     scales = torch.empty((*lead, c // BLOCK), device=x.device, dtype=torch.uint8)
-    _lib.call("dpa_mxfp4_quantize", x.data_ptr(), _DT[x.dtype], x.numel(), data.data_ptr(), scales.data_ptr(),
-              _lib.current_stream(x))
+    _call("dpa_mxfp4_quantize", x.data_ptr(), _DT[x.dtype], x.numel(), data.data_ptr(), scales.data_ptr(),
+              x)
     return MXFP4(data, scales)
 
 
@@ -103,8 +114,8 @@ def dequantize_mxfp4(q: MXFP4, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
     if data.data_ptr() % 4:
         data = data.clone()
     y = torch.empty(q.shape, device=data.device, dtype=dtype)
-    _lib.call("dpa_mxfp4_dequantize", data.data_ptr(), scales.data_ptr(), y.data_ptr(), _DT[dtype], y.numel(),
-              _lib.current_stream(data))
+    _call("dpa_mxfp4_dequantize", data.data_ptr(), scales.data_ptr(), y.data_ptr(), _DT[dtype], y.numel(),
+              data)
     return y
 
 
@@ -134,8 +145,8 @@ def _operands(x: torch.Tensor, rows: bool, cols: bool, seed: torch.Tensor | None
     r = _new_operand(m, k, x.device) if rows else None
     c = _new_operand(k, m, x.device) if cols else None
     if m:
-        _lib.call("dpa_mxfp4_operands", x.data_ptr(), _DT[x.dtype], m, k, x.stride(0) if m > 1 else k,
-                  _ptr(r and r.data), _ptr(c and c.data), _ptr(seed), _lib.current_stream(x))
+        _call("dpa_mxfp4_operands", x.data_ptr(), _DT[x.dtype], m, k, x.stride(0) if m > 1 else k,
+                  _ptr(r and r.data), _ptr(c and c.data), _ptr(seed), x)
     return r, c
 
 
@@ -161,8 +172,8 @@ def _product(a: MXFP4Operand, b: MXFP4Operand, bias: torch.Tensor | None, dtype:
     if m and n:
         nbytes = _lib.query("dpa_mxfp4_gemm_workspace_bytes", m, n, k)
         ws = _workspace(nbytes, a.data.device)
-        _lib.call("dpa_mxfp4_gemm", a.data.data_ptr(), b.data.data_ptr(), _ptr(bias), y.data_ptr(), _DT[dtype], m, n, k,
-                  _ptr(ws), nbytes, _lib.current_stream(a.data))
+        _call("dpa_mxfp4_gemm", a.data.data_ptr(), b.data.data_ptr(), _ptr(bias), y.data_ptr(), _DT[dtype], m, n, k,
+                  _ptr(ws), nbytes, a.data)
     return y
 
 
@@ -218,8 +229,8 @@ def linear_mxfp4_fwd(x: torch.Tensor, weight: torch.Tensor | MXFP4Operand, bias:
         ld = x2.stride(0) if m > 1 else k
         nbytes = _lib.query("dpa_mxfp4_linear_workspace_bytes", x2.data_ptr(), _DT[x2.dtype], ld, m, n, k)
         ws = _workspace(nbytes, x.device)
-        _lib.call("dpa_mxfp4_linear", x2.data_ptr(), _DT[x2.dtype], ld, w.data.data_ptr(), _ptr(b32), y.data_ptr(),
-                  _DT[dtype], m, n, k, _ptr(ws), nbytes, _lib.current_stream(x2))
+        _call("dpa_mxfp4_linear", x2.data_ptr(), _DT[x2.dtype], ld, w.data.data_ptr(), _ptr(b32), y.data_ptr(),
+                  _DT[dtype], m, n, k, _ptr(ws), nbytes, x2)
     return y.view(*x.shape[:-1], n)
 
 
@@ -266,8 +277,8 @@ def _column_sum(x: torch.Tensor) -> torch.Tensor:
     y = torch.empty(n, device=x.device, dtype=torch.float32)
     nbytes = _lib.query("dpa_column_sum_workspace_bytes", m, n)
     ws = _workspace(nbytes, x.device)
-    _lib.call("dpa_column_sum", x.data_ptr(), _DT[x.dtype], m, n, x.stride(0) if m > 1 else n, y.data_ptr(), _ptr(ws),
-              nbytes, _lib.current_stream(x))
+    _call("dpa_column_sum", x.data_ptr(), _DT[x.dtype], m, n, x.stride(0) if m > 1 else n, y.data_ptr(), _ptr(ws),
+              nbytes, x)
     return y
 
 
@@ -430,7 +441,7 @@ def cross_attention_mxfp4_fwd(q: torch.Tensor, kv: MXFP4, *, key_lengths: torch.
                       *(s for t in parts for s in _strides(t)), _DT[q.dtype], b, lq, lk, h, g, d, number)
     n = _lib.query("dpa_cross_attention_mxfp4_workspace_bytes", desc)
     ws = _workspace(n, q.device)
-    _lib.call("dpa_cross_attention_mxfp4", desc, _ptr(ws), n, _lib.current_stream(q))
+    _call("dpa_cross_attention_mxfp4", desc, _ptr(ws), n, q)
     return out, lse
 
 

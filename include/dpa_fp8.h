@@ -894,7 +894,7 @@ int dpa_column_sum(const void* x, int dtype, int64_t rows, int64_t cols, int64_t
 
 /* The forward of dpa_cross_attention_fwd over keys and values in MXFP4, head_dim a multiple of 32 up to
  * 128: elements of a head dense, 16-B aligned, strides of data and scales (batch, token, head) in bytes, those of
- * data multiples of 16. With fp16 queries a value of the cache is rounded to fp16. */
+ * data multiples of 16, those of tokens below 2^32. With fp16 queries a value of the cache is rounded to fp16. */
 typedef struct DpaCrossAttentionMxfp4 {
   const void *q, *k_data, *k_scales, *v_data, *v_scales;
   void* out;

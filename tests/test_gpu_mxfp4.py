@@ -390,3 +390,24 @@ def test_calls_on_two_streams_do_not_meet(M):
             outs.append(M.linear_mxfp4_fwd(x, w))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+def test_tensors_on_another_device_than_the_current_one(M, monkeypatch):
+    """Their device is the current one for each launch (shown with the question for the current device turned)."""
+    x, w = randn((70, 96), 61, torch.bfloat16).cuda(), randn((40, 96), 62, torch.bfloat16).cuda()
+    want = M.linear_mxfp4_fwd(x, w)
+    q4 = M.quantize_mxfp4(x)
+    entered = []
+
+    class On(torch.cuda.device):
+        def __enter__(self):
+            entered.append(self.idx)
+            return super().__enter__()
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 7)
+    monkeypatch.setattr(torch.cuda, "device", On)
+    assert torch.equal(M.linear_mxfp4_fwd(x, w), want) and entered == [0, 0]
+    kept = M.mxfp4_operand(w)
+    assert entered == [0, 0, 0]
+    monkeypatch.undo()
+    assert torch.equal(M.linear_mxfp4_fwd(x, kept), want)
+    assert torch.equal(M.quantize_mxfp4(x).data, q4.data)

@@ -140,6 +140,7 @@ def test_attention_entry_refuses_before_launch(lib, M):
     assert f(desc(scale=0.0), None, 0, None) == -2 and f(desc(lq=-1), None, 0, None) == -2
     assert f(desc(data_stride=8), None, 0, None) == -3 and f(desc(q_stride=4), None, 0, None) == -3
     assert f(desc(kd=0x1008), None, 0, None) == -3
+    assert f(desc(data_stride=1 << 32), None, 0, None) == -2 and f(desc(data_stride=-16), None, 0, None) == -2
     many = desc(lq=1, lk=100000)
     assert lib.dpa_cross_attention_mxfp4_workspace_bytes(many) > 0
     assert f(many, None, 0, None) == -5
