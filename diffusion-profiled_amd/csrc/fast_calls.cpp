@@ -443,8 +443,8 @@ PyObject* mxfp4_train_fwd(PyObject*, PyObject* const* o, Py_ssize_t count) {
              ws = bytes_like(*x, at_ws + gemm);
   uint8_t* p = (uint8_t*)ws.data_ptr();
   void* s = stream_of(device);
-  int status = mx_operands(x->data_ptr(), dtype_of(x->scalar_type()), m, k, k, p, xo.data_ptr(), nullptr, s);
-  if (!status) status = mx_operands(w->data_ptr(), dtype_of(w->scalar_type()), n, k, k, p + at_w, wo.data_ptr(), nullptr, s);
+  int status = mx_operands(x->data_ptr(), dtype_of(x->scalar_type()), m, k, k, p, xo.data_ptr(), nullptr, nullptr, s);
+  if (!status) status = mx_operands(w->data_ptr(), dtype_of(w->scalar_type()), n, k, k, p + at_w, wo.data_ptr(), nullptr, nullptr, s);
   if (status) return failed("dpa_mxfp4_operands", status);
   status = mx_gemm(p, p + at_w, bias ? (const float*)bias->data_ptr() : nullptr, y.data_ptr(), dtype_of(type), m, n, k, p + at_ws,
                    gemm, s);
@@ -475,8 +475,9 @@ PyObject* mxfp4_bwd(PyObject*, PyObject* const* o, Py_ssize_t count) {
       wo->scalar_type() != at::kByte || !xo->is_contiguous() || !wo->is_contiguous() || !aligned16(*xo) || !aligned16(*wo))
     return none();
   const bool bias = o[7] == Py_True;
-  const int64_t g1 = mx_gemm_bytes(m, k, n), g2 = mx_gemm_bytes(n, k, m), sums = bias ? column_sum_bytes(m, n) : 0;
-  const int64_t at_c = round256(dr), at_ws = at_c + round256(dc), most = std::max(std::max(g1, g2), sums);
+  const int64_t g1 = mx_gemm_bytes(m, k, n), g2 = mx_gemm_bytes(n, k, m);
+  const int64_t pieces = (m + 63) / 64, part = bias ? round256(pieces * n * 4) : 0, sums = bias ? column_sum_bytes(pieces, n) : 0;
+  const int64_t at_c = round256(dr), at_ws = at_c + round256(dc), most = std::max(std::max(g1, g2), part + sums);
   at::DimVector shape(dy->sizes().begin(), dy->sizes().end());
   shape.back() = k;
   at::Tensor dx = at::empty(shape, dy->options().dtype(dxt)), dw = at::empty({n, k}, dy->options().dtype(dwt)), db,
@@ -485,13 +486,14 @@ PyObject* mxfp4_bwd(PyObject*, PyObject* const* o, Py_ssize_t count) {
   uint8_t* p = (uint8_t*)ws.data_ptr();
   void* s = stream_of(device);
   const int type = dtype_of(dy->scalar_type());
-  int status = mx_operands(dy->data_ptr(), type, m, n, n, p, p + at_c, seed ? seed->data_ptr() : nullptr, s);
+  int status = mx_operands(dy->data_ptr(), type, m, n, n, p, p + at_c, bias ? (float*)(p + at_ws) : nullptr,
+                           seed ? seed->data_ptr() : nullptr, s);
   if (status) return failed("dpa_mxfp4_operands", status);
+  if (bias) status = column_sum(p + at_ws, DPA_DTYPE_F32, pieces, n, n, db.data_ptr(), p + at_ws + part, sums, s);
+  if (status) return failed("dpa_column_sum", status);
   status = mx_gemm(p, wo->data_ptr(), nullptr, dx.data_ptr(), dtype_of(dxt), m, k, n, p + at_ws, g1, s);
   if (!status) status = mx_gemm(p + at_c, xo->data_ptr(), nullptr, dw.data_ptr(), dtype_of(dwt), n, k, m, p + at_ws, g2, s);
   if (status) return failed("dpa_mxfp4_gemm", status);
-  if (bias) status = column_sum(dy->data_ptr(), type, m, n, n, db.data_ptr(), p + at_ws, sums, s);
-  if (status) return failed("dpa_column_sum", status);
   return tuple_of({dx, dw, db});
   END_HANDLE_TH_ERRORS
 }

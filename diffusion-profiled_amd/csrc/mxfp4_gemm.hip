@@ -871,7 +871,7 @@ extern "C" int dpa_mxfp4_linear(const void* x, int x_dtype, int64_t row_stride, 
     if (x_dtype == DPA_DTYPE_F16) return run_token<DPA_DTYPE_F16>(p, dtype, s);
     return run_token<DPA_DTYPE_F32>(p, dtype, s);
   }
-  const int quantized = dpa_mxfp4_operands(x, x_dtype, M, K, row_stride, ws, nullptr, nullptr, stream);
+  const int quantized = dpa_mxfp4_operands(x, x_dtype, M, K, row_stride, ws, nullptr, nullptr, nullptr, stream);
   if (quantized != DPA_OK) return quantized;
   p.a = ws, p.as = p.a + operand_data_bytes(M, K);
   p.part = (float*)(ws + align256(operand_bytes(M, K)));

@@ -153,6 +153,7 @@ struct BothArgs {
   int64_t rows, cols, ld;
   int col_tiles;
   uint32_t lines;  // of 256 rows x 256 columns
+  float* sums;     // [ceil(rows / 64)][cols] down the columns, or null
 };
 
 // Four neighbours of a row
@@ -270,6 +271,7 @@ __global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p) {
   __shared__ __attribute__((aligned(16))) uint8_t out[256 * kPitch];
   __shared__ __attribute__((aligned(16))) uint32_t tops[8][64 * kW];
   __shared__ __attribute__((aligned(8))) uint8_t bytes[2][256];
+  __shared__ __attribute__((aligned(16))) float sums[8][256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = wave >> 2, sub = wave & 3;
   // workgroups i, i + 8, i + 16, i + 24 of 32 (on one XCD): the tiles below each other of a line
@@ -292,6 +294,14 @@ __global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) top.take(x[i]);
   top.put(&tops[wave][lane * kW]);
+  if (p.sums) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] += x[i].get(j);
+    *reinterpret_cast<float4*>(&sums[wave][4 * lane]) = float4{s[0], s[1], s[2], s[3]};
+  }
   // rows
   if (p.row_data) {
     uint32_t mine = 0;  // lane 8 b + i: the scale of row i, block b
@@ -320,6 +330,12 @@ __global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p) {
   }
   wait_lgkmcnt0();
   lds_barrier();
+  if (p.sums && threadIdx.x < 256 && tc * 256 + threadIdx.x < p.cols && tr * 64 < p.rows) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += sums[w][threadIdx.x];
+    p.sums[tr * p.cols + tc * 256 + threadIdx.x] = s;
+  }
   // columns: word `sub` of block `half`
 #pragma unroll
   for (int w = 0; w < 4; ++w) top.join(&tops[4 * half + w][lane * kW]);
@@ -499,13 +515,14 @@ extern "C" int64_t dpa_mxfp4_operand_bytes(int64_t rows, int64_t cols) {
 }
 
 extern "C" int dpa_mxfp4_operands(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride,
-                                  void* by_rows, void* by_cols, const void* seed, void* stream) {
+                                  void* by_rows, void* by_cols, float* sums, const void* seed, void* stream) {
   if (!dtype_ok(dtype)) return DPA_ERR_SHAPE;
   if (!matrix_ok(rows, cols) || (row_stride < cols && rows > 1)) return DPA_ERR_SIZE;
-  if (!by_rows && !by_cols) return DPA_ERR_NULL;
+  if ((!by_rows && !by_cols) || (sums && !by_cols)) return DPA_ERR_NULL;
   if (rows == 0) return DPA_OK;
   if (!x) return DPA_ERR_NULL;
-  if (!aligned(x, size_of(dtype)) || !aligned(by_rows, 16) || !aligned(by_cols, 16) || !aligned(seed, 8)) return DPA_ERR_ALIGN;
+  if (!aligned(x, size_of(dtype)) || !aligned(by_rows, 16) || !aligned(by_cols, 16) || !aligned(sums, 4) || !aligned(seed, 8))
+    return DPA_ERR_ALIGN;
   RowArgs r{};
   r.x = x, r.data = (uint8_t*)by_rows, r.scales = r.data + operand_data_bytes(rows, cols), r.seed = (const uint64_t*)seed;
   r.rows = rows, r.cols = cols, r.ld = row_stride;
@@ -513,7 +530,7 @@ extern "C" int dpa_mxfp4_operands(const void* x, int dtype, int64_t rows, int64_
   BothArgs b{};
   b.x = x, b.row_data = r.data, b.row_scales = r.scales, b.seed = r.seed;
   b.col_data = (uint8_t*)by_cols, b.col_scales = b.col_data + operand_data_bytes(cols, rows);
-  b.rows = rows, b.cols = cols, b.ld = row_stride;
+  b.rows = rows, b.cols = cols, b.ld = row_stride, b.sums = sums;
   b.col_tiles = (int)ceil_div(cols, 256);
   b.lines = (uint32_t)(ceil_div(rows, 256) * b.col_tiles);
   // whole aligned vectors: 16 B of 8 elements (8 B of 4) of a 16-bit type, 16 B of 4 of fp32

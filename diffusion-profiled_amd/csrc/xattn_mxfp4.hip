@@ -442,8 +442,8 @@ __global__ __launch_bounds__(256, 2) void xattn_mxfp4_few_kernel(const MxArgs p)
 
 // ---------------------------------------------------------------------------------------
 // Up to 16 rows of a key head (single tokens, their heads sharing keys): as above, on v_mfma_f32_16x16x32, whose
-// columns are the rows. Bound by the bytes of the cache, so made for bytes in flight: half the registers, two tiles
-// of 32 keys a wave on their way, and as many waves as fit at once.
+// columns are the rows, a tile of 32 keys to a wave, two on their way. Bound by the conversions' instructions: a tile
+// takes 0.9 us of a SIMD's time whatever is on its way, the cache alone would be there in half of that.
 //   S^T (16 keys x 16 rows) = K Q^T: lane (key l & 15, q = l >> 4) takes dims [q D / 4, (q + 1) D / 4) of its key, 8 to
 //   a product. It receives the scores of row l & 15 at keys 4 q + t of each 16, which packed are the B operand of
 //   O^T += V^T P^T if the sum over 32 keys runs over {4 q + t, 16 + 4 q + t} in lane q: so the values' transpose
@@ -473,7 +473,7 @@ __device__ __forceinline__ float sum_quarters(float x) {
 }
 
 template <class T, int D>
-__global__ __launch_bounds__(256, 3) void xattn_mxfp4_token_kernel(const MxArgs p) {
+__global__ __launch_bounds__(256, 2) void xattn_mxfp4_token_kernel(const MxArgs p) {
   constexpr int KT = 32;
   constexpr int DP = D == 96 ? 128 : D;   // of the values' rows in LDS
   constexpr int NB = D / 32;              // blocks to a row, words of 8 dims to a lane's quarter of it
@@ -770,10 +770,10 @@ static void plan_mx(Args& p) {
   }
   p.tiles = 1;
   const int64_t groups = (int64_t)p.B * p.KVH;
-  // four workgroups to a CU, of which three are there at once and the others take the place of those whose keys
-  // end early; what fills the CUs without is not split, and no row into more than 64 parts, which the join would
-  // wait for
-  const int64_t want = groups >= 2 * num_cus() ? groups : std::min<int64_t>(4 * num_cus(), 64 * groups);
+  // two workgroups to a CU; what fills the CUs without is not split, and no row into more than 64 parts, which the
+  // join would wait for (16 queries over up to 8191 keys of 4 heads of 128, 48 MB of cache: 20.3 us, with three to a
+  // CU 22.7, with four 22.0: a wave's first and last tile cost as much as ten between)
+  const int64_t want = groups >= 2 * num_cus() ? groups : std::min<int64_t>(2 * num_cus(), 64 * groups);
   choose_splits(p, groups, ceil_div(p.Lk, 32), want, 8, kMaxRange / 32, 4);
   // A head's piece of a token is 16 to 64 B and its scales 1 to 4, so that cache lines hold those of several: the
   // heads of a split go to one XCD; splits are dealt out in turn, since lengths differ.

@@ -132,8 +132,8 @@ def _matrix(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
 
 
-def _operands(x: torch.Tensor, rows: bool, cols: bool, seed: torch.Tensor | None):
-    """x's operand, that of its transpose, or both."""
+def _operands(x: torch.Tensor, rows: bool, cols: bool, seed: torch.Tensor | None, sums: torch.Tensor | None = None):
+    """x's operand, that of its transpose, or both; with the latter the sums down the columns of every 64 rows."""
     _check_dtype("mxfp4 operand", x.dtype)
     if x.ndim != 2 or x.shape[1] == 0:
         raise ValueError(f"mxfp4 operand: a matrix of at least one column, got {tuple(x.shape)}")
@@ -146,7 +146,7 @@ def _operands(x: torch.Tensor, rows: bool, cols: bool, seed: torch.Tensor | None
     c = _new_operand(k, m, x.device) if cols else None
     if m:
         _call("dpa_mxfp4_operands", x.data_ptr(), _DT[x.dtype], m, k, x.stride(0) if m > 1 else k,
-                  _ptr(r and r.data), _ptr(c and c.data), _ptr(seed), x)
+                  _ptr(r and r.data), _ptr(c and c.data), _ptr(sums), _ptr(seed), x)
     return r, c
 
 
@@ -309,13 +309,17 @@ def linear_mxfp4_bwd(dy: torch.Tensor, kept: LinearKept, *, seed: torch.Tensor |
             _on_one_gpu(dy, o.data)
     dy2 = _matrix(dy.reshape(-1, n))
     dx = dw = None
+    summed = dy2
     if kept.weight is not None or kept.x is not None:
-        dyr, dyc = _operands(dy2, kept.weight is not None, kept.x is not None, seed)
+        part = None
+        if kept.bias and kept.x is not None:
+            part = summed = torch.empty((-(-dy2.shape[0] // 64), n), device=device, dtype=torch.float32)
+        dyr, dyc = _operands(dy2, kept.weight is not None, kept.x is not None, seed, part)
         if kept.weight is not None:
             dx = _product(dyr, kept.weight, None, kept.dtype).view(kept.shape)
         if kept.x is not None:
             dw = _product(dyc, kept.x, None, kept.weight_dtype)
-    return dx, dw, _column_sum(dy2) if kept.bias else None
+    return dx, dw, _column_sum(summed) if kept.bias else None
 
 
 class LinearMXFP4Function(torch.autograd.Function):

@@ -864,13 +864,14 @@ int dpa_mxfp4_dequantize(const void* data, const void* scales, void* y, int dtyp
  * them, in a buffer of *_bytes (16-B aligned, its order the kernels': ceil(cols / 256) * 128 B of data
  * a row, then ceil(cols / 512) * 16 scales a row). dpa_mxfp4_operands lays out x [rows][cols] (row_stride elements
  * apart) from one read: as it is (by_rows: blocks along the rows) and transposed (by_cols: an operand of `cols`
- * rows, blocks down the columns of x); NULL for the one that is not wanted. With seed (a uint64 in device
+ * rows, blocks down the columns of x); NULL for the one that is not wanted. With by_cols, sums (or NULL) gets the
+ * sums down the columns of every 64 rows, fp32 [ceil(rows / 64)][cols], for dpa_column_sum to add up. With seed (a uint64 in device
  * memory) elements are rounded up or down at random so that their mean is the element, the scale one power
  * higher where amax would pass 6 of it: 16 bits a element of splitmix64(seed + i / 4 * golden ratio),
  * i = row * (cols rounded up to 32) + col, for both arrangements. */
 int64_t dpa_mxfp4_operand_bytes(int64_t rows, int64_t cols);
 int dpa_mxfp4_operands(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride,
-                       void* by_rows, void* by_cols, const void* seed, void* stream);
+                       void* by_rows, void* by_cols, float* sums, const void* seed, void* stream);
 
 /* y [M][N] (bf16, fp16 or fp32) = a b^T + bias over operands a of M rows and b of N rows, K columns each;
  * bias fp32 [N] or NULL. fp32 sums in a fixed order. */

@@ -80,17 +80,18 @@ def test_c_entries_refuse_before_launch(lib):
     assert d(fake, nul, fake, 0, 32, nul) == -1 and d(fake, fake, odd, 0, 32, nul) == -3
     assert d(fake, fake, fake, 0, 16, nul) == -2 and d(fake, fake, fake, 7, 32, nul) == -4
     o = lib.dpa_mxfp4_operands
-    assert o(fake, 0, 4, 40, 40, nul, nul, nul, nul) == -1          # neither wanted
-    assert o(nul, 0, 4, 40, 40, fake, nul, nul, nul) == -1
-    assert o(fake, 0, 4, 40, 39, fake, nul, nul, nul) == -2         # rows that overlap
-    assert o(fake, 0, 4, 0, 40, fake, nul, nul, nul) == -2
-    assert o(fake, 0, -1, 40, 40, fake, nul, nul, nul) == -2
-    assert o(fake, 0, 1 << 25, 1 << 12, 1 << 12, fake, nul, nul, nul) == -2
-    assert o(fake, 5, 4, 40, 40, fake, nul, nul, nul) == -4
-    assert o(fake, 0, 4, 40, 40, odd, nul, nul, nul) == -3
-    assert o(fake, 0, 4, 40, 40, nul, odd, nul, nul) == -3
-    assert o(fake, 0, 4, 40, 40, fake, nul, odd, nul) == -3         # the seed
-    assert o(nul, 0, 0, 40, 40, fake, nul, nul, nul) == 0
+    assert o(fake, 0, 4, 40, 40, nul, nul, nul, nul, nul) == -1          # neither wanted
+    assert o(nul, 0, 4, 40, 40, fake, nul, nul, nul, nul) == -1
+    assert o(fake, 0, 4, 40, 39, fake, nul, nul, nul, nul) == -2         # rows that overlap
+    assert o(fake, 0, 4, 0, 40, fake, nul, nul, nul, nul) == -2
+    assert o(fake, 0, -1, 40, 40, fake, nul, nul, nul, nul) == -2
+    assert o(fake, 0, 1 << 25, 1 << 12, 1 << 12, fake, nul, nul, nul, nul) == -2
+    assert o(fake, 5, 4, 40, 40, fake, nul, nul, nul, nul) == -4
+    assert o(fake, 0, 4, 40, 40, odd, nul, nul, nul, nul) == -3
+    assert o(fake, 0, 4, 40, 40, nul, odd, nul, nul, nul) == -3
+    assert o(fake, 0, 4, 40, 40, fake, nul, nul, odd, nul) == -3         # the seed
+    assert o(fake, 0, 4, 40, 40, fake, nul, fake, nul, nul) == -1    # sums without the columns
+    assert o(nul, 0, 0, 40, 40, fake, nul, nul, nul, nul) == 0
     g = lib.dpa_mxfp4_gemm
     assert g(fake, nul, nul, fake, 0, 4, 4, 32, nul, 0, nul) == -1
     assert g(fake, fake, nul, fake, 0, 4, 4, 0, nul, 0, nul) == -2
