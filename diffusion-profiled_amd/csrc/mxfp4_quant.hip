@@ -264,14 +264,14 @@ __device__ __forceinline__ uint32_t down_pair(const Quad<DT>& a, const Quad<DT>&
   return perm_b32(j < 2 ? b.w.x : b.w.y, j < 2 ? a.w.x : a.w.y, j & 1 ? 0x07060302u : 0x05040100u);
 }
 
-template <int DT, bool kWide, bool SR>
+template <int DT, bool kWide, bool SR, bool kSum>
 __global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p) {
   constexpr int kPitch = 36;  // bytes of a column in LDS (lanes then lie in different banks)
   constexpr int kW = ColMax<DT>::kWords;
   __shared__ __attribute__((aligned(16))) uint8_t out[256 * kPitch];
   __shared__ __attribute__((aligned(16))) uint32_t tops[8][64 * kW];
   __shared__ __attribute__((aligned(8))) uint8_t bytes[2][256];
-  __shared__ __attribute__((aligned(16))) float sums[8][256];
+  __shared__ __attribute__((aligned(16))) float sums[kSum ? 8 : 1][256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = wave >> 2, sub = wave & 3;
   // workgroups i, i + 8, i + 16, i + 24 of 32 (on one XCD): the tiles below each other of a line
@@ -283,6 +283,14 @@ __global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p) {
   Quad<DT> x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = quad_at<DT, kWide>(p, r0 + i, c0);
+  if constexpr (kSum) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] += x[i].get(j);
+    *reinterpret_cast<float4*>(&sums[wave][4 * lane]) = float4{s[0], s[1], s[2], s[3]};
+  }
   uint32_t rnd[SR ? 8 : 1][4];
   if constexpr (SR) {
     const uint64_t z_row = (uint64_t)((p.cols + kBlock - 1) / kBlock) * (kBlock / 4) * kDropGolden;
@@ -294,14 +302,6 @@ __global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) top.take(x[i]);
   top.put(&tops[wave][lane * kW]);
-  if (p.sums) {
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] += x[i].get(j);
-    *reinterpret_cast<float4*>(&sums[wave][4 * lane]) = float4{s[0], s[1], s[2], s[3]};
-  }
   // rows
   if (p.row_data) {
     uint32_t mine = 0;  // lane 8 b + i: the scale of row i, block b
@@ -330,11 +330,13 @@ __global__ __launch_bounds__(512) void mxfp4_both_kernel(const BothArgs p) {
   }
   wait_lgkmcnt0();
   lds_barrier();
-  if (p.sums && threadIdx.x < 256 && tc * 256 + threadIdx.x < p.cols && tr * 64 < p.rows) {
-    float s = 0.f;
+  if constexpr (kSum) {
+    if (threadIdx.x < 256 && tc * 256 + threadIdx.x < p.cols && tr * 64 < p.rows) {
+      float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) s += sums[w][threadIdx.x];
-    p.sums[tr * p.cols + tc * 256 + threadIdx.x] = s;
+      for (int w = 0; w < 8; ++w) s += sums[w][threadIdx.x];
+      p.sums[tr * p.cols + tc * 256 + threadIdx.x] = s;
+    }
   }
   // columns: word `sub` of block `half`
 #pragma unroll
@@ -442,19 +444,24 @@ static int run_rows(const RowArgs& p, bool operand, bool wide, hipStream_t s) {
   return launch_status();
 }
 
-template <int DT, bool kWide>
+template <int DT, bool kWide, bool SR>
 static int run_both(const BothArgs& p, hipStream_t s) {
   const unsigned grid = (unsigned)(ceil_div(p.lines, 8) * 32);
-  if (p.seed)
-    mxfp4_both_kernel<DT, kWide, true><<<grid, 512, 0, s>>>(p);
+  if (p.sums)
+    mxfp4_both_kernel<DT, kWide, SR, true><<<grid, 512, 0, s>>>(p);
   else
-    mxfp4_both_kernel<DT, kWide, false><<<grid, 512, 0, s>>>(p);
+    mxfp4_both_kernel<DT, kWide, SR, false><<<grid, 512, 0, s>>>(p);
   return launch_status();
+}
+
+template <int DT, bool SR>
+static int run_both(const BothArgs& p, bool wide, hipStream_t s) {
+  return wide ? run_both<DT, true, SR>(p, s) : run_both<DT, false, SR>(p, s);
 }
 
 template <int DT>
 static int run_operands(const RowArgs& r, const BothArgs& b, bool wide, hipStream_t s) {
-  if (b.col_data) return wide ? run_both<DT, true>(b, s) : run_both<DT, false>(b, s);
+  if (b.col_data) return b.seed ? run_both<DT, true>(b, wide, s) : run_both<DT, false>(b, wide, s);
   return r.seed ? run_rows<DT, true>(r, true, wide, s) : run_rows<DT, false>(r, true, wide, s);
 }
 
