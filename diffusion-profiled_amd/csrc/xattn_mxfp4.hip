@@ -55,7 +55,9 @@ __device__ __forceinline__ void put_block(uint32_t at, int row, int blk, const R
 }
 
 // ---------------------------------------------------------------------------------------
-// Four waves of 32 query rows share tiles of 64 keys; a tile's blocks go through registers, one tile ahead.
+// Four waves of 32 query rows share tiles of 64 keys; a tile's blocks go through registers, one tile ahead. Bound as the
+// 16-bit form is, by the products and the softmax; the conversions cost what the shorter loads save: 8 x 1024 queries
+// of 8 heads of 128 over 4096 keys 152 us, there 150; 4 x 4096 of 8 heads of 64 over 1031 keys in fp16 55.5, there 52.2.
 // ---------------------------------------------------------------------------------------
 constexpr float kSlack = 8.f;
 
@@ -229,7 +231,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_mxfp4_fwd_kernel
 // ---------------------------------------------------------------------------------------
 // Few rows: four waves share 32 rows and take every fourth tile of 32 keys each, and join their softmaxes
 // in LDS. A lane's key goes straight to its A operand: dims [h DP / 2, (h + 1) DP / 2) of key l & 31, eight of
-// them to a product, and the queries likewise. Values pass through LDS, whose transpose reads turn them.
+// them to a product, and the queries likewise. Values pass through LDS, whose transpose reads turn them. 16 x 8
+// queries of 16 heads, four to a key head of 128, over 4096 keys 30.9 us with the join, in 16 bits 36.1.
 // ---------------------------------------------------------------------------------------
 template <class T, int DP>
 __global__ __launch_bounds__(256, 2) void xattn_mxfp4_few_kernel(const MxArgs p) {
@@ -701,7 +704,7 @@ __global__ __launch_bounds__(256, 2) void xattn_mxfp4_token_kernel(const MxArgs 
 
 // ---------------------------------------------------------------------------------------
 // Up to 128 keys: xattn_short.hpp over the values that a workgroup makes of them once. 128 x 1024 queries of 4 heads of
-// 64 dims over 77 keys 40 us by tiles of keys.
+// 64 dims over 77 keys 30.2 us, by tiles of keys 40, in 16 bits 30.3: bound by the queries and the output.
 // ---------------------------------------------------------------------------------------
 template <class T, int DP, int NB>
 __global__ __launch_bounds__(256, short_waves(DP)) void xattn_mxfp4_short_kernel(const MxArgs p) {
