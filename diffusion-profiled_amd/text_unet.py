@@ -66,7 +66,7 @@ class CrossAttentionBlock(nn.Module):
         """Keys and values [B, L, 2, heads, head_dim] of the states; a sampler keeps them over its
         steps."""
         b, l, _ = states.shape
-        return self.kv(states).view(b, l, 2, self.heads, -1)
+        return self.kv(states).view(b, l, 2, self.heads, self.norm.weight.numel() // self.heads)
 
     def forward(self, x: torch.Tensor, kv: torch.Tensor | MXFP4, key_mask: torch.Tensor | None) -> torch.Tensor:
         b, c, h, w = x.shape

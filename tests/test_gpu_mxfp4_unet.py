@@ -248,6 +248,71 @@ def test_operators_compile():
     assert not [str(w.message) for w in seen if "dpa_fast_calls" in str(w.message) or "builtin" in str(w.message)]
 
 
+def test_text_unet_compiles(seeds):
+    m = _model(text=_four()).train()
+    g = torch.Generator().manual_seed(13)
+    x, t, tokens = _images(2, g), torch.tensor([3, 70], device="cuda"), _tokens(2, 12, g)
+
+    def step(model):
+        m.zero_grad(set_to_none=True)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            y = model(x, t, tokens)
+        y.float().square().mean().backward()
+        return [y.detach()] + [p.grad.clone() for p in m.parameters()]
+    want = step(m)
+    torch._dynamo.reset()
+    fn = torch.compile(m, backend="aot_eager")
+    for _ in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(step(fn), want))
+    m.eval()
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        m.keep_prompt(tokens, bits=4)
+        m.keep_weights()
+        want = m(x, t)
+        assert torch.equal(fn(x, t), want)
+
+
+@pytest.mark.parametrize("length", [0, 1])
+def test_shortest_prompts_kept_in_four_bits(length):
+    g = torch.Generator().manual_seed(14)
+    m = _model(text=_four()).eval()
+    x, t = _images(2, g), torch.tensor([3, 70], device="cuda")
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        plain = m(x, t)
+        m.keep_prompt(torch.zeros((2, length), dtype=torch.int64, device="cuda"), bits=4)
+        assert torch.equal(m(x, t), plain)      # no token but the padding
+
+
+def test_two_graphs_and_eager_calls_between():
+    """Two captured graphs of split products and split keys, whose workspaces are their own, replayed in turn."""
+    g = torch.Generator().manual_seed(15)
+    w = M.mxfp4_operand(torch.randn((96, 8192), generator=g).bfloat16().cuda())
+    kv = M.quantize_mxfp4(torch.randn((2, 4000, 2, 1, 64), generator=g).bfloat16().cuda())
+    xs = [torch.zeros((100, 8192), device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+
+    def run(x):
+        y = M.linear_mxfp4_fwd(x, w)
+        return y, M.cross_attention_mxfp4(y[:, :64].reshape(2, 50, 1, 64)[:, :4], kv)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        run(xs[0])
+    torch.cuda.current_stream().wait_stream(stream)
+    graphs, outs = [], []
+    for x in xs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run(x))
+    for i in range(4):
+        for x in xs:
+            x.copy_(torch.randn(x.shape, generator=g).bfloat16())
+        graphs[i % 2].replay()
+        want = [run(x) for x in xs]
+        graphs[1 - i % 2].replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert all(torch.equal(u, v) for u, v in zip(a, b)), i
+
+
 def test_example_runs():
     spec = importlib.util.spec_from_file_location("text_to_image", os.path.join(ROOT, "examples", "text_to_image.py"))
     ex = importlib.util.module_from_spec(spec)
