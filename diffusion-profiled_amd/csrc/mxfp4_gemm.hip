@@ -54,17 +54,14 @@ __device__ __forceinline__ void dma16_from(const void* base, uint32_t off, uint3
 // live at once, and gives results other registers than the sums had (207 registers spilled of the 128 x 64
 // wave, 0.7 PFLOP/s). It does not know these for matrix instructions, so the waits are here: s_nop before a product
 // whose scales a vector instruction may just have written, and results_ready before the sums are read.
-template <int AT, bool kAcc>
+template <int AT>
 __device__ __forceinline__ void mfma_in_place(v4f& acc, u32x4 a, u32x4 b, uint32_t sa, uint32_t sb) {
-#define DPA_MFMA(SEL)                                                                                                     \
-  if constexpr (kAcc)                                                                                                     \
-    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " SEL " cbsz:4 blgp:4" : "+a"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb)); \
-  else                                                                                                                    \
-    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " SEL " cbsz:4 blgp:4" : "+v"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb))
-  if constexpr (AT == 0) { DPA_MFMA("op_sel_hi:[0,0,0]"); }
-  if constexpr (AT == 1) { DPA_MFMA("op_sel:[1,1,0] op_sel_hi:[0,0,0]"); }
-  if constexpr (AT == 2) { DPA_MFMA("op_sel_hi:[1,1,0]"); }
-  if constexpr (AT == 3) { DPA_MFMA("op_sel:[1,1,0] op_sel_hi:[1,1,0]"); }
+#define DPA_MFMA(SEL) \
+  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " SEL " cbsz:4 blgp:4" : "+v"(acc) : "v"(a), "v"(b), "v"(sa), "v"(sb))
+  if constexpr (AT == 0) DPA_MFMA("op_sel_hi:[0,0,0]");
+  if constexpr (AT == 1) DPA_MFMA("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
+  if constexpr (AT == 2) DPA_MFMA("op_sel_hi:[1,1,0]");
+  if constexpr (AT == 3) DPA_MFMA("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
 #undef DPA_MFMA
 }
 // 16 passes and more after the last product
@@ -89,10 +86,11 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_gemm_kernel(const GemmArgs
   constexpr int kXferB = BN / 16 / kWaves, kXferA = BM / 16 / kWaves, kXfer = kXferB + kXferA;
   static_assert(BN % (16 * kWaves) == 0 && BM % (16 * kWaves) == 0, "transfers of 16 rows");
   static_assert(FN % 2 == 0 && kWaves % 2 == 0 && NH % 4 == 0, "pairs of fragments; a row's place among 32; groups");
-  constexpr int kPieces = (BM + BN) / 64, kXferS = (kPieces + kWaves - 1) / kWaves;
-  constexpr bool kAcc = FM * FN >= 64;  // sums of 256 registers are the accumulation registers
-  // 8 rows of up to 64 of a wave's columns in turn, granule g of 4 columns of row r at g ^ r
-  constexpr int kCols = FN > 4 ? 64 : 16 * FN, kParts = 16 * FN / kCols;
+  constexpr int kPieces = (BM + BN) / 64;
+  static_assert(kPieces <= kWaves, "at most a transfer of scales to a wave");
+  // 8 rows of a wave's columns in turn, granule g of 4 columns of row r at g ^ r
+  constexpr int kCols = 16 * FN;
+  static_assert(kCols <= 64, "a row to a wave");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kS + kSlots * kBytesS + (vec ? 0 : kWaves * 8 * kCols * 4)];
   const uint32_t l0 = LDS_ADDR(lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -129,14 +127,11 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_gemm_kernel(const GemmArgs
   const uint32_t off_b = opaque(lr * 64 + (((lane & 3) ^ place_b(16 * wave + lr)) << 4));
   const uint32_t off_a = opaque(lr * 64 + (((lane & 3) ^ place_a(lr)) << 4));
   const int last_a = (int)padded_rows(p.M) - 16, last_b = (int)padded_rows(p.N) - 16;
+  const int part = wave % kPieces;
   auto fetch_scales = [&](int group, int slot) __attribute__((always_inline)) {
-#pragma unroll
-    for (int k = 0; k < kXferS; ++k) {
-      const int part = (k * kWaves + wave) % kPieces;
-      const uint8_t* from = part < BN / 64 ? p.bs + ((int64_t)group * p.N + c.n0 + 64 * part) * 16
-                                           : p.as + ((int64_t)group * p.M + c.m0 + 64 * (part - BN / 64)) * 16;
-      dma16_from(from, (uint32_t)lane * 16, l0 + kS + slot * kBytesS + part * 1024);
-    }
+    const uint8_t* from = part < BN / 64 ? p.bs + ((int64_t)group * p.N + c.n0 + 64 * part) * 16
+                                         : p.as + ((int64_t)group * p.M + c.m0 + 64 * (part - BN / 64)) * 16;
+    dma16_from(from, (uint32_t)lane * 16, l0 + kS + slot * kBytesS + part * 1024);
   };
   const uint8_t* from[kXfer];  // where each transfer goes on
   auto fetch1 = [&](int i, int buf) __attribute__((always_inline)) {
@@ -210,11 +205,11 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_gemm_kernel(const GemmArgs
       for (int i = 1; i <= NH - 2; ++i) n += (k + NH - i) % 4 == 0;
       return n;
     }(k);
-    constexpr int kBehind = (NH - 2) * kXfer + kGroups * kXferS;
+    constexpr int kBehind = (NH - 2) * kXfer + kGroups;
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
 #pragma unroll
-      for (int i = 0; i < FN; ++i) mfma_in_place<k % 4, kAcc>(acc[i][j], fb[t][i], fa[j], sb[i], sa[j]);
+      for (int i = 0; i < FN; ++i) mfma_in_place<k % 4>(acc[i][j], fb[t][i], fa[j], sb[i], sa[j]);
       if (j < kMeet) continue;
       if (j == kMeet) {
         __builtin_amdgcn_sched_barrier(0);
@@ -317,39 +312,36 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_gemm_kernel(const GemmArgs
     }
     // Rows that no vector fits: 8 of them turn in LDS, so that neighbouring lanes store neighbours (each lane its
     // 8 one by one: 3850 x 1023 of 513 in fp32 22.5 us, against 16.3)
+    const int col = lane % kCols, at = n + col;
+    const uint32_t off = at < p.N ? (uint32_t)(lane / kCols * p.N + at) * kSize : kNowhere;
 #pragma unroll
-    for (int h = 0; h < kParts; ++h) {
-      const int col = lane % kCols, at = n + h * kCols + col;
-      const uint32_t off = at < p.N ? (uint32_t)(lane / kCols * p.N + at) * kSize : kNowhere;
+    for (int j = 0; j < 2 * FM; ++j) {
+      if ((r >> 3) == (j & 1)) {
 #pragma unroll
-      for (int j = 0; j < 2 * FM; ++j) {
-        if ((r >> 3) == (j & 1)) {
+        for (int i = 0; i < kCols / 16; ++i) {
+          v4f v = acc[i][j / 2];
 #pragma unroll
-          for (int i = 0; i < kCols / 16; ++i) {
-            v4f v = acc[h * (kCols / 16) + i][j / 2];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += bias[h * (kCols / 32) + i / 2][4 * (i % 2) + e];
-            *reinterpret_cast<float4*>(turn + (r & 7) * kCols + (((8 * (i / 2) + 2 * q + i % 2) ^ (r & 7)) << 2)) =
-                float4{v[0], v[1], v[2], v[3]};
-          }
+          for (int e = 0; e < 4; ++e) v[e] += bias[i / 2][4 * (i % 2) + e];
+          *reinterpret_cast<float4*>(turn + (r & 7) * kCols + (((8 * (i / 2) + 2 * q + i % 2) ^ (r & 7)) << 2)) =
+              float4{v[0], v[1], v[2], v[3]};
         }
-        asm volatile("" ::: "memory");
-        const __amdgpu_buffer_rsrc_t rows = rows_at(m + 8 * j, 8);
-#pragma unroll
-        for (int i = 0; i < 8 * kCols / 64; ++i) {
-          const int row = i * (64 / kCols) + lane / kCols;
-          const float v = turn[row * kCols + (((col >> 2) ^ row) << 2) + (col & 3)];
-          const uint32_t from = off == kNowhere ? off : off + (uint32_t)(i * (64 / kCols) * p.N) * kSize;
-          if constexpr (DT == DPA_DTYPE_F32)
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rows, from, 0, 0);
-          else
-            __builtin_amdgcn_raw_buffer_store_b16((uint16_t)Elem<DT>::pack(v, v), rows, from, 0, 0);
-        }
-        asm volatile("" ::: "memory");
       }
+      asm volatile("" ::: "memory");
+      const __amdgpu_buffer_rsrc_t rows = rows_at(m + 8 * j, 8);
+#pragma unroll
+      for (int i = 0; i < 8 * kCols / 64; ++i) {
+        const int row = i * (64 / kCols) + lane / kCols;
+        const float v = turn[row * kCols + (((col >> 2) ^ row) << 2) + (col & 3)];
+        const uint32_t from = off == kNowhere ? off : off + (uint32_t)(i * (64 / kCols) * p.N) * kSize;
+        if constexpr (DT == DPA_DTYPE_F32)
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rows, from, 0, 0);
+        else
+          __builtin_amdgcn_raw_buffer_store_b16((uint16_t)Elem<DT>::pack(v, v), rows, from, 0, 0);
+      }
+      asm volatile("" ::: "memory");
     }
   };
-  constexpr int kAhead = (NH - 1) * kXfer + (NH / 4 - 1) * kXferS;  // transfers behind a tile's first
+  constexpr int kAhead = (NH - 1) * kXfer + NH / 4 - 1;  // transfers behind a tile's first
   static_assert(kAhead < 64, "vmcnt");
   begin();
   for (uint32_t id = blockIdx.x;;) {
@@ -753,7 +745,7 @@ static int run_tiles(GemmArgs p, hipStream_t s) {
     p.tiles_m = (int)ceil_div(p.M, kForms[1].side), p.tiles_n = (int)ceil_div(p.N, kForms[1].side);
   }
   const int64_t items = ceil_div((int64_t)p.tiles_m * p.tiles_n * p.splits, 8) * 8;
-  const unsigned grid = (unsigned)std::min<int64_t>(items, kForms[p.form].per_cu * num_cus());
+  const unsigned grid = (unsigned)std::min<int64_t>(items, kForms[p.form].per_cu * num_cus() / 8 * 8);
   if (p.form == 0)
     mxfp4_gemm_kernel<2, 4, 8, 4, 4, DT, true><<<grid, 512, 0, s>>>(p);
   else if (p.form == 1)
