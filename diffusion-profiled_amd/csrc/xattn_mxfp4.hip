@@ -445,8 +445,10 @@ __global__ __launch_bounds__(256, 2) void xattn_mxfp4_few_kernel(const MxArgs p)
 
 // ---------------------------------------------------------------------------------------
 // Up to 16 rows of a key head (single tokens, their heads sharing keys): as above, on v_mfma_f32_16x16x32, whose
-// columns are the rows, a tile of 32 keys to a wave, two on their way. Bound by the conversions' instructions: a tile
-// takes 0.9 us of a SIMD's time whatever is on its way, the cache alone would be there in half of that.
+// columns are the rows, a tile of 32 keys to a wave, two on their way. Bound by a wave's chain of a tile, 1.5 us from its
+// loads to its second product, of which a wave has eight in a row over 8192 keys of 64 heads: three or four tiles on
+// their way did not shorten it (20.3 us there, 23 and 24), nor did keys that went into the product in 4 bits, against
+// queries split into sums of e4m3 (half the conversions, 20.4).
 //   S^T (16 keys x 16 rows) = K Q^T: lane (key l & 15, q = l >> 4) takes dims [q D / 4, (q + 1) D / 4) of its key, 8 to
 //   a product. It receives the scores of row l & 15 at keys 4 q + t of each 16, which packed are the B operand of
 //   O^T += V^T P^T if the sum over 32 keys runs over {4 q + t, 16 + 4 q + t} in lane q: so the values' transpose
@@ -494,7 +496,11 @@ __global__ __launch_bounds__(256, 2) void xattn_mxfp4_token_kernel(const MxArgs 
   if (id >= p.total) return;
   // the heads of a batch's keys beside each other: their pieces of a token share cache lines
   const uint32_t bs = id / (uint32_t)p.KVH;
-  const int g = id - bs * p.KVH, b = bs / (uint32_t)p.splits, split = bs - b * p.splits, bkv = b * p.KVH + g;
+  const int g = id - bs * p.KVH, b = bs / (uint32_t)p.splits, bkv = b * p.KVH + g;
+  // (a batch's first split is another one each time: with a multiple of 8 of them the first ones, which have keys when
+  // others have none, would all go to one XCD. Lengths of 1024 in 8191, 16 batches of 4 heads: 19.4 us against 20.7)
+  const int turned = bs - b * p.splits + (uint32_t)b % (uint32_t)p.splits;
+  const int split = turned < p.splits ? turned : turned - p.splits;
 
   const int klen = __builtin_amdgcn_readfirstlane(keys_of(p, b));
   const int nt = (klen + KT - 1) / KT;
@@ -775,7 +781,7 @@ static void plan_mx(Args& p) {
   const int64_t groups = (int64_t)p.B * p.KVH;
   // two workgroups to a CU; what fills the CUs without is not split, and no row into more than 64 parts, which the
   // join would wait for (16 queries over up to 8191 keys of 4 heads of 128, 48 MB of cache: 20.3 us, with three to a
-  // CU 22.7, with four 22.0: a wave's first and last tile cost as much as ten between)
+  // CU 22.7, with four 22.0; lengths of 1024 in 8191 19.4, 15.5 and 16.4)
   const int64_t want = groups >= 2 * num_cus() ? groups : std::min<int64_t>(2 * num_cus(), 64 * groups);
   choose_splits(p, groups, ceil_div(p.Lk, 32), want, 8, kMaxRange / 32, 4);
   // A head's piece of a token is 16 to 64 B and its scales 1 to 4, so that cache lines hold those of several: the
