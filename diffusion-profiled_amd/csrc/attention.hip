@@ -110,7 +110,7 @@ __device__ __forceinline__ void att_dma(const uint16_t* src, int64_t pitch, int 
 
 // 4 B per lane to lds + 4 * lane (lds wave-uniform), from any 4-byte aligned source.
 __device__ __forceinline__ void dma4_lds(const void* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "m0");
 }
 
 struct AttnArgs {

@@ -310,15 +310,17 @@ struct Elem<DPA_DTYPE_F16> {
 // lists it as clobbered; clang warns that m0 is a reserved register whose value it may not
 // preserve around the statement. In the kernels built here nothing else uses m0 (in the
 // compiled igemm / hwgrad / wgrad / attention code every m0 access is the s_mov of such a pair,
-// or of attention's 4-B one), so no compiler-held value is live across it.
+// or of attention's 4-B one), so no compiler-held value is live across it. One wait state lies
+// between the scalar write of m0 and the load that reads it (s_nop 0), which the ISA asks of
+// software before a load to LDS and the compiler puts there for its own.
 __device__ __forceinline__ void dma16(const void* src, const void* lds) {
   const uint32_t l = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)LDS_PTR(lds));
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(l) : "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(l) : "m0");
 }
 
 // Same DMA with the LDS destination given as a 32-bit LDS address (wave-uniform).
 __device__ __forceinline__ void dma16_lds(const void* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "m0");
 }
 
 // 32-bit LDS address of a __shared__ object (no generic-pointer null check).

@@ -46,7 +46,7 @@ __device__ __forceinline__ uint32_t opaque(uint32_t x) {
 __device__ __forceinline__ u32x4 lds16(uint32_t a) { return *(const __attribute__((address_space(3))) u32x4*)(a); }
 
 __device__ __forceinline__ void dma16_from(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "m0");
 }
 
 // acc += the product, in its own registers (AT: the byte of both scale words). As instructions of their own, in

@@ -203,12 +203,12 @@ __device__ __forceinline__ void dma_rows(uint32_t lds, int c0, int lane, int D, 
 
 // 16 B per lane from base (wave-uniform) + off bytes
 __device__ __forceinline__ void dma16_lds_from(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "m0");
 }
 
 // 4 B per lane to lds + 4 * lane (lds wave-uniform).
 __device__ __forceinline__ void dma4_lds(const void* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "m0");
 }
 
 // Which keys of a workgroup's range [k0, k1) are visible, in words of 32 or 64 keys. Mask bytes are
