@@ -252,6 +252,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dpa_mxfp4_dequantize": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p]),
     "dpa_mxfp4_operand_bytes": (c_int64, [c_int64, c_int64]),
     "dpa_mxfp4_operands": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64] + [c_void_p] * 5),
+    "dpa_mxfp4_gemm_plan": (c_int, [c_int64] * 3 + [c_int, c_void_p]),
     "dpa_mxfp4_gemm_workspace_bytes": (c_int64, [c_int64] * 3),
     "dpa_mxfp4_gemm": (c_int, [c_void_p] * 4 + [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
     "dpa_mxfp4_linear_workspace_bytes": (c_int64, [c_void_p, c_int] + [c_int64] * 4),

@@ -53,7 +53,7 @@ __device__ __forceinline__ void dma16_from(const void* base, uint32_t off, uint3
 // their place: the compiler moves products of its own freely between the halves of a step, until all their fragments
 // live at once, and gives results other registers than the sums had (207 registers spilled of the 128 x 64
 // wave, 0.7 PFLOP/s). It does not know these for matrix instructions, so the waits are here: s_nop before a product
-// whose scales a vector instruction may just have written, and results_ready before the sums are read.
+// whose scales or sums a vector instruction may just have written, and results_ready before the sums are read.
 template <int AT>
 __device__ __forceinline__ void mfma_in_place(v4f& acc, u32x4 a, u32x4 b, uint32_t sa, uint32_t sb) {
 #define DPA_MFMA(SEL) \
@@ -195,6 +195,16 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_gemm_kernel(const GemmArgs
 #pragma unroll
       for (int j = 0; j < FM; ++j) sa[j] = sa_next[j];
       slot = slot + 1 == kSlots ? 0 : slot + 1;
+      // Scales, and the sums of a tile's first panel, are vector instructions' results (the sums zeros, which the
+      // compiler would otherwise write anew in front of the products): all of them in front of this wait
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        asm volatile("" : "+v"(sb[i]));
+#pragma unroll
+        for (int j = 0; j < FM; ++j) asm volatile("" : "+v"(acc[i][j]));
+      }
+#pragma unroll
+      for (int j = 0; j < FM; ++j) asm volatile("" : "+v"(sa[j]));
       __builtin_amdgcn_sched_barrier(0);
       asm volatile("s_nop 3");
     }
@@ -737,15 +747,23 @@ static int join(const GemmArgs& p, hipStream_t s) {
   return launch_status();
 }
 
-template <int DT>
-static int run_tiles(GemmArgs p, hipStream_t s) {
-  const bool vec = p.N % (16 / Elem<DT>::size) == 0 && aligned(p.y, 16);
+// Whether 16 B of y at a time fit its rows
+static bool whole_vectors(int64_t N, int dtype) { return N % (16 / size_of(dtype)) == 0; }
+
+// The form for a y that vectors fit or not, and its workgroups
+static unsigned settle(GemmArgs& p, bool vec) {
   if (!vec && p.form == 0) {  // (the largest tiles leave no registers to turn rows)
     p.form = 1;
     p.tiles_m = (int)ceil_div(p.M, kForms[1].side), p.tiles_n = (int)ceil_div(p.N, kForms[1].side);
   }
   const int64_t items = ceil_div((int64_t)p.tiles_m * p.tiles_n * p.splits, 8) * 8;
-  const unsigned grid = (unsigned)std::min<int64_t>(items, kForms[p.form].per_cu * num_cus() / 8 * 8);
+  return (unsigned)std::min<int64_t>(items, kForms[p.form].per_cu * num_cus() / 8 * 8);
+}
+
+template <int DT>
+static int run_tiles(GemmArgs p, hipStream_t s) {
+  const bool vec = whole_vectors(p.N, DT) && aligned(p.y, 16);
+  const unsigned grid = settle(p, vec);
   if (p.form == 0)
     mxfp4_gemm_kernel<2, 4, 8, 4, 4, DT, true><<<grid, 512, 0, s>>>(p);
   else if (p.form == 1)
@@ -809,6 +827,27 @@ static bool takes_token(const void* x, int dtype, int64_t ld, int64_t M, int64_t
 
 using namespace dpa;
 using namespace dpa::mx;
+
+extern "C" int dpa_mxfp4_gemm_plan(int64_t M, int64_t N, int64_t K, int dtype, DpaMxfp4GemmPlan* out) {
+  if (!dtype_ok(dtype)) return DPA_ERR_SHAPE;
+  const int st = check_gemm(M, N, K);
+  if (st != DPA_OK) return st;
+  if (!out) return DPA_ERR_NULL;
+  *out = DpaMxfp4GemmPlan{};
+  if (M == 0 || N == 0) return DPA_OK;
+  GemmArgs p = plan(M, N, K, false);
+  out->splits = p.splits;
+  if (M <= kFewRows) {
+    out->workgroups = p.tiles_n * p.splits;
+    out->tiles = out->workgroups;
+    return DPA_OK;
+  }
+  out->vectors = whole_vectors(N, p.splits > 1 ? DPA_DTYPE_F32 : dtype);
+  out->workgroups = (int32_t)settle(p, out->vectors != 0);
+  out->side = kForms[p.form].side;
+  out->tiles = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+  return DPA_OK;
+}
 
 extern "C" int64_t dpa_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   return check_gemm(M, N, K) == DPA_OK ? part_bytes(plan(M, N, K, false)) : 0;

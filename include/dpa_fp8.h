@@ -879,6 +879,16 @@ int64_t dpa_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int dpa_mxfp4_gemm(const void* a, const void* b, const float* bias, void* y, int dtype, int64_t M, int64_t N,
                    int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* What dpa_mxfp4_gemm would launch, on a device like the current one, for a 16-B aligned y: tiles of side x side (0: a form for
+ * up to 64 rows) of y and of the `splits` of K, taken in turn by `workgroups`; vectors: whether y leaves by
+ * 16 B. Launches nothing; DPA_ERR_SIZE for a size that dpa_mxfp4_gemm refuses. */
+typedef struct DpaMxfp4GemmPlan {
+  int32_t side, vectors, splits, workgroups;
+  int64_t tiles;
+} DpaMxfp4GemmPlan;
+
+int dpa_mxfp4_gemm_plan(int64_t M, int64_t N, int64_t K, int dtype, DpaMxfp4GemmPlan* plan);
+
 /* The same from x [M][K] itself (rows row_stride elements apart), rounded to nearest: for few rows within the
  * product's launch, else laid out in the workspace first (x's alignment has a say in it; the query reads
  * nothing). */

@@ -86,3 +86,10 @@ def kernels_of(assembly: str) -> dict[str, Kernel]:
 def m0_too_close(kernel: Kernel) -> list[str]:
     """One state from a scalar write of m0 to a load to LDS, which reads it."""
     return kernel.closer(1, lambda c: c.writes_m0, lambda c, d: d.to_lds)
+
+
+def products_too_close(kernel: Kernel) -> list[str]:
+    """Two states from a vector instruction's result to a matrix instruction that reads it, twelve from a matrix instruction
+    of eight passes to any other that touches its result."""
+    return (kernel.closer(2, lambda c: c.vector and c.writes, lambda c, d: d.matrix and c.writes & d.touches)
+            + kernel.closer(12, lambda c: c.matrix, lambda c, d: not d.matrix and c.writes & d.touches))
