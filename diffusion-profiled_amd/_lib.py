@@ -320,7 +320,7 @@ _FAST_ENTRIES = ("dpa_cross_attention_fwd", "dpa_cross_attention_fwd_workspace_b
                  "dpa_cross_attention_bwd", "dpa_cross_attention_bwd_workspace_bytes", "dpa_dropout",
                  "dpa_embedding_fwd", "dpa_embedding_bwd", "dpa_embedding_bwd_workspace_bytes",
                  "dpa_status_string", "dpa_mxfp4_quantize", "dpa_mxfp4_dequantize", "dpa_mxfp4_operand_bytes",
-                 "dpa_mxfp4_operands", "dpa_mxfp4_gemm", "dpa_mxfp4_gemm_workspace_bytes", "dpa_mxfp4_linear",
+                 "dpa_mxfp4_operands", "dpa_mxfp4_gemm", "dpa_mxfp4_gemm_workspace_bytes", "dpa_mxfp4_gemm_plan", "dpa_mxfp4_linear",
                  "dpa_mxfp4_linear_workspace_bytes", "dpa_column_sum", "dpa_column_sum_workspace_bytes",
                  "dpa_cross_attention_mxfp4", "dpa_cross_attention_mxfp4_workspace_bytes")
 

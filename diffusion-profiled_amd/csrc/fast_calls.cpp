@@ -34,6 +34,7 @@ decltype(&dpa_mxfp4_operand_bytes) mx_operand_bytes;
 decltype(&dpa_mxfp4_operands) mx_operands;
 decltype(&dpa_mxfp4_gemm) mx_gemm;
 decltype(&dpa_mxfp4_gemm_workspace_bytes) mx_gemm_bytes;
+decltype(&dpa_mxfp4_gemm_plan) mx_plan;
 decltype(&dpa_mxfp4_linear) mx_linear;
 decltype(&dpa_mxfp4_linear_workspace_bytes) mx_linear_bytes;
 decltype(&dpa_column_sum) column_sum;
@@ -435,7 +436,10 @@ PyObject* mxfp4_train_fwd(PyObject*, PyObject* const* o, Py_ssize_t count) {
       !bias_ok(bias, n))
     return none();
   const int64_t xr = mx_operand_bytes(m, k), xc = mx_operand_bytes(k, m), wr = mx_operand_bytes(n, k), wc = mx_operand_bytes(k, n);
-  if (!xr || !xc || !wr || !wc) return none();
+  // (of the gradients' products too: sizes that one of them does not take are refused before a launch)
+  if (!xr || !xc || !wr || !wc || mx_plan(m, n, k, DPA_DTYPE_F32, nullptr) || mx_plan(m, k, n, DPA_DTYPE_F32, nullptr) ||
+      mx_plan(n, k, m, DPA_DTYPE_F32, nullptr))
+    return none();
   const int64_t gemm = mx_gemm_bytes(m, n, k), at_w = round256(xr), at_ws = at_w + round256(wr);
   at::DimVector shape(x->sizes().begin(), x->sizes().end());
   shape.back() = n;
@@ -546,7 +550,7 @@ PyObject* init(PyObject*, PyObject* const* o, Py_ssize_t n) {
   void** const to[] = {(void**)&attn_fwd, (void**)&attn_fwd_bytes, (void**)&attn_bwd, (void**)&attn_bwd_bytes, (void**)&drop,
                        (void**)&emb_fwd, (void**)&emb_bwd, (void**)&emb_bwd_bytes, (void**)&status_string,
                        (void**)&mx_quant, (void**)&mx_dequant, (void**)&mx_operand_bytes, (void**)&mx_operands,
-                       (void**)&mx_gemm, (void**)&mx_gemm_bytes, (void**)&mx_linear, (void**)&mx_linear_bytes,
+                       (void**)&mx_gemm, (void**)&mx_gemm_bytes, (void**)&mx_plan, (void**)&mx_linear, (void**)&mx_linear_bytes,
                        (void**)&column_sum, (void**)&column_sum_bytes, (void**)&mx_attn, (void**)&mx_attn_bytes};
   if (n != (Py_ssize_t)(sizeof(to) / sizeof(to[0]))) {
     PyErr_Format(PyExc_TypeError, "init takes %d addresses, got %d", (int)(sizeof(to) / sizeof(to[0])), (int)n);

@@ -831,8 +831,7 @@ using namespace dpa::mx;
 extern "C" int dpa_mxfp4_gemm_plan(int64_t M, int64_t N, int64_t K, int dtype, DpaMxfp4GemmPlan* out) {
   if (!dtype_ok(dtype)) return DPA_ERR_SHAPE;
   const int st = check_gemm(M, N, K);
-  if (st != DPA_OK) return st;
-  if (!out) return DPA_ERR_NULL;
+  if (st != DPA_OK || !out) return st;
   *out = DpaMxfp4GemmPlan{};
   if (M == 0 || N == 0) return DPA_OK;
   GemmArgs p = plan(M, N, K, false);

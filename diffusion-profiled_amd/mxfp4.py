@@ -204,7 +204,9 @@ def linear_mxfp4_fwd(x: torch.Tensor, weight: torch.Tensor | MXFP4Operand, bias:
                      out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """Q(x) Q(weight)^T + bias in out_dtype (x's by default): x [..., K] and weight [N, K] rounded to MXFP4 with
     blocks along K, sums and bias in fp32, one rounding. weight: bf16, fp16 or fp32, or an operand made of it
-    before (``mxfp4_operand``). Any sizes; the last block of a row may be shorter."""
+    before (``mxfp4_operand``). The last block of a row may be shorter. Sizes: a matrix of r rows and c columns has
+    (r rounded up to 16) * ceil(c / 512) below 2^25, and the same with r and c exchanged; K is at most 2^24 and the output
+    has less than 2^33 elements."""
     if torch.compiler.is_dynamo_compiling():
         return _between_graphs(linear_mxfp4_fwd, x, weight, bias, out_dtype=out_dtype)
     if isinstance(weight, MXFP4Operand):
@@ -246,12 +248,23 @@ class LinearKept(NamedTuple):
     bias: bool
 
 
+def _check_products(m: int, n: int, k: int, want_dx: bool, want_dw: bool) -> None:
+    """Refuses, before anything is launched, sizes of which one of a training step's products is beyond the kernels."""
+    if m == 0 or n == 0:
+        return
+    for what, size in (("output", (m, n, k)), ("dx", (m, k, n) if want_dx else None), ("dweight", (n, k, m) if want_dw else None)):
+        if size and _lib.query("dpa_mxfp4_gemm_plan", *size, 0, None):
+            raise ValueError(f"linear_mxfp4: {m} rows of {k} with a weight [{n}, {k}]: the product of {what}, {size[0]} x {size[1]} "
+                             f"over {size[2]}, is beyond what the kernels take")
+
+
 def _train_fwd(x, weight, bias, out_dtype, want_dx: bool, want_dw: bool):
     if weight.ndim != 2:
         raise ValueError(f"linear_mxfp4: the weight is [N, K], got {tuple(weight.shape)}")
     _on_one_gpu(x, weight)
     n, k = weight.shape
     x2, b32, dtype = _check_linear(x, n, k, bias, out_dtype)
+    _check_products(x2.shape[0], n, k, want_dx, want_dw)
     xr, xc = _operands(x2, True, want_dw, None)
     wr, wc = _operands(weight, True, want_dx, None)
     y = _product(xr, wr, b32, dtype).view(*x.shape[:-1], n)
@@ -261,7 +274,8 @@ def _train_fwd(x, weight, bias, out_dtype, want_dx: bool, want_dw: bool):
 def linear_mxfp4_train_fwd(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                            out_dtype: torch.dtype | None = None) -> tuple[torch.Tensor, LinearKept]:
     """``linear_mxfp4_fwd``, and what ``linear_mxfp4_bwd`` needs of it (17/32 byte an element of x and of
-    the weight)."""
+    the weight). Sizes whose gradients are products beyond the kernels (more than 2^24 rows of x or of the weight) are
+    refused here."""
     if torch.compiler.is_dynamo_compiling():
         return _between_graphs(linear_mxfp4_train_fwd, x, weight, bias, out_dtype=out_dtype)
     done = _fast().mxfp4_train_fwd(x, weight, bias, out_dtype)

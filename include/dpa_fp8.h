@@ -881,7 +881,7 @@ int dpa_mxfp4_gemm(const void* a, const void* b, const float* bias, void* y, int
 
 /* What dpa_mxfp4_gemm would launch, on a device like the current one, for a 16-B aligned y: tiles of side x side (0: a form for
  * up to 64 rows) of y and of the `splits` of K, taken in turn by `workgroups`; vectors: whether y leaves by
- * 16 B. Launches nothing; DPA_ERR_SIZE for a size that dpa_mxfp4_gemm refuses. */
+ * 16 B. Launches nothing; DPA_ERR_SIZE for a size that dpa_mxfp4_gemm refuses. plan may be NULL, for that alone. */
 typedef struct DpaMxfp4GemmPlan {
   int32_t side, vectors, splits, workgroups;
   int64_t tiles;

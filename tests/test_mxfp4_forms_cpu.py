@@ -24,4 +24,4 @@ def test_few_rows_and_refusals():
     assert plan(0, 512, 512, torch.bfloat16)["workgroups"] == 0
     entry, out = dpa_mod("_lib").load().dpa_mxfp4_gemm_plan, bytes(PLAN.size)
     assert entry(1 << 27, 4, 32, 0, out) == -2 and entry(4, 1 << 25, 32, 0, out) == -2
-    assert entry(4, 4, 0, 0, out) == -2 and entry(4, 4, 32, 7, out) == -4 and entry(4, 4, 32, 0, None) == -1
+    assert entry(4, 4, 0, 0, out) == -2 and entry(4, 4, 32, 7, out) == -4 and entry(4, 4, 32, 0, None) == 0
