@@ -22,6 +22,7 @@ from typing import Any, NamedTuple
 import torch
 import torch.nn as nn
 from torch.amp.autocast_mode import custom_bwd, custom_fwd
+from torch.autograd import forward_ad
 
 from . import _lib
 from .conditioning import (_DT, _between_graphs, _check_masks, _check_seed, _fast, _on_one_gpu, _ptr, _rows,
@@ -67,6 +68,13 @@ def _call(entry: str, *args) -> None:
     else:
         with torch.cuda.device(on.device):
             _lib.call(entry, *args, _lib.current_stream(on))
+
+
+def _has_tangent(*tensors: torch.Tensor | None) -> bool:
+    """Whether one of them is a dual tensor of forward-mode differentiation (with gradients off too)."""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 # ---- quantisation ------------------------------------------------------------------------
@@ -366,14 +374,15 @@ def linear_mxfp4(x: torch.Tensor, weight: torch.Tensor | MXFP4Operand, bias: tor
     """Differentiable ``linear_mxfp4_fwd`` with the gradients of ``linear_mxfp4_bwd`` (straight through the
     roundings). stochastic: the output's gradient is rounded stochastically, by ``seed`` or one drawn from
     torch's generator (a captured graph draws a new one each replay). Under autocast the output of an fp32 x is
-    in the autocast dtype. An operand as the weight carries no gradient, and x must not ask for one."""
+    in the autocast dtype. An operand as the weight carries no gradient, and x must not ask for one. There is no
+    forward-mode derivative: dual tensors are refused."""
     if torch.compiler.is_dynamo_compiling():
         return _between_graphs(linear_mxfp4, x, weight, bias, stochastic=stochastic, seed=seed)
     out_dtype = x.dtype
     if x.dtype == torch.float32 and torch.is_autocast_enabled("cuda"):
         out_dtype = torch.get_autocast_dtype("cuda")
     if isinstance(weight, MXFP4Operand):
-        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        if (torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad))) or _has_tangent(x, bias):
             raise ValueError("linear_mxfp4: gradients need the weight itself, not an operand made of it")
         return linear_mxfp4_fwd(x, weight, bias, out_dtype=out_dtype)
     if stochastic and seed is None and torch.is_grad_enabled():
@@ -399,7 +408,7 @@ class LinearMXFP4(nn.Linear):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not x.is_cuda:
             return super().forward(x)
-        if self._kept is not None and not torch.is_grad_enabled():
+        if self._kept is not None and not torch.is_grad_enabled() and not _has_tangent(self.weight):
             return linear_mxfp4(x, self._kept, self.bias)
         return linear_mxfp4(x, self.weight, self.bias, stochastic=True)
 
@@ -466,8 +475,8 @@ def cross_attention_mxfp4_fwd(q: torch.Tensor, kv: MXFP4, *, key_lengths: torch.
 def cross_attention_mxfp4(q: torch.Tensor, kv: MXFP4, *, key_lengths: torch.Tensor | None = None,
                           key_mask: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
     """``cross_attention_mxfp4_fwd``'s first output, for sampling and serving: it has no gradient, and refuses
-    queries that ask for one. Under autocast fp32 queries are rounded to the autocast dtype first."""
-    if torch.is_grad_enabled() and q.requires_grad:
+    queries that ask for one or carry a tangent. Under autocast fp32 queries are rounded to the autocast dtype first."""
+    if (torch.is_grad_enabled() and q.requires_grad) or _has_tangent(q):
         raise ValueError("cross attention over MXFP4 keys and values has no gradient")
     if q.dtype == torch.float32 and torch.is_autocast_enabled("cuda"):
         q = q.to(torch.get_autocast_dtype("cuda"))
