@@ -561,7 +561,8 @@ extern "C" int64_t dpa_column_sum_workspace_bytes(int64_t rows, int64_t cols) {
 extern "C" int dpa_column_sum(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, void* y,
                               void* workspace, int64_t workspace_bytes, void* stream) {
   if (!dtype_ok(dtype)) return DPA_ERR_SHAPE;
-  if (rows <= 0 || cols <= 0 || rows >= (1 << 30) || cols >= (1 << 30) || (row_stride < cols && rows > 1)) return DPA_ERR_SIZE;
+  if (rows <= 0 || cols <= 0 || rows >= (1 << 30) || cols > 64 * kMaxGroups256 || (row_stride < cols && rows > 1))
+    return DPA_ERR_SIZE;
   if (!x || !y) return DPA_ERR_NULL;
   if (!workspace || workspace_bytes < dpa_column_sum_workspace_bytes(rows, cols)) return DPA_ERR_WORKSPACE;
   if (!aligned(x, size_of(dtype)) || !aligned(y, 4) || !aligned(workspace, 4)) return DPA_ERR_ALIGN;

@@ -898,7 +898,7 @@ int dpa_mxfp4_linear(const void* x, int x_dtype, int64_t row_stride, const void*
                      int64_t workspace_bytes, void* stream);
 
 /* y [cols] fp32 = sums down the columns of x [rows][cols] (bf16, fp16 or fp32, rows row_stride elements
- * apart), in fp32, in a fixed order. */
+ * apart), in fp32, in a fixed order. Less than 2^30 rows, at most 2^30 - 64 columns. */
 int64_t dpa_column_sum_workspace_bytes(int64_t rows, int64_t cols);
 int dpa_column_sum(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, void* y,
                    void* workspace, int64_t workspace_bytes, void* stream);

@@ -1,6 +1,8 @@
 """A linear step on MXFP4 operands whose backward would be refused is refused in its forward."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 
 from conftest import dpa_mod
@@ -20,3 +22,11 @@ def test_sizes_that_are_refused(m, n, k, wanted, what):
         check(m, n, k, *wanted)
     if what != "output":        # taken where that gradient is not wanted
         check(m, n, k, False, False)
+
+
+@pytest.mark.parametrize("cols", [(1 << 30) - 63, (1 << 30) - 1, 1 << 30])
+def test_column_sums_of_more_workgroups_than_a_launch_has(cols):
+    """64 columns to a workgroup of 256: beyond 2^24 - 1 of them their number would wrap."""
+    lib = dpa_mod("_lib").load()
+    fake = ctypes.c_void_p(0x1000)      # never dereferenced
+    assert lib.dpa_column_sum(fake, 0, 4, cols, cols, fake, fake, 1 << 40, None) == -2
