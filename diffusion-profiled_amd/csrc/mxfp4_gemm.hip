@@ -28,7 +28,7 @@ struct GemmArgs {
 // columns of y in a row and four lanes 64 B: row r of fragment i is row 32 (i / 2) + 8 (r / 4) + 4 (i % 2) + r % 4 of
 // the wave's. The 16-B piece c of a row lies at c ^ turned(its r / 4): the 16 lanes that LDS serves together (rows
 // 0-3 and 12-15 at one piece, 4-11 at the one beside it) then lie in 16 different places of the banks.
-// Measured: 4096 x 8192 of 8192 125 us, 4.4 PFLOP/s, the matrix instructions busy 54 % of the time at 1.96 GHz. The same
+// Measured: 4096 x 8192 of 8192 122 to 125 us, 4.4 PFLOP/s, the matrix instructions busy 54 % of the time at 1.96 GHz. The same
 // without transfers 109, without reads of LDS 111, without both 100, without the meetings too 93: the products alone,
 // whose power holds the clock below its 2.4 GHz (a loop of nothing else on random operands: 6.9 PFLOP/s).
 // (Four waves of 128 x 128 for 256 x 256: less read of LDS, but nothing to run while a wave waits, 161 us.)
@@ -752,7 +752,9 @@ static bool whole_vectors(int64_t N, int dtype) { return N % (16 / size_of(dtype
 
 // The form for a y that vectors fit or not, and its workgroups
 static unsigned settle(GemmArgs& p, bool vec) {
-  if (!vec && p.form == 0) {  // (the largest tiles leave no registers to turn rows)
+  // (The largest tiles leave no registers to turn rows. plan_tiles does not know y: such a product is costed as one of 256 x 256
+  // tiles, keeps its splits, of which large ones have none, and runs as 128 x 128. Other choices were not measured.)
+  if (!vec && p.form == 0) {
     p.form = 1;
     p.tiles_m = (int)ceil_div(p.M, kForms[1].side), p.tiles_n = (int)ceil_div(p.N, kForms[1].side);
   }

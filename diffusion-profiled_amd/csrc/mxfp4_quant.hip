@@ -146,8 +146,9 @@ __global__ __launch_bounds__(256) void mxfp4_rows_kernel(const RowArgs p) {
 // through LDS. The columns' codes turn in LDS and leave as 32 B of a column; the tiles below each other, which fill
 // a line of 128 B, go to one XCD, whose L2 joins them. (Two or four tiles to a workgroup, the next one's loads ahead, is slower,
 // from cold caches: 8192 x 4096 of bf16 37.7 and 36.2 us against 34.2, 768 x 256 of fp32 10.8 and 16.8 against 7.6.)
-// Within a step 8192 x 4096 of bf16 takes 28 us, stochastically 38, 104 MB at 3.7 and 2.7 TB/s: between the bytes and
-// the conversions, a workgroup's loads, conversions and stores following each other; three workgroups to a CU overlap
+// Within a step 8192 x 4096 of bf16 takes 28 us, stochastically 36, 104 MB at 3.7 and 2.9 TB/s: between the bytes and
+// the conversions (vector instructions hold a SIMD for 10 and 24 us of these, by the counters), a workgroup's loads,
+// conversions and stores following each other; three workgroups to a CU overlap
 // theirs (two, when the sums below cost registers in every variant: 27.2 us for 32768 x 768, with three 25.3).
 // ---------------------------------------------------------------------------------------
 struct BothArgs {

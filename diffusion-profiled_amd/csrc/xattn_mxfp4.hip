@@ -2,6 +2,10 @@
 // xattn_fwd.hip, with values of the operands' type made from the 4-bit ones on the way to the products.
 // The products stay those of bf16 or fp16: queries and probabilities in 4 bits would lose what the cache
 // keeps. A value of the cache is exact in bf16; in fp16 it is one that fp16 holds if it was quantised from fp16.
+// Scores, maxima and sums are fp32; a probability is rounded to the queries' type for the product with the values, as in
+// the 16-bit forms (the sum l takes it before): the product has no operand of fp32, and the sum of two 16-bit ones would be
+// twice the products. Against 64 bits outputs are then 2.1e-3 off in bf16 and 2.9e-4 in fp16 (relative norms), with
+// probabilities in fp32 1.7e-3 and 2.1e-4, which the output's own rounding makes.
 #include <algorithm>
 #include <type_traits>
 
@@ -56,8 +60,10 @@ __device__ __forceinline__ void put_block(uint32_t at, int row, int blk, const R
 
 // ---------------------------------------------------------------------------------------
 // Four waves of 32 query rows share tiles of 64 keys; a tile's blocks go through registers, one tile ahead. Bound as the
-// 16-bit form is, by the products and the softmax; the conversions cost what the shorter loads save: 8 x 1024 queries
-// of 8 heads of 128 over 4096 keys 152 us, there 150; 4 x 4096 of 8 heads of 64 over 1031 keys in fp16 55.5, there 52.2.
+// 16-bit form is, by the products and the softmax, and by the conversions, which cost more than the shorter loads save: 8 x 1024 queries
+// of 8 heads of 128 over 4096 keys 149 us, there 143; 4 x 4096 of 8 heads of 64, two to a key head, over 1031 keys in fp16 52.3,
+// there 47.2. (Of 64 dims four workgroups share a CU, with 128 registers a lane, of which four addresses of
+// put_block lie in scratch: every second step loads them again, one after the other.)
 // ---------------------------------------------------------------------------------------
 constexpr float kSlack = 8.f;
 
@@ -232,7 +238,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void xattn_mxfp4_fwd_kernel
 // Few rows: four waves share 32 rows and take every fourth tile of 32 keys each, and join their softmaxes
 // in LDS. A lane's key goes straight to its A operand: dims [h DP / 2, (h + 1) DP / 2) of key l & 31, eight of
 // them to a product, and the queries likewise. Values pass through LDS, whose transpose reads turn them. 16 x 8
-// queries of 16 heads, four to a key head of 128, over 4096 keys 30.9 us with the join, in 16 bits 36.1.
+// queries of 16 heads, four to a key head of 128, over 4096 keys 29.8 us with the join, in 16 bits 35.4.
 // ---------------------------------------------------------------------------------------
 template <class T, int DP>
 __global__ __launch_bounds__(256, 2) void xattn_mxfp4_few_kernel(const MxArgs p) {
@@ -455,7 +461,6 @@ __global__ __launch_bounds__(256, 2) void xattn_mxfp4_few_kernel(const MxArgs p)
 //   reads fetch rows 4 q .. and 16 + 4 q ...
 // ---------------------------------------------------------------------------------------
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 template <class T>
 __device__ __forceinline__ v4f mfma16(uint4 a, uint4 b, v4f c) {
@@ -710,7 +715,7 @@ __global__ __launch_bounds__(256, 2) void xattn_mxfp4_token_kernel(const MxArgs 
 
 // ---------------------------------------------------------------------------------------
 // Up to 128 keys: xattn_short.hpp over the values that a workgroup makes of them once. 128 x 1024 queries of 4 heads of
-// 64 dims over 77 keys 30.2 us, by tiles of keys 40, in 16 bits 30.3: bound by the queries and the output.
+// 64 dims over 77 keys 28.7 us, by tiles of keys 40, in 16 bits 30.3: bound by the queries and the output.
 // ---------------------------------------------------------------------------------------
 template <class T, int DP, int NB>
 __global__ __launch_bounds__(256, short_waves(DP)) void xattn_mxfp4_short_kernel(const MxArgs p) {

@@ -425,8 +425,8 @@ def cross_attention_mxfp4_fwd(q: torch.Tensor, kv: MXFP4, *, key_lengths: torch.
 
     q [B, Lq, H, D] in bf16 or fp16, kv of the shape [B, Lk, 2, G, D] (keys, then values:
     ``quantize_mxfp4`` of what ``cross_attention_kv`` takes), D a multiple of 32 up to 128, G dividing H.
-    Products, softmax and sums are those of q's dtype; with fp16, a value of the cache beyond fp16's
-    range is an infinity (one that was quantised from fp16 is exact). Any strides with dense heads whose
+    Products are those of q's dtype, to which the probabilities are rounded; scores, softmax and sums are fp32. With
+    fp16, a value of the cache beyond fp16's range is an infinity (one that was quantised from fp16 is exact). Any strides with dense heads whose
     data lies in multiples of 16 bytes are read in place (``expand`` over the batch, a part of a longer
     cache), others through a copy. Lengths, mask and what hidden keys hold: as there."""
     if torch.compiler.is_dynamo_compiling():
